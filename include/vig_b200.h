@@ -374,6 +374,57 @@ VIG_API int vig_linear_swiglu_preferred(int64_t M, int K, int I, int dtype);   /
 VIG_API int vig_linear_swiglu_fwd(const void* x, int64_t ldx, const void* w, void* out, int64_t ldo,
                           int64_t M, int K, int I, int dtype, int32_t* status_dev, void* stream);
 
+/* ---- training and serving of a block with a gated recurrence -------------------------------------------------------------------------- */
+#define VIG_OUT_E4M3 0
+#define VIG_OUT_INT8 1
+
+/*
+ * Gated linear recurrence with one state per channel: h_t = a_t h_{t-1} + x_t (reverse: h_t = a_t h_{t+1} + x_t), a_t = exp(g_t), or with
+ * gate_logit_normalizer n > 0 from raw logits, a_t = sigmoid(g_t)^(1/n).  x, g, h: [B, L, D] with unit stride over D and element strides
+ * (b, l) (NULL = contiguous); any alignment; h may not overlap x or g.  h0 (optional), h_final (optional): fp32 [B, D] with row strides
+ * ld_h0, ld_final; h_final may be h0 itself (a state updated in place), and L may be 0 (the state is handed on) or 1 (one new token).
+ */
+VIG_API int vig_gated_recurrence_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final,
+                                     int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,
+                                     float gate_logit_normalizer, int reverse, int dtype, void* stream);
+/* Its gradients: from g, the output h, h0 (NULL as in the forward), d_h and d_final (optional, fp32 [B, D]): d_x and d_g ([B, L, D] contiguous;
+ * d_g with respect to what g holds) and d_h0 (optional, fp32 [B, D]). */
+VIG_API int vig_gated_recurrence_bwd(const void* g, const void* h, const float* h0, const void* d_h, const float* d_final, void* d_x, void* d_g, float* d_h0,
+                                     int B, int L, int D, const int64_t* strides_g, const int64_t* strides_h, const int64_t* strides_dh,
+                                     float gate_logit_normalizer, int reverse, int dtype, void* stream);
+
+/*
+ * Optional residual add and RMSNorm with 8-bit rows out: s = x (+ residual), y = s * rsqrt(mean(s^2) + eps) * w, and for every group of
+ * `group` channels (32, 64 or 128, dividing N; 0 or N: the row) scale = max|y| / top and q = round(y / scale), top = 448 (e4m3) or 127 (int8);
+ * a group of zeros has scale 0.  y is taken from the fp32 sum and is not rounded before q.  x, residual: [rows, N] with row strides ldx,
+ * ldr; w: [N] of w_dtype (the rows' dtype or fp32); q: [rows, N] bytes; scales: fp32 [rows, N / group]; residual_out (optional): [rows, N], s.
+ */
+VIG_API int vig_add_rmsnorm_8bit_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* w, int w_dtype, void* q, float* scales,
+                                     void* residual_out, int64_t rows, int N, int group, float eps, int out_type, int dtype, void* stream);
+/* The same norm with y in the rows' dtype, any N and alignment: the forward of a trained norm. */
+VIG_API int vig_add_rmsnorm_train_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* w, int w_dtype, void* y,
+                                      void* residual_out, int64_t rows, int N, float eps, int dtype, void* stream);
+/* Its gradients from dy, the sum r (residual_out, or x where there was no residual) and optionally d_r, the gradient of r itself:
+ * dx [rows, N] contiguous (of x and of the residual alike) and dw [N] of w_dtype.  Row strides ldy, ldr, ld_dr.  The workspace holds the
+ * blocks' shares of dw, which are added in a fixed order. */
+VIG_API size_t vig_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int N);
+VIG_API int vig_add_rmsnorm_bwd(const void* dy, int64_t ldy, const void* r, int64_t ldr, const void* w, int w_dtype, const void* d_r, int64_t ld_dr,
+                                void* dx, void* dw, int64_t rows, int N, float eps, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One AdamW step over `count` tensors: m = b1 m + (1-b1) g, v = b2 v + (1-b2) g^2,
+ * p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps).  All arrays are on the HOST, with one entry a tensor:
+ * device pointers, numbers of values, dtype codes of parameter and gradient.  masters (optional, entries optional): fp32 copies of the
+ * parameters, which are then what is stepped, the parameter being their rounding.  States are fp32, or, for a tensor with entries in both
+ * exp_avg_scales and exp_avg_sq_scales (fp32, one value per 256 values begun), e4m3 codes of m / scale and of sqrt(v) / scale; a root that is
+ * not zero never gets the code 0.  grad_scale (optional, one fp32 on the device): what gradients are multiplied by first; found_inf (optional,
+ * one fp32 on the device): where it is not 0, nothing is written.  No two tensors may overlap.
+ */
+VIG_API int vig_adamw_step(int count, void* const* params, const void* const* grads, void* const* exp_avgs, void* const* exp_avg_sqs,
+                           float* const* masters, float* const* exp_avg_scales, float* const* exp_avg_sq_scales, const int64_t* numels,
+                           const int* param_dtypes, const int* grad_dtypes, int64_t step, double lr, double beta1, double beta2, double eps,
+                           double weight_decay, const float* grad_scale, const float* found_inf, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

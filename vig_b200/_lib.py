@@ -4,7 +4,7 @@ There is no fallback: if the library is missing or a call is rejected, a ``Runti
 """
 import ctypes
 import os
-from ctypes import c_float, c_int, c_int32, c_int64, c_size_t, c_void_p, POINTER
+from ctypes import c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p, POINTER
 
 import torch
 
@@ -61,6 +61,13 @@ _SIGNATURES = {
     "vig_stem_fold_fwd": (c_int, [c_void_p, c_void_p] + [c_int] * 5 + [c_void_p]),
     "vig_stem_conv_ln_supported": (c_int, [c_int] * 6),
     "vig_stem_conv_ln_fwd": (c_int, [c_void_p] * 6 + [c_int] * 5 + [c_float, c_int, c_int, c_void_p, c_void_p]),
+    "vig_gated_recurrence_fwd": (c_int, [c_void_p] * 3 + [c_int64] + [c_void_p] * 2 + [c_int64] + [c_int] * 3 + [_P64] * 3 + [c_float, c_int, c_int, c_void_p]),
+    "vig_gated_recurrence_bwd": (c_int, [c_void_p] * 8 + [c_int] * 3 + [_P64] * 3 + [c_float, c_int, c_int, c_void_p]),
+    "vig_add_rmsnorm_8bit_fwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p, c_int] + [c_void_p] * 3 + [c_int64, c_int, c_int, c_float, c_int, c_int, c_void_p]),
+    "vig_add_rmsnorm_train_fwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p, c_int] + [c_void_p] * 2 + [c_int64, c_int, c_float, c_int, c_void_p]),
+    "vig_add_rmsnorm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "vig_add_rmsnorm_bwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p, c_int] + [c_void_p, c_int64] + [c_void_p] * 2 + [c_int64, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "vig_adamw_step": (c_int, [c_int] + [POINTER(c_void_p)] * 7 + [_P64] + [POINTER(c_int)] * 2 + [c_int64] + [c_double] * 5 + [c_void_p] * 3),
     "vig_swiglu_fwd": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int64, c_int64, c_int, c_void_p]),
 }
 EXPORTS = tuple(_SIGNATURES)

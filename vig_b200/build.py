@@ -9,8 +9,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libvig_b200.so")
 HOST = os.path.join(HERE, "_host.so")
-HOST_SOURCES = ["host_ops.cpp", "host_model.cpp"]
-SOURCES = ["abi.cu", "bigla_simt.cu", "bigla_tc.cu", "bigla_wave.cu", "elementwise.cu", "noalloc.cu", "bigla_bwd_simt.cu", "bigla_bwd_mma.cu", "bigla_seg.cu", "block_tail.cu", "conv_proj.cu", "embed_conv.cu", "gemm_swiglu.cu", "gemm_pair.cu", "gemm_pair_norm.cu", "gemm_addnorm.cu", "dwconv_tma.cu", "gemm_bias.cu", "gemm_stem.cu"]
+HOST_SOURCES = ["host_ops.cpp", "host_model.cpp", "host_train.cpp"]
+SOURCES = ["abi.cu", "bigla_simt.cu", "bigla_tc.cu", "bigla_wave.cu", "elementwise.cu", "noalloc.cu", "bigla_bwd_simt.cu", "bigla_bwd_mma.cu", "bigla_seg.cu", "block_tail.cu", "conv_proj.cu", "embed_conv.cu", "gemm_swiglu.cu", "gemm_pair.cu", "gemm_pair_norm.cu", "gemm_addnorm.cu", "dwconv_tma.cu", "gemm_bias.cu", "gemm_stem.cu",
+           "gated_recurrence.cu", "rmsnorm_rows.cu", "adamw.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 

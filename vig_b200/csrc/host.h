@@ -17,7 +17,9 @@ namespace py = pybind11;
     X(vig_dwconv3x3_fwd) X(vig_gate_inject_fwd) X(vig_add_rmsnorm_fwd) X(vig_layernorm_act_fwd) X(vig_layernorm_act_add_fwd)  \
     X(vig_layernorm_act_add_rmsnorm_fwd) X(vig_linear_swiglu_fwd) X(vig_linear_swiglu_preferred) X(vig_linear_add_rmsnorm_fwd) X(vig_linear_add_rmsnorm_preferred) \
     X(vig_stem_fold_fwd) X(vig_stem_unfold_fwd) X(vig_stem_conv_ln_fwd)                   \
-    X(vig_stem_conv_ln_supported) X(vig_swiglu_fwd) X(vig_add_layernorm_fwd) X(vig_chain_launches) X(vig_token_mean_fwd) X(vig_embed_conv_ln_fwd) X(vig_linear_pair_preferred) X(vig_linear_pair_fwd) X(vig_conv_proj_preferred) X(vig_conv_proj_fwd) X(vig_block_tail_preferred) X(vig_block_tail_fwd)
+    X(vig_stem_conv_ln_supported) X(vig_swiglu_fwd) X(vig_add_layernorm_fwd) X(vig_chain_launches) X(vig_token_mean_fwd) X(vig_embed_conv_ln_fwd) X(vig_linear_pair_preferred) X(vig_linear_pair_fwd) X(vig_conv_proj_preferred) X(vig_conv_proj_fwd) X(vig_block_tail_preferred) X(vig_block_tail_fwd) \
+    X(vig_gated_recurrence_fwd) X(vig_gated_recurrence_bwd) X(vig_add_rmsnorm_8bit_fwd) X(vig_add_rmsnorm_train_fwd) X(vig_add_rmsnorm_bwd) \
+    X(vig_add_rmsnorm_bwd_workspace_bytes) X(vig_adamw_step)
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
     VIG_HOST_API(X)
@@ -53,5 +55,6 @@ void bi_gla_into(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
                  double norm, double clamp, const Tensor& init_f, const Tensor& init_b, const Tensor& final_f, const Tensor& final_b, int dir_mask, int impl);
 
 void bind_model(py::module_& m);
+void bind_train(py::module_& m);
 
 }  // namespace vig_host

@@ -165,4 +165,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("bi_gla_stacked", &bi_gla_stacked);
     m.def("scan", &scan);
     bind_model(m);
+    bind_train(m);
 }

@@ -4,8 +4,8 @@
 ``fused_chunk_gla`` mirrors ``fla/ops/gla/chunk_fuse.py:554-572`` and ``chunk_gla``
 ``fla/ops/gla/chunk.py:561-580``; ``bi_gla`` is the explicit form of the merged operator.
 Tensors are ``[B, H, L, d]`` views with a contiguous last dimension; no copies are made.
-``bi_gla`` and the one-direction entry points are differentiable (``vig_bigla_bwd_full``); the block's other kernels
-are inference-only.
+``bi_gla`` and the one-direction entry points are differentiable (``vig_bigla_bwd_full``), and so are ``gated_recurrence`` and
+``add_rmsnorm_train``; the block's other kernels are inference-only.
 """
 import math
 
@@ -653,3 +653,65 @@ def linear_bias(x, weight, bias=None):
 def swiglu_linear(x, y, weight, bias):
     """``fla/modules/activations.py:150-174``: ``F.linear(swiglu(x, y), weight, bias)``."""
     return torch.nn.functional.linear(swiglu(x, y), weight, bias)
+
+
+# --------------------------------------------------------------------------------------------------
+# Training and serving of a block with a gated recurrence: checks, outputs and autograd nodes are in ``csrc/host_train.cpp``.
+OUT_8BIT = {torch.float8_e4m3fn: 0, torch.int8: 1}
+
+
+def gated_recurrence(x, g, initial_state=None, output_final_state=False, *, reverse=False, gate_logit_normalizer=0.0):
+    """``h_t = a_t * h_{t-1} + x_t`` with one state per channel (``reverse``: from the last token to the first), ``a_t = exp(g_t)``; with
+    ``gate_logit_normalizer`` n > 0 ``g`` holds raw logits and ``a_t = exp(logsigmoid(g_t) / n)``, as in ``bi_gla``.
+
+    ``x``, ``g``: ``[B, L, D]`` of one dtype, any strides with a contiguous last dimension.  ``initial_state``: fp32 ``[B, D]``.  Returns
+    ``(h, final_state)``, ``h`` in ``x``'s dtype, ``final_state`` fp32 or None.  States and sums are fp32.  Log-gates may be ``-inf`` (the
+    state starts anew at that token).  Differentiable in ``x``, ``g`` and ``initial_state``, through both results."""
+    return _lib.host().gated_recurrence(x, g, initial_state, output_final_state, reverse, gate_logit_normalizer)
+
+
+def gated_recurrence_step(x, g, state, *, gate_logit_normalizer=0.0):
+    """One new token of ``gated_recurrence``: ``x``, ``g`` ``[B, D]``; ``state`` (fp32 ``[B, D]``, rows may be a slice of a larger table) is
+    updated in place.  Returns ``h`` ``[B, D]``.  No gradient."""
+    return _lib.host().gated_recurrence_step(x, g, state, gate_logit_normalizer)
+
+
+def add_rmsnorm_8bit(x, weight, residual=None, eps=1e-6, dtype=torch.float8_e4m3fn, group=None, prenorm=False):
+    """``add_rmsnorm`` with 8-bit rows out, for a product in 8 bits: ``(q, scales)``, or ``(q, scales, x + residual)`` with ``prenorm``.
+
+    ``q`` (``float8_e4m3fn`` or ``int8``, ``x``'s shape) times ``scales`` (fp32 ``[..., N / group]``; ``group`` None: one scale a row) is the
+    normed row; ``scales = max|y| / 448`` (or 127), 0 where all of a group is zero.  ``group``: 32, 64 or 128.  Any N, any row strides.
+    ``weight`` in ``x``'s dtype or fp32.  The norm is taken from the fp32 sum.  No gradient."""
+    try:
+        out = OUT_8BIT[dtype]
+    except KeyError:
+        raise TypeError(f"unsupported 8-bit dtype {dtype}; expected float8_e4m3fn or int8") from None
+    q, scales, r = _lib.host().add_rmsnorm_8bit(x, weight, residual, eps, out, group or 0, prenorm)
+    return (q, scales, r) if prenorm else (q, scales)
+
+
+def add_rmsnorm_train(x, weight, residual=None, eps=1e-6):
+    """``(y, r)``: ``r = x + residual`` (``x`` itself without one), ``y = RMSNorm(r) * weight``; differentiable in ``x``, ``weight`` and
+    ``residual``, through both results.  Any N, any row strides; ``weight`` in ``x``'s dtype or fp32 (its gradient has the same).  The norm is
+    taken from the fp32 sum, where ``add_rmsnorm`` rounds the sum first."""
+    return _lib.host().add_rmsnorm_train(x, weight, residual, eps)
+
+
+def add_rmsnorm_backward(d_y, r, weight, eps=1e-6, d_r=None):
+    """Gradients of ``add_rmsnorm_train`` at the sum ``r``: ``(dx, dweight)``; ``dx`` is the residual's gradient too.  ``d_r``: what comes to
+    ``r`` from elsewhere."""
+    return _lib.host().add_rmsnorm_backward(d_y, r, weight, eps, d_r)
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, masters=None,
+               exp_avg_scales=None, exp_avg_sq_scales=None, grad_scale=None, found_inf=None):
+    """One AdamW step over lists of tensors, in place and in one launch for up to 400 of them (see ``vig_adamw_step`` for the formula).
+
+    ``params``, ``grads``: fp32, bf16 or fp16, mixed as they come; ``step`` counts from 1.  ``masters`` (entries may be None): fp32 copies that
+    are stepped in the parameters' place, these being their rounding.  States are fp32 tensors like the parameters, or, for tensors with
+    entries in both lists of scales (fp32, one value per 256 values begun, in memory order), ``float8_e4m3fn`` codes: ``exp_avg = code * scale``,
+    ``sqrt(exp_avg_sq) = code * scale``.  ``grad_scale`` / ``found_inf``: fp32 tensors of one value; gradients are multiplied by the first, and
+    nothing is written where the second is not 0.  Tensors must not overlap."""
+    beta1, beta2 = betas
+    _lib.host().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, masters, exp_avg_scales, exp_avg_sq_scales,
+                           grad_scale, found_inf)

@@ -1,0 +1,51 @@
+"""A causal block on the gated recurrence: norm -> one projection to ``[x | gate logits | output gate]`` -> recurrence -> ``h * silu(gate)`` ->
+output projection, with the residual stream handed from block to block as in ``GLABlock.forward_deferred``.  ``forward`` trains it and
+reads a prefix in; ``step`` serves one token at a time, with 8-bit products once ``quantize`` has been called."""
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from . import ops
+from .modules import RMSNorm
+
+
+class GatedRecurrence(nn.Module):
+    def __init__(self, d_model, d_inner=None, gate_logit_normalizer=16.0, eps=1e-6):
+        super().__init__()
+        self.d_model, self.d_inner = d_model, d_inner or d_model
+        self.gate_logit_normalizer = gate_logit_normalizer
+        self.norm = RMSNorm(d_model, eps=eps)
+        self.in_proj = nn.Linear(d_model, 3 * self.d_inner, bias=False)
+        self.out_proj = nn.Linear(self.d_inner, d_model, bias=False)
+        self._in_8bit = None
+
+    def forward(self, hidden, residual=None, state=None, output_final_state=False):
+        """``hidden`` ``[B, L, d_model]`` and the residual stream (None: it begins with ``hidden``); ``state``: fp32 ``[B, d_inner]`` of the tokens
+        before.  Returns ``(output, residual, final_state)``; differentiable."""
+        y, residual = ops.add_rmsnorm_train(hidden, self.norm.weight, residual, self.norm.eps)
+        x, g, o = self.in_proj(y).chunk(3, -1)
+        h, final = ops.gated_recurrence(x, g, state, output_final_state, gate_logit_normalizer=self.gate_logit_normalizer)
+        return self.out_proj(h * F.silu(o)), residual, final
+
+    @torch.no_grad()
+    def quantize(self):
+        """Lays out the input projection for ``step`` as e4m3 codes with a scale per output channel; weights that change later need another call."""
+        w = self.in_proj.weight.float()
+        scale = (w.abs().amax(1) / 448.0).clamp_min(torch.finfo(torch.float32).tiny)
+        self._in_8bit = ((w / scale[:, None]).to(torch.float8_e4m3fn), scale)
+        return self
+
+    @torch.no_grad()
+    def step(self, hidden, residual, state):
+        """One token: ``hidden``, ``residual`` ``[B, d_model]`` (``residual`` may be None), ``state`` fp32 ``[B, d_inner]``, updated in place.
+        Returns ``(output, residual)``."""
+        if self._in_8bit is not None:
+            w, w_scale = self._in_8bit
+            q, scale, residual = ops.add_rmsnorm_8bit(hidden, self.norm.weight, residual, self.norm.eps, prenorm=True)
+            z = torch._scaled_mm(q, w.t(), scale_a=scale, scale_b=w_scale[None], out_dtype=torch.bfloat16).to(hidden.dtype)
+        else:
+            y, residual = ops.add_rmsnorm_train(hidden, self.norm.weight, residual, self.norm.eps)
+            z = self.in_proj(y)
+        x, g, o = z.chunk(3, -1)
+        h = ops.gated_recurrence_step(x, g, state, gate_logit_normalizer=self.gate_logit_normalizer)
+        return self.out_proj(h * F.silu(o)), residual
