@@ -383,6 +383,7 @@ VIG_API int vig_linear_swiglu_fwd(const void* x, int64_t ldx, const void* w, voi
  * gate_logit_normalizer n > 0 from raw logits, a_t = sigmoid(g_t)^(1/n).  x, g, h: [B, L, D] with unit stride over D and element strides
  * (b, l) (NULL = contiguous); any alignment; h may not overlap x or g.  h0 (optional), h_final (optional): fp32 [B, D] with row strides
  * ld_h0, ld_final; h_final may be h0 itself (a state updated in place), and L may be 0 (the state is handed on) or 1 (one new token).
+ * B * D < 2^31, L < 2^30.
  */
 VIG_API int vig_gated_recurrence_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final,
                                      int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,

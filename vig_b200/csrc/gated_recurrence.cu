@@ -25,9 +25,15 @@ struct RecParams {
     int from_end;                   // the scan at hand starts at token L-1
 };
 
-// decay of one token
-template <bool LOGITS> __device__ __forceinline__ float decay_of(float g, float inv_norm) {
-    return expf(LOGITS ? log_sigmoid(g) * inv_norm : g);
+// decay of one token.  16-bit types: two or three MUFU instructions, right to about 2^-21 of the decay; fp32: the exact functions
+template <typename T, bool LOGITS> __device__ __forceinline__ float decay_of(float g, float inv_norm) {
+    if (sizeof(T) == 4) return expf(LOGITS ? log_sigmoid(g) * inv_norm : g);
+    if (!LOGITS) return __expf(g);
+    return __expf((fminf(g, 0.f) - __logf(1.f + __expf(-fabsf(g)))) * inv_norm);
+}
+// d logsigmoid(z) / dz
+template <typename T> __device__ __forceinline__ float rest_of(float z) {
+    return sizeof(T) == 4 ? 1.f / (1.f + expf(z)) : __fdividef(1.f, 1.f + __expf(z));
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -45,7 +51,7 @@ __global__ void __launch_bounds__(128) rec_serial_kernel(const RecParams p) {
     float s = p.s0 ? p.s0[b * p.ld_s0 + d] : 0.f;
     for (int k = 0; k < p.L; ++k) {
         const int64_t t = p.from_end ? p.L - 1 - k : k;
-        const float gv = DType<T>::to_f(g[t * p.sg[1]]), a = decay_of<LOGITS>(gv, p.inv_norm);
+        const float gv = DType<T>::to_f(g[t * p.sg[1]]), a = decay_of<T, LOGITS>(gv, p.inv_norm);
         const float xv = DType<T>::to_f(x[t * p.sx[1]]);
         if (!BWD) {
             s = fmaf(a, s, xv);
@@ -56,7 +62,7 @@ __global__ void __launch_bounds__(128) rec_serial_kernel(const RecParams p) {
             const int64_t before = p.from_end ? t - 1 : t + 1;
             const float hb = k + 1 < p.L ? DType<T>::to_f(hin[before * p.sh[1]]) : p.h0 ? p.h0[(int64_t)b * p.D + d] : 0.f;
             float dg = s * hb;
-            if (LOGITS) dg *= p.inv_norm / (1.f + expf(gv));
+            if (LOGITS) dg *= p.inv_norm * rest_of<T>(gv);
             out[t * p.so[1]] = DType<T>::from_f(dx);
             outg[t * p.sog[1]] = DType<T>::from_f(dg);
         }
@@ -64,11 +70,224 @@ __global__ void __launch_bounds__(128) rec_serial_kernel(const RecParams p) {
     if (p.s_end) p.s_end[b * p.ld_end + d] = s;
 }
 
+// ---------------------------------------------------------------------------------------------------
+// A cluster of CTAs owns a strip of 32 * V channels of one sequence and walks it in steps of (CTAs x 8 warps x RUN) tokens.  A warp's lanes
+// are channels (rows of a strip are read whole), a thread holds RUN consecutive tokens of its channels in registers.  In a step every
+// thread scans its tokens from a zero state, which gives the product of their decays and their own contribution; these pairs meet in shared
+// memory, the CTAs' totals in the shared memory of every CTA of the cluster, at one cluster barrier; each thread then joins the pairs ahead
+// of it to the state that the step began with and walks its tokens again from there, now in the order of the definition.  The next step's
+// tokens are requested before the first meeting.  Every value is read and written once.  No state is rounded, no order depends on timing.
+// A pair is joined to a state by h + a s, except that a state of 0 gives h: products of decays above one may overflow.
+template <typename T, int V> struct Raw;
+template <> struct Raw<float, 1> {
+    using type = float;
+    static __device__ void get(float r, float* f) { f[0] = r; }
+    static __device__ float put(const float* f) { return f[0]; }
+};
+template <typename T> struct Raw<T, 1> {
+    using type = T;
+    static __device__ void get(T r, float* f) { f[0] = DType<T>::to_f(r); }
+    static __device__ T put(const float* f) { return DType<T>::from_f(f[0]); }
+};
+template <> struct Raw<__nv_bfloat16, 2> {
+    using type = __nv_bfloat162;
+    static __device__ void get(type r, float* f) { const float2 v = __bfloat1622float2(r); f[0] = v.x; f[1] = v.y; }
+    static __device__ type put(const float* f) { return __floats2bfloat162_rn(f[0], f[1]); }
+};
+template <> struct Raw<__half, 2> {
+    using type = __half2;
+    static __device__ void get(type r, float* f) { const float2 v = __half22float2(r); f[0] = v.x; f[1] = v.y; }
+    static __device__ type put(const float* f) { return __floats2half2_rn(f[0], f[1]); }
+};
+
+constexpr int RW = 8;                 // warps of a CTA
+constexpr int RC = 8;                 // CTAs of a cluster, at most
+
+__device__ __forceinline__ float join(float a, float h, float s) { return s == 0.f ? h : fmaf(a, s, h); }
+
+template <typename T, bool LOGITS, bool BWD, int V, int RUN>
+__global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p) {
+    using R = typename Raw<T, V>::type;
+    __shared__ float2 own[2][RW][32 * V];          // (product of decays, contribution) of each warp's tokens
+    __shared__ float2 all[2][RC][32 * V];          // of each CTA's
+    uint32_t rank, ctas;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");       // I run; waited for before the first CTA's memory is written
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int strips = (p.D + 32 * V - 1) / (32 * V);
+    const int strip = blockIdx.x / ctas, b = strip / strips, d = (strip % strips) * 32 * V + lane * V;
+    const bool live = d < p.D;
+    const T* x = (const T*)p.x + b * p.sx[0] + d;
+    const T* g = (const T*)p.g + b * p.sg[0] + d;
+    const T* hin = BWD ? (const T*)p.h_in + b * p.sh[0] + d : nullptr;
+    T* out = (T*)p.out + b * p.so[0] + d;
+    T* outg = BWD ? (T*)p.out_g + b * p.sog[0] + d : nullptr;
+    const int per = (int)ctas * RW * RUN;          // tokens of a step
+    float carry[V], first[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        carry[v] = live && p.s0 ? p.s0[b * p.ld_s0 + d + v] : 0.f;
+        first[v] = BWD && live && p.h0 ? p.h0[(int64_t)b * p.D + d + v] : 0.f;
+    }
+    const auto at = [&](int k) { return (int64_t)(p.from_end ? p.L - 1 - k : k); };
+    R xn[RUN], gn[RUN], hn[BWD ? RUN : 1];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+            const int k = k0 + i;
+            if (live && k < p.L) {
+                const int64_t t = at(k);
+                xn[i] = *(const R*)(x + t * p.sx[1]);
+                gn[i] = *(const R*)(g + t * p.sg[1]);
+                if (BWD && k + 1 < p.L) hn[i] = *(const R*)(hin + at(k + 1) * p.sh[1]);
+            }
+        }
+    };
+    const int mine = ((int)rank * RW + wid) * RUN;
+    fetch(mine);
+    for (int base = 0, buf = 0; base < p.L; base += per, buf ^= 1) {
+        const int k0 = base + mine;
+        float a[RUN][V], A[V], H[V];
+        R xr[RUN], gr[BWD && LOGITS ? RUN : 1], hr[BWD ? RUN : 1];
+#pragma unroll
+        for (int v = 0; v < V; ++v) { A[v] = 1.f; H[v] = 0.f; }
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+            const bool in = live && k0 + i < p.L;
+            float gf[V], xf[V];
+            Raw<T, V>::get(gn[i], gf);
+            Raw<T, V>::get(xn[i], xf);
+            xr[i] = xn[i];
+            if (BWD && LOGITS) gr[i] = gn[i];
+            if (BWD) hr[i] = hn[i];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                a[i][v] = in ? decay_of<T, LOGITS>(gf[v], p.inv_norm) : 1.f;
+                if (in) H[v] = BWD ? a[i][v] * (xf[v] + H[v]) : fmaf(a[i][v], H[v], xf[v]);
+                A[v] *= a[i][v];
+            }
+        }
+        if (base + per < p.L) fetch(k0 + per);
+#pragma unroll
+        for (int v = 0; v < V; ++v) own[buf][wid][lane * V + v] = make_float2(A[v], H[v]);
+        __syncthreads();
+        // joined: the tokens of the CTA ahead of this warp's; and all of them
+        float pa[V], ph[V], ta[V], th[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            pa[v] = ta[v] = 1.f; ph[v] = th[v] = 0.f;
+#pragma unroll
+            for (int w = 0; w < RW; ++w) {
+                if (w == wid) { pa[v] = ta[v]; ph[v] = th[v]; }
+                const float2 e = own[buf][w][lane * V + v];
+                th[v] = join(e.x, e.y, th[v]);
+                ta[v] *= e.x;
+            }
+        }
+        float s[V];
+        if (ctas > 1) {
+            if (base == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+            for (uint32_t to = wid; to < ctas; to += RW) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const uint32_t here = (uint32_t)__cvta_generic_to_shared(&all[buf][rank][lane * V + v]);
+                    uint32_t there;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(to));
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(ta[v]), "f"(th[v]) : "memory");
+                }
+            }
+            asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                s[v] = carry[v];
+                for (uint32_t r = 0; r < ctas; ++r) {
+                    if (r == rank) s[v] = carry[v];
+                    const float2 e = all[buf][r][lane * V + v];
+                    carry[v] = join(e.x, e.y, carry[v]);
+                }
+                s[v] = join(pa[v], ph[v], s[v]);
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                s[v] = join(pa[v], ph[v], carry[v]);
+                carry[v] = join(ta[v], th[v], carry[v]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) {
+            const int k = k0 + i;
+            if (!live || k >= p.L) continue;
+            const int64_t t = at(k);
+            float xf[V], o[V];
+            Raw<T, V>::get(xr[i], xf);
+            if (!BWD) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[v] = s[v] = fmaf(a[i][v], s[v], xf[v]);
+                *(R*)(out + t * p.so[1]) = Raw<T, V>::put(o);
+            } else {
+                float hf[V], gf[V], og[V];
+                Raw<T, V>::get(hr[i], hf);
+                if (LOGITS) Raw<T, V>::get(gr[i], gf);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    o[v] = xf[v] + s[v];
+                    s[v] = a[i][v] * o[v];
+                    og[v] = s[v] * (k + 1 < p.L ? hf[v] : first[v]);
+                    if (LOGITS) og[v] *= p.inv_norm * rest_of<T>(gf[v]);
+                }
+                *(R*)(out + t * p.so[1]) = Raw<T, V>::put(o);
+                *(R*)(outg + t * p.sog[1]) = Raw<T, V>::put(og);
+            }
+        }
+        // the state behind the last token, as that token's output was rounded from it
+        if (p.s_end && live && k0 < p.L && k0 + RUN >= p.L) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) p.s_end[b * p.ld_end + d + v] = s[v];
+        }
+    }
+}
+
+// CTAs of a cluster: enough to fill the SMs twice over, no more than the sequence has steps for
+template <int RUN> int rec_ctas(int64_t strips, int L) {
+    const int64_t room = 2ll * device_sms() / strips;
+    const int need = (L + RW * RUN - 1) / (RW * RUN);
+    int c = (int)(room < 1 ? 1 : room > RC ? RC : room);
+    return c < need ? c : need;
+}
+
+template <typename T, bool LOGITS, bool BWD, int V, int RUN>
+int rec_strips(const RecParams& p, cudaStream_t s) {
+    const int64_t strips = (int64_t)p.B * ((p.D + 32 * V - 1) / (32 * V));
+    int c = rec_ctas<RUN>(strips, p.L);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(strips * c)); cfg.blockDim = dim3(RW * 32); cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = c; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, rec_strip_kernel<T, LOGITS, BWD, V, RUN>, p);
+    return (int)(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+// Whether rows of two values begin on their size
+template <typename T> bool in_pairs(const RecParams& p, bool bwd) {
+    auto fits = [](const void* q, const int64_t* st) { return (uintptr_t)q % (2 * sizeof(T)) == 0 && st[0] % 2 == 0 && st[1] % 2 == 0; };
+    return p.D % 2 == 0 && fits(p.x, p.sx) && fits(p.g, p.sg) && fits(p.out, p.so) && (!bwd || (fits(p.h_in, p.sh) && fits(p.out_g, p.sog)));
+}
+
 template <typename T, bool LOGITS, bool BWD>
 int rec_launch(const RecParams& p, cudaStream_t s) {
     const int64_t n = (int64_t)p.B * p.D;
-    rec_serial_kernel<T, LOGITS, BWD><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
-    return (int)cudaGetLastError();
+    if (p.L < 16) {
+        rec_serial_kernel<T, LOGITS, BWD><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
+        return (int)cudaGetLastError();
+    }
+    constexpr int RUN = BWD ? 8 : 16;
+    if constexpr (sizeof(T) == 2) if (in_pairs<T>(p, BWD)) return rec_strips<T, LOGITS, BWD, 2, RUN>(p, s);
+    return rec_strips<T, LOGITS, BWD, 1, RUN>(p, s);
 }
 
 template <bool BWD> int rec_dispatch(const RecParams& p, int dtype, cudaStream_t s) {
@@ -80,10 +299,10 @@ template <bool BWD> int rec_dispatch(const RecParams& p, int dtype, cudaStream_t
     return VIG_ERR_DTYPE;
 }
 
-// sizes every call has to have; VIG_OK with *empty set where there is nothing to do
+// what every call is asked; token numbers are 32-bit with room for a step behind the last one
 static int rec_check(int B, int L, int D, float norm, int dtype) {
     if (dtype < VIG_DTYPE_F32 || dtype > VIG_DTYPE_F16) return VIG_ERR_DTYPE;
-    if (B < 0 || L < 0 || D < 0 || (int64_t)B * D >= (1ll << 31)) return VIG_ERR_SHAPE;
+    if (B < 0 || L < 0 || L >= (1 << 30) || D < 0 || (int64_t)B * D >= (1ll << 31)) return VIG_ERR_SHAPE;
     if (!(norm >= 0.f) || norm > 3.4e38f) return VIG_ERR_ARG;
     return VIG_OK;
 }
