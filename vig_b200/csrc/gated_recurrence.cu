@@ -6,6 +6,7 @@
 // dz_t = dg_t (1 - sigmoid(z_t)) / n,  dh_{-1} = u_0.  States, decays and sums are fp32; h is rounded once, to x's type, and the
 // backward reads h_{t-1} as it was rounded, so that x is not read again.
 // Bound by memory: 3 tensors forward (x, g in, h out), 5 backward (g, h, dh in, dx, dg out), about one exponential and a multiply-add a value.
+#include <type_traits>
 #include "common.cuh"
 
 namespace vig {
@@ -25,15 +26,28 @@ struct RecParams {
     int from_end;                   // the scan at hand starts at token L-1
 };
 
-// decay of one token.  16-bit types: two or three MUFU instructions, right to about 2^-21 of the decay; fp32: the exact functions
-template <typename T, bool LOGITS> __device__ __forceinline__ float decay_of(float g, float inv_norm) {
-    if (sizeof(T) == 4) return expf(LOGITS ? log_sigmoid(g) * inv_norm : g);
-    if (!LOGITS) return __expf(g);
-    return __expf((fminf(g, 0.f) - __logf(1.f + __expf(-fabsf(g)))) * inv_norm);
-}
-// d logsigmoid(z) / dz
-template <typename T> __device__ __forceinline__ float rest_of(float z) {
-    return sizeof(T) == 4 ? 1.f / (1.f + expf(z)) : __fdividef(1.f, 1.f + __expf(z));
+// The exponential and logarithm of base two of the MUFU unit, without the scaling that denormal arguments and results would take
+// (decays and their logarithms that small make no difference to a sum in fp32).
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+constexpr float LOG2E = 1.4426950408889634f;
+
+// Decays of V tokens' values g, and with REST also d logsigmoid(z) / dz = sigmoid(-z).  16-bit types: one MUFU instruction for a log-gate, three
+// for a raw logit (and one for REST), right to about 2^-21; fp32: the exact functions.
+template <typename T, bool LOGITS, bool REST, int V> __device__ __forceinline__ void decays(const float* g, float inv_norm, float* a, float* rest) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if (sizeof(T) == 4) {
+            a[v] = expf(LOGITS ? log_sigmoid(g[v]) * inv_norm : g[v]);
+            if (LOGITS && REST) rest[v] = 1.f / (1.f + expf(g[v]));
+        } else if (!LOGITS) {
+            a[v] = ex2(g[v] * LOG2E);
+        } else {
+            const float z = g[v] * LOG2E, t = fminf(z, 0.f) - lg2(1.f + ex2(-fabsf(z)));          // log2 of the sigmoid
+            a[v] = ex2(t * inv_norm);
+            if (REST) rest[v] = ex2(t - z);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -51,7 +65,9 @@ __global__ void __launch_bounds__(128) rec_serial_kernel(const RecParams p) {
     float s = p.s0 ? p.s0[b * p.ld_s0 + d] : 0.f;
     for (int k = 0; k < p.L; ++k) {
         const int64_t t = p.from_end ? p.L - 1 - k : k;
-        const float gv = DType<T>::to_f(g[t * p.sg[1]]), a = decay_of<T, LOGITS>(gv, p.inv_norm);
+        const float gv = DType<T>::to_f(g[t * p.sg[1]]);
+        float a, rest;
+        decays<T, LOGITS, BWD, 1>(&gv, p.inv_norm, &a, &rest);
         const float xv = DType<T>::to_f(x[t * p.sx[1]]);
         if (!BWD) {
             s = fmaf(a, s, xv);
@@ -62,7 +78,7 @@ __global__ void __launch_bounds__(128) rec_serial_kernel(const RecParams p) {
             const int64_t before = p.from_end ? t - 1 : t + 1;
             const float hb = k + 1 < p.L ? DType<T>::to_f(hin[before * p.sh[1]]) : p.h0 ? p.h0[(int64_t)b * p.D + d] : 0.f;
             float dg = s * hb;
-            if (LOGITS) dg *= p.inv_norm * rest_of<T>(gv);
+            if (LOGITS) dg *= p.inv_norm * rest;
             out[t * p.so[1]] = DType<T>::from_f(dx);
             outg[t * p.sog[1]] = DType<T>::from_f(dg);
         }
@@ -77,7 +93,7 @@ __global__ void __launch_bounds__(128) rec_serial_kernel(const RecParams p) {
 // memory, the CTAs' totals in the shared memory of every CTA of the cluster, at one cluster barrier; each thread then joins the pairs ahead
 // of it to the state that the step began with and walks its tokens again from there, now in the order of the definition.  The next step's
 // tokens are requested before the first meeting.  Every value is read and written once.  No state is rounded, no order depends on timing.
-// A pair is joined to a state by h + a s, except that a state of 0 gives h: products of decays above one may overflow.
+// (Decays may exceed one, as long as their product over a step's tokens stays below 3.4e38.)
 template <typename T, int V> struct Raw;
 template <> struct Raw<float, 1> {
     using type = float;
@@ -103,13 +119,30 @@ template <> struct Raw<__half, 2> {
 constexpr int RW = 8;                 // warps of a CTA
 constexpr int RC = 8;                 // CTAs of a cluster, at most
 
-__device__ __forceinline__ float join(float a, float h, float s) { return s == 0.f ? h : fmaf(a, s, h); }
+// two values at a time where there are two
+template <int V> __device__ __forceinline__ void fma_v(float* d, const float* a, const float* b, const float* c) {
+    if constexpr (V == 2)
+        asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
+    else
+        d[0] = fmaf(a[0], b[0], c[0]);
+}
+template <int V> __device__ __forceinline__ void mul_v(float* d, const float* a, const float* b) {
+    if constexpr (V == 2)
+        asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+    else
+        d[0] = a[0] * b[0];
+}
+
+// The product of decays of a stretch of tokens, kept finite: 0 times it stays 0.  (Were a decay NaN, the stretch's contribution is NaN.)
+__device__ __forceinline__ float finite(float a) { return fminf(a, 3.4028235e38f); }
 
 template <typename T, bool LOGITS, bool BWD, int V, int RUN>
 __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p) {
     using R = typename Raw<T, V>::type;
-    __shared__ float2 own[2][RW][32 * V];          // (product of decays, contribution) of each warp's tokens
-    __shared__ float2 all[2][RC][32 * V];          // of each CTA's
+    __shared__ float2 own[2][RW][V][32];           // (product of decays, contribution) of each warp's tokens
+    __shared__ float2 all[2][RC][V][32];           // of each CTA's
     uint32_t rank, ctas;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
@@ -118,11 +151,14 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
     const int strips = (p.D + 32 * V - 1) / (32 * V);
     const int strip = blockIdx.x / ctas, b = strip / strips, d = (strip % strips) * 32 * V + lane * V;
     const bool live = d < p.D;
-    const T* x = (const T*)p.x + b * p.sx[0] + d;
-    const T* g = (const T*)p.g + b * p.sg[0] + d;
-    const T* hin = BWD ? (const T*)p.h_in + b * p.sh[0] + d : nullptr;
-    T* out = (T*)p.out + b * p.so[0] + d;
-    T* outg = BWD ? (T*)p.out_g + b * p.sog[0] + d : nullptr;
+    // tokens are numbered as the scan meets them: k-th token at base + k * step bytes
+    struct Walk { char* base; int step; };
+    auto walk = [&](const void* q, const int64_t* st) {
+        const int64_t last = p.from_end ? (int64_t)(p.L - 1) * st[1] : 0;
+        return Walk{(char*)((T*)q + b * st[0] + last + d), (int)((p.from_end ? -st[1] : st[1]) * (int64_t)sizeof(T))};
+    };
+    const Walk x = walk(p.x, p.sx), g = walk(p.g, p.sg), out = walk(p.out, p.so), hin = BWD ? walk(p.h_in, p.sh) : x, outg = BWD ? walk(p.out_g, p.sog) : x;
+    auto cell = [](const Walk& w, int k) { return (R*)(w.base + (int64_t)k * w.step); };
     const int per = (int)ctas * RW * RUN;          // tokens of a step
     float carry[V], first[V];
 #pragma unroll
@@ -130,68 +166,80 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
         carry[v] = live && p.s0 ? p.s0[b * p.ld_s0 + d + v] : 0.f;
         first[v] = BWD && live && p.h0 ? p.h0[(int64_t)b * p.D + d + v] : 0.f;
     }
-    const auto at = [&](int k) { return (int64_t)(p.from_end ? p.L - 1 - k : k); };
     R xn[RUN], gn[RUN], hn[BWD ? RUN : 1];
     auto fetch = [&](int k0) {
+        if (!live) return;
+        if (k0 + RUN < p.L) {
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) {
-            const int k = k0 + i;
-            if (live && k < p.L) {
-                const int64_t t = at(k);
-                xn[i] = *(const R*)(x + t * p.sx[1]);
-                gn[i] = *(const R*)(g + t * p.sg[1]);
-                if (BWD && k + 1 < p.L) hn[i] = *(const R*)(hin + at(k + 1) * p.sh[1]);
+            for (int i = 0; i < RUN; ++i) {
+                xn[i] = *cell(x, k0 + i);
+                gn[i] = *cell(g, k0 + i);
+                if (BWD) hn[i] = *cell(hin, k0 + i + 1);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) {
+                if (k0 + i < p.L) { xn[i] = *cell(x, k0 + i); gn[i] = *cell(g, k0 + i); }
+                if (BWD && k0 + i + 1 < p.L) hn[i] = *cell(hin, k0 + i + 1);
             }
         }
     };
     const int mine = ((int)rank * RW + wid) * RUN;
     fetch(mine);
     for (int base = 0, buf = 0; base < p.L; base += per, buf ^= 1) {
-        const int k0 = base + mine;
-        float a[RUN][V], A[V], H[V];
-        R xr[RUN], gr[BWD && LOGITS ? RUN : 1], hr[BWD ? RUN : 1];
+        const int k0 = base + mine, left = live ? p.L - k0 : 0;        // tokens behind the last one leave the state as it is
+        float a[RUN][V], rest[BWD && LOGITS ? RUN : 1][V], A[V], H[V];
+        R xr[RUN], hr[BWD ? RUN : 1];
 #pragma unroll
         for (int v = 0; v < V; ++v) { A[v] = 1.f; H[v] = 0.f; }
+        auto local = [&](auto whole) {
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) {
-            const bool in = live && k0 + i < p.L;
-            float gf[V], xf[V];
-            Raw<T, V>::get(gn[i], gf);
-            Raw<T, V>::get(xn[i], xf);
-            xr[i] = xn[i];
-            if (BWD && LOGITS) gr[i] = gn[i];
-            if (BWD) hr[i] = hn[i];
+            for (int i = 0; i < RUN; ++i) {
+                float gf[V], xf[V];
+                Raw<T, V>::get(gn[i], gf);
+                Raw<T, V>::get(xn[i], xf);
+                decays<T, LOGITS, BWD, V>(gf, p.inv_norm, a[i], rest[BWD && LOGITS ? i : 0]);
+                if (!decltype(whole)::value && i >= left) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                a[i][v] = in ? decay_of<T, LOGITS>(gf[v], p.inv_norm) : 1.f;
-                if (in) H[v] = BWD ? a[i][v] * (xf[v] + H[v]) : fmaf(a[i][v], H[v], xf[v]);
-                A[v] *= a[i][v];
+                    for (int v = 0; v < V; ++v) { a[i][v] = 1.f; xf[v] = 0.f; }
+                }
+                xr[i] = xn[i];
+                if (BWD) {
+                    hr[i] = hn[i];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) H[v] += xf[v];
+                    mul_v<V>(H, a[i], H);
+                } else {
+                    fma_v<V>(H, a[i], H, xf);
+                }
+                mul_v<V>(A, A, a[i]);
             }
-        }
+        };
+        if (left >= RUN) local(std::true_type()); else local(std::false_type());
         if (base + per < p.L) fetch(k0 + per);
 #pragma unroll
-        for (int v = 0; v < V; ++v) own[buf][wid][lane * V + v] = make_float2(A[v], H[v]);
+        for (int v = 0; v < V; ++v) own[buf][wid][v][lane] = make_float2(finite(A[v]), H[v]);
         __syncthreads();
-        // joined: the tokens of the CTA ahead of this warp's; and all of them
-        float pa[V], ph[V], ta[V], th[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            pa[v] = ta[v] = 1.f; ph[v] = th[v] = 0.f;
-#pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                if (w == wid) { pa[v] = ta[v]; ph[v] = th[v]; }
-                const float2 e = own[buf][w][lane * V + v];
-                th[v] = join(e.x, e.y, th[v]);
-                ta[v] *= e.x;
-            }
-        }
         float s[V];
         if (ctas > 1) {
+            // joined: the tokens of the CTA ahead of this warp's; and all of them
+            float pa[V], ph[V], ta[V], th[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                pa[v] = ta[v] = 1.f; ph[v] = th[v] = 0.f;
+#pragma unroll
+                for (int w = 0; w < RW; ++w) {
+                    if (w == wid) { pa[v] = ta[v]; ph[v] = th[v]; }
+                    const float2 e = own[buf][w][v][lane];
+                    th[v] = fmaf(e.x, th[v], e.y);
+                    ta[v] = finite(ta[v] * e.x);
+                }
+            }
             if (base == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
             for (uint32_t to = wid; to < ctas; to += RW) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const uint32_t here = (uint32_t)__cvta_generic_to_shared(&all[buf][rank][lane * V + v]);
+                    const uint32_t here = (uint32_t)__cvta_generic_to_shared(&all[buf][rank][v][lane]);
                     uint32_t there;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(to));
                     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(ta[v]), "f"(th[v]) : "memory");
@@ -203,46 +251,53 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
                 s[v] = carry[v];
                 for (uint32_t r = 0; r < ctas; ++r) {
                     if (r == rank) s[v] = carry[v];
-                    const float2 e = all[buf][r][lane * V + v];
-                    carry[v] = join(e.x, e.y, carry[v]);
+                    const float2 e = all[buf][r][v][lane];
+                    carry[v] = fmaf(e.x, carry[v], e.y);
                 }
-                s[v] = join(pa[v], ph[v], s[v]);
+                s[v] = fmaf(pa[v], s[v], ph[v]);
             }
         } else {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                s[v] = join(pa[v], ph[v], carry[v]);
-                carry[v] = join(ta[v], th[v], carry[v]);
-            }
-        }
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) {
-            const int k = k0 + i;
-            if (!live || k >= p.L) continue;
-            const int64_t t = at(k);
-            float xf[V], o[V];
-            Raw<T, V>::get(xr[i], xf);
-            if (!BWD) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) o[v] = s[v] = fmaf(a[i][v], s[v], xf[v]);
-                *(R*)(out + t * p.so[1]) = Raw<T, V>::put(o);
-            } else {
-                float hf[V], gf[V], og[V];
-                Raw<T, V>::get(hr[i], hf);
-                if (LOGITS) Raw<T, V>::get(gr[i], gf);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    o[v] = xf[v] + s[v];
-                    s[v] = a[i][v] * o[v];
-                    og[v] = s[v] * (k + 1 < p.L ? hf[v] : first[v]);
-                    if (LOGITS) og[v] *= p.inv_norm * rest_of<T>(gf[v]);
+                for (int w = 0; w < RW; ++w) {
+                    if (w == wid) s[v] = carry[v];
+                    const float2 e = own[buf][w][v][lane];
+                    carry[v] = fmaf(e.x, carry[v], e.y);
                 }
-                *(R*)(out + t * p.so[1]) = Raw<T, V>::put(o);
-                *(R*)(outg + t * p.sog[1]) = Raw<T, V>::put(og);
             }
         }
+        auto outputs = [&](auto whole) {
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) {
+                if (!decltype(whole)::value && i >= left) break;
+                float xf[V], o[V];
+                Raw<T, V>::get(xr[i], xf);
+                if (!BWD) {
+                    fma_v<V>(s, a[i], s, xf);
+                    *cell(out, k0 + i) = Raw<T, V>::put(s);
+                } else {
+                    float hf[V];
+                    Raw<T, V>::get(hr[i], hf);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        if (!decltype(whole)::value && i + 1 >= left) hf[v] = first[v];
+                        o[v] = xf[v] + s[v];
+                    }
+                    mul_v<V>(s, a[i], o);
+                    *cell(out, k0 + i) = Raw<T, V>::put(o);
+                    mul_v<V>(o, s, hf);
+                    if (LOGITS) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) o[v] *= p.inv_norm * rest[i][v];
+                    }
+                    *cell(outg, k0 + i) = Raw<T, V>::put(o);
+                }
+            }
+        };
+        if (left > RUN) outputs(std::true_type()); else outputs(std::false_type());
         // the state behind the last token, as that token's output was rounded from it
-        if (p.s_end && live && k0 < p.L && k0 + RUN >= p.L) {
+        if (p.s_end && left > 0 && left <= RUN) {
 #pragma unroll
             for (int v = 0; v < V; ++v) p.s_end[b * p.ld_end + d + v] = s[v];
         }
@@ -272,6 +327,13 @@ int rec_strips(const RecParams& p, cudaStream_t s) {
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
+// Whether a step over all three or five tensors is a 32-bit number of bytes
+inline bool short_steps(const RecParams& p, bool bwd) {
+    const int64_t most = (1ll << 29) - 1;
+    auto fits = [&](const int64_t* st) { return st[1] <= most && st[1] >= -most; };
+    return fits(p.sx) && fits(p.sg) && fits(p.so) && (!bwd || (fits(p.sh) && fits(p.sog)));
+}
+
 // Whether rows of two values begin on their size
 template <typename T> bool in_pairs(const RecParams& p, bool bwd) {
     auto fits = [](const void* q, const int64_t* st) { return (uintptr_t)q % (2 * sizeof(T)) == 0 && st[0] % 2 == 0 && st[1] % 2 == 0; };
@@ -281,7 +343,7 @@ template <typename T> bool in_pairs(const RecParams& p, bool bwd) {
 template <typename T, bool LOGITS, bool BWD>
 int rec_launch(const RecParams& p, cudaStream_t s) {
     const int64_t n = (int64_t)p.B * p.D;
-    if (p.L < 16) {
+    if (p.L < 16 || !short_steps(p, BWD)) {
         rec_serial_kernel<T, LOGITS, BWD><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
         return (int)cudaGetLastError();
     }
