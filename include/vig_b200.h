@@ -383,16 +383,16 @@ VIG_API int vig_linear_swiglu_fwd(const void* x, int64_t ldx, const void* w, voi
  * gate_logit_normalizer n > 0 from raw logits, a_t = sigmoid(g_t)^(1/n).  x, g, h: [B, L, D] with unit stride over D and element strides
  * (b, l) (NULL = contiguous); any alignment; h may not overlap x or g.  h0 (optional), h_final (optional): fp32 [B, D] with row strides
  * ld_h0, ld_final; h_final may be h0 itself (a state updated in place), and L may be 0 (the state is handed on) or 1 (one new token).
- * B * D < 2^31, L < 2^30.
+ * B * D < 2^31, L < 2^30.  status_dev: optional int32 on the device, bit 0 = a bounded wait ran out.
  */
 VIG_API int vig_gated_recurrence_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final,
                                      int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,
-                                     float gate_logit_normalizer, int reverse, int dtype, void* stream);
+                                     float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream);
 /* Its gradients: from g, the output h, h0 (NULL as in the forward), d_h and d_final (optional, fp32 [B, D]): d_x and d_g ([B, L, D] contiguous;
  * d_g with respect to what g holds) and d_h0 (optional, fp32 [B, D]). */
 VIG_API int vig_gated_recurrence_bwd(const void* g, const void* h, const float* h0, const void* d_h, const float* d_final, void* d_x, void* d_g, float* d_h0,
                                      int B, int L, int D, const int64_t* strides_g, const int64_t* strides_h, const int64_t* strides_dh,
-                                     float gate_logit_normalizer, int reverse, int dtype, void* stream);
+                                     float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream);
 
 /*
  * Optional residual add and RMSNorm with 8-bit rows out: s = x (+ residual), y = s * rsqrt(mean(s^2) + eps) * w, and for every group of

@@ -289,6 +289,6 @@ def test_refusals():
 def test_c_entry_refuses_before_any_launch():
     from vig_b200 import _lib
     L_ = _lib.lib()
-    fwd = lambda B=1, L=4, D=8, norm=0.0, dtype=0, ptr=None: L_.vig_gated_recurrence_fwd(ptr, ptr, None, 0, ptr, None, 0, B, L, D, None, None, None, norm, 0, dtype, None)  # noqa: E731
+    fwd = lambda B=1, L=4, D=8, norm=0.0, dtype=0, ptr=None: L_.vig_gated_recurrence_fwd(ptr, ptr, None, 0, ptr, None, 0, B, L, D, None, None, None, norm, 0, dtype, None, None)  # noqa: E731
     assert fwd() == -1 and fwd(dtype=3) == -3 and fwd(B=-1) == -2 and fwd(norm=-1.0) == -6 and fwd(norm=float("nan")) == -6 and fwd(L=0) == 0
-    assert L_.vig_gated_recurrence_bwd(None, None, None, None, None, None, None, None, 1, 4, 8, None, None, None, 0.0, 0, 0, None) == -1
+    assert L_.vig_gated_recurrence_bwd(None, None, None, None, None, None, None, None, 1, 4, 8, None, None, None, 0.0, 0, 0, None, None) == -1

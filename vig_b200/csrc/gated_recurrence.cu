@@ -7,7 +7,7 @@
 // backward reads h_{t-1} as it was rounded, so that x is not read again.
 // Bound by memory: 3 tensors forward (x, g in, h out), 5 backward (g, h, dh in, dx, dg out), about one exponential and a multiply-add a value.
 #include <type_traits>
-#include "common.cuh"
+#include "tc_common.cuh"
 
 namespace vig {
 
@@ -24,6 +24,7 @@ struct RecParams {
     int B, L, D;
     float inv_norm;                 // > 0: g holds raw logits
     int from_end;                   // the scan at hand starts at token L-1
+    int32_t* status;
 };
 
 // The exponential and logarithm of base two of the MUFU unit, without the scaling that denormal arguments and results would take
@@ -90,9 +91,10 @@ __global__ void __launch_bounds__(128) rec_serial_kernel(const RecParams p) {
 // A cluster of CTAs owns a strip of 32 * V channels of one sequence and walks it in steps of (CTAs x 8 warps x RUN) tokens.  A warp's lanes
 // are channels (rows of a strip are read whole), a thread holds RUN consecutive tokens of its channels in registers.  In a step every
 // thread scans its tokens from a zero state, which gives the product of their decays and their own contribution; these pairs meet in shared
-// memory, the CTAs' totals in the shared memory of every CTA of the cluster, at one cluster barrier; each thread then joins the pairs ahead
-// of it to the state that the step began with and walks its tokens again from there, now in the order of the definition.  The next step's
-// tokens are requested before the first meeting.  Every value is read and written once.  No state is rounded, no order depends on timing.
+// memory, the CTAs' totals in the shared memory of every CTA of the cluster (stores that its mbarrier counts: a cluster barrier would
+// also wait for the outputs of the step before).  Each thread then joins the pairs ahead of it to the state that the step began with and
+// walks its tokens again from there, in the order of the definition.  The next step's tokens are requested before the first meeting.
+// Every value is read and written once.  No state is rounded, no order depends on timing.
 // (Decays may exceed one, as long as their product over a step's tokens stays below 3.4e38.)
 template <typename T, int V> struct Raw;
 template <> struct Raw<float, 1> {
@@ -141,12 +143,19 @@ __device__ __forceinline__ float finite(float a) { return fminf(a, 3.4028235e38f
 template <typename T, bool LOGITS, bool BWD, int V, int RUN>
 __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p) {
     using R = typename Raw<T, V>::type;
-    __shared__ float2 own[2][RW][V][32];           // (product of decays, contribution) of each warp's tokens
-    __shared__ float2 all[2][RC][V][32];           // of each CTA's
-    uint32_t rank, ctas;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
-    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");       // I run; waited for before the first CTA's memory is written
+    struct alignas(8 * V) Pair { float a[V], h[V]; };                 // product of decays and contribution of a stretch of tokens
+    __shared__ Pair own[2][RW][32];                // of each warp's tokens
+    __shared__ Pair all[2][RC][32];                // of each CTA's
+    __shared__ uint64_t landed[2];                 // counts the bytes of `all`
+    const uint32_t rank = tc::cluster_rank(), ctas = tc::cluster_size(), bar = tc::smem_u32(landed);
+    if (ctas > 1) {
+        if (threadIdx.x == 0) {
+            tc::mbar_init(bar, 1);
+            tc::mbar_init(bar + 8, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");       // I run; waited for before the first CTA's memory is written
+    }
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     const int strips = (p.D + 32 * V - 1) / (32 * V);
     const int strip = blockIdx.x / ctas, b = strip / strips, d = (strip % strips) * 32 * V + lane * V;
@@ -158,7 +167,8 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
         return Walk{(char*)((T*)q + b * st[0] + last + d), (int)((p.from_end ? -st[1] : st[1]) * (int64_t)sizeof(T))};
     };
     const Walk x = walk(p.x, p.sx), g = walk(p.g, p.sg), out = walk(p.out, p.so), hin = BWD ? walk(p.h_in, p.sh) : x, outg = BWD ? walk(p.out_g, p.sog) : x;
-    auto cell = [](const Walk& w, int k) { return (R*)(w.base + (int64_t)k * w.step); };
+    auto to = [](const Walk& w, int k) { return w.base + (int64_t)k * w.step; };
+    auto cell = [](char* at, const Walk& w, int i) { return (R*)(at + (int64_t)i * w.step); };
     const int per = (int)ctas * RW * RUN;          // tokens of a step
     float carry[V], first[V];
 #pragma unroll
@@ -169,24 +179,27 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
     R xn[RUN], gn[RUN], hn[BWD ? RUN : 1];
     auto fetch = [&](int k0) {
         if (!live) return;
+        char *px = to(x, k0), *pg = to(g, k0), *ph = to(hin, k0);
         if (k0 + RUN < p.L) {
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                xn[i] = *cell(x, k0 + i);
-                gn[i] = *cell(g, k0 + i);
-                if (BWD) hn[i] = *cell(hin, k0 + i + 1);
+                xn[i] = *cell(px, x, i);
+                gn[i] = *cell(pg, g, i);
+                if (BWD) hn[i] = *cell(ph, hin, i + 1);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                if (k0 + i < p.L) { xn[i] = *cell(x, k0 + i); gn[i] = *cell(g, k0 + i); }
-                if (BWD && k0 + i + 1 < p.L) hn[i] = *cell(hin, k0 + i + 1);
+                if (k0 + i < p.L) { xn[i] = *cell(px, x, i); gn[i] = *cell(pg, g, i); }
+                if (BWD && k0 + i + 1 < p.L) hn[i] = *cell(ph, hin, i + 1);
             }
         }
     };
     const int mine = ((int)rank * RW + wid) * RUN;
     fetch(mine);
+    uint32_t phase = 0;
     for (int base = 0, buf = 0; base < p.L; base += per, buf ^= 1) {
+        if (ctas > 1 && threadIdx.x == 0) tc::mbar_expect_tx(bar + 8 * buf, ctas * 32 * (uint32_t)sizeof(Pair));
         const int k0 = base + mine, left = live ? p.L - k0 : 0;        // tokens behind the last one leave the state as it is
         float a[RUN][V], rest[BWD && LOGITS ? RUN : 1][V], A[V], H[V];
         R xr[RUN], hr[BWD ? RUN : 1];
@@ -217,56 +230,70 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
         };
         if (left >= RUN) local(std::true_type()); else local(std::false_type());
         if (base + per < p.L) fetch(k0 + per);
+        Pair me;
 #pragma unroll
-        for (int v = 0; v < V; ++v) own[buf][wid][v][lane] = make_float2(finite(A[v]), H[v]);
+        for (int v = 0; v < V; ++v) { me.a[v] = finite(A[v]); me.h[v] = H[v]; }
+        own[buf][wid][lane] = me;
         __syncthreads();
         float s[V];
         if (ctas > 1) {
             // joined: the tokens of the CTA ahead of this warp's; and all of them
-            float pa[V], ph[V], ta[V], th[V];
+            float pa[V], ph[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                pa[v] = ta[v] = 1.f; ph[v] = th[v] = 0.f;
+            for (int v = 0; v < V; ++v) { me.a[v] = 1.f; me.h[v] = 0.f; }
 #pragma unroll
-                for (int w = 0; w < RW; ++w) {
-                    if (w == wid) { pa[v] = ta[v]; ph[v] = th[v]; }
-                    const float2 e = own[buf][w][v][lane];
-                    th[v] = fmaf(e.x, th[v], e.y);
-                    ta[v] = finite(ta[v] * e.x);
+            for (int w = 0; w < RW; ++w) {
+                const Pair e = own[buf][w][lane];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (w == wid) { pa[v] = me.a[v]; ph[v] = me.h[v]; }
+                    me.h[v] = fmaf(e.a[v], me.h[v], e.h[v]);
+                    me.a[v] = finite(me.a[v] * e.a[v]);
                 }
             }
             if (base == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-            for (uint32_t to = wid; to < ctas; to += RW) {
+            for (uint32_t other = wid; other < ctas; other += RW) {
+                const uint32_t at = tc::map_rank(tc::smem_u32(&all[buf][rank][lane]), other), count = tc::map_rank(bar + 8 * buf, other);
+                if constexpr (V == 2)
+                    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                                 ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.a[1])), "r"(__float_as_uint(me.h[0])), "r"(__float_as_uint(me.h[1])), "r"(count) : "memory");
+                else
+                    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
+                                 ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.h[0])), "r"(count) : "memory");
+            }
+            int tries = 0;
+            while (!tc::mbar_try_wait_parked(bar + 8 * buf, (phase >> buf) & 1, 1000000)) {
+                if (++tries > 2000) {                                  // about a second or two: say so, and finish with what is there
+                    if (p.status && lane == 0) atomicOr(p.status, 1);
+                    break;
+                }
+            }
+            phase ^= 1u << buf;
+#pragma unroll
+            for (int v = 0; v < V; ++v) s[v] = carry[v];
+#pragma unroll 4
+            for (uint32_t r = 0; r < ctas; ++r) {
+                const Pair e = all[buf][r][lane];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const uint32_t here = (uint32_t)__cvta_generic_to_shared(&all[buf][rank][v][lane]);
-                    uint32_t there;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(to));
-                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(ta[v]), "f"(th[v]) : "memory");
-                }
-            }
-            asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                s[v] = carry[v];
-                for (uint32_t r = 0; r < ctas; ++r) {
                     if (r == rank) s[v] = carry[v];
-                    const float2 e = all[buf][r][v][lane];
-                    carry[v] = fmaf(e.x, carry[v], e.y);
+                    carry[v] = fmaf(e.a[v], carry[v], e.h[v]);
                 }
-                s[v] = fmaf(pa[v], s[v], ph[v]);
             }
+#pragma unroll
+            for (int v = 0; v < V; ++v) s[v] = fmaf(pa[v], s[v], ph[v]);
         } else {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
+            for (int w = 0; w < RW; ++w) {
+                const Pair e = own[buf][w][lane];
 #pragma unroll
-                for (int w = 0; w < RW; ++w) {
+                for (int v = 0; v < V; ++v) {
                     if (w == wid) s[v] = carry[v];
-                    const float2 e = own[buf][w][v][lane];
-                    carry[v] = fmaf(e.x, carry[v], e.y);
+                    carry[v] = fmaf(e.a[v], carry[v], e.h[v]);
                 }
             }
         }
+        char *po = to(out, k0), *pog = to(outg, k0);
         auto outputs = [&](auto whole) {
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
@@ -275,7 +302,7 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
                 Raw<T, V>::get(xr[i], xf);
                 if (!BWD) {
                     fma_v<V>(s, a[i], s, xf);
-                    *cell(out, k0 + i) = Raw<T, V>::put(s);
+                    *cell(po, out, i) = Raw<T, V>::put(s);
                 } else {
                     float hf[V];
                     Raw<T, V>::get(hr[i], hf);
@@ -285,13 +312,13 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
                         o[v] = xf[v] + s[v];
                     }
                     mul_v<V>(s, a[i], o);
-                    *cell(out, k0 + i) = Raw<T, V>::put(o);
+                    *cell(po, out, i) = Raw<T, V>::put(o);
                     mul_v<V>(o, s, hf);
                     if (LOGITS) {
 #pragma unroll
                         for (int v = 0; v < V; ++v) o[v] *= p.inv_norm * rest[i][v];
                     }
-                    *cell(outg, k0 + i) = Raw<T, V>::put(o);
+                    *cell(pog, outg, i) = Raw<T, V>::put(o);
                 }
             }
         };
@@ -301,6 +328,11 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
 #pragma unroll
             for (int v = 0; v < V; ++v) p.s_end[b * p.ld_end + d + v] = s[v];
         }
+    }
+    // no CTA leaves while another may still write to it (one that gave up waiting)
+    if (ctas > 1) {
+        asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+        asm volatile("barrier.cluster.wait;" ::: "memory");
     }
 }
 
@@ -387,7 +419,7 @@ using namespace vig;
 
 extern "C" int vig_gated_recurrence_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final,
                                         int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,
-                                        float gate_logit_normalizer, int reverse, int dtype, void* stream) {
+                                        float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
     if (const int e = rec_check(B, L, D, gate_logit_normalizer, dtype)) return e;
     if (B > 1 && ((h0 && ld_h0 < 0) || (h_final && ld_final < D))) return VIG_ERR_ARG;
     if (!B || !D || !L) return rec_empty(h0, ld_h0, h_final, ld_final, B, D, (cudaStream_t)stream);
@@ -398,12 +430,13 @@ extern "C" int vig_gated_recurrence_fwd(const void* x, const void* g, const floa
     p.B = B; p.L = L; p.D = D;
     p.inv_norm = gate_logit_normalizer > 0.f ? 1.f / gate_logit_normalizer : 0.f;
     p.from_end = reverse != 0;
+    p.status = status_dev;
     return rec_dispatch<false>(p, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int vig_gated_recurrence_bwd(const void* g, const void* h, const float* h0, const void* d_h, const float* d_final, void* d_x, void* d_g, float* d_h0,
                                         int B, int L, int D, const int64_t* strides_g, const int64_t* strides_h, const int64_t* strides_dh,
-                                        float gate_logit_normalizer, int reverse, int dtype, void* stream) {
+                                        float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
     if (const int e = rec_check(B, L, D, gate_logit_normalizer, dtype)) return e;
     if (!B || !D || !L) return rec_empty(d_final, D, d_h0, D, B, D, (cudaStream_t)stream);
     if (!g || !h || !d_h || !d_x || !d_g) return VIG_ERR_NULL;
@@ -413,5 +446,6 @@ extern "C" int vig_gated_recurrence_bwd(const void* g, const void* h, const floa
     p.B = B; p.L = L; p.D = D;
     p.inv_norm = gate_logit_normalizer > 0.f ? 1.f / gate_logit_normalizer : 0.f;
     p.from_end = reverse == 0;
+    p.status = status_dev;
     return rec_dispatch<true>(p, dtype, (cudaStream_t)stream);
 }

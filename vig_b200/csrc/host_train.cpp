@@ -75,7 +75,7 @@ void check_rec(const Tensor& x, const Tensor& g, int dim, double norm) {
 void rec_forward(const Tensor& x, const Tensor& g, const Tensor& h0, const Tensor& h, const Tensor& fin, bool reverse, double norm) {
     const S2 sx(x), sg(g), sh(h);
     ok(api.vig_gated_recurrence_fwd(ptr(x), ptr(g), (const float*)ptr(h0), h0.defined() ? h0.stride(0) : 0, ptr(h), (float*)ptr(fin), fin.defined() ? fin.stride(0) : 0,
-                                    (int)x.size(0), (int)x.size(1), (int)x.size(2), sx.s, sg.s, sh.s, (float)norm, reverse, dtype_code(x), stream()),
+                                    (int)x.size(0), (int)x.size(1), (int)x.size(2), sx.s, sg.s, sh.s, (float)norm, reverse, dtype_code(x), status_ptr(x.get_device()), stream()),
        "vig_gated_recurrence_fwd");
 }
 
@@ -106,25 +106,27 @@ struct Rec : torch::autograd::Function<Rec> {
         const S2 sg(g), sh(h), sd(dh);
         ok(api.vig_gated_recurrence_bwd(ptr(g), ptr(h), (const float*)ptr(h0), ptr(dh), (const float*)ptr(df), ptr(dx), ptr(dg), (float*)ptr(d0), (int)h.size(0),
                                         (int)h.size(1), (int)h.size(2), sg.s, sh.s, sd.s, (float)ctx->saved_data["norm"].toDouble(),
-                                        ctx->saved_data["reverse"].toBool(), dtype_code(h), stream()), "vig_gated_recurrence_bwd");
+                                        ctx->saved_data["reverse"].toBool(), dtype_code(h), status_ptr(h.get_device()), stream()), "vig_gated_recurrence_bwd");
         return {dx, dg, d0, Tensor(), Tensor(), Tensor()};
     }
 };
 
-std::pair<Tensor, OptT> gated_recurrence(const Tensor& x, const Tensor& g, const OptT& h0_, bool want_final, bool reverse, double norm) {
+// nullopt: the device's error word has to be registered first
+std::optional<std::pair<Tensor, OptT>> gated_recurrence(const Tensor& x, const Tensor& g, const OptT& h0_, bool want_final, bool reverse, double norm) {
     check_rec(x, g, 3, norm);
+    if (!status_known(x.get_device())) return std::nullopt;
     const Tensor h0 = get(h0_);
     if (h0.defined()) check_state(h0, x, "initial_state");
     c10::cuda::CUDAGuard dev(x.device());
     if (wants_grad({&x, &g, &h0})) {
         const auto out = Rec::apply(x, g, h0_, want_final, reverse, norm);
-        return {out[0], want_final ? OptT(out[1]) : std::nullopt};
+        return std::make_pair(out[0], want_final ? OptT(out[1]) : OptT());
     }
     const Tensor h = at::empty(x.sizes(), x.options());
     Tensor fin;
     if (want_final) fin = at::empty({x.size(0), x.size(2)}, x.options().dtype(at::kFloat));
     rec_forward(x, g, h0, h, fin, reverse, norm);
-    return {h, want_final ? OptT(fin) : std::nullopt};
+    return std::make_pair(h, want_final ? OptT(fin) : OptT());
 }
 
 Tensor gated_recurrence_step(const Tensor& x, const Tensor& g, const Tensor& state, double norm) {
@@ -137,7 +139,7 @@ Tensor gated_recurrence_step(const Tensor& x, const Tensor& g, const Tensor& sta
     const Tensor h = at::empty(x.sizes(), x.options());
     const int64_t sx[2] = {x.stride(0), 0}, sg[2] = {g.stride(0), 0}, sh[2] = {h.stride(0), 0};
     ok(api.vig_gated_recurrence_fwd(ptr(x), ptr(g), (const float*)ptr(state), state.stride(0), ptr(h), (float*)ptr(state), state.stride(0), (int)x.size(0), 1, (int)x.size(1),
-                                    sx, sg, sh, (float)norm, 0, dtype_code(x), stream()), "vig_gated_recurrence_fwd");
+                                    sx, sg, sh, (float)norm, 0, dtype_code(x), status_ptr(x.get_device()), stream()), "vig_gated_recurrence_fwd");
     return h;
 }
 

@@ -667,7 +667,12 @@ def gated_recurrence(x, g, initial_state=None, output_final_state=False, *, reve
     ``x``, ``g``: ``[B, L, D]`` of one dtype, any strides with a contiguous last dimension.  ``initial_state``: fp32 ``[B, D]``.  Returns
     ``(h, final_state)``, ``h`` in ``x``'s dtype, ``final_state`` fp32 or None.  States and sums are fp32.  Log-gates may be ``-inf`` (the
     state starts anew at that token).  Differentiable in ``x``, ``g`` and ``initial_state``, through both results."""
-    return _lib.host().gated_recurrence(x, g, initial_state, output_final_state, reverse, gate_logit_normalizer)
+    args = (x, g, initial_state, output_final_state, reverse, gate_logit_normalizer)
+    res = _lib.host().gated_recurrence(*args)
+    if res is None:                         # the device's first call
+        status_word(x.device)
+        res = _lib.host().gated_recurrence(*args)
+    return res
 
 
 def gated_recurrence_step(x, g, state, *, gate_logit_normalizer=0.0):
