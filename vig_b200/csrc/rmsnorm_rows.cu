@@ -20,6 +20,7 @@ struct NormParams {
     int64_t ldx, ldr, rows;
     int N, group, w_f32;
     float eps;
+    int whole = 0;                   // rows of all tensors are whole 16-byte vectors on 16 bytes
 };
 
 struct NormBwdParams {
@@ -29,6 +30,7 @@ struct NormBwdParams {
     int64_t ldy, ldr, lddr, rows;
     int N, w_f32, blocks;
     float eps;
+    int whole = 0;
 };
 
 template <int OUT> __device__ __forceinline__ float out_top() { return OUT == VIG_OUT_INT8 ? 127.f : 448.f; }
@@ -76,7 +78,8 @@ __device__ __forceinline__ float block_top(float v, float* sh) {
     return __uint_as_float(u);
 }
 
-// Rows of any width and alignment: a CTA takes a row a value at a time, and reads it again for every step.
+// Rows too wide for the registers of a CTA (more than 16384 values of 16 bits, 8192 of fp32): a CTA takes a row a value at a time, and reads
+// it again for every step.
 template <typename T, int OUT>
 __global__ void __launch_bounds__(NT) norm_any_kernel(const NormParams p) {
     __shared__ float sh[NT / 32];
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(NT) norm_any_kernel(const NormParams p) {
     }
 }
 
-// Backward, rows of any width and alignment: a CTA's share of dw stays in its row of the workspace (only the thread that owns a
+// Backward, rows too wide for registers: a CTA's share of dw stays in its row of the workspace (only the thread that owns a
 // channel touches it), and a second launch adds the CTAs' shares in their order, so results do not depend on timing.
 template <typename T>
 __global__ void __launch_bounds__(NT) norm_bwd_any_kernel(const NormBwdParams p) {
@@ -172,20 +175,363 @@ __global__ void __launch_bounds__(NT) norm_dw_kernel(const NormBwdParams p) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------------
+// TPR threads share a row; a thread holds VPT vectors of 16 bytes of it (vector t + m * TPR) and their weights in registers, and its next
+// row is in flight while it works on one.  Everything about a row that needs the other threads -- the sum of squares and max|r w| --
+// comes out of one reading and one reduction.  TPR below 32: a warp takes several rows; above: a CTA takes one.  Rows that are no whole
+// vectors, or do not begin on 16 bytes, are read and written a value at a time in the same arrangement: the same bits come out.
+template <typename T> __device__ __forceinline__ void take(Vec16<T>& v, const T* row, int vi, int N, int whole) {
+    constexpr int V = DType<T>::VEC;
+    if (whole) {
+        v.load(row + vi * V);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v.e[i] = vi * V + i < N ? row[vi * V + i] : DType<T>::from_f(0.f);
+    }
+}
+template <typename T> __device__ __forceinline__ void give(const Vec16<T>& v, T* row, int vi, int N, int whole) {
+    constexpr int V = DType<T>::VEC;
+    if (whole) {
+        v.store(row + vi * V);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (vi * V + i < N) row[vi * V + i] = v.e[i];
+    }
+}
+template <typename T> __device__ __forceinline__ void weights_of(const void* w, int w_f32, int vi, int N, int whole, float* f) {
+    constexpr int V = DType<T>::VEC;
+    if (w_f32) {
+        Vec16<float> v[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            take<float>(v[i], (const float*)w, vi * (V / 4) + i, N, whole);
+            v[i].to_float(f + 4 * i);
+        }
+    } else {
+        Vec16<T> v;
+        take<T>(v, (const T*)w, vi, N, whole);
+        v.to_float(f);
+    }
+}
+
+__device__ __forceinline__ float top_of(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
+
+// a summed and b summed (or, MAX, its largest value by bits) over the TPR threads of a row
+template <int TPR, bool MAX> __device__ __forceinline__ void over_row(float& a, float& b, float (*sh)[2], int& buf) {
+#pragma unroll
+    for (int m = (TPR < 32 ? TPR : 32) / 2; m; m >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, m);
+        const float o = __shfl_xor_sync(0xffffffffu, b, m);
+        b = MAX ? top_of(b, o) : b + o;
+    }
+    if (TPR > 32) {
+        constexpr int W = TPR / 32;
+        float (*s)[2] = sh + buf * W;                            // two buffers in turn, so that one barrier a reduction is enough
+        buf ^= 1;
+        if ((threadIdx.x & 31) == 0) { s[threadIdx.x >> 5][0] = a; s[threadIdx.x >> 5][1] = b; }
+        __syncthreads();
+        a = s[0][0]; b = s[0][1];
+#pragma unroll
+        for (int i = 1; i < W; ++i) { a += s[i][0]; b = MAX ? top_of(b, s[i][1]) : b + s[i][1]; }
+    }
+}
+
+template <int OUT, int V> __device__ __forceinline__ void store_codes(uint8_t* row, int vi, int N, int whole, const float* t, float by) {
+    uint32_t word[V / 4];
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) {
+        if (OUT == VIG_OUT_E4M3) {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * j] * by, t[4 * j + 1] * by), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * j + 2] * by, t[4 * j + 3] * by), __NV_SATFINITE, __NV_E4M3);
+            word[j] = lo | hi << 16;
+        } else {
+            word[j] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) word[j] |= (uint32_t)(uint8_t)(int8_t)__float2int_rn(t[4 * j + i] * by) << (8 * i);
+        }
+    }
+    uint8_t* q = row + vi * V;
+    if (!whole) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (vi * V + i < N) q[i] = (uint8_t)(word[i / 4] >> (8 * (i % 4)));
+    } else if constexpr (V == 8) {
+        *(uint2*)q = make_uint2(word[0], word[1]);
+    } else {
+        *(uint32_t*)q = word[0];
+    }
+}
+
+template <int TPR> constexpr int norm_threads = TPR > 128 ? TPR : 128;
+
+template <typename T, int OUT, int TPR, int VPT>
+__global__ void __launch_bounds__(norm_threads<TPR>) norm_rows_kernel(const NormParams p) {
+    constexpr int V = DType<T>::VEC, THREADS = norm_threads<TPR>, RPB = THREADS / TPR;            // RPB: rows of a CTA at a time
+    static_assert(TPR <= 32 || RPB == 1, "a row's threads are part of a warp, or a CTA");
+    __shared__ float sh[2 * (THREADS / 32)][2];
+    int buf = 0;
+    const int t = threadIdx.x % TPR, nv = (p.N + V - 1) / V, lanes = p.group / V;
+    const int64_t hop = (int64_t)gridDim.x * RPB;
+    float wf[VPT][V];
+#pragma unroll
+    for (int m = 0; m < VPT; ++m)
+        if (t + m * TPR < nv) weights_of<T>(p.w, p.w_f32, t + m * TPR, p.N, p.whole, wf[m]);
+    Vec16<T> xn[VPT], rn[VPT];
+    auto fetch = [&](int64_t row) {
+        if (row >= p.rows) return;
+        const T *x = (const T*)p.x + row * p.ldx, *res = p.res ? (const T*)p.res + row * p.ldr : nullptr;
+#pragma unroll
+        for (int m = 0; m < VPT; ++m) {
+            const int vi = t + m * TPR;
+            if (vi < nv) {
+                take<T>(xn[m], x, vi, p.N, p.whole);
+                if (res) take<T>(rn[m], res, vi, p.N, p.whole);
+            }
+        }
+    };
+    int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    fetch(row);
+    // a CTA's threads leave together: all of them take part in every reduction
+    for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += hop, row += hop) {
+        const bool in = row < p.rows;
+        float v[VPT][V], gt[VPT], ss = 0.f, top = 0.f;
+#pragma unroll
+        for (int m = 0; m < VPT; ++m) {
+            const int vi = t + m * TPR;
+            gt[m] = 0.f;
+            if (in && vi < nv) {
+                xn[m].to_float(v[m]);
+                if (p.res) {
+                    float rf[V];
+                    rn[m].to_float(rf);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[m][i] += rf[i];
+                }
+                if (p.r) { Vec16<T> o; o.from_float(v[m]); give<T>(o, (T*)p.r + row * p.N, vi, p.N, p.whole); }
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    ss = fmaf(v[m][i], v[m][i], ss);
+                    v[m][i] *= wf[m][i];
+                    if (OUT != OUT_SAME) gt[m] = top_of(gt[m], fabsf(v[m][i]));
+                }
+                top = top_of(top, gt[m]);
+            }
+        }
+        fetch(row + hop);
+        over_row<TPR, true>(ss, top, sh, buf);
+        const float rstd = 1.f / sqrtf(ss / (float)p.N + p.eps);
+        float inv = 0.f;
+        if (OUT != OUT_SAME && p.group == p.N) {
+            const float scale = scale_of<OUT>(top * rstd, &inv);
+            if (in && t == 0) p.scales[row] = scale;
+        }
+#pragma unroll
+        for (int m = 0; m < VPT; ++m) {
+            const int vi = t + m * TPR;
+            if (OUT != OUT_SAME && p.group != p.N) {             // group / V neighbouring threads share a group
+                float g = gt[m];
+                for (int k = lanes / 2; k; k >>= 1) g = top_of(g, __shfl_xor_sync(0xffffffffu, g, k));
+                const float scale = scale_of<OUT>(g * rstd, &inv);
+                if (in && vi < nv && vi % lanes == 0) p.scales[row * (p.N / p.group) + vi / lanes] = scale;
+            }
+            if (in && vi < nv) {
+                if constexpr (OUT == OUT_SAME) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[m][i] *= rstd;
+                    Vec16<T> o;
+                    o.from_float(v[m]);
+                    give<T>(o, (T*)p.y + row * p.N, vi, p.N, p.whole);
+                } else {
+                    store_codes<OUT, V>((uint8_t*)p.y + row * p.N, vi, p.N, p.whole, v[m], rstd * inv);
+                }
+            }
+        }
+    }
+}
+
+// Backward of the same rows: sum of squares and sum of r w dy in one reduction; a thread's share of dw stays in registers over all of its
+// rows (the weights come from the first-level cache each time: the registers are worth more to the next row), the CTA's rows of threads are added at the end, and a second launch adds the CTAs' shares in their order.
+template <int TPR> constexpr int norm_bwd_threads = TPR > 256 ? TPR : 256;
+
+template <typename T, int TPR, int VPT>
+__global__ void __launch_bounds__(norm_bwd_threads<TPR>, TPR > 256 ? 1 : 2) norm_bwd_rows_kernel(const NormBwdParams p) {
+    constexpr int V = DType<T>::VEC, THREADS = norm_bwd_threads<TPR>, RPB = THREADS / TPR;
+    static_assert(TPR <= 32 || RPB == 1, "a row's threads are part of a warp, or a CTA");
+    __shared__ float sh[2 * (THREADS / 32)][2];
+    extern __shared__ float share[];                             // [RPB][N]
+    int buf = 0;
+    const int t = threadIdx.x % TPR, nv = (p.N + V - 1) / V;
+    const int64_t hop = (int64_t)gridDim.x * RPB;
+    float acc[VPT][V];
+#pragma unroll
+    for (int m = 0; m < VPT; ++m)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[m][i] = 0.f;
+    Vec16<T> rn[VPT], dn[VPT], en[VPT];
+    auto fetch = [&](int64_t row) {
+        if (row >= p.rows) return;
+        const T *r = (const T*)p.r + row * p.ldr, *dy = (const T*)p.dy + row * p.ldy, *dr = p.dr ? (const T*)p.dr + row * p.lddr : nullptr;
+#pragma unroll
+        for (int m = 0; m < VPT; ++m) {
+            const int vi = t + m * TPR;
+            if (vi < nv) {
+                take<T>(rn[m], r, vi, p.N, p.whole);
+                take<T>(dn[m], dy, vi, p.N, p.whole);
+                if (dr) take<T>(en[m], dr, vi, p.N, p.whole);
+            }
+        }
+    };
+    int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    fetch(row);
+    for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += hop, row += hop) {
+        const bool in = row < p.rows;
+        Vec16<T> r[VPT], d[VPT], e[VPT];
+        float ss = 0.f, dot = 0.f;
+#pragma unroll
+        for (int m = 0; m < VPT; ++m) {
+            r[m] = rn[m]; d[m] = dn[m]; e[m] = en[m];
+            if (in && t + m * TPR < nv) {
+                float rf[V], df[V], wf[V];
+                r[m].to_float(rf);
+                d[m].to_float(df);
+                weights_of<T>(p.w, p.w_f32, t + m * TPR, p.N, p.whole, wf);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    ss = fmaf(rf[i], rf[i], ss);
+                    dot = fmaf(rf[i], df[i] * wf[i], dot);
+                }
+            }
+        }
+        fetch(row + hop);
+        over_row<TPR, false>(ss, dot, sh, buf);
+        const float rstd = 1.f / sqrtf(ss / (float)p.N + p.eps), c = dot / (float)p.N * rstd * rstd;
+#pragma unroll
+        for (int m = 0; m < VPT; ++m) {
+            const int vi = t + m * TPR;
+            if (in && vi < nv) {
+                float rf[V], df[V], wf[V], o[V];
+                r[m].to_float(rf);
+                d[m].to_float(df);
+                weights_of<T>(p.w, p.w_f32, vi, p.N, p.whole, wf);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    acc[m][i] = fmaf(df[i], rf[i] * rstd, acc[m][i]);
+                    o[i] = rstd * (df[i] * wf[i] - rf[i] * c);
+                }
+                if (p.dr) {
+                    float ef[V];
+                    e[m].to_float(ef);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] += ef[i];
+                }
+                Vec16<T> v;
+                v.from_float(o);
+                give<T>(v, (T*)p.dx + row * p.N, vi, p.N, p.whole);
+            }
+        }
+    }
+    float* part = p.partial + (int64_t)blockIdx.x * p.N;
+#pragma unroll
+    for (int m = 0; m < VPT; ++m) {
+        const int vi = t + m * TPR;
+        if (vi < nv) {
+            float* to = RPB > 1 ? share + (threadIdx.x / TPR) * p.N : part;
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) give<float>(*(const Vec16<float>*)(acc[m] + 4 * i), to, vi * (V / 4) + i, p.N, p.whole);
+        }
+    }
+    if (RPB > 1) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < p.N; i += THREADS) {
+            float v = 0.f;
+#pragma unroll
+            for (int k = 0; k < RPB; ++k) v += share[k * p.N + i];
+            part[i] = v;
+        }
+    }
+}
+
+// CTAs of the backward, whose shares of dw the workspace holds: two an SM
 static int norm_blocks(int64_t rows) {
-    const int64_t most = (int64_t)device_sms() * 4;
+    const int64_t most = (int64_t)device_sms() * 2;
     return (int)(rows < most ? rows : most);
 }
 
-template <typename T, int OUT> int norm_launch(const NormParams& p, cudaStream_t s) {
+// threads a row of nv vectors: a power of two of which three or four vectors a thread make the row (fewer where a group or a warp wants more)
+static int threads_a_row(int nv, int least) {
+    int tpr = least;
+    while (tpr * 4 < nv) tpr *= 2;
+    return tpr;
+}
+
+static bool on_16(const void* q, int64_t ld, int size) { return (uintptr_t)q % 16 == 0 && ld * size % 16 == 0; }
+
+template <typename T, int OUT, int TPR> int norm_rows_launch(const NormParams& p, int nv, cudaStream_t s) {
+    constexpr int THREADS = norm_threads<TPR>, RPB = THREADS / TPR;
+    const int vpt = (nv + TPR - 1) / TPR;
+    const int64_t need = (p.rows + RPB - 1) / RPB, most = (int64_t)device_sms() * (2048 / THREADS);
+    const unsigned grid = (unsigned)(need < most ? need : most);
+    switch (vpt) {
+        case 1: norm_rows_kernel<T, OUT, TPR, 1><<<grid, THREADS, 0, s>>>(p); break;
+        case 2: norm_rows_kernel<T, OUT, TPR, 2><<<grid, THREADS, 0, s>>>(p); break;
+        case 3: norm_rows_kernel<T, OUT, TPR, 3><<<grid, THREADS, 0, s>>>(p); break;
+        default: norm_rows_kernel<T, OUT, TPR, 4><<<grid, THREADS, 0, s>>>(p); break;
+    }
+    return (int)cudaGetLastError();
+}
+
+template <typename T, int OUT> int norm_launch(NormParams p, cudaStream_t s) {
+    constexpr int V = DType<T>::VEC;
+    const int size = (int)sizeof(T);
+    p.whole = p.N % V == 0 && on_16(p.x, p.ldx, size) && (!p.res || on_16(p.res, p.ldr, size)) && on_16(p.w, 0, 1) && on_16(p.y, 0, 1) && (!p.r || on_16(p.r, 0, 1));
+    const int nv = (p.N + V - 1) / V;
+    switch (threads_a_row(nv, p.group != p.N ? 32 : 8)) {
+        case 8: return norm_rows_launch<T, OUT, 8>(p, nv, s);
+        case 16: return norm_rows_launch<T, OUT, 16>(p, nv, s);
+        case 32: return norm_rows_launch<T, OUT, 32>(p, nv, s);
+        case 64: case 128: return norm_rows_launch<T, OUT, 128>(p, nv, s);
+        case 256: return norm_rows_launch<T, OUT, 256>(p, nv, s);
+        case 512: return norm_rows_launch<T, OUT, 512>(p, nv, s);
+    }
     const int64_t most = (int64_t)device_sms() * 8;
     norm_any_kernel<T, OUT><<<(unsigned)(p.rows < most ? p.rows : most), NT, 0, s>>>(p);
     return (int)cudaGetLastError();
 }
 
-template <typename T> int norm_bwd_launch(const NormBwdParams& p, cudaStream_t s) {
-    norm_bwd_any_kernel<T><<<p.blocks, NT, 0, s>>>(p);
-    if (const cudaError_t e = cudaGetLastError()) return (int)e;
+template <typename T, int TPR> int norm_bwd_rows_launch(const NormBwdParams& p, int nv, cudaStream_t s) {
+    constexpr int THREADS = norm_bwd_threads<TPR>, RPB = THREADS / TPR;
+    const size_t smem = RPB > 1 ? (size_t)RPB * p.N * sizeof(float) : 0;            // at most 32 KB
+    switch ((nv + TPR - 1) / TPR) {
+        case 1: norm_bwd_rows_kernel<T, TPR, 1><<<p.blocks, THREADS, smem, s>>>(p); break;
+        case 2: norm_bwd_rows_kernel<T, TPR, 2><<<p.blocks, THREADS, smem, s>>>(p); break;
+        case 3: norm_bwd_rows_kernel<T, TPR, 3><<<p.blocks, THREADS, smem, s>>>(p); break;
+        default: norm_bwd_rows_kernel<T, TPR, 4><<<p.blocks, THREADS, smem, s>>>(p); break;
+    }
+    return (int)cudaGetLastError();
+}
+
+template <typename T> int norm_bwd_launch(NormBwdParams p, cudaStream_t s) {
+    constexpr int V = DType<T>::VEC;
+    const int size = (int)sizeof(T);
+    p.whole = p.N % V == 0 && on_16(p.r, p.ldr, size) && on_16(p.dy, p.ldy, size) && (!p.dr || on_16(p.dr, p.lddr, size)) && on_16(p.w, 0, 1) && on_16(p.dx, 0, 1) &&
+                         on_16(p.partial, 0, 1);
+    const int nv = (p.N + V - 1) / V, tpr = threads_a_row(nv, 8);
+    int e;
+    if (tpr <= 512) {
+        const int rpb = tpr > 32 ? 1 : 256 / tpr;
+        const int64_t need = (p.rows + rpb - 1) / rpb;
+        if (need < p.blocks) p.blocks = (int)need;
+        switch (tpr) {
+            case 8: e = norm_bwd_rows_launch<T, 8>(p, nv, s); break;
+            case 16: e = norm_bwd_rows_launch<T, 16>(p, nv, s); break;
+            case 32: e = norm_bwd_rows_launch<T, 32>(p, nv, s); break;
+            case 512: e = norm_bwd_rows_launch<T, 512>(p, nv, s); break;
+            default: e = norm_bwd_rows_launch<T, 256>(p, nv, s); break;
+        }
+    } else {
+        norm_bwd_any_kernel<T><<<p.blocks, NT, 0, s>>>(p);
+        e = (int)cudaGetLastError();
+    }
+    if (e) return e;
     norm_dw_kernel<T><<<(p.N + 31) / 32, NT, 0, s>>>(p);
     return (int)cudaGetLastError();
 }
