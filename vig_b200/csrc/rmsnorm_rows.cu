@@ -157,19 +157,24 @@ __global__ void __launch_bounds__(NT) norm_bwd_any_kernel(const NormBwdParams p)
     }
 }
 
-// dw = the CTAs' shares, added in their order: 32 channels x 8 warps
+// dw = the CTAs' shares, added in a fixed order: 32 channels x 32 warps
+constexpr int DW = 32;
+
 template <typename T>
-__global__ void __launch_bounds__(NT) norm_dw_kernel(const NormBwdParams p) {
-    __shared__ float sh[NT / 32][32];
+__global__ void __launch_bounds__(DW * 32) norm_dw_kernel(const NormBwdParams p) {
+    __shared__ float sh[DW][32];
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+    pdl_wait();
     float s = 0.f;
-    if (i < p.N)
-        for (int b = wid; b < p.blocks; b += NT / 32) s += p.partial[(int64_t)b * p.N + i];
+    if (i < p.N) {
+#pragma unroll 16
+        for (int b = wid; b < p.blocks; b += DW) s += p.partial[(int64_t)b * p.N + i];
+    }
     sh[wid][lane] = s;
     __syncthreads();
     if (wid == 0 && i < p.N) {
 #pragma unroll
-        for (int k = 1; k < NT / 32; ++k) s += sh[k][lane];
+        for (int k = 1; k < DW; ++k) s += sh[k][lane];
         if (p.w_f32) ((float*)p.dw)[i] = s;
         else ((T*)p.dw)[i] = DType<T>::from_f(s);
     }
@@ -349,11 +354,13 @@ __global__ void __launch_bounds__(norm_threads<TPR>) norm_rows_kernel(const Norm
 }
 
 // Backward of the same rows: sum of squares and sum of r w dy in one reduction; a thread's share of dw stays in registers over all of its
-// rows (the weights come from the first-level cache each time: the registers are worth more to the next row), the CTA's rows of threads are added at the end, and a second launch adds the CTAs' shares in their order.
+// rows.  The weights come from the first-level cache each time and no row is requested ahead: the registers are worth more as warps.  At the end the CTA's rows of threads are added at the end, and a second launch adds the CTAs' shares in their order.
 template <int TPR> constexpr int norm_bwd_threads = TPR > 256 ? TPR : 256;
 
+template <int TPR, int VALUES> constexpr int norm_bwd_ctas = TPR > 256 ? 1 : VALUES <= 24 ? 3 : 2;       // CTAs of an SM, by the values a thread holds
+
 template <typename T, int TPR, int VPT>
-__global__ void __launch_bounds__(norm_bwd_threads<TPR>, TPR > 256 ? 1 : 2) norm_bwd_rows_kernel(const NormBwdParams p) {
+__global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT * DType<T>::VEC>) norm_bwd_rows_kernel(const NormBwdParams p) {
     constexpr int V = DType<T>::VEC, THREADS = norm_bwd_threads<TPR>, RPB = THREADS / TPR;
     static_assert(TPR <= 32 || RPB == 1, "a row's threads are part of a warp, or a CTA");
     __shared__ float sh[2 * (THREADS / 32)][2];
@@ -366,29 +373,26 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, TPR > 256 ? 1 : 2) norm
     for (int m = 0; m < VPT; ++m)
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[m][i] = 0.f;
-    Vec16<T> rn[VPT], dn[VPT], en[VPT];
-    auto fetch = [&](int64_t row) {
-        if (row >= p.rows) return;
-        const T *r = (const T*)p.r + row * p.ldr, *dy = (const T*)p.dy + row * p.ldy, *dr = p.dr ? (const T*)p.dr + row * p.lddr : nullptr;
-#pragma unroll
-        for (int m = 0; m < VPT; ++m) {
-            const int vi = t + m * TPR;
-            if (vi < nv) {
-                take<T>(rn[m], r, vi, p.N, p.whole);
-                take<T>(dn[m], dy, vi, p.N, p.whole);
-                if (dr) take<T>(en[m], dr, vi, p.N, p.whole);
-            }
-        }
-    };
+    pdl_launch();
     int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-    fetch(row);
     for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += hop, row += hop) {
         const bool in = row < p.rows;
         Vec16<T> r[VPT], d[VPT], e[VPT];
         float ss = 0.f, dot = 0.f;
+        if (in) {
+            const T *pr = (const T*)p.r + row * p.ldr, *dy = (const T*)p.dy + row * p.ldy, *dr = p.dr ? (const T*)p.dr + row * p.lddr : nullptr;
+#pragma unroll
+            for (int m = 0; m < VPT; ++m) {
+                const int vi = t + m * TPR;
+                if (vi < nv) {
+                    take<T>(r[m], pr, vi, p.N, p.whole);
+                    take<T>(d[m], dy, vi, p.N, p.whole);
+                    if (dr) take<T>(e[m], dr, vi, p.N, p.whole);
+                }
+            }
+        }
 #pragma unroll
         for (int m = 0; m < VPT; ++m) {
-            r[m] = rn[m]; d[m] = dn[m]; e[m] = en[m];
             if (in && t + m * TPR < nv) {
                 float rf[V], df[V], wf[V];
                 r[m].to_float(rf);
@@ -401,7 +405,6 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, TPR > 256 ? 1 : 2) norm
                 }
             }
         }
-        fetch(row + hop);
         over_row<TPR, false>(ss, dot, sh, buf);
         const float rstd = 1.f / sqrtf(ss / (float)p.N + p.eps), c = dot / (float)p.N * rstd * rstd;
 #pragma unroll
@@ -450,9 +453,9 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, TPR > 256 ? 1 : 2) norm
     }
 }
 
-// CTAs of the backward, whose shares of dw the workspace holds: two an SM
+// CTAs of the backward, whose shares of dw the workspace holds: at most three an SM
 static int norm_blocks(int64_t rows) {
-    const int64_t most = (int64_t)device_sms() * 2;
+    const int64_t most = (int64_t)device_sms() * 3;
     return (int)(rows < most ? rows : most);
 }
 
@@ -484,7 +487,7 @@ template <typename T, int OUT> int norm_launch(NormParams p, cudaStream_t s) {
     const int size = (int)sizeof(T);
     p.whole = p.N % V == 0 && on_16(p.x, p.ldx, size) && (!p.res || on_16(p.res, p.ldr, size)) && on_16(p.w, 0, 1) && on_16(p.y, 0, 1) && (!p.r || on_16(p.r, 0, 1));
     const int nv = (p.N + V - 1) / V;
-    switch (threads_a_row(nv, p.group != p.N ? 32 : 8)) {
+    switch (threads_a_row(nv, p.group != p.N && p.group / V > 8 ? p.group / V : 8)) {
         case 8: return norm_rows_launch<T, OUT, 8>(p, nv, s);
         case 16: return norm_rows_launch<T, OUT, 16>(p, nv, s);
         case 32: return norm_rows_launch<T, OUT, 32>(p, nv, s);
@@ -497,16 +500,21 @@ template <typename T, int OUT> int norm_launch(NormParams p, cudaStream_t s) {
     return (int)cudaGetLastError();
 }
 
-template <typename T, int TPR> int norm_bwd_rows_launch(const NormBwdParams& p, int nv, cudaStream_t s) {
+template <typename T, int TPR, int VPT> int norm_bwd_rows(NormBwdParams& p, cudaStream_t s) {
     constexpr int THREADS = norm_bwd_threads<TPR>, RPB = THREADS / TPR;
-    const size_t smem = RPB > 1 ? (size_t)RPB * p.N * sizeof(float) : 0;            // at most 32 KB
-    switch ((nv + TPR - 1) / TPR) {
-        case 1: norm_bwd_rows_kernel<T, TPR, 1><<<p.blocks, THREADS, smem, s>>>(p); break;
-        case 2: norm_bwd_rows_kernel<T, TPR, 2><<<p.blocks, THREADS, smem, s>>>(p); break;
-        case 3: norm_bwd_rows_kernel<T, TPR, 3><<<p.blocks, THREADS, smem, s>>>(p); break;
-        default: norm_bwd_rows_kernel<T, TPR, 4><<<p.blocks, THREADS, smem, s>>>(p); break;
-    }
+    const int64_t need = (p.rows + RPB - 1) / RPB, room = (int64_t)device_sms() * norm_bwd_ctas<TPR, VPT * DType<T>::VEC>;
+    p.blocks = (int)(need < room ? need : room);
+    norm_bwd_rows_kernel<T, TPR, VPT><<<p.blocks, THREADS, RPB > 1 ? (size_t)RPB * p.N * sizeof(float) : 0, s>>>(p);       // at most 32 KB
     return (int)cudaGetLastError();
+}
+
+template <typename T, int TPR> int norm_bwd_rows_launch(NormBwdParams& p, int nv, cudaStream_t s) {
+    switch ((nv + TPR - 1) / TPR) {
+        case 1: return norm_bwd_rows<T, TPR, 1>(p, s);
+        case 2: return norm_bwd_rows<T, TPR, 2>(p, s);
+        case 3: return norm_bwd_rows<T, TPR, 3>(p, s);
+        default: return norm_bwd_rows<T, TPR, 4>(p, s);
+    }
 }
 
 template <typename T> int norm_bwd_launch(NormBwdParams p, cudaStream_t s) {
@@ -517,9 +525,6 @@ template <typename T> int norm_bwd_launch(NormBwdParams p, cudaStream_t s) {
     const int nv = (p.N + V - 1) / V, tpr = threads_a_row(nv, 8);
     int e;
     if (tpr <= 512) {
-        const int rpb = tpr > 32 ? 1 : 256 / tpr;
-        const int64_t need = (p.rows + rpb - 1) / rpb;
-        if (need < p.blocks) p.blocks = (int)need;
         switch (tpr) {
             case 8: e = norm_bwd_rows_launch<T, 8>(p, nv, s); break;
             case 16: e = norm_bwd_rows_launch<T, 16>(p, nv, s); break;
@@ -532,8 +537,7 @@ template <typename T> int norm_bwd_launch(NormBwdParams p, cudaStream_t s) {
         e = (int)cudaGetLastError();
     }
     if (e) return e;
-    norm_dw_kernel<T><<<(p.N + 31) / 32, NT, 0, s>>>(p);
-    return (int)cudaGetLastError();
+    return (int)launch_next(norm_dw_kernel<T>, dim3((p.N + 31) / 32), dim3(DW * 32), 0, s, p);
 }
 
 template <int OUT> int norm_dispatch(const NormParams& p, int dtype, cudaStream_t s) {
