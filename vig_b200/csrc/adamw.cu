@@ -24,7 +24,8 @@ struct AdamTensor {
     float *master, *ms, *vs;         // ms, vs: scales of 8-bit states, or NULL
     int64_t n;
     uint32_t first;                  // its first chunk
-    uint16_t pt, gt;                 // dtype codes
+    uint8_t pt, gt;                  // dtype codes
+    uint8_t whole;                   // everything begins on four values
 };
 
 struct AdamTable {
@@ -47,21 +48,136 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float x)
 __device__ __forceinline__ float from_e4m3(uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
 __device__ __forceinline__ uint8_t to_e4m3(float x) { return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
 
-// A warp takes blocks of 256 values, 8 of them a lane.
-__global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant__ AdamTable tab) {
-    if (tab.found_inf && *tab.found_inf != 0.f) return;
-    int lo = 0, hi = tab.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (tab.t[mid].first <= blockIdx.x) lo = mid; else hi = mid - 1;
+// One value: gradient, states and weight in, states and weight out; returns the root of the new v.  Written so that every path rounds alike.
+__device__ __forceinline__ float adam_value(const AdamTable& tab, float g, float& m, float& v, float& p) {
+    m = fmaf(tab.b1, m, __fmul_rn(tab.c1, g));
+    v = fmaf(tab.b2, v, __fmul_rn(tab.c2, __fmul_rn(g, g)));
+    const float root = sqrtf(v);
+    p = fmaf(p, tab.keep, -__fdiv_rn(__fmul_rn(tab.rate, m), fmaf(root, tab.root, tab.eps)));
+    return root;
+}
+// scale of a block from its largest magnitude, and what its values are multiplied by; a scale without a reciprocal makes all codes 0
+__device__ __forceinline__ float adam_scale(uint32_t top, float* inv) {
+    const float s = __uint_as_float(__reduce_max_sync(0xffffffffu, top)) * (1.f / 448.f);
+    *inv = s >= 1.17549435e-38f ? 1.f / s : s - s;
+    return s;
+}
+__device__ __forceinline__ uint32_t bits_of(float x) { return __float_as_uint(x) & 0x7fffffffu; }      // magnitudes order like these, and a NaN comes out on top
+
+// four values of T as one load, and one store
+template <typename T> struct Four;
+template <> struct Four<float> {
+    float4 r;
+    __device__ void load(const void* p, int64_t i) { r = *(const float4*)((const float*)p + i); }
+    __device__ void get(float* f) const { f[0] = r.x; f[1] = r.y; f[2] = r.z; f[3] = r.w; }
+    static __device__ void store(void* p, int64_t i, const float* f) { *(float4*)((float*)p + i) = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <typename T> struct Four {
+    uint2 r;
+    __device__ void load(const void* p, int64_t i) { r = *(const uint2*)((const T*)p + i); }
+    __device__ void get(float* f) const {
+        const T* e = (const T*)&r;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = DType<T>::to_f(e[k]);
     }
-    const AdamTensor& t = tab.t[lo];
+    static __device__ void store(void* p, int64_t i, const float* f) {
+        uint2 r;
+        T* e = (T*)&r;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = DType<T>::from_f(f[k]);
+        *(uint2*)((T*)p + i) = r;
+    }
+};
+__device__ __forceinline__ void codes_get(uint32_t c, float* f) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float2 v = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> (16 * k)), __NV_E4M3)));
+        f[2 * k] = v.x; f[2 * k + 1] = v.y;
+    }
+}
+template <bool ROOT> __device__ __forceinline__ uint32_t codes_put(const float* f, float by) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        c |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2 * k] * by, f[2 * k + 1] * by), __NV_SATFINITE, __NV_E4M3) << (16 * k);
+    if (ROOT) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (f[k] > 0.f && !(c & 0xffu << (8 * k))) c |= 1u << (8 * k);
+    }
+    return c;
+}
+
+// A whole block of 256 values that begin on four: a lane takes two groups of four, and every load of the block is under way before the
+// first is used.
+template <typename P, typename G, bool EIGHT>
+__device__ __forceinline__ void adam_whole(const AdamTable& tab, const AdamTensor& t, int64_t block, float gs) {
     const int lane = threadIdx.x & 31;
-    const float gs = tab.grad_scale ? *tab.grad_scale : 1.f;
-    const int64_t block = (int64_t)(blockIdx.x - t.first) * (AW_CHUNK / AW_BLOCK) + (threadIdx.x >> 5);
+    const int64_t at = block * AW_BLOCK + 4 * lane;
+    Four<P> pr[2];
+    Four<G> gr[2];
+    Four<float> wr[2], mr[2], vr[2];
+    uint32_t mc[2], vc[2];
+    float sm = 1.f, sv = 1.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t i = at + 128 * j;
+        gr[j].load(t.g, i);
+        if (EIGHT) {
+            mc[j] = *(const uint32_t*)((const uint8_t*)t.m + i);
+            vc[j] = *(const uint32_t*)((const uint8_t*)t.v + i);
+        } else {
+            mr[j].load(t.m, i);
+            vr[j].load(t.v, i);
+        }
+        if (t.master) wr[j].load(t.master, i); else pr[j].load(t.p, i);
+    }
+    if (EIGHT) { sm = t.ms[block]; sv = t.vs[block]; }
+    float m[2][4], v[2][4];
+    uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int64_t i = at + 128 * j;
+        float g[4], w[4];
+        gr[j].get(g);
+        if (t.master) wr[j].get(w); else pr[j].get(w);
+        if (EIGHT) { codes_get(mc[j], m[j]); codes_get(vc[j], v[j]); } else { mr[j].get(m[j]); vr[j].get(v[j]); }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (EIGHT) {
+                m[j][k] = __fmul_rn(m[j][k], sm);
+                const float root = __fmul_rn(v[j][k], sv);
+                v[j][k] = __fmul_rn(root, root);
+            }
+            const float root = adam_value(tab, __fmul_rn(g[k], gs), m[j][k], v[j][k], w[k]);
+            if (EIGHT) {
+                v[j][k] = root;
+                top_m = max(top_m, bits_of(m[j][k]));
+                top_v = max(top_v, bits_of(root));
+            }
+        }
+        if (t.master) Four<float>::store(t.master, i, w);
+        Four<P>::store(t.p, i, w);
+        if (!EIGHT) { Four<float>::store(t.m, i, m[j]); Four<float>::store(t.v, i, v[j]); }
+    }
+    if (EIGHT) {
+        float im, iv;
+        const float nm = adam_scale(top_m, &im), nv = adam_scale(top_v, &iv);
+        if (lane == 0) { t.ms[block] = nm; t.vs[block] = nv; }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            *(uint32_t*)((uint8_t*)t.m + at + 128 * j) = codes_put<false>(m[j], im);
+            *(uint32_t*)((uint8_t*)t.v + at + 128 * j) = codes_put<true>(v[j], iv);
+        }
+    }
+}
+
+// Any block: the last of a tensor, or one that begins anywhere; a value at a time.
+__device__ __noinline__ void adam_any(const AdamTable& tab, const AdamTensor& t, int64_t block, float gs) {
+    const int lane = threadIdx.x & 31;
     const int64_t at = block * AW_BLOCK;
-    if (at >= t.n) return;
-    const float sm = t.ms ? t.ms[block] : 1.f, sv = t.vs ? t.vs[block] : 1.f;
+    const bool eight = t.ms != nullptr;
+    const float sm = eight ? t.ms[block] : 1.f, sv = eight ? t.vs[block] : 1.f;
     float m[8], v[8];
     uint32_t top_m = 0, top_v = 0;
 #pragma unroll
@@ -69,37 +185,31 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
         const int64_t i = at + lane + 32 * j;
         m[j] = v[j] = 0.f;
         if (i < t.n) {
-            const float g = load_as(t.g, i, t.gt) * gs;
-            float root = 0.f;
-            if (t.ms) {
-                m[j] = from_e4m3(((const uint8_t*)t.m)[i]) * sm;
-                root = from_e4m3(((const uint8_t*)t.v)[i]) * sv;
-                v[j] = root * root;
+            if (eight) {
+                m[j] = __fmul_rn(from_e4m3(((const uint8_t*)t.m)[i]), sm);
+                const float root = __fmul_rn(from_e4m3(((const uint8_t*)t.v)[i]), sv);
+                v[j] = __fmul_rn(root, root);
             } else {
                 m[j] = ((const float*)t.m)[i];
                 v[j] = ((const float*)t.v)[i];
             }
-            m[j] = fmaf(tab.b1, m[j], tab.c1 * g);
-            v[j] = fmaf(tab.b2, v[j], tab.c2 * (g * g));
-            root = sqrtf(v[j]);
             float p = t.master ? t.master[i] : load_as(t.p, i, t.pt);
-            p = fmaf(p, tab.keep, -(tab.rate * m[j] / fmaf(root, tab.root, tab.eps)));
+            const float root = adam_value(tab, __fmul_rn(load_as(t.g, i, t.gt), gs), m[j], v[j], p);
             if (t.master) t.master[i] = p;
             store_as(t.p, i, t.pt, p);
-            if (t.ms) {
+            if (eight) {
                 v[j] = root;
-                top_m = max(top_m, __float_as_uint(fabsf(m[j])));
-                top_v = max(top_v, __float_as_uint(root) & 0x7fffffffu);
+                top_m = max(top_m, bits_of(m[j]));
+                top_v = max(top_v, bits_of(root));
             } else {
                 ((float*)t.m)[i] = m[j];
                 ((float*)t.v)[i] = v[j];
             }
         }
     }
-    if (!t.ms) return;
-    const float nm = __uint_as_float(__reduce_max_sync(0xffffffffu, top_m)) * (1.f / 448.f);
-    const float nv = __uint_as_float(__reduce_max_sync(0xffffffffu, top_v)) * (1.f / 448.f);
-    const float im = nm >= 1.17549435e-38f ? 1.f / nm : nm - nm, iv = nv >= 1.17549435e-38f ? 1.f / nv : nv - nv;
+    if (!eight) return;
+    float im, iv;
+    const float nm = adam_scale(top_m, &im), nv = adam_scale(top_v, &iv);
     if (lane == 0) { t.ms[block] = nm; t.vs[block] = nv; }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -111,6 +221,29 @@ __global__ void __launch_bounds__(AW_THREADS) adamw_kernel(const __grid_constant
             ((uint8_t*)t.v)[i] = c;
         }
     }
+}
+
+// A warp takes a block of 256 values, a CTA eight of them.
+__global__ void __launch_bounds__(AW_THREADS, 4) adamw_kernel(const __grid_constant__ AdamTable tab) {
+    if (tab.found_inf && *tab.found_inf != 0.f) return;
+    int lo = 0, hi = tab.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab.t[mid].first <= blockIdx.x) lo = mid; else hi = mid - 1;
+    }
+    const AdamTensor& t = tab.t[lo];
+    const float gs = tab.grad_scale ? *tab.grad_scale : 1.f;
+    const int64_t block = (int64_t)(blockIdx.x - t.first) * (AW_CHUNK / AW_BLOCK) + (threadIdx.x >> 5);
+    if (block * AW_BLOCK >= t.n) return;
+    if (!t.whole || (block + 1) * AW_BLOCK > t.n || (t.gt != t.pt && t.gt != VIG_DTYPE_F32)) {
+        adam_any(tab, t, block, gs);
+        return;
+    }
+#define VIG_AW(P, G) do { if (t.ms) adam_whole<P, G, true>(tab, t, block, gs); else adam_whole<P, G, false>(tab, t, block, gs); } while (0)
+    if (t.pt == VIG_DTYPE_F32) VIG_AW(float, float);
+    else if (t.pt == VIG_DTYPE_BF16) { if (t.gt == VIG_DTYPE_BF16) VIG_AW(__nv_bfloat16, __nv_bfloat16); else VIG_AW(__nv_bfloat16, float); }
+    else { if (t.gt == VIG_DTYPE_F16) VIG_AW(__half, __half); else VIG_AW(__half, float); }
+#undef VIG_AW
 }
 
 }  // namespace vig
@@ -146,7 +279,11 @@ extern "C" int vig_adamw_step(int count, void* const* params, const void* const*
             if (more > 0x7fffffff) return VIG_ERR_SHAPE;
             if (chunks + more > 0x7fffffff) break;
             tab.t[tab.count++] = {params[i], grads[i], exp_avgs[i], exp_avg_sqs[i], masters ? masters[i] : nullptr, exp_avg_scales ? exp_avg_scales[i] : nullptr,
-                                  exp_avg_sq_scales ? exp_avg_sq_scales[i] : nullptr, numels[i], (uint32_t)chunks, (uint16_t)param_dtypes[i], (uint16_t)grad_dtypes[i]};
+                                  exp_avg_sq_scales ? exp_avg_sq_scales[i] : nullptr, numels[i], (uint32_t)chunks, (uint8_t)param_dtypes[i], (uint8_t)grad_dtypes[i], 0};
+            AdamTensor& t = tab.t[tab.count - 1];
+            auto on = [](const void* q, int size) { return (uintptr_t)q % (4 * size) == 0; };
+            auto size = [](int dtype) { return dtype == VIG_DTYPE_F32 ? 4 : 2; };
+            t.whole = on(t.p, size(t.pt)) && on(t.g, size(t.gt)) && on(t.m, t.ms ? 1 : 4) && on(t.v, t.ms ? 1 : 4) && on(t.master, 4);
             chunks += more;
         }
         if (!tab.count) break;

@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(norm_threads<TPR>) norm_rows_kernel(const Norm
 // rows.  The weights come from the first-level cache each time and no row is requested ahead: the registers are worth more as warps.  At the end the CTA's rows of threads are added at the end, and a second launch adds the CTAs' shares in their order.
 template <int TPR> constexpr int norm_bwd_threads = TPR > 256 ? TPR : 256;
 
-template <int TPR, int VALUES> constexpr int norm_bwd_ctas = TPR > 256 ? 1 : VALUES <= 24 ? 3 : 2;       // CTAs of an SM, by the values a thread holds
+template <int TPR, int VALUES> constexpr int norm_bwd_ctas = TPR > 256 ? 1 : VALUES <= 16 ? 3 : 2;       // CTAs of an SM, by the values a thread holds
 
 template <typename T, int TPR, int VPT>
 __global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT * DType<T>::VEC>) norm_bwd_rows_kernel(const NormBwdParams p) {
