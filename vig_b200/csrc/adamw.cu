@@ -8,6 +8,7 @@
 // Bound by memory: p, g, m, v in, p, m, v out -- 28 bytes a value in full precision, 16 (and two scales in 256 values) with 16-bit weights, a
 // full-precision copy of them and states in 8 bits.
 #include <cuda_fp8.h>
+#include <algorithm>
 #include "common.cuh"
 
 namespace vig {
@@ -15,7 +16,8 @@ namespace vig {
 constexpr int AW_BLOCK = 256;        // values that share a scale
 constexpr int AW_CHUNK = 2048;       // values of a CTA
 constexpr int AW_THREADS = 256;
-constexpr int AW_MAX = 400;          // tensors of a launch: the table travels in the launch's parameters (at most 32764 bytes)
+constexpr int AW_MAX = 400;          // tensors of a launch: the table travels in the launch's parameters (at most 32764 bytes) ...
+constexpr int AW_FEW = 48;           // ... and a short one in fewer of them
 
 struct AdamTensor {
     void* p;
@@ -28,13 +30,15 @@ struct AdamTensor {
     uint8_t whole;                   // everything begins on four values
 };
 
-struct AdamTable {
-    AdamTensor t[AW_MAX];
-    int count;
+struct AdamScalars {
     float keep, b1, c1, b2, c2, rate, root, eps;      // 1 - lr wd, b1, 1 - b1, b2, 1 - b2, lr / (1 - b1^t), 1 / sqrt(1 - b2^t), eps
     const float *grad_scale, *found_inf;
 };
-static_assert(sizeof(AdamTable) <= 32764, "the parameters of a launch");
+template <int MAX> struct AdamTable : AdamScalars {
+    int count;
+    AdamTensor t[MAX];
+};
+static_assert(sizeof(AdamTable<AW_MAX>) <= 32764, "the parameters of a launch");
 
 __device__ __forceinline__ float load_as(const void* p, int64_t i, int dtype) {
     return dtype == VIG_DTYPE_F32 ? ((const float*)p)[i] : dtype == VIG_DTYPE_BF16 ? __bfloat162float(((const __nv_bfloat16*)p)[i]) : __half2float(((const __half*)p)[i]);
@@ -49,11 +53,15 @@ __device__ __forceinline__ float from_e4m3(uint8_t c) { return __half2float(__ha
 __device__ __forceinline__ uint8_t to_e4m3(float x) { return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
 
 // One value: gradient, states and weight in, states and weight out; returns the root of the new v.  Written so that every path rounds alike.
-__device__ __forceinline__ float adam_value(const AdamTable& tab, float g, float& m, float& v, float& p) {
+__device__ __forceinline__ float adam_value(const AdamScalars& tab, float g, float& m, float& v, float& p) {
     m = fmaf(tab.b1, m, __fmul_rn(tab.c1, g));
     v = fmaf(tab.b2, v, __fmul_rn(tab.c2, __fmul_rn(g, g)));
-    const float root = sqrtf(v);
-    p = fmaf(p, tab.keep, -__fdiv_rn(__fmul_rn(tab.rate, m), fmaf(root, tab.root, tab.eps)));
+    // root and quotient of the MUFU unit, each right to 2^-23 or so of itself: the step is off by that much of itself, the weight by far less.
+    // (A v below the smallest normal number has the root 0: beside eps it makes no difference.)  The exact forms cost four times the
+    // instructions and bound the 8-bit states: 85 M values 270 us with them.
+    float root;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v));
+    p = fmaf(p, tab.keep, -__fdividef(__fmul_rn(tab.rate, m), fmaf(root, tab.root, tab.eps)));
     return root;
 }
 // scale of a block from its largest magnitude, and what its values are multiplied by; a scale without a reciprocal makes all codes 0
@@ -97,21 +105,21 @@ __device__ __forceinline__ void codes_get(uint32_t c, float* f) {
 }
 template <bool ROOT> __device__ __forceinline__ uint32_t codes_put(const float* f, float by) {
     uint32_t c = 0;
+    float t[4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-        c |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2 * k] * by, f[2 * k + 1] * by), __NV_SATFINITE, __NV_E4M3) << (16 * k);
-    if (ROOT) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (f[k] > 0.f && !(c & 0xffu << (8 * k))) c |= 1u << (8 * k);
+    for (int k = 0; k < 4; ++k) {
+        t[k] = f[k] * by;
+        if (ROOT && f[k] > 0.f) t[k] = fmaxf(t[k], 0x1p-9f);           // the smallest code that is not 0
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) c |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(t[2 * k], t[2 * k + 1]), __NV_SATFINITE, __NV_E4M3) << (16 * k);
     return c;
 }
 
 // A whole block of 256 values that begin on four: a lane takes two groups of four, and every load of the block is under way before the
 // first is used.
 template <typename P, typename G, bool EIGHT>
-__device__ __forceinline__ void adam_whole(const AdamTable& tab, const AdamTensor& t, int64_t block, float gs) {
+__device__ __forceinline__ void adam_whole(const AdamScalars& tab, const AdamTensor& t, int64_t block, float gs) {
     const int lane = threadIdx.x & 31;
     const int64_t at = block * AW_BLOCK + 4 * lane;
     Four<P> pr[2];
@@ -173,7 +181,7 @@ __device__ __forceinline__ void adam_whole(const AdamTable& tab, const AdamTenso
 }
 
 // Any block: the last of a tensor, or one that begins anywhere; a value at a time.
-__device__ __noinline__ void adam_any(const AdamTable& tab, const AdamTensor& t, int64_t block, float gs) {
+__device__ __noinline__ void adam_any(const AdamScalars& tab, const AdamTensor& t, int64_t block, float gs) {
     const int lane = threadIdx.x & 31;
     const int64_t at = block * AW_BLOCK;
     const bool eight = t.ms != nullptr;
@@ -216,15 +224,14 @@ __device__ __noinline__ void adam_any(const AdamTable& tab, const AdamTensor& t,
         const int64_t i = at + lane + 32 * j;
         if (i < t.n) {
             ((uint8_t*)t.m)[i] = to_e4m3(m[j] * im);
-            uint8_t c = to_e4m3(v[j] * iv);
-            if (c == 0 && v[j] > 0.f) c = 1;
-            ((uint8_t*)t.v)[i] = c;
+            ((uint8_t*)t.v)[i] = to_e4m3(v[j] > 0.f ? fmaxf(v[j] * iv, 0x1p-9f) : v[j] * iv);
         }
     }
 }
 
 // A warp takes a block of 256 values, a CTA eight of them.
-__global__ void __launch_bounds__(AW_THREADS, 4) adamw_kernel(const __grid_constant__ AdamTable tab) {
+template <int MAX>
+__global__ void __launch_bounds__(AW_THREADS, 4) adamw_kernel(const __grid_constant__ AdamTable<MAX> tab) {
     if (tab.found_inf && *tab.found_inf != 0.f) return;
     int lo = 0, hi = tab.count - 1;
     while (lo < hi) {
@@ -263,7 +270,7 @@ extern "C" int vig_adamw_step(int count, void* const* params, const void* const*
         if (param_dtypes[i] < 0 || param_dtypes[i] > 2 || grad_dtypes[i] < 0 || grad_dtypes[i] > 2) return VIG_ERR_DTYPE;
         if ((exp_avg_scales && exp_avg_scales[i]) != (exp_avg_sq_scales && exp_avg_sq_scales[i])) return VIG_ERR_NULL;
     }
-    AdamTable tab;
+    AdamTable<AW_MAX> tab;
     tab.keep = (float)(1. - lr * weight_decay);
     tab.b1 = (float)beta1; tab.c1 = (float)(1. - beta1); tab.b2 = (float)beta2; tab.c2 = (float)(1. - beta2);
     tab.rate = (float)(lr / (1. - pow(beta1, (double)step)));
@@ -287,7 +294,15 @@ extern "C" int vig_adamw_step(int count, void* const* params, const void* const*
             chunks += more;
         }
         if (!tab.count) break;
-        adamw_kernel<<<(unsigned)chunks, AW_THREADS, 0, (cudaStream_t)stream>>>(tab);
+        if (tab.count <= AW_FEW) {
+            AdamTable<AW_FEW> few;
+            static_cast<AdamScalars&>(few) = tab;
+            few.count = tab.count;
+            std::copy(tab.t, tab.t + tab.count, few.t);
+            adamw_kernel<AW_FEW><<<(unsigned)chunks, AW_THREADS, 0, (cudaStream_t)stream>>>(few);
+        } else {
+            adamw_kernel<AW_MAX><<<(unsigned)chunks, AW_THREADS, 0, (cudaStream_t)stream>>>(tab);
+        }
         if (const cudaError_t e = cudaGetLastError()) return (int)e;
     }
     return VIG_OK;
