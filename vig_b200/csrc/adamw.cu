@@ -25,7 +25,6 @@ struct AdamTensor {
     void *m, *v;
     float *master, *ms, *vs;         // ms, vs: scales of 8-bit states, or NULL
     int64_t n;
-    uint32_t first;                  // its first chunk
     uint8_t pt, gt;                  // dtype codes
     uint8_t whole;                   // everything begins on four values
 };
@@ -36,6 +35,7 @@ struct AdamScalars {
 };
 template <int MAX> struct AdamTable : AdamScalars {
     int count;
+    uint32_t first[MAX];             // the tensors' first chunks, close together: every CTA searches them
     AdamTensor t[MAX];
 };
 static_assert(sizeof(AdamTable<AW_MAX>) <= 32764, "the parameters of a launch");
@@ -236,11 +236,11 @@ __global__ void __launch_bounds__(AW_THREADS, 4) adamw_kernel(const __grid_const
     int lo = 0, hi = tab.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (tab.t[mid].first <= blockIdx.x) lo = mid; else hi = mid - 1;
+        if (tab.first[mid] <= blockIdx.x) lo = mid; else hi = mid - 1;
     }
     const AdamTensor& t = tab.t[lo];
     const float gs = tab.grad_scale ? *tab.grad_scale : 1.f;
-    const int64_t block = (int64_t)(blockIdx.x - t.first) * (AW_CHUNK / AW_BLOCK) + (threadIdx.x >> 5);
+    const int64_t block = (int64_t)(blockIdx.x - tab.first[lo]) * (AW_CHUNK / AW_BLOCK) + (threadIdx.x >> 5);
     if (block * AW_BLOCK >= t.n) return;
     if (!t.whole || (block + 1) * AW_BLOCK > t.n || (t.gt != t.pt && t.gt != VIG_DTYPE_F32)) {
         adam_any(tab, t, block, gs);
@@ -285,8 +285,9 @@ extern "C" int vig_adamw_step(int count, void* const* params, const void* const*
             if (!more) continue;
             if (more > 0x7fffffff) return VIG_ERR_SHAPE;
             if (chunks + more > 0x7fffffff) break;
+            tab.first[tab.count] = (uint32_t)chunks;
             tab.t[tab.count++] = {params[i], grads[i], exp_avgs[i], exp_avg_sqs[i], masters ? masters[i] : nullptr, exp_avg_scales ? exp_avg_scales[i] : nullptr,
-                                  exp_avg_sq_scales ? exp_avg_sq_scales[i] : nullptr, numels[i], (uint32_t)chunks, (uint8_t)param_dtypes[i], (uint8_t)grad_dtypes[i], 0};
+                                  exp_avg_sq_scales ? exp_avg_sq_scales[i] : nullptr, numels[i], (uint8_t)param_dtypes[i], (uint8_t)grad_dtypes[i], 0};
             AdamTensor& t = tab.t[tab.count - 1];
             auto on = [](const void* q, int size) { return (uintptr_t)q % (4 * size) == 0; };
             auto size = [](int dtype) { return dtype == VIG_DTYPE_F32 ? 4 : 2; };
@@ -298,6 +299,7 @@ extern "C" int vig_adamw_step(int count, void* const* params, const void* const*
             AdamTable<AW_FEW> few;
             static_cast<AdamScalars&>(few) = tab;
             few.count = tab.count;
+            std::copy(tab.first, tab.first + tab.count, few.first);
             std::copy(tab.t, tab.t + tab.count, few.t);
             adamw_kernel<AW_FEW><<<(unsigned)chunks, AW_THREADS, 0, (cudaStream_t)stream>>>(few);
         } else {
