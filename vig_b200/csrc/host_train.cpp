@@ -21,8 +21,9 @@ std::string shape_of(const Tensor& t) {
     s << t.sizes();
     return s.str();
 }
-void want(bool ok, const std::string& msg) { if (!ok) throw py::value_error(msg); }
-void want_type(bool ok, const std::string& msg) { if (!ok) throw py::type_error(msg); }
+// the message is only put together where it is needed: these calls are a few microseconds long
+#define want(ok, msg) do { if (!(ok)) throw py::value_error(msg); } while (0)
+#define want_type(ok, msg) do { if (!(ok)) throw py::type_error(msg); } while (0)
 
 void on_gpu(const Tensor& t) { if (!t.is_cuda()) throw std::runtime_error("vig_b200 kernels need CUDA tensors; there is no CPU path"); }
 void same_device(const Tensor& t, const Tensor& like, const char* name) {
@@ -66,7 +67,7 @@ void check_rec(const Tensor& x, const Tensor& g, int dim, double norm) {
     same_device(g, x, "g");
     code(x);
     want_type(g.scalar_type() == x.scalar_type(), "x and g must share one dtype");
-    want(x.dim() == dim && g.sizes() == x.sizes(), std::string(dim == 3 ? "x and g must be [B, L, D]" : "x and g must be [B, D]") + "; got " + shape_of(x) + " and " + shape_of(g));
+    want(x.dim() == dim && g.sizes() == x.sizes(), (dim == 3 ? "x and g must be [B, L, D]; got " : "x and g must be [B, D]; got ") + shape_of(x) + " and " + shape_of(g));
     want(unit_last(x) && unit_last(g), "the last dimension of x and g must be contiguous");
     want(norm >= 0 && std::isfinite(norm), "gate_logit_normalizer must be 0 (log-gates) or positive (raw logits)");
     want(x.size(0) * x.size(-1) < (1ll << 31) && (dim == 2 || x.size(1) < (1ll << 30)), "B * D must be below 2^31 and L below 2^30");
