@@ -33,6 +33,22 @@ __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32
 __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 constexpr float LOG2E = 1.4426950408889634f;
 
+// two values at a time where there are two
+template <int V> __device__ __forceinline__ void fma_v(float* d, const float* a, const float* b, const float* c) {
+    if constexpr (V == 2)
+        asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
+    else
+        d[0] = fmaf(a[0], b[0], c[0]);
+}
+template <int V> __device__ __forceinline__ void mul_v(float* d, const float* a, const float* b) {
+    if constexpr (V == 2)
+        asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+    else
+        d[0] = a[0] * b[0];
+}
+
 // Decays of V tokens' values g, and with REST also d logsigmoid(z) / dz = sigmoid(-z).  16-bit types: one MUFU instruction for a log-gate, three
 // for a raw logit (and one for REST), right to about 2^-21; fp32: the exact functions.
 template <typename T, bool LOGITS, bool REST, int V> __device__ __forceinline__ void decays(const float* g, float inv_norm, float* a, float* rest) {
@@ -43,10 +59,25 @@ template <typename T, bool LOGITS, bool REST, int V> __device__ __forceinline__ 
             if (LOGITS && REST) rest[v] = 1.f / (1.f + expf(g[v]));
         } else if (!LOGITS) {
             a[v] = ex2(g[v] * LOG2E);
-        } else {
-            const float z = g[v] * LOG2E, t = fminf(z, 0.f) - lg2(1.f + ex2(-fabsf(z)));          // log2 of the sigmoid
-            a[v] = ex2(t * inv_norm);
-            if (REST) rest[v] = ex2(t - z);
+        }
+    }
+    if constexpr (sizeof(T) == 2 && LOGITS) {
+        const float l2e[2] = {LOG2E, LOG2E}, one[2] = {1.f, 1.f}, minus[2] = {-1.f, -1.f}, inv[2] = {inv_norm, inv_norm};
+        float z[V], e[V], t[V];
+        mul_v<V>(z, g, l2e);
+#pragma unroll
+        for (int v = 0; v < V; ++v) e[v] = ex2(-fabsf(z[v]));
+        fma_v<V>(e, e, one, one);
+#pragma unroll
+        for (int v = 0; v < V; ++v) { e[v] = lg2(e[v]); t[v] = fminf(z[v], 0.f); }
+        fma_v<V>(t, e, minus, t);                                // log2 of the sigmoid: min(z, 0) - log2(1 + 2^-|z|)
+        mul_v<V>(e, t, inv);
+#pragma unroll
+        for (int v = 0; v < V; ++v) a[v] = ex2(e[v]);
+        if (REST) {
+            fma_v<V>(t, z, minus, t);
+#pragma unroll
+            for (int v = 0; v < V; ++v) rest[v] = ex2(t[v]);
         }
     }
 }
@@ -120,22 +151,6 @@ template <> struct Raw<__half, 2> {
 
 constexpr int RW = 8;                 // warps of a CTA
 constexpr int RC = 8;                 // CTAs of a cluster, at most
-
-// two values at a time where there are two
-template <int V> __device__ __forceinline__ void fma_v(float* d, const float* a, const float* b, const float* c) {
-    if constexpr (V == 2)
-        asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
-            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
-    else
-        d[0] = fmaf(a[0], b[0], c[0]);
-}
-template <int V> __device__ __forceinline__ void mul_v(float* d, const float* a, const float* b) {
-    if constexpr (V == 2)
-        asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
-            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
-    else
-        d[0] = a[0] * b[0];
-}
 
 // The product of decays of a stretch of tokens, kept finite: 0 times it stays 0.  (Were a decay NaN, the stretch's contribution is NaN.)
 __device__ __forceinline__ float finite(float a) { return fminf(a, 3.4028235e38f); }
@@ -336,27 +351,294 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
     }
 }
 
-// CTAs of a cluster: enough to fill the SMs twice over, no more than the sequence has steps for
-template <int RUN> int rec_ctas(int64_t strips, int L) {
-    const int64_t room = 2ll * device_sms() / strips;
-    const int need = (L + RW * RUN - 1) / (RW * RUN);
-    int c = (int)(room < 1 ? 1 : room > RC ? RC : room);
-    return c < need ? c : need;
+// ---------------------------------------------------------------------------------------------------
+// The same walk for rows of whole 16-byte pieces, which come to shared memory by asynchronous copies.  A chunk is RUN tokens of 4 bytes a
+// lane (V channels) times LPC lanes; a warp holds 32 / LPC chunks side by side (its lanes, LPC by LPC), brings their rows itself, STAGES steps
+// ahead, and reads them twice: for the chunk's pair, and for the outputs.  So no registers wait for memory, and three CTAs share an SM.
+// Narrow strips (LPC 16 or 8) are the finer pieces of work where 32 lanes a strip would leave SMs idle; pairs of a warp's own chunks
+// meet by shuffles.
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+
+template <bool BWD> constexpr int tile_run = BWD ? 8 : 16;
+constexpr int tile_stages = 2;
+// bytes of a chunk of one tensor, with the shift that keeps the chunks of a warp in different banks
+template <int LPC, int RUN> constexpr int tile_chunk = RUN * LPC * 4 + (LPC < 32 ? LPC * 4 : 0);
+template <bool BWD, int LPC> constexpr int tile_warp = (BWD ? 3 : 2) * (32 / LPC) * tile_chunk<LPC, tile_run<BWD>>;      // of a warp and stage
+template <bool BWD, int LPC> constexpr int tile_smem = RW * tile_stages * tile_warp<BWD, LPC>;
+
+template <typename T, bool LOGITS, bool BWD, int LPC>
+__global__ void __launch_bounds__(RW * 32, BWD ? 2 : 3) rec_tile_kernel(const RecParams p) {
+    constexpr int V = 4 / (int)sizeof(T), RUN = tile_run<BWD>, NC = 32 / LPC, ROW = LPC * 4, PIECES = ROW / 16, NT = BWD ? 3 : 2;
+    constexpr int CHUNK = tile_chunk<LPC, RUN>;
+    using R = typename Raw<T, V>::type;
+    struct alignas(8 * V) Pair { float a[V], h[V]; };
+    extern __shared__ __align__(128) uint8_t tiles[];
+    __shared__ Pair own[2][RW][LPC];               // of each warp's tokens
+    __shared__ Pair all[2][RC][LPC];               // of each CTA's
+    __shared__ float behind[2][LPC][V];            // the state behind a step, from the threads that walked its last tokens (one CTA)
+    __shared__ uint64_t landed[2];
+    const uint32_t rank = tc::cluster_rank(), ctas = tc::cluster_size(), bar = tc::smem_u32(landed);
+    if (ctas > 1) {
+        if (threadIdx.x == 0) {
+            tc::mbar_init(bar, 1);
+            tc::mbar_init(bar + 8, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");       // I run; waited for before the first CTA's memory is written
+    }
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, q = lane / LPC, l = lane % LPC;
+    const int strips = (p.D + LPC * V - 1) / (LPC * V);
+    const int strip = blockIdx.x / ctas, b = strip / strips, d0 = (strip % strips) * LPC * V, d = d0 + l * V;
+    const bool live = d < p.D;
+    const int per = (int)ctas * RW * NC * RUN;     // tokens of a step
+    const int first_of_warp = ((int)rank * RW + wid) * NC * RUN, mine = first_of_warp + q * RUN;
+    // ---- the warp's copies: piece `pc` of rows r0, r0 + 32 / PIECES, ... of its NC * RUN rows
+    const int pc = lane % PIECES, r0 = lane / PIECES;
+    const uint32_t ring = tc::smem_u32(tiles) + wid * tile_stages * tile_warp<BWD, LPC>;
+    struct Walk { const char* base; int step; };   // tokens are numbered as the scan meets them: the k-th at base + k * step bytes
+    auto walk = [&](const void* at, const int64_t* st, int channel) {
+        const int64_t last = p.from_end ? (int64_t)(p.L - 1) * st[1] : 0;
+        return Walk{(const char*)((const T*)at + b * st[0] + last + channel), (int)((p.from_end ? -st[1] : st[1]) * (int64_t)sizeof(T))};
+    };
+    const bool piece = d0 + pc * (16 / (int)sizeof(T)) < p.D;
+    const int pd = piece ? d0 + pc * (16 / (int)sizeof(T)) : 0;
+    const Walk src[3] = {walk(p.x, p.sx, pd), walk(p.g, p.sg, pd), BWD ? walk(p.h_in, p.sh, pd) : Walk{}};
+    const uint32_t slot = ring + (r0 / RUN) * CHUNK + (r0 % RUN) * ROW + pc * 16;
+    constexpr int HOP = 32 / PIECES, AHEAD = HOP / RUN * CHUNK + HOP % RUN * ROW;      // rows from one copy of a lane to its next, and how far that is
+    static_assert(HOP % RUN == 0 || RUN % HOP == 0, "a lane's rows are evenly spaced, or lie in one chunk");
+    auto bring = [&](int base, int stage) {
+        const int k0 = base + first_of_warp;
+        if (k0 + NC * RUN + (BWD ? 1 : 0) <= p.L) {
+            if (piece) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const char* from = src[n].base + (int64_t)(k0 + r0 + (n == 2 ? 1 : 0)) * src[n].step;
+#pragma unroll
+                    for (int r = 0; r < NC * RUN / HOP; ++r)
+                        copy_16(slot + stage * tile_warp<BWD, LPC> + n * NC * CHUNK + (HOP >= RUN ? r * AHEAD : r / (RUN / HOP) * CHUNK + r % (RUN / HOP) * AHEAD),
+                                from + (int64_t)(r * HOP) * src[n].step);
+                }
+            }
+        } else if (piece && k0 < p.L) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                for (int r = 0; r < NC * RUN / HOP; ++r) {
+                    const int row = r * HOP + r0, k = k0 + row + (n == 2 ? 1 : 0);
+                    if (k < p.L)
+                        copy_16(ring + pc * 16 + stage * tile_warp<BWD, LPC> + n * NC * CHUNK + (row / RUN) * CHUNK + (row % RUN) * ROW, src[n].base + (int64_t)k * src[n].step);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int st = 0; st < tile_stages; ++st) bring(st * per, st);
+    const Walk out = walk(p.out, p.so, d), outg = BWD ? walk(p.out_g, p.sog, d) : out;
+    float carry[V], first[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        carry[v] = live && p.s0 ? p.s0[b * p.ld_s0 + d + v] : 0.f;
+        first[v] = BWD && live && p.h0 ? p.h0[(int64_t)b * p.D + d + v] : 0.f;
+    }
+    uint32_t phase = 0;
+    for (int base = 0, buf = 0; base < p.L; base += per, buf ^= 1) {
+        if (ctas > 1 && threadIdx.x == 0) tc::mbar_expect_tx(bar + 8 * buf, ctas * LPC * (uint32_t)sizeof(Pair));
+        asm volatile("cp.async.wait_group %0;" ::"n"(tile_stages - 1) : "memory");
+        __syncwarp();
+        const int k0 = base + mine, left = live ? p.L - k0 : 0;        // tokens behind the last one leave the state as it is
+        const uint8_t* tile = tiles + (wid * tile_stages + buf) * tile_warp<BWD, LPC> + q * CHUNK + l * 4;
+        auto cell = [&](int n, int i) { return *(const R*)(tile + n * NC * CHUNK + i * ROW); };
+        float a[RUN][V], rest[BWD && LOGITS ? RUN : 1][V], A[V], H[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) { A[v] = 1.f; H[v] = 0.f; }
+        auto local = [&](auto whole) {
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) {
+                float gf[V], xf[V];
+                Raw<T, V>::get(cell(1, i), gf);
+                Raw<T, V>::get(cell(0, i), xf);
+                decays<T, LOGITS, BWD, V>(gf, p.inv_norm, a[i], rest[BWD && LOGITS ? i : 0]);
+                if (!decltype(whole)::value && i >= left) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) { a[i][v] = 1.f; xf[v] = 0.f; }
+                }
+                if (BWD) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) H[v] += xf[v];
+                    mul_v<V>(H, a[i], H);
+                } else {
+                    fma_v<V>(H, a[i], H, xf);
+                }
+                mul_v<V>(A, A, a[i]);
+            }
+        };
+        if (left >= RUN) local(std::true_type()); else local(std::false_type());
+        __syncwarp();
+        // chunks of the warp ahead of mine: (ea, eh); the lanes of the last chunk then hold the warp's pair
+        float ea[V], eh[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) { A[v] = finite(A[v]); ea[v] = 1.f; eh[v] = 0.f; }
+#pragma unroll
+        for (int off = LPC; off < 32; off *= 2) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float oa = __shfl_up_sync(0xffffffffu, A[v], off), oh = __shfl_up_sync(0xffffffffu, H[v], off);
+                if (lane >= off) { H[v] = fmaf(A[v], oh, H[v]); A[v] = finite(A[v] * oa); }
+            }
+        }
+        if (LPC < 32) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float oa = __shfl_up_sync(0xffffffffu, A[v], LPC), oh = __shfl_up_sync(0xffffffffu, H[v], LPC);
+                if (lane >= LPC) { ea[v] = oa; eh[v] = oh; }
+            }
+        }
+        Pair me;
+        if (lane >= 32 - LPC) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) { me.a[v] = A[v]; me.h[v] = H[v]; }
+            own[buf][wid][l] = me;
+        }
+        __syncthreads();
+        float s[V];
+        if (ctas > 1) {
+            // joined: the tokens of the CTA ahead of this warp's; and all of them
+            float pa[V], ph[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) { me.a[v] = 1.f; me.h[v] = 0.f; }
+#pragma unroll
+            for (int w = 0; w < RW; ++w) {
+                const Pair e = own[buf][w][l];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (w == wid) { pa[v] = me.a[v]; ph[v] = me.h[v]; }
+                    me.h[v] = fmaf(e.a[v], me.h[v], e.h[v]);
+                    me.a[v] = finite(me.a[v] * e.a[v]);
+                }
+            }
+            if (base == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+            if (lane < LPC)
+                for (uint32_t other = wid; other < ctas; other += RW) {
+                    const uint32_t at = tc::map_rank(tc::smem_u32(&all[buf][rank][l]), other), count = tc::map_rank(bar + 8 * buf, other);
+                    if constexpr (V == 2)
+                        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                                     ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.a[1])), "r"(__float_as_uint(me.h[0])), "r"(__float_as_uint(me.h[1])), "r"(count) : "memory");
+                    else
+                        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
+                                     ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.h[0])), "r"(count) : "memory");
+                }
+            int tries = 0;
+            while (!tc::mbar_try_wait_parked(bar + 8 * buf, (phase >> buf) & 1, 1000000)) {
+                if (++tries > 2000) {                                  // about a second or two: say so, and finish with what is there
+                    if (p.status && lane == 0) atomicOr(p.status, 1);
+                    break;
+                }
+            }
+            phase ^= 1u << buf;
+#pragma unroll
+            for (int v = 0; v < V; ++v) s[v] = carry[v];
+#pragma unroll 4
+            for (uint32_t r = 0; r < ctas; ++r) {
+                const Pair e = all[buf][r][l];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (r == rank) s[v] = carry[v];
+                    carry[v] = fmaf(e.a[v], carry[v], e.h[v]);
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) s[v] = fmaf(pa[v], s[v], ph[v]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) s[v] = base ? behind[buf][l][v] : carry[v];
+#pragma unroll 1
+            for (int w = 0; w < wid; ++w) {
+                const Pair e = own[buf][w][l];
+                fma_v<V>(s, e.a, s, e.h);
+            }
+        }
+        if (LPC < 32) fma_v<V>(s, ea, s, eh);
+        char *po = (char*)out.base + (int64_t)k0 * out.step, *pog = (char*)outg.base + (int64_t)k0 * outg.step;
+        auto outputs = [&](auto whole) {
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) {
+                if (!decltype(whole)::value && i >= left) break;
+                float xf[V], o[V];
+                Raw<T, V>::get(cell(0, i), xf);
+                if (!BWD) {
+                    fma_v<V>(s, a[i], s, xf);
+                    *(R*)(po + (int64_t)i * out.step) = Raw<T, V>::put(s);
+                } else {
+                    float hf[V];
+                    Raw<T, V>::get(cell(2, i), hf);
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        if (!decltype(whole)::value && i + 1 >= left) hf[v] = first[v];
+                        o[v] = xf[v] + s[v];
+                    }
+                    mul_v<V>(s, a[i], o);
+                    *(R*)(po + (int64_t)i * out.step) = Raw<T, V>::put(o);
+                    mul_v<V>(o, s, hf);
+                    if (LOGITS) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) o[v] *= p.inv_norm * rest[i][v];
+                    }
+                    *(R*)(pog + (int64_t)i * outg.step) = Raw<T, V>::put(o);
+                }
+            }
+        };
+        if (left > RUN) outputs(std::true_type()); else outputs(std::false_type());
+        if (ctas == 1 && wid == RW - 1 && lane >= 32 - LPC) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) behind[buf ^ 1][l][v] = s[v];
+        }
+        // the state behind the last token, as that token's output was rounded from it
+        if (p.s_end && left > 0 && left <= RUN) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) p.s_end[b * p.ld_end + d + v] = s[v];
+        }
+        __syncwarp();
+        bring(base + tile_stages * per, buf);
+    }
+    // no CTA leaves while another may still write to it (one that gave up waiting)
+    if (ctas > 1) {
+        asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+        asm volatile("barrier.cluster.wait;" ::: "memory");
+    }
 }
 
-template <typename T, bool LOGITS, bool BWD, int V, int RUN>
-int rec_strips(const RecParams& p, cudaStream_t s) {
-    const int64_t strips = (int64_t)p.B * ((p.D + 32 * V - 1) / (32 * V));
-    int c = rec_ctas<RUN>(strips, p.L);
+static int rec_clusters(void (*kernel)(RecParams), const RecParams& p, int64_t strips, int c, size_t smem, cudaStream_t s) {
+    if (smem > 24 * 1024)                          // with what is static, more than a kernel has unasked
+        if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(strips * c)); cfg.blockDim = dim3(RW * 32); cfg.stream = s;
+    cfg.gridDim = dim3((unsigned)(strips * c)); cfg.blockDim = dim3(RW * 32); cfg.stream = s; cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = c; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, rec_strip_kernel<T, LOGITS, BWD, V, RUN>, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+// CTAs of a cluster, a power of two (others are placed badly): as many as still find room at once, no more than the sequence has steps for
+static int rec_ctas(int64_t strips, int L, int step, int slots) {
+    int c = 1;
+    while (c < RC && 2 * c * strips <= slots && c * (int64_t)step < L) c *= 2;
+    return c;
+}
+
+template <typename T, bool LOGITS, bool BWD>
+int rec_strips(const RecParams& p, cudaStream_t s) {
+    constexpr int RUN = BWD ? 8 : 16;
+    const int64_t strips = (int64_t)p.B * ((p.D + 31) / 32);
+    return rec_clusters(rec_strip_kernel<T, LOGITS, BWD, 1, RUN>, p, strips, rec_ctas(strips, p.L, RW * RUN, 2 * device_sms()), 0, s);
+}
+
+template <typename T, bool LOGITS, bool BWD, int LPC>
+int rec_tiles(const RecParams& p, int64_t strips, cudaStream_t s) {
+    const int slots = (BWD ? 2 : 3) * device_sms();
+    return rec_clusters(rec_tile_kernel<T, LOGITS, BWD, LPC>, p, strips, rec_ctas(strips, p.L, RW * (32 / LPC) * tile_run<BWD>, slots), tile_smem<BWD, LPC>, s);
 }
 
 // Whether a step over all three or five tensors is a 32-bit number of bytes
@@ -366,10 +648,10 @@ inline bool short_steps(const RecParams& p, bool bwd) {
     return fits(p.sx) && fits(p.sg) && fits(p.so) && (!bwd || (fits(p.sh) && fits(p.sog)));
 }
 
-// Whether rows of two values begin on their size
-template <typename T> bool in_pairs(const RecParams& p, bool bwd) {
-    auto fits = [](const void* q, const int64_t* st) { return (uintptr_t)q % (2 * sizeof(T)) == 0 && st[0] % 2 == 0 && st[1] % 2 == 0; };
-    return p.D % 2 == 0 && fits(p.x, p.sx) && fits(p.g, p.sg) && fits(p.out, p.so) && (!bwd || (fits(p.h_in, p.sh) && fits(p.out_g, p.sog)));
+// Whether all rows are 16-byte pieces
+template <typename T> bool in_pieces(const RecParams& p, bool bwd) {
+    auto fits = [](const void* q, const int64_t* st) { return (uintptr_t)q % 16 == 0 && st[0] * sizeof(T) % 16 == 0 && st[1] * sizeof(T) % 16 == 0; };
+    return p.D * sizeof(T) % 16 == 0 && fits(p.x, p.sx) && fits(p.g, p.sg) && fits(p.out, p.so) && (!bwd || (fits(p.h_in, p.sh) && fits(p.out_g, p.sog)));
 }
 
 template <typename T, bool LOGITS, bool BWD>
@@ -379,9 +661,12 @@ int rec_launch(const RecParams& p, cudaStream_t s) {
         rec_serial_kernel<T, LOGITS, BWD><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
         return (int)cudaGetLastError();
     }
-    constexpr int RUN = BWD ? 8 : 16;
-    if constexpr (sizeof(T) == 2) if (in_pairs<T>(p, BWD)) return rec_strips<T, LOGITS, BWD, 2, RUN>(p, s);
-    return rec_strips<T, LOGITS, BWD, 1, RUN>(p, s);
+    if (!in_pieces<T>(p, BWD)) return rec_strips<T, LOGITS, BWD>(p, s);
+    const int slots = (BWD ? 2 : 3) * device_sms();
+    auto strips = [&](int lpc) { const int w = lpc * (4 / (int)sizeof(T)); return (int64_t)p.B * ((p.D + w - 1) / w); };
+    if (strips(32) >= 2 * slots) return rec_tiles<T, LOGITS, BWD, 32>(p, strips(32), s);
+    if (strips(16) >= 2 * slots) return rec_tiles<T, LOGITS, BWD, 16>(p, strips(16), s);
+    return rec_tiles<T, LOGITS, BWD, 8>(p, strips(8), s);
 }
 
 template <bool BWD> int rec_dispatch(const RecParams& p, int dtype, cudaStream_t s) {
