@@ -149,7 +149,8 @@ template <> struct Raw<__half, 2> {
     static __device__ type put(const float* f) { return __floats2half2_rn(f[0], f[1]); }
 };
 
-constexpr int RW = 8;                 // warps of a CTA
+constexpr int RW = 8;                 // warps of a CTA, and of one below
+constexpr int TW = 4;
 constexpr int RC = 8;                 // CTAs of a cluster, at most
 
 // The product of decays of a stretch of tokens, kept finite: 0 times it stays 0.  (Were a decay NaN, the stretch's contribution is NaN.)
@@ -354,44 +355,40 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
 // ---------------------------------------------------------------------------------------------------
 // The same walk for rows of whole 16-byte pieces, which come to shared memory by asynchronous copies.  A chunk is RUN tokens of 4 bytes a
 // lane (V channels) times LPC lanes; a warp holds 32 / LPC chunks side by side (its lanes, LPC by LPC), brings their rows itself, STAGES steps
-// ahead, and reads them twice: for the chunk's pair, and for the outputs.  So no registers wait for memory, and three CTAs share an SM.
+// ahead, and reads them twice: for the chunk's pair, and for the outputs.  No registers wait for memory.
 // Narrow strips (LPC 16 or 8) are the finer pieces of work where 32 lanes a strip would leave SMs idle; pairs of a warp's own chunks
 // meet by shuffles.
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 
 template <bool BWD> constexpr int tile_run = BWD ? 8 : 16;
-constexpr int tile_stages = 2;
+constexpr int tile_stages = 3;
 // bytes of a chunk of one tensor, with the shift that keeps the chunks of a warp in different banks
 template <int LPC, int RUN> constexpr int tile_chunk = RUN * LPC * 4 + (LPC < 32 ? LPC * 4 : 0);
 template <bool BWD, int LPC> constexpr int tile_warp = (BWD ? 3 : 2) * (32 / LPC) * tile_chunk<LPC, tile_run<BWD>>;      // of a warp and stage
-template <bool BWD, int LPC> constexpr int tile_smem = RW * tile_stages * tile_warp<BWD, LPC>;
+template <bool BWD, int LPC> constexpr int tile_smem = TW * tile_stages * tile_warp<BWD, LPC>;
 
 template <typename T, bool LOGITS, bool BWD, int LPC>
-__global__ void __launch_bounds__(RW * 32, BWD ? 2 : 3) rec_tile_kernel(const RecParams p) {
+__global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p) {
     constexpr int V = 4 / (int)sizeof(T), RUN = tile_run<BWD>, NC = 32 / LPC, ROW = LPC * 4, PIECES = ROW / 16, NT = BWD ? 3 : 2;
     constexpr int CHUNK = tile_chunk<LPC, RUN>;
     using R = typename Raw<T, V>::type;
     struct alignas(8 * V) Pair { float a[V], h[V]; };
     extern __shared__ __align__(128) uint8_t tiles[];
-    __shared__ Pair own[2][RW][LPC];               // of each warp's tokens
+    __shared__ Pair own[2][TW][LPC];               // of each warp's tokens
     __shared__ Pair all[2][RC][LPC];               // of each CTA's
-    __shared__ float behind[2][LPC][V];            // the state behind a step, from the threads that walked its last tokens (one CTA)
-    __shared__ uint64_t landed[2];
+    float (*mail)[LPC][V] = (float (*)[LPC][V])own;                   // one CTA: the state ahead of each warp's tokens, from the warp before
+    __shared__ uint64_t landed[TW];   // several CTAs: 0 and 1 count the bytes of `all`; one: one a warp, its mail is there
     const uint32_t rank = tc::cluster_rank(), ctas = tc::cluster_size(), bar = tc::smem_u32(landed);
-    if (ctas > 1) {
-        if (threadIdx.x == 0) {
-            tc::mbar_init(bar, 1);
-            tc::mbar_init(bar + 8, 1);
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        }
-        asm volatile("barrier.cluster.arrive.release;" ::: "memory");       // I run; waited for before the first CTA's memory is written
-    }
+    if (threadIdx.x < TW) tc::mbar_init(bar + 8 * threadIdx.x, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");       // I run; waited for before the first CTA's memory is written
+    __syncthreads();
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, q = lane / LPC, l = lane % LPC;
     const int strips = (p.D + LPC * V - 1) / (LPC * V);
     const int strip = blockIdx.x / ctas, b = strip / strips, d0 = (strip % strips) * LPC * V, d = d0 + l * V;
     const bool live = d < p.D;
-    const int per = (int)ctas * RW * NC * RUN;     // tokens of a step
-    const int first_of_warp = ((int)rank * RW + wid) * NC * RUN, mine = first_of_warp + q * RUN;
+    const int per = (int)ctas * TW * NC * RUN;     // tokens of a step
+    const int first_of_warp = ((int)rank * TW + wid) * NC * RUN, mine = first_of_warp + q * RUN;
     // ---- the warp's copies: piece `pc` of rows r0, r0 + 32 / PIECES, ... of its NC * RUN rows
     const int pc = lane % PIECES, r0 = lane / PIECES;
     const uint32_t ring = tc::smem_u32(tiles) + wid * tile_stages * tile_warp<BWD, LPC>;
@@ -441,39 +438,65 @@ __global__ void __launch_bounds__(RW * 32, BWD ? 2 : 3) rec_tile_kernel(const Re
         first[v] = BWD && live && p.h0 ? p.h0[(int64_t)b * p.D + d + v] : 0.f;
     }
     uint32_t phase = 0;
-    for (int base = 0, buf = 0; base < p.L; base += per, buf ^= 1) {
-        if (ctas > 1 && threadIdx.x == 0) tc::mbar_expect_tx(bar + 8 * buf, ctas * LPC * (uint32_t)sizeof(Pair));
-        asm volatile("cp.async.wait_group %0;" ::"n"(tile_stages - 1) : "memory");
-        __syncwarp();
-        const int k0 = base + mine, left = live ? p.L - k0 : 0;        // tokens behind the last one leave the state as it is
-        const uint8_t* tile = tiles + (wid * tile_stages + buf) * tile_warp<BWD, LPC> + q * CHUNK + l * 4;
-        auto cell = [&](int n, int i) { return *(const R*)(tile + n * NC * CHUNK + i * ROW); };
-        float a[RUN][V], rest[BWD && LOGITS ? RUN : 1][V], A[V], H[V];
+    float a[RUN][V], rest[BWD && LOGITS ? RUN : 1][V], A[V], H[V], s[V];
+    const uint8_t* const mine_of_ring = tiles + wid * tile_stages * tile_warp<BWD, LPC> + q * CHUNK + l * 4;
+    auto cell = [&](int stage, int n, int i) { return *(const R*)(mine_of_ring + stage * tile_warp<BWD, LPC> + n * NC * CHUNK + i * ROW); };
+    // token i of a step: its decay, and the chunk's pair up to it
+    auto enter = [&](int stage, int i, bool in) {
+        float gf[V], xf[V];
+        Raw<T, V>::get(cell(stage, 1, i), gf);
+        Raw<T, V>::get(cell(stage, 0, i), xf);
+        decays<T, LOGITS, BWD, V>(gf, p.inv_norm, a[i], rest[BWD && LOGITS ? i : 0]);
+        if (!in) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) { a[i][v] = 1.f; xf[v] = 0.f; }
+        }
+        if (BWD) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) H[v] += xf[v];
+            mul_v<V>(H, a[i], H);
+        } else {
+            fma_v<V>(H, a[i], H, xf);
+        }
+        mul_v<V>(A, A, a[i]);
+    };
+    // token i of a step: its outputs from the state ahead of it
+    auto leave = [&](int stage, int i, char* po, char* pog, bool last) {
+        float xf[V], o[V];
+        Raw<T, V>::get(cell(stage, 0, i), xf);
+        if (!BWD) {
+            fma_v<V>(s, a[i], s, xf);
+            *(R*)(po + (int64_t)i * out.step) = Raw<T, V>::put(s);
+        } else {
+            float hf[V];
+            Raw<T, V>::get(cell(stage, 2, i), hf);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (last) hf[v] = first[v];
+                o[v] = xf[v] + s[v];
+            }
+            mul_v<V>(s, a[i], o);
+            *(R*)(po + (int64_t)i * out.step) = Raw<T, V>::put(o);
+            mul_v<V>(o, s, hf);
+            if (LOGITS) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[v] *= p.inv_norm * rest[i][v];
+            }
+            *(R*)(pog + (int64_t)i * outg.step) = Raw<T, V>::put(o);
+        }
+    };
+    auto begin = [&]() {
 #pragma unroll
         for (int v = 0; v < V; ++v) { A[v] = 1.f; H[v] = 0.f; }
-        auto local = [&](auto whole) {
+    };
+    asm volatile("cp.async.wait_group %0;" ::"n"(tile_stages - 1) : "memory");
+    __syncwarp();
+    begin();
 #pragma unroll
-            for (int i = 0; i < RUN; ++i) {
-                float gf[V], xf[V];
-                Raw<T, V>::get(cell(1, i), gf);
-                Raw<T, V>::get(cell(0, i), xf);
-                decays<T, LOGITS, BWD, V>(gf, p.inv_norm, a[i], rest[BWD && LOGITS ? i : 0]);
-                if (!decltype(whole)::value && i >= left) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) { a[i][v] = 1.f; xf[v] = 0.f; }
-                }
-                if (BWD) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) H[v] += xf[v];
-                    mul_v<V>(H, a[i], H);
-                } else {
-                    fma_v<V>(H, a[i], H, xf);
-                }
-                mul_v<V>(A, A, a[i]);
-            }
-        };
-        if (left >= RUN) local(std::true_type()); else local(std::false_type());
-        __syncwarp();
+    for (int i = 0; i < RUN; ++i) enter(0, i, live && mine + i < p.L);
+    for (int base = 0, buf = 0, stage = 0; base < p.L; base += per, buf ^= 1) {
+        if (ctas > 1 && threadIdx.x == 0) tc::mbar_expect_tx(bar + 8 * buf, ctas * LPC * (uint32_t)sizeof(Pair));
+        const int k0 = base + mine, left = live ? p.L - k0 : 0;        // tokens behind the last one leave the state as it is
         // chunks of the warp ahead of mine: (ea, eh); the lanes of the last chunk then hold the warp's pair
         float ea[V], eh[V];
 #pragma unroll
@@ -493,21 +516,29 @@ __global__ void __launch_bounds__(RW * 32, BWD ? 2 : 3) rec_tile_kernel(const Re
                 if (lane >= LPC) { ea[v] = oa; eh[v] = oh; }
             }
         }
-        Pair me;
-        if (lane >= 32 - LPC) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) { me.a[v] = A[v]; me.h[v] = H[v]; }
-            own[buf][wid][l] = me;
-        }
-        __syncthreads();
-        float s[V];
+        auto wait = [&](uint32_t what, uint32_t parity) {
+            int tries = 0;
+            while (!tc::mbar_try_wait_parked(what, parity, 1000000)) {
+                if (++tries > 2000) {                                  // about a second or two: say so, and finish with what is there
+                    if (p.status && lane == 0) atomicOr(p.status, 1);
+                    break;
+                }
+            }
+        };
         if (ctas > 1) {
+            Pair me;
+            if (lane >= 32 - LPC) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) { me.a[v] = A[v]; me.h[v] = H[v]; }
+                own[buf][wid][l] = me;
+            }
+            __syncthreads();
             // joined: the tokens of the CTA ahead of this warp's; and all of them
             float pa[V], ph[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) { me.a[v] = 1.f; me.h[v] = 0.f; }
 #pragma unroll
-            for (int w = 0; w < RW; ++w) {
+            for (int w = 0; w < TW; ++w) {
                 const Pair e = own[buf][w][l];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
@@ -518,7 +549,7 @@ __global__ void __launch_bounds__(RW * 32, BWD ? 2 : 3) rec_tile_kernel(const Re
             }
             if (base == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
             if (lane < LPC)
-                for (uint32_t other = wid; other < ctas; other += RW) {
+                for (uint32_t other = wid; other < ctas; other += TW) {
                     const uint32_t at = tc::map_rank(tc::smem_u32(&all[buf][rank][l]), other), count = tc::map_rank(bar + 8 * buf, other);
                     if constexpr (V == 2)
                         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
@@ -527,13 +558,7 @@ __global__ void __launch_bounds__(RW * 32, BWD ? 2 : 3) rec_tile_kernel(const Re
                         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
                                      ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.h[0])), "r"(count) : "memory");
                 }
-            int tries = 0;
-            while (!tc::mbar_try_wait_parked(bar + 8 * buf, (phase >> buf) & 1, 1000000)) {
-                if (++tries > 2000) {                                  // about a second or two: say so, and finish with what is there
-                    if (p.status && lane == 0) atomicOr(p.status, 1);
-                    break;
-                }
-            }
+            wait(bar + 8 * buf, (phase >> buf) & 1);
             phase ^= 1u << buf;
 #pragma unroll
             for (int v = 0; v < V; ++v) s[v] = carry[v];
@@ -549,48 +574,49 @@ __global__ void __launch_bounds__(RW * 32, BWD ? 2 : 3) rec_tile_kernel(const Re
 #pragma unroll
             for (int v = 0; v < V; ++v) s[v] = fmaf(pa[v], s[v], ph[v]);
         } else {
+            // from warp to warp, round and round: no barrier, so the warps stay apart and one's arithmetic runs under another's waiting
+            if (base || wid) {
+                wait(bar + 8 * wid, (phase >> 2) & 1);
+                phase ^= 4;
 #pragma unroll
-            for (int v = 0; v < V; ++v) s[v] = base ? behind[buf][l][v] : carry[v];
-#pragma unroll 1
-            for (int w = 0; w < wid; ++w) {
-                const Pair e = own[buf][w][l];
-                fma_v<V>(s, e.a, s, e.h);
+                for (int v = 0; v < V; ++v) s[v] = mail[wid][l][v];
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) s[v] = carry[v];
+            }
+            if (base + (wid == TW - 1 ? per : 0) < p.L) {
+                const int to = (wid + 1) % TW;
+                if (lane >= 32 - LPC) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) mail[to][l][v] = fmaf(A[v], s[v], H[v]);
+                }
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar + 8 * to) : "memory");
             }
         }
         if (LPC < 32) fma_v<V>(s, ea, s, eh);
         char *po = (char*)out.base + (int64_t)k0 * out.step, *pog = (char*)outg.base + (int64_t)k0 * outg.step;
-        auto outputs = [&](auto whole) {
+        const int ahead = stage + 1 < tile_stages ? stage + 1 : 0;
+        const bool more = base + per < p.L;
+        asm volatile("cp.async.wait_group %0;" ::"n"(tile_stages - 2) : "memory");
+        __syncwarp();
+        begin();
+        if (left - per >= RUN) {
+            // a token's decay is used for the last time, and in its place comes that of the next step: the MUFU unit works under the
+            // multiply-adds and stores (one after the other, the warps of an SM fall into step and leave it idle: 75 us instead of 55)
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                if (!decltype(whole)::value && i >= left) break;
-                float xf[V], o[V];
-                Raw<T, V>::get(cell(0, i), xf);
-                if (!BWD) {
-                    fma_v<V>(s, a[i], s, xf);
-                    *(R*)(po + (int64_t)i * out.step) = Raw<T, V>::put(s);
-                } else {
-                    float hf[V];
-                    Raw<T, V>::get(cell(2, i), hf);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        if (!decltype(whole)::value && i + 1 >= left) hf[v] = first[v];
-                        o[v] = xf[v] + s[v];
-                    }
-                    mul_v<V>(s, a[i], o);
-                    *(R*)(po + (int64_t)i * out.step) = Raw<T, V>::put(o);
-                    mul_v<V>(o, s, hf);
-                    if (LOGITS) {
-#pragma unroll
-                        for (int v = 0; v < V; ++v) o[v] *= p.inv_norm * rest[i][v];
-                    }
-                    *(R*)(pog + (int64_t)i * outg.step) = Raw<T, V>::put(o);
-                }
+                leave(stage, i, po, pog, false);
+                enter(ahead, i, true);
             }
-        };
-        if (left > RUN) outputs(std::true_type()); else outputs(std::false_type());
-        if (ctas == 1 && wid == RW - 1 && lane >= 32 - LPC) {
+        } else {
 #pragma unroll
-            for (int v = 0; v < V; ++v) behind[buf ^ 1][l][v] = s[v];
+            for (int i = 0; i < RUN; ++i)
+                if (i < left) leave(stage, i, po, pog, i + 1 == left);
+            if (more) {
+#pragma unroll
+                for (int i = 0; i < RUN; ++i) enter(ahead, i, i < left - per);
+            }
         }
         // the state behind the last token, as that token's output was rounded from it
         if (p.s_end && left > 0 && left <= RUN) {
@@ -598,7 +624,8 @@ __global__ void __launch_bounds__(RW * 32, BWD ? 2 : 3) rec_tile_kernel(const Re
             for (int v = 0; v < V; ++v) p.s_end[b * p.ld_end + d + v] = s[v];
         }
         __syncwarp();
-        bring(base + tile_stages * per, buf);
+        bring(base + tile_stages * per, stage);
+        stage = ahead;
     }
     // no CTA leaves while another may still write to it (one that gave up waiting)
     if (ctas > 1) {
@@ -607,11 +634,11 @@ __global__ void __launch_bounds__(RW * 32, BWD ? 2 : 3) rec_tile_kernel(const Re
     }
 }
 
-static int rec_clusters(void (*kernel)(RecParams), const RecParams& p, int64_t strips, int c, size_t smem, cudaStream_t s) {
+static int rec_clusters(void (*kernel)(RecParams), const RecParams& p, int64_t strips, int c, int warps, size_t smem, cudaStream_t s) {
     if (smem > 24 * 1024)                          // with what is static, more than a kernel has unasked
         if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(strips * c)); cfg.blockDim = dim3(RW * 32); cfg.stream = s; cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3((unsigned)(strips * c)); cfg.blockDim = dim3(warps * 32); cfg.stream = s; cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = c; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -621,10 +648,11 @@ static int rec_clusters(void (*kernel)(RecParams), const RecParams& p, int64_t s
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
-// CTAs of a cluster, a power of two (others are placed badly): as many as still find room at once, no more than the sequence has steps for
-static int rec_ctas(int64_t strips, int L, int step, int slots) {
+// CTAs of a cluster, a power of two (others are placed badly: three took longer than four): the fewest that make `want` of them in all, no more
+// than the sequence has steps for
+static int rec_ctas(int64_t strips, int L, int step, int64_t want) {
     int c = 1;
-    while (c < RC && 2 * c * strips <= slots && c * (int64_t)step < L) c *= 2;
+    while (c < RC && c * strips < want && c * (int64_t)step < L) c *= 2;
     return c;
 }
 
@@ -632,13 +660,12 @@ template <typename T, bool LOGITS, bool BWD>
 int rec_strips(const RecParams& p, cudaStream_t s) {
     constexpr int RUN = BWD ? 8 : 16;
     const int64_t strips = (int64_t)p.B * ((p.D + 31) / 32);
-    return rec_clusters(rec_strip_kernel<T, LOGITS, BWD, 1, RUN>, p, strips, rec_ctas(strips, p.L, RW * RUN, 2 * device_sms()), 0, s);
+    return rec_clusters(rec_strip_kernel<T, LOGITS, BWD, 1, RUN>, p, strips, rec_ctas(strips, p.L, RW * RUN, device_sms()), RW, 0, s);
 }
 
 template <typename T, bool LOGITS, bool BWD, int LPC>
-int rec_tiles(const RecParams& p, int64_t strips, cudaStream_t s) {
-    const int slots = (BWD ? 2 : 3) * device_sms();
-    return rec_clusters(rec_tile_kernel<T, LOGITS, BWD, LPC>, p, strips, rec_ctas(strips, p.L, RW * (32 / LPC) * tile_run<BWD>, slots), tile_smem<BWD, LPC>, s);
+int rec_tiles(const RecParams& p, int64_t strips, int c, cudaStream_t s) {
+    return rec_clusters(rec_tile_kernel<T, LOGITS, BWD, LPC>, p, strips, c, TW, tile_smem<BWD, LPC>, s);
 }
 
 // Whether a step over all three or five tensors is a 32-bit number of bytes
@@ -662,11 +689,23 @@ int rec_launch(const RecParams& p, cudaStream_t s) {
         return (int)cudaGetLastError();
     }
     if (!in_pieces<T>(p, BWD)) return rec_strips<T, LOGITS, BWD>(p, s);
-    const int slots = (BWD ? 2 : 3) * device_sms();
+    // Width of the strips and CTAs of a cluster.  Four CTAs find room on an SM.  Best is the widest strip of which there are enough by
+    // themselves (a cluster's meetings cost: 16 x 4096 x 768 bf16, forward / backward, 62 / 93 us with 32 channels and one CTA, 67 / 102 with 64
+    // and two): 6/10 of the room, for the backward with its five tensors 4.5/10 (24 x 4096 x 768: 288 strips of 64 channels 146 us, 576 of 32
+    // 201, too many rows of memory at once).  Else the widest that reaches 6/10 in clusters (4 x 4096 x 384: 12.8 / 17.8 us with 32 channels and
+    // eight CTAs, 13.6 / 19.2 with 16 and four); else the narrowest (1 x 16384 x 768: 25 / 38 us with 16 channels, 32 / 52 with 32).
+    const int64_t room = 4 * device_sms(), alone = room * (BWD ? 45 : 60) / 100, joined = room * 60 / 100;
     auto strips = [&](int lpc) { const int w = lpc * (4 / (int)sizeof(T)); return (int64_t)p.B * ((p.D + w - 1) / w); };
-    if (strips(32) >= 2 * slots) return rec_tiles<T, LOGITS, BWD, 32>(p, strips(32), s);
-    if (strips(16) >= 2 * slots) return rec_tiles<T, LOGITS, BWD, 16>(p, strips(16), s);
-    return rec_tiles<T, LOGITS, BWD, 8>(p, strips(8), s);
+    auto ctas = [&](int lpc) { return rec_ctas(strips(lpc), p.L, TW * (32 / lpc) * tile_run<BWD>, joined); };
+    int lpc = 0, c = 1;
+    for (int w = 32; w >= 8 && !lpc; w /= 2) if (strips(w) >= alone) lpc = w;
+    for (int w = 32; w >= 8 && !lpc; w /= 2) if (strips(w) * ctas(w) >= joined) { lpc = w; c = ctas(w); }
+    if (!lpc) { lpc = 8; c = ctas(8); }
+    switch (lpc) {
+        case 32: return rec_tiles<T, LOGITS, BWD, 32>(p, strips(32), c, s);
+        case 16: return rec_tiles<T, LOGITS, BWD, 16>(p, strips(16), c, s);
+        default: return rec_tiles<T, LOGITS, BWD, 8>(p, strips(8), c, s);
+    }
 }
 
 template <bool BWD> int rec_dispatch(const RecParams& p, int dtype, cudaStream_t s) {
