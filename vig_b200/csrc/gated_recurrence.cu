@@ -558,6 +558,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
                         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
                                      ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.h[0])), "r"(count) : "memory");
                 }
+            if (base) bring(base + (tile_stages - 1) * per, stage ? stage - 1 : tile_stages - 1);      // what the step before has read, while totals are under way
             wait(bar + 8 * buf, (phase >> buf) & 1);
             phase ^= 1u << buf;
 #pragma unroll
@@ -624,7 +625,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
             for (int v = 0; v < V; ++v) p.s_end[b * p.ld_end + d + v] = s[v];
         }
         __syncwarp();
-        bring(base + tile_stages * per, stage);
+        if (ctas == 1) bring(base + tile_stages * per, stage);
         stage = ahead;
     }
     // no CTA leaves while another may still write to it (one that gave up waiting)
