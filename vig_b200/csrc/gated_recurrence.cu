@@ -62,65 +62,132 @@ template <typename T, bool LOGITS, bool REST, int V> __device__ __forceinline__ 
         }
     }
     if constexpr (sizeof(T) == 2 && LOGITS) {
+        constexpr int W = V > 1 ? 2 : 1;
         const float l2e[2] = {LOG2E, LOG2E}, one[2] = {1.f, 1.f}, minus[2] = {-1.f, -1.f}, inv[2] = {inv_norm, inv_norm};
-        float z[V], e[V], t[V];
-        mul_v<V>(z, g, l2e);
 #pragma unroll
-        for (int v = 0; v < V; ++v) e[v] = ex2(-fabsf(z[v]));
-        fma_v<V>(e, e, one, one);
+        for (int v = 0; v < V; v += W) {
+            float z[W], e[W], t[W];
+            mul_v<W>(z, g + v, l2e);
 #pragma unroll
-        for (int v = 0; v < V; ++v) { e[v] = lg2(e[v]); t[v] = fminf(z[v], 0.f); }
-        fma_v<V>(t, e, minus, t);                                // log2 of the sigmoid: min(z, 0) - log2(1 + 2^-|z|)
-        mul_v<V>(e, t, inv);
+            for (int w = 0; w < W; ++w) e[w] = ex2(-fabsf(z[w]));
+            fma_v<W>(e, e, one, one);
 #pragma unroll
-        for (int v = 0; v < V; ++v) a[v] = ex2(e[v]);
-        if (REST) {
-            fma_v<V>(t, z, minus, t);
+            for (int w = 0; w < W; ++w) { e[w] = lg2(e[w]); t[w] = fminf(z[w], 0.f); }
+            fma_v<W>(t, e, minus, t);                            // log2 of the sigmoid: min(z, 0) - log2(1 + 2^-|z|)
+            mul_v<W>(e, t, inv);
 #pragma unroll
-            for (int v = 0; v < V; ++v) rest[v] = ex2(t[v]);
+            for (int w = 0; w < W; ++w) a[v + w] = ex2(e[w]);
+            if (REST) {
+                fma_v<W>(t, z, minus, t);
+#pragma unroll
+                for (int w = 0; w < W; ++w) rest[v + w] = ex2(t[w]);
+            }
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------------
-// A thread owns a channel and walks its sequence.
-template <typename T, bool LOGITS, bool BWD>
-__global__ void __launch_bounds__(128) rec_serial_kernel(const RecParams p) {
+// Few tokens: a thread owns V channels (one, or 16 bytes of them) and walks their tokens, the loads of up to four tokens under way together.
+template <typename T, int V> struct Few {
+    T e[V];
+    __device__ void load(const T* p) {
+        if constexpr (V > 1) *(uint4*)e = *(const uint4*)p;
+        else e[0] = *p;
+    }
+    __device__ void get(float* f) const {
+#pragma unroll
+        for (int v = 0; v < V; ++v) f[v] = DType<T>::to_f(e[v]);
+    }
+    static __device__ void store(T* p, const float* f) {
+        Few o;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o.e[v] = DType<T>::from_f(f[v]);
+        if constexpr (V > 1) *(uint4*)p = *(const uint4*)o.e;
+        else *p = o.e[0];
+    }
+};
+template <int V> __device__ __forceinline__ void state_in(float* s, const float* p) {
+    if constexpr (V > 1) {
+#pragma unroll
+        for (int v = 0; v < V; v += 4) *(float4*)(s + v) = *(const float4*)(p + v);
+    } else {
+        s[0] = *p;
+    }
+}
+template <int V> __device__ __forceinline__ void state_out(float* p, const float* s) {
+    if constexpr (V > 1) {
+#pragma unroll
+        for (int v = 0; v < V; v += 4) *(float4*)(p + v) = *(const float4*)(s + v);
+    } else {
+        *p = s[0];
+    }
+}
+
+template <typename T, bool LOGITS, bool BWD, int V>
+__global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
+    constexpr int U = 4;
     const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    if (i >= (int64_t)p.B * p.D) return;
-    const int b = (int)(i / p.D), d = (int)(i % p.D);
+    const int per = p.D / V;
+    if (i >= (int64_t)p.B * per) return;
+    const int b = (int)(i / per), d = (int)(i % per) * V;
     const T* x = (const T*)p.x + b * p.sx[0] + d;
     const T* g = (const T*)p.g + b * p.sg[0] + d;
     const T* hin = BWD ? (const T*)p.h_in + b * p.sh[0] + d : nullptr;
     T* out = (T*)p.out + b * p.so[0] + d;
     T* outg = BWD ? (T*)p.out_g + b * p.sog[0] + d : nullptr;
-    float s = p.s0 ? p.s0[b * p.ld_s0 + d] : 0.f;
-    for (int k = 0; k < p.L; ++k) {
-        const int64_t t = p.from_end ? p.L - 1 - k : k;
-        const float gv = DType<T>::to_f(g[t * p.sg[1]]);
-        float a, rest;
-        decays<T, LOGITS, BWD, 1>(&gv, p.inv_norm, &a, &rest);
-        const float xv = DType<T>::to_f(x[t * p.sx[1]]);
-        if (!BWD) {
-            s = fmaf(a, s, xv);
-            out[t * p.so[1]] = DType<T>::from_f(s);
-        } else {
-            const float dx = xv + s;
-            s = a * dx;
-            const int64_t before = p.from_end ? t - 1 : t + 1;
-            const float hb = k + 1 < p.L ? DType<T>::to_f(hin[before * p.sh[1]]) : p.h0 ? p.h0[(int64_t)b * p.D + d] : 0.f;
-            float dg = s * hb;
-            if (LOGITS) dg *= p.inv_norm * rest;
-            out[t * p.so[1]] = DType<T>::from_f(dx);
-            outg[t * p.sog[1]] = DType<T>::from_f(dg);
+    auto at = [&](int k) { return (int64_t)(p.from_end ? p.L - 1 - k : k); };
+    float s[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = 0.f;
+    if (p.s0) state_in<V>(s, p.s0 + b * p.ld_s0 + d);
+    for (int k0 = 0; k0 < p.L; k0 += U) {
+        Few<T, V> xr[U], gr[U], hr[BWD ? U : 1];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u < p.L) {
+                xr[u].load(x + at(k0 + u) * p.sx[1]);
+                gr[u].load(g + at(k0 + u) * p.sg[1]);
+                if (BWD && k0 + u + 1 < p.L) hr[u].load(hin + at(k0 + u + 1) * p.sh[1]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u >= p.L) break;
+            float xf[V], gf[V], a[V], rest[V];
+            xr[u].get(xf);
+            gr[u].get(gf);
+            decays<T, LOGITS, BWD, V>(gf, p.inv_norm, a, rest);
+            if (!BWD) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) s[v] = fmaf(a[v], s[v], xf[v]);
+                Few<T, V>::store(out + at(k0 + u) * p.so[1], s);
+            } else {
+                float hb[V], og[V];
+                if (k0 + u + 1 < p.L) {
+                    hr[u].get(hb);
+                } else {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) hb[v] = 0.f;
+                    if (p.h0) state_in<V>(hb, p.h0 + (int64_t)b * p.D + d);
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    xf[v] += s[v];
+                    s[v] = a[v] * xf[v];
+                    og[v] = s[v] * hb[v];
+                    if (LOGITS) og[v] *= p.inv_norm * rest[v];
+                }
+                Few<T, V>::store(out + at(k0 + u) * p.so[1], xf);
+                Few<T, V>::store(outg + at(k0 + u) * p.sog[1], og);
+            }
         }
     }
-    if (p.s_end) p.s_end[b * p.ld_end + d] = s;
+    if (p.s_end) state_out<V>(p.s_end + b * p.ld_end + d, s);
 }
 
 // ---------------------------------------------------------------------------------------------------
-// A cluster of CTAs owns a strip of 32 * V channels of one sequence and walks it in steps of (CTAs x 8 warps x RUN) tokens.  A warp's lanes
-// are channels (rows of a strip are read whole), a thread holds RUN consecutive tokens of its channels in registers.  In a step every
+// Rows of any alignment.  A cluster of CTAs owns a strip of 32 channels of one sequence and walks it in steps of (CTAs x 8 warps x RUN)
+// tokens.  A warp's lanes are channels, a thread holds RUN consecutive tokens of its channel in registers.  In a step every
 // thread scans its tokens from a zero state, which gives the product of their decays and their own contribution; these pairs meet in shared
 // memory, the CTAs' totals in the shared memory of every CTA of the cluster (stores that its mbarrier counts: a cluster barrier would
 // also wait for the outputs of the step before).  Each thread then joins the pairs ahead of it to the state that the step began with and
@@ -156,8 +223,9 @@ constexpr int RC = 8;                 // CTAs of a cluster, at most
 // The product of decays of a stretch of tokens, kept finite: 0 times it stays 0.  (Were a decay NaN, the stretch's contribution is NaN.)
 __device__ __forceinline__ float finite(float a) { return fminf(a, 3.4028235e38f); }
 
-template <typename T, bool LOGITS, bool BWD, int V, int RUN>
+template <typename T, bool LOGITS, bool BWD, int RUN>
 __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p) {
+    constexpr int V = 1;
     using R = typename Raw<T, V>::type;
     struct alignas(8 * V) Pair { float a[V], h[V]; };                 // product of decays and contribution of a stretch of tokens
     __shared__ Pair own[2][RW][32];                // of each warp's tokens
@@ -270,12 +338,8 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
             if (base == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
             for (uint32_t other = wid; other < ctas; other += RW) {
                 const uint32_t at = tc::map_rank(tc::smem_u32(&all[buf][rank][lane]), other), count = tc::map_rank(bar + 8 * buf, other);
-                if constexpr (V == 2)
-                    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
-                                 ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.a[1])), "r"(__float_as_uint(me.h[0])), "r"(__float_as_uint(me.h[1])), "r"(count) : "memory");
-                else
-                    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
-                                 ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.h[0])), "r"(count) : "memory");
+                asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
+                             ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.h[0])), "r"(count) : "memory");
             }
             int tries = 0;
             while (!tc::mbar_try_wait_parked(bar + 8 * buf, (phase >> buf) & 1, 1000000)) {
@@ -661,7 +725,7 @@ template <typename T, bool LOGITS, bool BWD>
 int rec_strips(const RecParams& p, cudaStream_t s) {
     constexpr int RUN = BWD ? 8 : 16;
     const int64_t strips = (int64_t)p.B * ((p.D + 31) / 32);
-    return rec_clusters(rec_strip_kernel<T, LOGITS, BWD, 1, RUN>, p, strips, rec_ctas(strips, p.L, RW * RUN, device_sms()), RW, 0, s);
+    return rec_clusters(rec_strip_kernel<T, LOGITS, BWD, RUN>, p, strips, rec_ctas(strips, p.L, RW * RUN, device_sms()), RW, 0, s);
 }
 
 template <typename T, bool LOGITS, bool BWD, int LPC>
@@ -684,12 +748,22 @@ template <typename T> bool in_pieces(const RecParams& p, bool bwd) {
 
 template <typename T, bool LOGITS, bool BWD>
 int rec_launch(const RecParams& p, cudaStream_t s) {
-    const int64_t n = (int64_t)p.B * p.D;
-    if (p.L < 16 || !short_steps(p, BWD)) {
-        rec_serial_kernel<T, LOGITS, BWD><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
+    const bool pieces = in_pieces<T>(p, BWD);
+    // A strip's CTA is made for 64 tokens and more: below 16 a thread that walks them is as fast (8 x 768 channels, 15 tokens: 3.7 us, 16 in strips
+    // 4.8), and below 48 where the strips are more than find room at once (256 x 1024 channels, 16 tokens: 29 us in strips, 9 this way).
+    const int64_t wide = (int64_t)p.B * ((p.D * (int)sizeof(T) + 127) / 128);
+    if (p.L < (wide >= 4 * device_sms() ? 48 : 16) || !short_steps(p, BWD)) {
+        // 16 bytes a thread once there are threads enough for every SM
+        constexpr int V = 16 / (int)sizeof(T);
+        const int64_t n = (int64_t)p.B * p.D;
+        auto state = [](const float* q, int64_t ld) { return (uintptr_t)q % 16 == 0 && ld % 4 == 0; };
+        if (pieces && n / V >= 256ll * device_sms() && state(p.s0, p.ld_s0) && state(p.s_end, p.ld_end) && state(p.h0, 0))
+            rec_few_kernel<T, LOGITS, BWD, V><<<(unsigned)((n / V + 127) / 128), 128, 0, s>>>(p);
+        else
+            rec_few_kernel<T, LOGITS, BWD, 1><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
         return (int)cudaGetLastError();
     }
-    if (!in_pieces<T>(p, BWD)) return rec_strips<T, LOGITS, BWD>(p, s);
+    if (!pieces) return rec_strips<T, LOGITS, BWD>(p, s);
     // Width of the strips and CTAs of a cluster.  Four CTAs find room on an SM.  Best is the widest strip of which there are enough by
     // themselves (a cluster's meetings cost: 16 x 4096 x 768 bf16, forward / backward, 62 / 93 us with 32 channels and one CTA, 67 / 102 with 64
     // and two): 6/10 of the room, for the backward with its five tensors 4.5/10 (24 x 4096 x 768: 288 strips of 64 channels 146 us, 576 of 32
