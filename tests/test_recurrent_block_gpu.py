@@ -81,3 +81,13 @@ def test_training_and_serving():
                 err = float((residual + h - whole[:, t]).float().norm() / whole[:, t].float().norm())
                 # 16 bits: a handful of roundings of 2^-9 a block; 8-bit products: codes of 1/16, averaged over 128 terms, three projections wide
                 assert err < (0.1 if quantized else 0.02), (quantized, t, err)
+
+
+def test_example_runs():
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    import recurrent_stream
+    losses, far = recurrent_stream.main(["--steps", "30", "--width", "64", "--length", "48", "--batch", "4"])
+    # the loss falls; 8-bit products against 16-bit ones as above
+    assert losses[-1] < losses[0] and far < 0.1
