@@ -292,3 +292,37 @@ def test_c_entry_refuses_before_any_launch():
     fwd = lambda B=1, L=4, D=8, norm=0.0, dtype=0, ptr=None: L_.vig_gated_recurrence_fwd(ptr, ptr, None, 0, ptr, None, 0, B, L, D, None, None, None, norm, 0, dtype, None, None)  # noqa: E731
     assert fwd() == -1 and fwd(dtype=3) == -3 and fwd(B=-1) == -2 and fwd(norm=-1.0) == -6 and fwd(norm=float("nan")) == -6 and fwd(L=0) == 0
     assert L_.vig_gated_recurrence_bwd(None, None, None, None, None, None, None, None, 1, 4, 8, None, None, None, 0.0, 0, 0, None, None) == -1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("L", [5, 90])
+def test_masked_logits(L, dtype):
+    """Raw logits of -inf or the type's lowest value shut the state out, +inf and the highest keep it whole; gradients there are 0 and the
+    others what they are without them."""
+    x, g, _ = make(2, L, 24, dtype, 16.0, seed=12, state=False)
+    shut, keep = L // 2, L // 3
+    g[0, shut], g[1, shut] = float("-inf"), torch.finfo(dtype).min
+    g[0, keep], g[1, keep] = float("inf"), torch.finfo(dtype).max
+    leaf = [x.cuda().requires_grad_(True), g.cuda().requires_grad_(True)]
+    h, _ = vig_b200.gated_recurrence(*leaf, gate_logit_normalizer=16.0)
+    dx, dg = torch.autograd.grad(h, leaf, torch.ones_like(h))
+    h, dx, dg = h.detach().cpu(), dx.cpu(), dg.cpu()
+    assert torch.isfinite(h).all() and torch.isfinite(dx).all() and torch.isfinite(dg).all()
+    # sigmoid(lowest fp16)^(1/16) = e^-4094 and less: nothing of the state before is left
+    assert torch.equal(h[:, shut], x[:, shut]) and (dg[:, shut] == 0).all() and (dg[:, keep] == 0).all()
+    ref = h.float()[:, keep - 1] + x.float()[:, keep]
+    off = (h.float()[:, keep] - ref).abs()
+    assert (off <= 3 * UNIT[dtype] * (ref.abs() + h.float()[:, keep - 1].abs())).all()
+
+
+def test_no_token_hands_on_any_state():
+    x = torch.zeros(3, 0, 20, device="cuda")
+    for h0 in (torch.randn(1, 20, device="cuda").expand(3, 20), torch.randn(3, 50, device="cuda")[:, 7:27], torch.randn(20, device="cuda")[None].expand(3, 20)):
+        assert torch.equal(vig_b200.gated_recurrence(x, x, h0, True)[1], h0)
+
+
+def test_normalizers_that_no_float_holds_are_refused():
+    x = torch.zeros(1, 4, 8, device="cuda")
+    for n in (1e-50, 1e-40, 1e40, float("inf")):
+        with pytest.raises(ValueError):
+            vig_b200.gated_recurrence(x, x, gate_logit_normalizer=n)

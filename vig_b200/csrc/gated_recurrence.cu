@@ -80,7 +80,7 @@ template <typename T, bool LOGITS, bool REST, int V> __device__ __forceinline__ 
             if (REST) {
                 fma_v<W>(t, z, minus, t);
 #pragma unroll
-                for (int w = 0; w < W; ++w) rest[v + w] = ex2(t[w]);
+                for (int w = 0; w < W; ++w) rest[v + w] = ex2(fminf(t[w], 0.f));         // (a logit of -inf: -inf + inf, for 0)
             }
         }
     }
@@ -796,15 +796,18 @@ template <bool BWD> int rec_dispatch(const RecParams& p, int dtype, cudaStream_t
 static int rec_check(int B, int L, int D, float norm, int dtype) {
     if (dtype < VIG_DTYPE_F32 || dtype > VIG_DTYPE_F16) return VIG_ERR_DTYPE;
     if (B < 0 || L < 0 || L >= (1 << 30) || D < 0 || (int64_t)B * D >= (1ll << 31)) return VIG_ERR_SHAPE;
-    if (!(norm >= 0.f) || norm > 3.4e38f) return VIG_ERR_ARG;
+    if (norm != 0.f && !(norm >= 1e-30f && norm <= 1e30f)) return VIG_ERR_ARG;
     return VIG_OK;
 }
 
 // no token: the state that enters is the state that leaves
 static int rec_empty(const float* s0, int64_t ld0, float* s_end, int64_t ld_end, int B, int D, cudaStream_t s) {
-    if (!s_end || s_end == s0 || !B || !D) return VIG_OK;
-    return (int)(s0 ? cudaMemcpy2DAsync(s_end, ld_end * 4, s0, ld0 * 4, (size_t)D * 4, B, cudaMemcpyDeviceToDevice, s)
-                    : cudaMemset2DAsync(s_end, ld_end * 4, 0, (size_t)D * 4, B, s));
+    const int64_t n = (int64_t)B * D;
+    if (!s_end || !n) return VIG_OK;
+    RecParams p{};
+    p.s0 = s0; p.ld_s0 = ld0; p.s_end = s_end; p.ld_end = ld_end; p.B = B; p.D = D;
+    rec_few_kernel<float, false, false, 1><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
+    return (int)cudaGetLastError();
 }
 
 static void two(int64_t* dst, const int64_t* src, int L, int D) {

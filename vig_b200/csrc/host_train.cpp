@@ -3,6 +3,7 @@
 #include "host.h"
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 namespace vig_host {
 
@@ -50,6 +51,10 @@ void once(const variable_list& ds, const variable_list& saved) {
 }
 Tensor rows(const Tensor& t) { return t.defined() && !unit_last(t) ? t.contiguous() : t; }
 
+// an output on the device of `like`: the allocator's call without the dispatcher's way to it, which is a tenth of a short call
+Tensor fresh(at::IntArrayRef sizes, const Tensor& like, at::ScalarType type) { return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt)); }
+Tensor fresh(at::IntArrayRef sizes, const Tensor& like) { return fresh(sizes, like, like.scalar_type()); }
+
 struct S2 {                                    // (b, l) element strides of a [B, L, D] view
     int64_t s[2];
     explicit S2(const Tensor& t) { if (t.defined()) { s[0] = t.stride(0); s[1] = t.stride(1); } }
@@ -69,7 +74,7 @@ void check_rec(const Tensor& x, const Tensor& g, int dim, double norm) {
     want_type(g.scalar_type() == x.scalar_type(), "x and g must share one dtype");
     want(x.dim() == dim && g.sizes() == x.sizes(), (dim == 3 ? "x and g must be [B, L, D]; got " : "x and g must be [B, D]; got ") + shape_of(x) + " and " + shape_of(g));
     want(unit_last(x) && unit_last(g), "the last dimension of x and g must be contiguous");
-    want(norm >= 0 && std::isfinite(norm), "gate_logit_normalizer must be 0 (log-gates) or positive (raw logits)");
+    want(norm == 0 || (norm >= 1e-30 && norm <= 1e30), "gate_logit_normalizer must be 0 (log-gates) or positive (raw logits; 1e-30 to 1e30)");
     want(x.size(0) * x.size(-1) < (1ll << 31) && (dim == 2 || x.size(1) < (1ll << 30)), "B * D must be below 2^31 and L below 2^30");
 }
 
@@ -83,9 +88,9 @@ void rec_forward(const Tensor& x, const Tensor& g, const Tensor& h0, const Tenso
 struct Rec : torch::autograd::Function<Rec> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const OptT& h0_, bool want_final, bool reverse, double norm) {
         at::AutoDispatchBelowADInplaceOrView guard;
-        const Tensor h0 = get(h0_), h = at::empty(x.sizes(), x.options());
+        const Tensor h0 = get(h0_), h = fresh(x.sizes(), x);
         Tensor fin;
-        if (want_final) fin = at::empty({x.size(0), x.size(2)}, x.options().dtype(at::kFloat));
+        if (want_final) fin = fresh({x.size(0), x.size(2)}, x, at::kFloat);
         rec_forward(x, g, h0, h, fin, reverse, norm);
         ctx->save_for_backward({g, h, h0});
         ctx->saved_data["reverse"] = reverse;
@@ -101,9 +106,9 @@ struct Rec : torch::autograd::Function<Rec> {
         c10::cuda::CUDAGuard dev(g.device());
         const Tensor dh = d[0].defined() ? rows(d[0]) : at::zeros(h.sizes(), h.options());
         const Tensor df = d.size() > 1 && d[1].defined() ? d[1].contiguous() : Tensor();
-        const Tensor dx = at::empty(h.sizes(), h.options()), dg = at::empty(h.sizes(), h.options());
+        const Tensor dx = fresh(h.sizes(), h), dg = fresh(h.sizes(), h);
         Tensor d0;
-        if (h0.defined()) d0 = at::empty(h0.sizes(), h0.options());
+        if (h0.defined()) d0 = fresh(h0.sizes(), h0);
         const S2 sg(g), sh(h), sd(dh);
         ok(api.vig_gated_recurrence_bwd(ptr(g), ptr(h), (const float*)ptr(h0), ptr(dh), (const float*)ptr(df), ptr(dx), ptr(dg), (float*)ptr(d0), (int)h.size(0),
                                         (int)h.size(1), (int)h.size(2), sg.s, sh.s, sd.s, (float)ctx->saved_data["norm"].toDouble(),
@@ -123,9 +128,9 @@ std::optional<std::pair<Tensor, OptT>> gated_recurrence(const Tensor& x, const T
         const auto out = Rec::apply(x, g, h0_, want_final, reverse, norm);
         return std::make_pair(out[0], want_final ? OptT(out[1]) : OptT());
     }
-    const Tensor h = at::empty(x.sizes(), x.options());
+    const Tensor h = fresh(x.sizes(), x);
     Tensor fin;
-    if (want_final) fin = at::empty({x.size(0), x.size(2)}, x.options().dtype(at::kFloat));
+    if (want_final) fin = fresh({x.size(0), x.size(2)}, x, at::kFloat);
     rec_forward(x, g, h0, h, fin, reverse, norm);
     return std::make_pair(h, want_final ? OptT(fin) : OptT());
 }
@@ -137,7 +142,7 @@ Tensor gated_recurrence_step(const Tensor& x, const Tensor& g, const Tensor& sta
     if (wants_grad({&x, &g, &state})) not_implemented("gated_recurrence_step updates its state in place and has no gradient: use gated_recurrence, or torch.no_grad()");
     c10::cuda::CUDAGuard dev(x.device());
     state.unsafeGetTensorImpl()->bump_version();
-    const Tensor h = at::empty(x.sizes(), x.options());
+    const Tensor h = fresh(x.sizes(), x);
     const int64_t sx[2] = {x.stride(0), 0}, sg[2] = {g.stride(0), 0}, sh[2] = {h.stride(0), 0};
     ok(api.vig_gated_recurrence_fwd(ptr(x), ptr(g), (const float*)ptr(state), state.stride(0), ptr(h), (float*)ptr(state), state.stride(0), (int)x.size(0), 1, (int)x.size(1),
                                     sx, sg, sh, (float)norm, 0, dtype_code(x), status_ptr(x.get_device()), stream()), "vig_gated_recurrence_fwd");
@@ -177,11 +182,11 @@ std::tuple<Tensor, Tensor, Tensor> add_rmsnorm_8bit(const Tensor& x_, const Tens
     c10::cuda::CUDAGuard dev(x_.device());
     const Tensor x = as_rows(x_), res = res0.defined() ? as_rows(res0) : res0;
     auto sizes = x_.sizes().vec();
-    const Tensor q = at::empty(sizes, x.options().dtype(out_type == VIG_OUT_E4M3 ? at::kFloat8_e4m3fn : at::kChar));
+    const Tensor q = fresh(sizes, x, out_type == VIG_OUT_E4M3 ? at::kFloat8_e4m3fn : at::kChar);
     Tensor r;
-    if (prenorm && res.defined()) r = at::empty(sizes, x.options());
+    if (prenorm && res.defined()) r = fresh(sizes, x);
     sizes.back() = group ? N / group : 1;
-    const Tensor scales = at::empty(sizes, x.options().dtype(at::kFloat));
+    const Tensor scales = fresh(sizes, x, at::kFloat);
     ok(api.vig_add_rmsnorm_8bit_fwd(ptr(x), ld(x), ptr(res), ld(res), ptr(w), dtype_code(w), ptr(q), (float*)ptr(scales), ptr(r), x.size(0), (int)N, (int)group,
                                     (float)eps, (int)out_type, dtype_code(x), stream()), "vig_add_rmsnorm_8bit_fwd");
     return {q, scales, r.defined() ? r : x_};
@@ -189,9 +194,9 @@ std::tuple<Tensor, Tensor, Tensor> add_rmsnorm_8bit(const Tensor& x_, const Tens
 
 std::pair<Tensor, Tensor> norm_forward(const Tensor& x_, const Tensor& w, const Tensor& res0, double eps) {
     const Tensor x = as_rows(x_), res = res0.defined() ? as_rows(res0) : res0;
-    const Tensor y = at::empty(x_.sizes(), x.options());
+    const Tensor y = fresh(x_.sizes(), x);
     Tensor r;
-    if (res.defined()) r = at::empty(x_.sizes(), x.options());
+    if (res.defined()) r = fresh(x_.sizes(), x);
     ok(api.vig_add_rmsnorm_train_fwd(ptr(x), ld(x), ptr(res), ld(res), ptr(w), dtype_code(w), ptr(y), ptr(r), x.size(0), (int)x.size(1), (float)eps, dtype_code(x), stream()),
        "vig_add_rmsnorm_train_fwd");
     return {y, r};
@@ -199,10 +204,10 @@ std::pair<Tensor, Tensor> norm_forward(const Tensor& x_, const Tensor& w, const 
 
 std::pair<Tensor, Tensor> norm_backward(const Tensor& dy_, const Tensor& r_, const Tensor& w, const Tensor& dr_, double eps) {
     const Tensor r = as_rows(r_), dy = as_rows(dy_), dr = dr_.defined() ? as_rows(dr_) : dr_;
-    const Tensor dx = at::empty(r_.sizes(), r.options()), dw = at::empty(w.sizes(), w.options());
+    const Tensor dx = fresh(r_.sizes(), r), dw = fresh(w.sizes(), w);
     const size_t n = api.vig_add_rmsnorm_bwd_workspace_bytes(r.size(0), (int)r.size(1));
     Tensor ws;
-    if (n) ws = at::empty({(int64_t)n}, r.options().dtype(at::kByte));
+    if (n) ws = fresh({(int64_t)n}, r, at::kByte);
     ok(api.vig_add_rmsnorm_bwd(ptr(dy), ld(dy), ptr(r), ld(r), ptr(w), dtype_code(w), ptr(dr), ld(dr), ptr(dx), ptr(dw), r.size(0), (int)r.size(1), (float)eps,
                                dtype_code(r), ptr(ws), n, stream()), "vig_add_rmsnorm_bwd");
     return {dx, dw};
