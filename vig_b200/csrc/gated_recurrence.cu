@@ -5,7 +5,11 @@
 // Gradients: u_t = a_t (dh_t + u_{t+1}), the same recurrence from the other end;  dx_t = dh_t + u_{t+1},  dg_t = u_t h_{t-1},
 // dz_t = dg_t (1 - sigmoid(z_t)) / n,  dh_{-1} = u_0.  States, decays and sums are fp32; h is rounded once, to x's type, and the
 // backward reads h_{t-1} as it was rounded, so that x is not read again.
-// Bound by memory: 3 tensors forward (x, g in, h out), 5 backward (g, h, dh in, dx, dg out), about one exponential and a multiply-add a value.
+// Bound by memory where sequences are many (3 tensors forward: x, g in, h out; 5 backward: g, h, dh in, dx, dg out), and by the MUFU unit
+// beside it: a raw logit of 16 bits is three of its instructions (four backward), 3/4 of its rate at the copy bandwidth.  16 x 4096 x 768 bf16
+// from raw logits: forward 62 us (4.9 TB/s), backward 91 us (5.5 TB/s); 1 x 16384 x 768, 48 strips on 384 CTAs, 24 us.
+// Three forms, by the rule in rec_launch: rows of 16-byte pieces through shared memory (rec_tile_kernel), rows of any alignment through
+// registers (rec_strip_kernel), few tokens a thread at a time (rec_few_kernel).
 #include <type_traits>
 #include "tc_common.cuh"
 
@@ -40,6 +44,13 @@ template <int V> __device__ __forceinline__ void fma_v(float* d, const float* a,
             : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
     else
         d[0] = fmaf(a[0], b[0], c[0]);
+}
+template <int V> __device__ __forceinline__ void add_v(float* d, const float* a, const float* b) {
+    if constexpr (V == 2)
+        asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+    else
+        d[0] = a[0] + b[0];
 }
 template <int V> __device__ __forceinline__ void mul_v(float* d, const float* a, const float* b) {
     if constexpr (V == 2)
@@ -417,11 +428,17 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
 }
 
 // ---------------------------------------------------------------------------------------------------
-// The same walk for rows of whole 16-byte pieces, which come to shared memory by asynchronous copies.  A chunk is RUN tokens of 4 bytes a
-// lane (V channels) times LPC lanes; a warp holds 32 / LPC chunks side by side (its lanes, LPC by LPC), brings their rows itself, STAGES steps
-// ahead, and reads them twice: for the chunk's pair, and for the outputs.  No registers wait for memory.
-// Narrow strips (LPC 16 or 8) are the finer pieces of work where 32 lanes a strip would leave SMs idle; pairs of a warp's own chunks
-// meet by shuffles.
+// The same walk for rows of whole 16-byte pieces, which come to shared memory by asynchronous copies, two steps ahead.  A chunk is RUN tokens of
+// 4 bytes a lane (V channels) times LPC lanes; a warp holds 32 / LPC chunks side by side (its lanes, LPC by LPC) and brings their rows
+// itself.  No registers wait for memory.  Narrow strips (LPC 16 or 8) are the finer pieces of work where 32 lanes a strip would leave SMs idle;
+// the pairs of a warp's own chunks meet by shuffles.  What it measured on the way, forward, raw bf16 logits (us):
+//   loads a step ahead in registers, pairs over a barrier           16 x 4096 x 768   92     1 x 16384 x 768   41
+//   rows in shared memory, three CTAs of eight warps an SM                            75                       26
+//   decays of the next step under the outputs of this one                             67                       28
+//   the state handed from warp to warp, no barrier                                    62                       28
+//   four CTAs of four warps an SM, requests under the exchange                        62 (backward 103 -> 91)  24
+// Also tried: every warp adding up all pairs behind flags instead of the hand-over (the warps then keep step: 71), 32 tokens a thread
+// (1 x 16384 x 768 26), prefetch hints on the copies (no difference).
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 
 template <bool BWD> constexpr int tile_run = BWD ? 8 : 16;
@@ -516,8 +533,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
             for (int v = 0; v < V; ++v) { a[i][v] = 1.f; xf[v] = 0.f; }
         }
         if (BWD) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) H[v] += xf[v];
+            add_v<V>(H, H, xf);
             mul_v<V>(H, a[i], H);
         } else {
             fma_v<V>(H, a[i], H, xf);
@@ -534,17 +550,18 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
         } else {
             float hf[V];
             Raw<T, V>::get(cell(stage, 2, i), hf);
+            if (last) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (last) hf[v] = first[v];
-                o[v] = xf[v] + s[v];
+                for (int v = 0; v < V; ++v) hf[v] = first[v];
             }
+            add_v<V>(o, xf, s);
             mul_v<V>(s, a[i], o);
             *(R*)(po + (int64_t)i * out.step) = Raw<T, V>::put(o);
             mul_v<V>(o, s, hf);
             if (LOGITS) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) o[v] *= p.inv_norm * rest[i][v];
+                const float inv[2] = {p.inv_norm, p.inv_norm};
+                mul_v<V>(o, o, inv);
+                mul_v<V>(o, o, rest[i]);
             }
             *(R*)(pog + (int64_t)i * outg.step) = Raw<T, V>::put(o);
         }
@@ -570,10 +587,14 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float oa = __shfl_up_sync(0xffffffffu, A[v], off), oh = __shfl_up_sync(0xffffffffu, H[v], off);
-                if (lane >= off) { H[v] = fmaf(A[v], oh, H[v]); A[v] = finite(A[v] * oa); }
+                if (lane >= off) {
+                    H[v] = fmaf(A[v], oh, H[v]);
+                    A[v] = finite(A[v] * oa);
+                    if (NC == 2) { ea[v] = oa; eh[v] = oh; }
+                }
             }
         }
-        if (LPC < 32) {
+        if (NC > 2) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float oa = __shfl_up_sync(0xffffffffu, A[v], LPC), oh = __shfl_up_sync(0xffffffffu, H[v], LPC);
@@ -668,7 +689,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
         begin();
         if (left - per >= RUN) {
             // a token's decay is used for the last time, and in its place comes that of the next step: the MUFU unit works under the
-            // multiply-adds and stores (one after the other, the warps of an SM fall into step and leave it idle: 75 us instead of 55)
+            // multiply-adds and stores (one after the other, the warps of an SM fall into step and leave it idle)
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
                 leave(stage, i, po, pog, false);
