@@ -66,12 +66,14 @@ def main(argv=None):
     with torch.no_grad():
         whole, _ = model(x)
         _, states = model(x[:, :prefix])
+        model.step(x[:, prefix], [s.clone() for s in states])              # the first step loads its kernels
         torch.cuda.synchronize()
         began = time.perf_counter()
         served = torch.stack([model.step(x[:, t], states) for t in range(prefix, a.length)], 1)
         torch.cuda.synchronize()
+        took = time.perf_counter() - began
     far = float((served - whole[:, prefix:]).float().norm() / whole[:, prefix:].float().norm())
-    print(f"served 16 tokens of {a.batch} streams in {(time.perf_counter() - began) * 1e3:.2f} ms, {far:.3f} from the whole sequence in 16 bits")
+    print(f"served 16 tokens of {a.batch} streams in {took * 1e3:.2f} ms, {far:.3f} from the whole sequence in 16 bits")
     vig_b200.check_status()
     return losses, far
 

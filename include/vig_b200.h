@@ -381,10 +381,10 @@ VIG_API int vig_linear_swiglu_fwd(const void* x, int64_t ldx, const void* w, voi
 /*
  * Gated linear recurrence with one state per channel: h_t = a_t h_{t-1} + x_t (reverse: h_t = a_t h_{t+1} + x_t), a_t = exp(g_t), or with
  * gate_logit_normalizer n > 0 (1e-30 to 1e30) from raw logits, a_t = sigmoid(g_t)^(1/n).  Decays may exceed 1 as
- * long as their products over up to 2048 tokens stay below 3.4e38.  x, g, h: [B, L, D] with unit stride over D and element strides
+ * long as their products over up to 4096 tokens stay below 3.4e38.  x, g, h: [B, L, D] with unit stride over D and element strides
  * (b, l) (NULL = contiguous); any alignment; h may not overlap x or g.  h0 (optional), h_final (optional): fp32 [B, D] with row strides
  * ld_h0, ld_final; h_final may be h0 itself (a state updated in place), and L may be 0 (the state is handed on) or 1 (one new token).
- * B * D < 2^31, L < 2^30.  status_dev: optional int32 on the device, bit 0 = a bounded wait ran out.
+ * B * D < 2^31, D < 2^28, L < 2^30.  status_dev: optional int32 on the device, bit 0 = a bounded wait ran out.
  */
 VIG_API int vig_gated_recurrence_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final,
                                      int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,

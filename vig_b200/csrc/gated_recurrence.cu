@@ -229,7 +229,7 @@ template <> struct Raw<__half, 2> {
 
 constexpr int RW = 8;                 // warps of a CTA, and of one below
 constexpr int TW = 4;
-constexpr int RC = 8;                 // CTAs of a cluster, at most
+constexpr int RC = 8;                 // CTAs of a cluster of this kernel, at most
 
 // The product of decays of a stretch of tokens, kept finite: 0 times it stays 0.  (Were a decay NaN, the stretch's contribution is NaN.)
 __device__ __forceinline__ float finite(float a) { return fminf(a, 3.4028235e38f); }
@@ -447,6 +447,8 @@ constexpr int tile_stages = 3;
 template <int LPC, int RUN> constexpr int tile_chunk = RUN * LPC * 4 + (LPC < 32 ? LPC * 4 : 0);
 template <bool BWD, int LPC> constexpr int tile_warp = (BWD ? 3 : 2) * (32 / LPC) * tile_chunk<LPC, tile_run<BWD>>;      // of a warp and stage
 template <bool BWD, int LPC> constexpr int tile_smem = TW * tile_stages * tile_warp<BWD, LPC>;
+// ... and of what its warps, or its cluster's CTAs, tell one another (a pair is 8 bytes a channel)
+template <int LPC, int V> int tile_words(int ctas) { return ctas == 1 ? TW * LPC * V * 4 : 2 * (TW + ctas) * LPC * V * 8; }
 
 template <typename T, bool LOGITS, bool BWD, int LPC>
 __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p) {
@@ -455,11 +457,12 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
     using R = typename Raw<T, V>::type;
     struct alignas(8 * V) Pair { float a[V], h[V]; };
     extern __shared__ __align__(128) uint8_t tiles[];
-    __shared__ Pair own[2][TW][LPC];               // of each warp's tokens
-    __shared__ Pair all[2][RC][LPC];               // of each CTA's
-    float (*mail)[LPC][V] = (float (*)[LPC][V])own;                   // one CTA: the state ahead of each warp's tokens, from the warp before
-    __shared__ uint64_t landed[TW];   // several CTAs: 0 and 1 count the bytes of `all`; one: one a warp, its mail is there
+    __shared__ uint64_t landed[TW];                // one CTA: one a warp, its mail is there; several: 0 and 1 count the bytes of `all`
     const uint32_t rank = tc::cluster_rank(), ctas = tc::cluster_size(), bar = tc::smem_u32(landed);
+    // behind the tiles, one CTA: the state ahead of each warp's tokens, from the warp before; several: the pair of each warp's tokens and of each
+    // CTA's, for this step and the one before
+    float (*mail)[LPC][V] = (float (*)[LPC][V])(tiles + tile_smem<BWD, LPC>);
+    Pair (*own)[TW][LPC] = (Pair (*)[TW][LPC])(tiles + tile_smem<BWD, LPC>), *all = (Pair*)(own + 2);
     if (threadIdx.x < TW) tc::mbar_init(bar + 8 * threadIdx.x, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (ctas > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");       // I run; waited for before the first CTA's memory is written
@@ -635,7 +638,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
             if (base == 0) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
             if (lane < LPC)
                 for (uint32_t other = wid; other < ctas; other += TW) {
-                    const uint32_t at = tc::map_rank(tc::smem_u32(&all[buf][rank][l]), other), count = tc::map_rank(bar + 8 * buf, other);
+                    const uint32_t at = tc::map_rank(tc::smem_u32(all + (buf * ctas + rank) * LPC + l), other), count = tc::map_rank(bar + 8 * buf, other);
                     if constexpr (V == 2)
                         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
                                      ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.a[1])), "r"(__float_as_uint(me.h[0])), "r"(__float_as_uint(me.h[1])), "r"(count) : "memory");
@@ -650,7 +653,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
             for (int v = 0; v < V; ++v) s[v] = carry[v];
 #pragma unroll 4
             for (uint32_t r = 0; r < ctas; ++r) {
-                const Pair e = all[buf][r][l];
+                const Pair e = all[(buf * ctas + r) * LPC + l];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     if (r == rank) s[v] = carry[v];
@@ -720,25 +723,49 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
     }
 }
 
-static int rec_clusters(void (*kernel)(RecParams), const RecParams& p, int64_t strips, int c, int warps, size_t smem, cudaStream_t s) {
-    if (smem > 24 * 1024)                          // with what is static, more than a kernel has unasked
-        if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
-    cudaLaunchConfig_t cfg{};
+static cudaError_t rec_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, void (*kernel)(RecParams), int64_t strips, int c, int warps, size_t smem, cudaStream_t s) {
+    cfg = {};
     cfg.gridDim = dim3((unsigned)(strips * c)); cfg.blockDim = dim3(warps * 32); cfg.stream = s; cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = c; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = c; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
     cfg.numAttrs = 1;
+    if (smem > 24 * 1024)                          // with what is static, more than a kernel has unasked
+        if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
+    return c > 8 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) : cudaSuccess;
+}
+
+static int rec_clusters(void (*kernel)(RecParams), const RecParams& p, int64_t strips, int c, int warps, size_t smem, cudaStream_t s) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    if (const cudaError_t e = rec_config(cfg, attr, kernel, strips, c, warps, smem, s)) return (int)e;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
-// CTAs of a cluster, a power of two (others are placed badly: three took longer than four): the fewest that make `want` of them in all, no more
-// than the sequence has steps for
+// Whether this device places clusters of 16 of a kernel: more than is promised, so it is asked once.
+template <typename T, bool LOGITS, bool BWD, int LPC> bool places_16() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    int k = known[dev].load(std::memory_order_relaxed);
+    if (!k) {
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute attr;
+        int n = 0;
+        auto kernel = rec_tile_kernel<T, LOGITS, BWD, LPC>;
+        const bool yes = rec_config(cfg, attr, kernel, 1, 16, TW, tile_smem<BWD, LPC> + tile_words<LPC, 4 / (int)sizeof(T)>(16), nullptr) == cudaSuccess && cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
+        if (!yes) cudaGetLastError();
+        known[dev].store(k = yes ? 1 : 2, std::memory_order_relaxed);
+    }
+    return k == 1;
+}
+
+// CTAs of a cluster, a power of two up to 8 (others are placed badly: three took longer than four): the fewest that make `want` of them in
+// all, no more than the sequence has steps for
 static int rec_ctas(int64_t strips, int L, int step, int64_t want) {
     int c = 1;
-    while (c < RC && c * strips < want && c * (int64_t)step < L) c *= 2;
+    while (c < 8 && c * strips < want && c * (int64_t)step < L) c *= 2;
     return c;
 }
 
@@ -751,7 +778,7 @@ int rec_strips(const RecParams& p, cudaStream_t s) {
 
 template <typename T, bool LOGITS, bool BWD, int LPC>
 int rec_tiles(const RecParams& p, int64_t strips, int c, cudaStream_t s) {
-    return rec_clusters(rec_tile_kernel<T, LOGITS, BWD, LPC>, p, strips, c, TW, tile_smem<BWD, LPC>, s);
+    return rec_clusters(rec_tile_kernel<T, LOGITS, BWD, LPC>, p, strips, c, TW, tile_smem<BWD, LPC> + tile_words<LPC, 4 / (int)sizeof(T)>(c), s);
 }
 
 // Whether a step over all three or five tensors is a 32-bit number of bytes
@@ -763,7 +790,7 @@ inline bool short_steps(const RecParams& p, bool bwd) {
 
 // Whether all rows are 16-byte pieces
 template <typename T> bool in_pieces(const RecParams& p, bool bwd) {
-    auto fits = [](const void* q, const int64_t* st) { return (uintptr_t)q % 16 == 0 && st[0] * sizeof(T) % 16 == 0 && st[1] * sizeof(T) % 16 == 0; };
+    auto fits = [&](const void* q, const int64_t* st) { return (uintptr_t)q % 16 == 0 && (p.B == 1 || st[0] * sizeof(T) % 16 == 0) && (p.L == 1 || st[1] * sizeof(T) % 16 == 0); };
     return p.D * sizeof(T) % 16 == 0 && fits(p.x, p.sx) && fits(p.g, p.sg) && fits(p.out, p.so) && (!bwd || (fits(p.h_in, p.sh) && fits(p.out_g, p.sog)));
 }
 
@@ -772,7 +799,7 @@ int rec_launch(const RecParams& p, cudaStream_t s) {
     const bool pieces = in_pieces<T>(p, BWD);
     // A strip's CTA is made for 64 tokens and more: below 16 a thread that walks them is as fast (8 x 768 channels, 15 tokens: 3.7 us, 16 in strips
     // 4.8), and below 48 where the strips are more than find room at once (256 x 1024 channels, 16 tokens: 29 us in strips, 9 this way).
-    const int64_t wide = (int64_t)p.B * ((p.D * (int)sizeof(T) + 127) / 128);
+    const int64_t wide = (int64_t)p.B * ((p.D * (int64_t)sizeof(T) + 127) / 128);
     if (p.L < (wide >= 4 * device_sms() ? 48 : 16) || !short_steps(p, BWD)) {
         // 16 bytes a thread once there are threads enough for every SM
         constexpr int V = 16 / (int)sizeof(T);
@@ -786,17 +813,25 @@ int rec_launch(const RecParams& p, cudaStream_t s) {
     }
     if (!pieces) return rec_strips<T, LOGITS, BWD>(p, s);
     // Width of the strips and CTAs of a cluster.  Four CTAs find room on an SM.  Best is the widest strip of which there are enough by
-    // themselves (a cluster's meetings cost: 16 x 4096 x 768 bf16, forward / backward, 62 / 93 us with 32 channels and one CTA, 67 / 102 with 64
-    // and two): 6/10 of the room, for the backward with its five tensors 4.5/10 (24 x 4096 x 768: 288 strips of 64 channels 146 us, 576 of 32
-    // 201, too many rows of memory at once).  Else the widest that reaches 6/10 in clusters (4 x 4096 x 384: 12.8 / 17.8 us with 32 channels and
-    // eight CTAs, 13.6 / 19.2 with 16 and four); else the narrowest (1 x 16384 x 768: 25 / 38 us with 16 channels, 32 / 52 with 32).
-    const int64_t room = 4 * device_sms(), alone = room * (BWD ? 45 : 60) / 100, joined = room * 60 / 100;
+    // themselves, 6/10 of the room (a cluster's meetings cost: 16 x 4096 x 768 bf16, forward, 62 us with 32 channels and one CTA, 66 with 64 and
+    // two); else the widest that reaches that in clusters (4 x 4096 x 384, forward / backward: 12.8 / 17.8 us with 32 channels and eight CTAs,
+    // 13.6 / 19.2 with 16 and four); else the narrowest (1 x 16384 x 768: 25 / 38 us with 16 channels, 31 / 48 with 32).  The backward writes two
+    // tensors, and half rows of them cost once many are under way (24 x 4096 x 768: 203 us with 32 channels, 131 with 64 and two CTAs, 148 with
+    // one; 16 x 4096 x 768: 93 with 32 channels, 104 with 64 and two): strips of 64 channels from 35/100 of the room, narrower ones by themselves
+    // from 45/100.
+    const int64_t room = 4 * device_sms(), joined = room * 60 / 100, alone = BWD ? room * 45 / 100 : joined, whole_rows = BWD ? room * 35 / 100 : joined;
     auto strips = [&](int lpc) { const int w = lpc * (4 / (int)sizeof(T)); return (int64_t)p.B * ((p.D + w - 1) / w); };
     auto ctas = [&](int lpc) { return rec_ctas(strips(lpc), p.L, TW * (32 / lpc) * tile_run<BWD>, joined); };
     int lpc = 0, c = 1;
-    for (int w = 32; w >= 8 && !lpc; w /= 2) if (strips(w) >= alone) lpc = w;
+    if (strips(32) >= whole_rows) { lpc = 32; c = ctas(32); }
+    for (int w = 16; w >= 8 && !lpc; w /= 2) if (strips(w) >= alone) lpc = w;
     for (int w = 32; w >= 8 && !lpc; w /= 2) if (strips(w) * ctas(w) >= joined) { lpc = w; c = ctas(w); }
-    if (!lpc) { lpc = 8; c = ctas(8); }
+    if (!lpc) {
+        lpc = 8;
+        c = ctas(8);
+        // twice as many where they still find room at once (1 x 65536 x 192: 50 / 82 us with eight, 37 / 58 with sixteen)
+        if (c == 8 && 16 * strips(8) <= room && 8ll * TW * 4 * tile_run<BWD> < p.L && places_16<T, LOGITS, BWD, 8>()) c = 16;
+    }
     switch (lpc) {
         case 32: return rec_tiles<T, LOGITS, BWD, 32>(p, strips(32), c, s);
         case 16: return rec_tiles<T, LOGITS, BWD, 16>(p, strips(16), c, s);
@@ -816,7 +851,7 @@ template <bool BWD> int rec_dispatch(const RecParams& p, int dtype, cudaStream_t
 // what every call is asked; token numbers are 32-bit with room for a step behind the last one
 static int rec_check(int B, int L, int D, float norm, int dtype) {
     if (dtype < VIG_DTYPE_F32 || dtype > VIG_DTYPE_F16) return VIG_ERR_DTYPE;
-    if (B < 0 || L < 0 || L >= (1 << 30) || D < 0 || (int64_t)B * D >= (1ll << 31)) return VIG_ERR_SHAPE;
+    if (B < 0 || L < 0 || L >= (1 << 30) || D < 0 || D >= (1 << 28) || (int64_t)B * D >= (1ll << 31)) return VIG_ERR_SHAPE;
     if (norm != 0.f && !(norm >= 1e-30f && norm <= 1e30f)) return VIG_ERR_ARG;
     return VIG_OK;
 }

@@ -75,7 +75,7 @@ void check_rec(const Tensor& x, const Tensor& g, int dim, double norm) {
     want(x.dim() == dim && g.sizes() == x.sizes(), (dim == 3 ? "x and g must be [B, L, D]; got " : "x and g must be [B, D]; got ") + shape_of(x) + " and " + shape_of(g));
     want(unit_last(x) && unit_last(g), "the last dimension of x and g must be contiguous");
     want(norm == 0 || (norm >= 1e-30 && norm <= 1e30), "gate_logit_normalizer must be 0 (log-gates) or positive (raw logits; 1e-30 to 1e30)");
-    want(x.size(0) * x.size(-1) < (1ll << 31) && (dim == 2 || x.size(1) < (1ll << 30)), "B * D must be below 2^31 and L below 2^30");
+    want(x.size(0) * x.size(-1) < (1ll << 31) && x.size(-1) < (1ll << 28) && (dim == 2 || x.size(1) < (1ll << 30)), "B * D must be below 2^31, D below 2^28 and L below 2^30");
 }
 
 void rec_forward(const Tensor& x, const Tensor& g, const Tensor& h0, const Tensor& h, const Tensor& fin, bool reverse, double norm) {
