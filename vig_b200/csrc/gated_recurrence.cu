@@ -824,6 +824,9 @@ int rec_launch(const RecParams& p, cudaStream_t s) {
     auto ctas = [&](int lpc) { return rec_ctas(strips(lpc), p.L, TW * (32 / lpc) * tile_run<BWD>, joined); };
     int lpc = 0, c = 1;
     if (strips(32) >= whole_rows) { lpc = 32; c = ctas(32); }
+    // a few more than find room at once would make a second round of their own: in halves (56 x 1024 x 768, 672 strips of 64 channels: backward 89
+    // us, 79 with 32; 50 x 2048 x 768, 600 strips: forward 98, 88)
+    if (strips(32) > room && strips(32) * 10 <= room * (BWD ? 15 : 11)) { lpc = 16; c = 1; }
     for (int w = 16; w >= 8 && !lpc; w /= 2) if (strips(w) >= alone) lpc = w;
     for (int w = 32; w >= 8 && !lpc; w /= 2) if (strips(w) * ctas(w) >= joined) { lpc = w; c = ctas(w); }
     if (!lpc) {
