@@ -400,6 +400,7 @@ VIG_API int vig_gated_recurrence_bwd(const void* g, const void* h, const float* 
  * `group` channels (32, 64 or 128, dividing N; 0 or N: the row) scale = max|y| / top and q = round(y / scale), top = 448 (e4m3) or 127 (int8);
  * a group of zeros has scale 0.  y is taken from the fp32 sum and is not rounded before q.  x, residual: [rows, N] with row strides ldx,
  * ldr; w: [N] of w_dtype (the rows' dtype or fp32); q: [rows, N] bytes; scales: fp32 [rows, N / group]; residual_out (optional): [rows, N], s.
+ * N < 2^30.
  */
 VIG_API int vig_add_rmsnorm_8bit_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* w, int w_dtype, void* q, float* scales,
                                      void* residual_out, int64_t rows, int N, int group, float eps, int out_type, int dtype, void* stream);

@@ -241,3 +241,30 @@ def test_no_rows_and_refusals():
     call = lambda rows=1, N=64, group=0, dtype=0, wd=0, out=0: L_.vig_add_rmsnorm_8bit_fwd(None, 64, None, 0, None, wd, None, None, None, rows, N, group, 1e-6, out, dtype, None)  # noqa: E731
     assert call() == -1 and call(dtype=5) == -3 and call(wd=1) == -3 and call(rows=-1) == -2 and call(N=0) == -2 and call(rows=0) == 0
     assert call(rows=0, group=48) == -2 and call(rows=0, out=2) == -6
+
+
+@pytest.mark.parametrize("out", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("N", [192, 193, 20000])
+def test_small_scales(N, out):
+    """Rows whose scale is hardly above the smallest normal number, though the norm lifts them by a thousand."""
+    top = 448 if out == torch.float8_e4m3fn else 127
+    x = torch.full((1, N), 2.0 ** -30)
+    x[0, ::2] = 0
+    w = torch.full((N,), 2.0 ** -126 * top * 2.0 ** 21)       # y up to 1.5 times the smallest normal scale's range
+    q, s = vig_b200.add_rmsnorm_8bit(x.cuda(), w.cuda(), eps=1e-6, dtype=out)
+    assert 1.17549435e-38 <= float(s) < 2.4e-38
+    assert (q[0, ::2].float() == 0).all() and (q[0, 1::2].float() == top).all()
+
+
+def test_gradient_of_small_rows_without_eps():
+    """eps = 0 and rows of 1e-15: rstd is 1e15 and its cube out of range, the gradient is not."""
+    x, w, _ = make(3, 64, torch.float32, 4, False)
+    x, dy = x * 1e-15, torch.randn(3, 64, generator=torch.Generator().manual_seed(6))
+    dx, dw = vig_b200.add_rmsnorm_backward(dy.cuda(), x.cuda(), w.cuda(), eps=0.0)
+    r = x.double()
+    rstd = r.square().mean(-1, keepdim=True).rsqrt()
+    t, xh = dy.double() * w.double(), r * rstd
+    m = (t * xh).mean(-1, keepdim=True)
+    rel = rel_rstd(64) + 4 * U
+    assert ((dx.cpu().double() - rstd * (t - xh * m)).abs() <= 4 * rel * rstd * (t.abs() + xh.abs() * (t * xh).abs().mean(-1, keepdim=True))).all()
+    assert ((dw.cpu().double() - (dy.double() * xh).sum(0)).abs() <= (rel + 16 * U) * (dy.double() * xh).abs().sum(0)).all()

@@ -163,7 +163,7 @@ void check_norm(const Tensor& x, const Tensor& w, const Tensor& res) {
     on_gpu(x);
     same_device(w, x, "weight");
     code(x);
-    want(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) < (1ll << 31), "x must be [..., N] with N > 0");
+    want(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) < (1ll << 30), "x must be [..., N] with 0 < N < 2^30");
     want(w.dim() == 1 && w.size(0) == x.size(-1) && w.is_contiguous(), "weight must be a contiguous [N] tensor");
     want_type(w.scalar_type() == x.scalar_type() || w.scalar_type() == at::kFloat, "weight must have x's dtype or float32");
     if (res.defined()) {

@@ -243,18 +243,19 @@ template <int TPR, bool MAX> __device__ __forceinline__ void over_row(float& a, 
     }
 }
 
-template <int OUT, int V> __device__ __forceinline__ void store_codes(uint8_t* row, int vi, int N, int whole, const float* t, float by) {
+template <int OUT, int V> __device__ __forceinline__ void store_codes(uint8_t* row, int vi, int N, int whole, const float* t, float rstd, float inv) {
+    // y first: rstd times the scale's reciprocal may be out of range where neither is
     uint32_t word[V / 4];
 #pragma unroll
     for (int j = 0; j < V / 4; ++j) {
         if (OUT == VIG_OUT_E4M3) {
-            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * j] * by, t[4 * j + 1] * by), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * j + 2] * by, t[4 * j + 3] * by), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * j] * rstd * inv, t[4 * j + 1] * rstd * inv), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * j + 2] * rstd * inv, t[4 * j + 3] * rstd * inv), __NV_SATFINITE, __NV_E4M3);
             word[j] = lo | hi << 16;
         } else {
             word[j] = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) word[j] |= (uint32_t)(uint8_t)(int8_t)__float2int_rn(t[4 * j + i] * by) << (8 * i);
+            for (int i = 0; i < 4; ++i) word[j] |= (uint32_t)(uint8_t)(int8_t)__float2int_rn(t[4 * j + i] * rstd * inv) << (8 * i);
         }
     }
     uint8_t* q = row + vi * V;
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(norm_threads<TPR>) norm_rows_kernel(const Norm
                     o.from_float(v[m]);
                     give<T>(o, (T*)p.y + row * p.N, vi, p.N, p.whole);
                 } else {
-                    store_codes<OUT, V>((uint8_t*)p.y + row * p.N, vi, p.N, p.whole, v[m], rstd * inv);
+                    store_codes<OUT, V>((uint8_t*)p.y + row * p.N, vi, p.N, p.whole, v[m], rstd, inv);
                 }
             }
         }
@@ -357,7 +358,7 @@ __global__ void __launch_bounds__(norm_threads<TPR>) norm_rows_kernel(const Norm
 
 // Backward of the same rows: sum of squares and sum of r w dy in one reduction; a thread's share of dw stays in registers over all of its
 // rows.  The next rows are on their way to shared memory meanwhile (262144 x 192 bf16: 68 us; 81 without rows ahead, 169 with
-// the row ahead in registers).  At the end the CTA's rows of threads are added at the end, and a second launch adds the CTAs' shares in their order.
+// the row ahead in registers).  At the end the CTA's rows of threads are added, and a second launch adds the CTAs' shares in their order.
 template <int TPR> constexpr int norm_bwd_threads = TPR > 256 ? TPR : TPR > 32 ? 256 : 128;
 
 // CTAs of an SM, by the values a thread holds: as many as their registers allow without spilling (262144 x 192 bf16, 24 values: 68 us with 512
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT 
             }
         }
         over_row<TPR, false>(ss, dot, sh, buf);
-        const float rstd = 1.f / sqrtf(ss / (float)p.N + p.eps), c = -dot / (float)p.N * rstd * rstd * rstd;
+        const float rstd = 1.f / sqrtf(ss / (float)p.N + p.eps), c = -dot / (float)p.N * rstd * rstd;
 #pragma unroll
         for (int m = 0; m < VPT; ++m) {
             const int vi = t + m * TPR;
@@ -445,8 +446,9 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT 
                 }
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    acc[m][i] = fmaf(df[i], rf[i] * rstd, acc[m][i]);
-                    o[i] = fmaf(df[i] * wf[m][i], rstd, fmaf(rf[i], c, o[i]));      // rstd (t - xh mean(t xh)) + d_r
+                    const float xh = rf[i] * rstd;
+                    acc[m][i] = fmaf(df[i], xh, acc[m][i]);
+                    o[i] = fmaf(df[i] * wf[m][i], rstd, fmaf(xh, c, o[i]));         // rstd (t - xh mean(t xh)) + d_r
                 }
                 Vec16<T> v;
                 v.from_float(o);
@@ -526,9 +528,10 @@ template <typename T, int OUT> int norm_launch(NormParams p, cudaStream_t s) {
 
 template <typename T, int TPR, int VPT> int norm_bwd_rows(NormBwdParams& p, cudaStream_t s) {
     constexpr int THREADS = norm_bwd_threads<TPR>, RPB = THREADS / TPR;
-    const int64_t need = (p.rows + RPB - 1) / RPB, room = (int64_t)device_sms() * norm_bwd_ctas<TPR, VPT * DType<T>::VEC>;
-    p.blocks = (int)(need < room ? need : room);
     constexpr int smem = norm_bwd_ring<TPR, VPT>;                // more than RPB rows of N values in fp32
+    constexpr int ctas = norm_bwd_ctas<TPR, VPT * DType<T>::VEC>, fit = 227 * 1024 / (smem + 2048);
+    const int64_t need = (p.rows + RPB - 1) / RPB, room = (int64_t)device_sms() * (ctas < fit ? ctas : fit);
+    p.blocks = (int)(need < room ? need : room);
     static_assert(smem >= RPB * TPR * VPT * DType<T>::VEC * 4, "the shares of dw find room where the ring was");
     void (*const kernel)(NormBwdParams) = p.whole ? norm_bwd_rows_kernel<T, TPR, VPT, true> : norm_bwd_rows_kernel<T, TPR, VPT, false>;
     if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return (int)e;
@@ -579,7 +582,7 @@ template <int OUT> int norm_dispatch(const NormParams& p, int dtype, cudaStream_
 
 static int norm_check(const void* x, const void* w, const void* y, int64_t rows, int N, int w_dtype, int dtype) {
     if (dtype < VIG_DTYPE_F32 || dtype > VIG_DTYPE_F16 || (w_dtype != dtype && w_dtype != VIG_DTYPE_F32)) return VIG_ERR_DTYPE;
-    if (rows < 0 || N <= 0) return VIG_ERR_SHAPE;
+    if (rows < 0 || N <= 0 || N >= (1 << 30)) return VIG_ERR_SHAPE;
     if (rows && (!x || !w || !y)) return VIG_ERR_NULL;
     return VIG_OK;
 }

@@ -30,6 +30,8 @@ class GatedRecurrence(nn.Module):
     @torch.no_grad()
     def quantize(self):
         """Lays out the input projection for ``step`` as e4m3 codes with a scale per output channel; weights that change later need another call."""
+        if self.d_model % 16 or 3 * self.d_inner % 16:
+            raise ValueError(f"8-bit products want widths of whole 16s; got {self.d_model} and {self.d_inner}")
         w = self.in_proj.weight.float()
         scale = (w.abs().amax(1) / 448.0).clamp_min(torch.finfo(torch.float32).tiny)
         self._in_8bit = ((w / scale[:, None]).to(torch.float8_e4m3fn), scale)
