@@ -252,3 +252,21 @@ def test_refusals():
         call(g=[torch.zeros(8)])
     with pytest.raises(ValueError):
         vig_b200.AdamW([f(8).requires_grad_(True)], state_bits=4)
+
+
+def test_offsets_beyond_32_bits():
+    """A tensor of more than 2^31 values: its last blocks as a call on them alone gives them, bit for bit."""
+    n, k = (1 << 31) + 1000, 256 * 40 + 1000                  # the tail begins on a block
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    p, g = (torch.empty(n, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2))
+    m, v = (torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+    scales = [torch.zeros((n + 255) // 256, device="cuda") for _ in range(2)]
+    tail = [t[-k:].clone() for t in (p, g, m.view(torch.uint8), v.view(torch.uint8))]
+    tail[2], tail[3] = (t.view(torch.float8_e4m3fn) for t in tail[2:])
+    small = [torch.zeros((k + 255) // 256, device="cuda") for _ in range(2)]
+    for step in (1, 2):
+        vig_b200.adamw_step([p], [g], [m], [v], step, exp_avg_scales=scales[:1], exp_avg_sq_scales=scales[1:])
+        vig_b200.adamw_step(*[[t] for t in tail], step, exp_avg_scales=small[:1], exp_avg_sq_scales=small[1:])
+    assert torch.equal(p[-k:], tail[0])
+    assert torch.equal(m[-k:].view(torch.uint8), tail[2].view(torch.uint8)) and torch.equal(v[-k:].view(torch.uint8), tail[3].view(torch.uint8))
+    assert torch.equal(scales[0][-len(small[0]):], small[0]) and torch.equal(scales[1][-len(small[1]):], small[1])

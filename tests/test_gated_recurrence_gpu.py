@@ -326,3 +326,17 @@ def test_normalizers_that_no_float_holds_are_refused():
     for n in (1e-50, 1e-40, 1e40, float("inf")):
         with pytest.raises(ValueError):
             vig_b200.gated_recurrence(x, x, gate_logit_normalizer=n)
+
+
+@pytest.mark.parametrize("D,reverse", [(1024, False), (1024, True), (1001, False)])
+def test_offsets_beyond_32_bits(D, reverse):
+    """More than 2^31 values: the far end against a call on its last 3000 tokens alone.  With decays of a sigmoid of normal logits 4000 tokens
+    forget what was before them; both calls then round states that agree to 1e-6."""
+    L, n = 2_300_000, 3000
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    x, g = (torch.empty(1, L, D, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2))
+    kw = dict(gate_logit_normalizer=1.0, reverse=reverse)
+    h, _ = vig_b200.gated_recurrence(x, g, **kw)
+    state = None if reverse else vig_b200.gated_recurrence(x[:, -n - 4000:-n], g[:, -n - 4000:-n], None, True, **kw)[1]
+    ref = vig_b200.gated_recurrence(x[:, -n:], g[:, -n:], state, **kw)[0].float()
+    assert ((h[:, -n:].float() - ref).abs() <= 2 * UNIT[torch.bfloat16] * ref.abs() + 1e-5).all()

@@ -268,3 +268,15 @@ def test_gradient_of_small_rows_without_eps():
     rel = rel_rstd(64) + 4 * U
     assert ((dx.cpu().double() - rstd * (t - xh * m)).abs() <= 4 * rel * rstd * (t.abs() + xh.abs() * (t * xh).abs().mean(-1, keepdim=True))).all()
     assert ((dw.cpu().double() - (dy.double() * xh).sum(0)).abs() <= (rel + 16 * U) * (dy.double() * xh).abs().sum(0)).all()
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values: the last rows as a call on them alone gives them, bit for bit (a row's arithmetic does not depend on its place)."""
+    M, N = 2_900_000, 768
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    x, res = (torch.empty(M, N, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2))
+    w = torch.ones(N, dtype=torch.bfloat16, device="cuda")
+    got, ref = vig_b200.add_rmsnorm_8bit(x, w, res, prenorm=True), vig_b200.add_rmsnorm_8bit(x[-40:], w, res[-40:], prenorm=True)
+    assert all(torch.equal(a[-40:].view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, ref))
+    dx, _ = vig_b200.add_rmsnorm_backward(x, got[2], w)
+    assert torch.equal(dx[-40:], vig_b200.add_rmsnorm_backward(x[-40:], got[2][-40:], w)[0])
