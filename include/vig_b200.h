@@ -407,12 +407,12 @@ VIG_API int vig_add_rmsnorm_8bit_fwd(const void* x, int64_t ldx, const void* res
 /* The same norm with y in the rows' dtype, any N and alignment: the forward of a trained norm. */
 VIG_API int vig_add_rmsnorm_train_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* w, int w_dtype, void* y,
                                       void* residual_out, int64_t rows, int N, float eps, int dtype, void* stream);
-/* Its gradients from dy, the sum r (residual_out, or x where there was no residual) and optionally d_r, the gradient of r itself:
- * dx [rows, N] contiguous (of x and of the residual alike) and dw [N] of w_dtype.  Row strides ldy, ldr, ld_dr.  The workspace holds the
- * blocks' shares of dw, which are added in a fixed order. */
+/* Its gradients from dy, x and the residual (NULL where there was none, or where x is their sum already) and optionally d_r, the gradient
+ * of the sum itself: dx [rows, N] contiguous (of x and of the residual alike) and dw [N] of w_dtype.  Row strides ldy, ldx, ldr, ld_dr.  The
+ * workspace holds the blocks' shares of dw, which are added in a fixed order. */
 VIG_API size_t vig_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int N);
-VIG_API int vig_add_rmsnorm_bwd(const void* dy, int64_t ldy, const void* r, int64_t ldr, const void* w, int w_dtype, const void* d_r, int64_t ld_dr,
-                                void* dx, void* dw, int64_t rows, int N, float eps, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+VIG_API int vig_add_rmsnorm_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* w, int w_dtype,
+                                const void* d_r, int64_t ld_dr, void* dx, void* dw, int64_t rows, int N, float eps, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * One AdamW step over `count` tensors: m = b1 m + (1-b1) g, v = b2 v + (1-b2) g^2,

@@ -180,7 +180,7 @@ def test_backward_by_itself_and_strided_gradients():
     leaf = [t.clone().requires_grad_(True) for t in (x, w, res)]
     y, _ = vig_b200.add_rmsnorm_train(*leaf)
     y.sum().backward()                         # a gradient of stride 0
-    ones = vig_b200.add_rmsnorm_backward(torch.ones_like(y), r, w)
+    ones = vig_b200.add_rmsnorm_backward(torch.ones_like(y), x, w, residual=res)         # the sum as the forward had it, in fp32
     assert torch.equal(leaf[0].grad, ones[0]) and torch.equal(leaf[1].grad, ones[1])
 
 

@@ -51,7 +51,7 @@ def test_norm_entries():
     assert fwd() == -1 and fwd(dtype=5) == -3 and fwd(wd=1) == -3 and fwd(rows=-1) == -2 and fwd(N=0) == -2
     assert fwd(rows=0) == 0 and fwd(rows=0, group=48) == -2 and fwd(rows=0, N=40, group=32) == -2 and fwd(rows=0, out=2) == -6
     assert L_.vig_add_rmsnorm_train_fwd(None, 8, None, 0, None, 0, None, None, 1, 8, 1e-6, 0, None) == -1
-    assert L_.vig_add_rmsnorm_bwd(None, 8, None, 8, None, 0, None, 0, None, None, 1, 8, 1e-6, 0, None, 0, None) == -1
+    assert L_.vig_add_rmsnorm_bwd(None, 8, None, 8, None, 0, None, 0, None, 0, None, None, 1, 8, 1e-6, 0, None, 0, None) == -1
     assert L_.vig_add_rmsnorm_bwd_workspace_bytes(0, 64) == 0 and L_.vig_add_rmsnorm_bwd_workspace_bytes(10, 64) >= 64 * 4
 
 

@@ -66,7 +66,7 @@ _SIGNATURES = {
     "vig_add_rmsnorm_8bit_fwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p, c_int] + [c_void_p] * 3 + [c_int64, c_int, c_int, c_float, c_int, c_int, c_void_p]),
     "vig_add_rmsnorm_train_fwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p, c_int] + [c_void_p] * 2 + [c_int64, c_int, c_float, c_int, c_void_p]),
     "vig_add_rmsnorm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int]),
-    "vig_add_rmsnorm_bwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p, c_int] + [c_void_p, c_int64] + [c_void_p] * 2 + [c_int64, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "vig_add_rmsnorm_bwd": (c_int, [c_void_p, c_int64] * 3 + [c_void_p, c_int] + [c_void_p, c_int64] + [c_void_p] * 2 + [c_int64, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
     "vig_adamw_step": (c_int, [c_int] + [POINTER(c_void_p)] * 7 + [_P64] + [POINTER(c_int)] * 2 + [c_int64] + [c_double] * 5 + [c_void_p] * 3),
     "vig_swiglu_fwd": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int64, c_int64, c_int, c_void_p]),
 }

@@ -202,14 +202,14 @@ std::pair<Tensor, Tensor> norm_forward(const Tensor& x_, const Tensor& w, const 
     return {y, r};
 }
 
-std::pair<Tensor, Tensor> norm_backward(const Tensor& dy_, const Tensor& r_, const Tensor& w, const Tensor& dr_, double eps) {
-    const Tensor r = as_rows(r_), dy = as_rows(dy_), dr = dr_.defined() ? as_rows(dr_) : dr_;
-    const Tensor dx = fresh(r_.sizes(), r), dw = fresh(w.sizes(), w);
-    const size_t n = api.vig_add_rmsnorm_bwd_workspace_bytes(r.size(0), (int)r.size(1));
+std::pair<Tensor, Tensor> norm_backward(const Tensor& dy_, const Tensor& x_, const Tensor& res_, const Tensor& w, const Tensor& dr_, double eps) {
+    const Tensor x = as_rows(x_), dy = as_rows(dy_), dr = dr_.defined() ? as_rows(dr_) : dr_, res = res_.defined() ? as_rows(res_) : res_;
+    const Tensor dx = fresh(x_.sizes(), x), dw = fresh(w.sizes(), w);
+    const size_t n = api.vig_add_rmsnorm_bwd_workspace_bytes(x.size(0), (int)x.size(1));
     Tensor ws;
-    if (n) ws = fresh({(int64_t)n}, r, at::kByte);
-    ok(api.vig_add_rmsnorm_bwd(ptr(dy), ld(dy), ptr(r), ld(r), ptr(w), dtype_code(w), ptr(dr), ld(dr), ptr(dx), ptr(dw), r.size(0), (int)r.size(1), (float)eps,
-                               dtype_code(r), ptr(ws), n, stream()), "vig_add_rmsnorm_bwd");
+    if (n) ws = fresh({(int64_t)n}, x, at::kByte);
+    ok(api.vig_add_rmsnorm_bwd(ptr(dy), ld(dy), ptr(x), ld(x), ptr(res), ld(res), ptr(w), dtype_code(w), ptr(dr), ld(dr), ptr(dx), ptr(dw), x.size(0), (int)x.size(1),
+                               (float)eps, dtype_code(x), ptr(ws), n, stream()), "vig_add_rmsnorm_bwd");
     return {dx, dw};
 }
 
@@ -217,7 +217,9 @@ struct Norm : torch::autograd::Function<Norm> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptT& res, double eps) {
         at::AutoDispatchBelowADInplaceOrView guard;
         const auto [y, r] = norm_forward(x, w, get(res), eps);
-        ctx->save_for_backward({r.defined() ? r : x, w});
+        // fp32: the sum, which is what it was; 16 bits: what was added, because the sum was rounded
+        if (r.defined() && r.scalar_type() != at::kFloat) ctx->save_for_backward({x, w, *res});
+        else ctx->save_for_backward({r.defined() ? r : x, w, Tensor()});
         ctx->saved_data["eps"] = eps;
         variable_list out{y};
         if (r.defined()) out.push_back(r);
@@ -226,10 +228,10 @@ struct Norm : torch::autograd::Function<Norm> {
     static variable_list backward(AutogradContext* ctx, variable_list d) {
         const auto saved = ctx->get_saved_variables();
         once(d, saved);
-        const Tensor r = saved[0], w = saved[1];
-        c10::cuda::CUDAGuard dev(r.device());
-        const Tensor dy = d[0].defined() ? d[0] : at::zeros(r.sizes(), r.options());
-        const auto [dx, dw] = norm_backward(dy, r, w, d.size() > 1 ? d[1] : Tensor(), ctx->saved_data["eps"].toDouble());
+        const Tensor x = saved[0], w = saved[1], res = saved[2];
+        c10::cuda::CUDAGuard dev(x.device());
+        const Tensor dy = d[0].defined() ? d[0] : at::zeros(x.sizes(), x.options());
+        const auto [dx, dw] = norm_backward(dy, x, res, w, d.size() > 1 ? d[1] : Tensor(), ctx->saved_data["eps"].toDouble());
         return {dx, dw, d.size() > 1 ? dx : Tensor(), Tensor()};
     }
 };
@@ -247,13 +249,14 @@ std::pair<Tensor, Tensor> add_rmsnorm_train(const Tensor& x, const Tensor& w, co
     return {y, r.defined() ? r : x};
 }
 
-std::pair<Tensor, Tensor> add_rmsnorm_backward(const Tensor& dy, const Tensor& r, const Tensor& w, double eps, const OptT& dr_) {
-    const Tensor dr = get(dr_);
+std::pair<Tensor, Tensor> add_rmsnorm_backward(const Tensor& dy, const Tensor& r, const Tensor& w, double eps, const OptT& dr_, const OptT& res_) {
+    const Tensor dr = get(dr_), res = get(res_);
     check_norm(r, w, dy);
     check_norm(r, w, dr);
+    check_norm(r, w, res);
     want(eps >= 0, "eps must not be negative");
     c10::cuda::CUDAGuard dev(r.device());
-    return norm_backward(dy, r, w, dr, eps);
+    return norm_backward(dy, r, res, w, dr, eps);
 }
 
 // ---- AdamW ----

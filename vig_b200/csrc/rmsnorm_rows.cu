@@ -5,9 +5,10 @@
 // 8 bits: a row, or each group of 32, 64 or 128 channels of it, has the scale s = max|y| / top (448 for e4m3, 127 for int8) and the codes
 // round(y/s); where all of y is zero (or s below the smallest normal number), s and the codes are 0, and a NaN makes s NaN.  y is never rounded to 16 bits on the way.
 // Backward, with t = w dy and xh = r rstd:  dr = rstd (t - xh mean(t xh)) + d_r,  dw = sum over rows of dy xh; rstd is computed again from r.
-// The backward takes r as it was rounded to its type: x and the residual would be two tensors to read instead of one.
+// In 16 bits the backward takes the sum from x and the residual again: r as it was rounded would be one tensor instead of two (8 in all instead
+// of 9, backward 68 us instead of 86), but its roundings stand in dw beside dw's own, 2.5e-3 from 64 bits instead of 1.8e-3 in bf16.
 // Bound by memory: x, residual in, r and one byte a value out; backward dy, r, d_r in, dr out.  131072 x 768 bf16 to e4m3 114 us (6.2 TB/s);
-// 262144 x 192 bf16 forward 65 us (6.2 TB/s), backward 68 us (5.9 TB/s); one row of 768 2.5 us, a launch.
+// 262144 x 192 bf16 forward 65 us (6.2 TB/s), backward 86 us (5.8 TB/s); one row of 768 2.5 us, a launch.
 #include <cuda_fp8.h>
 #include "common.cuh"
 
@@ -26,10 +27,10 @@ struct NormParams {
 };
 
 struct NormBwdParams {
-    const void *dy, *r, *w, *dr;
+    const void *dy, *x, *res, *w, *dr;       // r = x + res (x itself where res is NULL)
     void *dx, *dw;
     float* partial;                  // [blocks][N]
-    int64_t ldy, ldr, lddr, rows;
+    int64_t ldy, ldx, ldr, lddr, rows;
     int N, w_f32, blocks;
     float eps;
     int whole = 0;
@@ -137,12 +138,14 @@ __global__ void __launch_bounds__(NT) norm_bwd_any_kernel(const NormBwdParams p)
     float* part = p.partial + (int64_t)blockIdx.x * p.N;
     for (int i = tid; i < p.N; i += NT) part[i] = 0.f;
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T* r = (const T*)p.r + row * p.ldr;
+        const T* x = (const T*)p.x + row * p.ldx;
+        const T* res = p.res ? (const T*)p.res + row * p.ldr : nullptr;
         const T* dy = (const T*)p.dy + row * p.ldy;
         const T* dr = p.dr ? (const T*)p.dr + row * p.lddr : nullptr;
+        auto sum = [&](int i) { return DType<T>::to_f(x[i]) + (res ? DType<T>::to_f(res[i]) : 0.f); };
         float ss = 0.f, dot = 0.f;
         for (int i = tid; i < p.N; i += NT) {
-            const float v = DType<T>::to_f(r[i]);
+            const float v = sum(i);
             ss = fmaf(v, v, ss);
             dot = fmaf(v, DType<T>::to_f(dy[i]) * weight_at<T>(p.w, i, p.w_f32), dot);
         }
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(NT) norm_bwd_any_kernel(const NormBwdParams p)
         dot = block_sum(dot, sh);
         const float rstd = 1.f / sqrtf(ss / (float)p.N + p.eps), c = dot / (float)p.N * rstd;
         for (int i = tid; i < p.N; i += NT) {
-            const float xh = DType<T>::to_f(r[i]) * rstd, d = DType<T>::to_f(dy[i]);
+            const float xh = sum(i) * rstd, d = DType<T>::to_f(dy[i]);
             part[i] = fmaf(d, xh, part[i]);
             float v = rstd * (d * weight_at<T>(p.w, i, p.w_f32) - xh * c);
             if (dr) v += DType<T>::to_f(dr[i]);
@@ -357,19 +360,21 @@ __global__ void __launch_bounds__(norm_threads<TPR>) norm_rows_kernel(const Norm
 }
 
 // Backward of the same rows: sum of squares and sum of r w dy in one reduction; a thread's share of dw stays in registers over all of its
-// rows.  The next rows are on their way to shared memory meanwhile (262144 x 192 bf16: 68 us; 81 without rows ahead, 169 with
+// rows.  The next rows are on their way to shared memory meanwhile (262144 x 192 bf16, from the sum: 68 us; 81 without rows ahead, 169 with
 // the row ahead in registers).  At the end the CTA's rows of threads are added, and a second launch adds the CTAs' shares in their order.
 template <int TPR> constexpr int norm_bwd_threads = TPR > 256 ? TPR : TPR > 32 ? 256 : 128;
 
-// CTAs of an SM, by the values a thread holds: as many as their registers allow without spilling (262144 x 192 bf16, 24 values: 68 us with 512
+// CTAs of an SM, by the values a thread holds: as many as their registers allow without spilling (the same, 24 values: 68 us with 512
 // threads an SM, 92 with 768 that spill)
 template <int TPR, int VALUES> constexpr int norm_bwd_ctas = TPR > 256 ? 1 : TPR > 32 ? (VALUES <= 16 ? 3 : 2) : VALUES <= 24 ? 4 : 3;
-constexpr int BWD_AHEAD = 2;         // rows of a thread that are under way or at hand
-template <int TPR, int VPT> constexpr int norm_bwd_ring = norm_bwd_threads<TPR> * BWD_AHEAD * 3 * VPT * 16;
+// rows of a thread that are under way or at hand, four tensors each: two where that leaves room for another CTA
+template <int TPR, int VPT> constexpr int norm_bwd_row = norm_bwd_threads<TPR> * 4 * VPT * 16;
+template <int TPR, int VPT> constexpr int norm_bwd_ahead = 2 * norm_bwd_row<TPR, VPT> <= 112 * 1024 ? 2 : 1;
+template <int TPR, int VPT> constexpr int norm_bwd_ring = norm_bwd_ahead<TPR, VPT> * norm_bwd_row<TPR, VPT>;
 
 template <typename T, int TPR, int VPT, bool WHOLE>
 __global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT * DType<T>::VEC>) norm_bwd_rows_kernel(const NormBwdParams p) {
-    constexpr int V = DType<T>::VEC, THREADS = norm_bwd_threads<TPR>, RPB = THREADS / TPR;
+    constexpr int V = DType<T>::VEC, THREADS = norm_bwd_threads<TPR>, RPB = THREADS / TPR, AHEAD = norm_bwd_ahead<TPR, VPT>;
     static_assert(TPR <= 32 || RPB == 1, "a row's threads are part of a warp, or a CTA");
     __shared__ float sh[2 * (THREADS / 32)][2];
     extern __shared__ __align__(16) float share[];               // the ring; at the end [RPB][N]
@@ -386,13 +391,15 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT 
     pdl_launch();
     // whole rows come to shared memory, every thread's vectors into slots of its own; others are read where they are
     const uint8_t* const ring = (const uint8_t*)share + threadIdx.x * 16;
-    const auto slot = [&](int stage, int n, int m) { return ring + ((stage * 3 + n) * VPT + m) * THREADS * 16; };
-    const auto source = [&](int n, int64_t row) { return n == 0 ? (const T*)p.r + row * p.ldr : n == 1 ? (const T*)p.dy + row * p.ldy : (const T*)p.dr + row * p.lddr; };
+    const auto slot = [&](int stage, int n, int m) { return ring + ((stage * 4 + n) * VPT + m) * THREADS * 16; };
+    const auto source = [&](int n, int64_t row) {
+        return n == 0 ? (const T*)p.x + row * p.ldx : n == 1 ? (const T*)p.dy + row * p.ldy : n == 2 ? (const T*)p.dr + row * p.lddr : (const T*)p.res + row * p.ldr;
+    };
     auto bring = [&](int64_t row, int stage) {
         if (WHOLE && row < p.rows) {
 #pragma unroll
-            for (int n = 0; n < 3; ++n) {
-                if (n == 2 && !p.dr) break;
+            for (int n = 0; n < 4; ++n) {
+                if ((n == 2 && !p.dr) || (n == 3 && !p.res)) continue;
                 const T* from = source(n, row);
 #pragma unroll
                 for (int m = 0; m < VPT; ++m)
@@ -404,23 +411,32 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT 
     };
     int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
 #pragma unroll
-    for (int k = 0; k < BWD_AHEAD; ++k) bring(row + k * hop, k);
+    for (int k = 0; k < AHEAD; ++k) bring(row + k * hop, k);
     int stage = 0;
-    for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += hop, row += hop, stage = stage + 1 < BWD_AHEAD ? stage + 1 : 0) {
+    for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += hop, row += hop, stage = stage + 1 < AHEAD ? stage + 1 : 0) {
         const bool in = row < p.rows;
-        asm volatile("cp.async.wait_group %0;" ::"n"(BWD_AHEAD - 1) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
         const auto get = [&](int n, int m, float* f) {
             Vec16<T> v;
             if (WHOLE) v.load((const T*)slot(stage, n, m));
             else take<T>(v, source(n, row), t + m * TPR, p.N, 0);
             v.to_float(f);
         };
+        const auto sum = [&](int m, float* f) {
+            get(0, m, f);
+            if (p.res) {
+                float o[V];
+                get(3, m, o);
+#pragma unroll
+                for (int i = 0; i < V; ++i) f[i] += o[i];
+            }
+        };
         float ss = 0.f, dot = 0.f;
 #pragma unroll
         for (int m = 0; m < VPT; ++m) {
             if (in && t + m * TPR < nv) {
                 float rf[V], df[V];
-                get(0, m, rf);
+                sum(m, rf);
                 get(1, m, df);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -436,7 +452,7 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT 
             const int vi = t + m * TPR;
             if (in && vi < nv) {
                 float rf[V], df[V], o[V];
-                get(0, m, rf);
+                sum(m, rf);
                 get(1, m, df);
                 if (p.dr) {
                     get(2, m, o);
@@ -455,7 +471,7 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT 
                 give<T>(v, (T*)p.dx + row * p.N, vi, p.N, WHOLE);
             }
         }
-        bring(row + BWD_AHEAD * hop, stage);
+        bring(row + AHEAD * hop, stage);
     }
     if (RPB > 1) __syncthreads();                                // the ring's room is taken for the CTA's shares of dw
     float* part = p.partial + (int64_t)blockIdx.x * p.N;
@@ -551,7 +567,7 @@ template <typename T, int TPR> int norm_bwd_rows_launch(NormBwdParams& p, int nv
 template <typename T> int norm_bwd_launch(NormBwdParams p, cudaStream_t s) {
     constexpr int V = DType<T>::VEC;
     const int size = (int)sizeof(T);
-    p.whole = p.N % V == 0 && on_16(p.r, p.ldr, size) && on_16(p.dy, p.ldy, size) && (!p.dr || on_16(p.dr, p.lddr, size)) && on_16(p.w, 0, 1) && on_16(p.dx, 0, 1) &&
+    p.whole = p.N % V == 0 && on_16(p.x, p.ldx, size) && (!p.res || on_16(p.res, p.ldr, size)) && on_16(p.dy, p.ldy, size) && (!p.dr || on_16(p.dr, p.lddr, size)) && on_16(p.w, 0, 1) && on_16(p.dx, 0, 1) &&
                          on_16(p.partial, 0, 1);
     const int nv = (p.N + V - 1) / V, tpr = threads_a_row(nv, 8);
     int e;
@@ -615,13 +631,13 @@ extern "C" size_t vig_add_rmsnorm_bwd_workspace_bytes(int64_t rows, int N) {
     return rows > 0 && N > 0 ? (size_t)norm_blocks(rows) * N * sizeof(float) : 0;
 }
 
-extern "C" int vig_add_rmsnorm_bwd(const void* dy, int64_t ldy, const void* r, int64_t ldr, const void* w, int w_dtype, const void* d_r, int64_t ld_dr,
+extern "C" int vig_add_rmsnorm_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* w, int w_dtype, const void* d_r, int64_t ld_dr,
                                    void* dx, void* dw, int64_t rows, int N, float eps, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-    if (const int e = norm_check(r, w, dx, rows, N, w_dtype, dtype)) return e;
+    if (const int e = norm_check(x, w, dx, rows, N, w_dtype, dtype)) return e;
     if (!dw || (rows && !dy)) return VIG_ERR_NULL;
     if (!rows) return (int)cudaMemsetAsync(dw, 0, (size_t)N * (w_dtype == VIG_DTYPE_F32 ? 4 : 2), (cudaStream_t)stream);
     if (!workspace || workspace_bytes < vig_add_rmsnorm_bwd_workspace_bytes(rows, N)) return VIG_ERR_WORKSPACE;
-    const NormBwdParams p{dy, r, w, d_r, dx, dw, (float*)workspace, ldy, ldr, ld_dr, rows, N, w_dtype == VIG_DTYPE_F32 && dtype != VIG_DTYPE_F32,
+    const NormBwdParams p{dy, x, residual, w, d_r, dx, dw, (float*)workspace, ldy, ldx, ldr, ld_dr, rows, N, w_dtype == VIG_DTYPE_F32 && dtype != VIG_DTYPE_F32,
                           norm_blocks(rows), eps};
     switch (dtype) {
         case VIG_DTYPE_F32: return norm_bwd_launch<float>(p, (cudaStream_t)stream);

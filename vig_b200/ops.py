@@ -702,10 +702,10 @@ def add_rmsnorm_train(x, weight, residual=None, eps=1e-6):
     return _lib.host().add_rmsnorm_train(x, weight, residual, eps)
 
 
-def add_rmsnorm_backward(d_y, r, weight, eps=1e-6, d_r=None):
-    """Gradients of ``add_rmsnorm_train`` at the sum ``r``: ``(dx, dweight)``; ``dx`` is the residual's gradient too.  ``d_r``: what comes to
-    ``r`` from elsewhere."""
-    return _lib.host().add_rmsnorm_backward(d_y, r, weight, eps, d_r)
+def add_rmsnorm_backward(d_y, r, weight, eps=1e-6, d_r=None, residual=None):
+    """Gradients of ``add_rmsnorm_train`` at the sum ``r``, or at ``r + residual`` (taken in fp32: in 16 bits a rounded sum costs the weight's
+    gradient a third of its precision): ``(dx, dweight)``; ``dx`` is the residual's gradient too.  ``d_r``: what comes to the sum from elsewhere."""
+    return _lib.host().add_rmsnorm_backward(d_y, r, weight, eps, d_r, residual)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, masters=None,
