@@ -6,7 +6,7 @@
 // dz_t = dg_t (1 - sigmoid(z_t)) / n,  dh_{-1} = u_0.  States, decays and sums are fp32; h is rounded once, to x's type, and the
 // backward reads h_{t-1} as it was rounded, so that x is not read again.
 // Bound by memory where sequences are many (3 tensors forward: x, g in, h out; 5 backward: g, h, dh in, dx, dg out), and by the MUFU unit
-// beside it: a raw logit of 16 bits is three of its instructions (four backward), 3/4 of its rate at the copy bandwidth.  16 x 4096 x 768 bf16
+// beside it: a raw logit is two of its instructions (three backward) and seven multiply-adds, half of its rate at the copy bandwidth.  16 x 4096 x 768 bf16
 // from raw logits: forward 62 us (4.9 TB/s), backward 91 us (5.5 TB/s); 1 x 16384 x 768, 48 strips on 384 CTAs, 24 us.
 // Three forms, by the rule in rec_launch: rows of 16-byte pieces through shared memory (rec_tile_kernel), rows of any alignment through
 // registers (rec_strip_kernel), few tokens a thread at a time (rec_few_kernel).
@@ -31,10 +31,9 @@ struct RecParams {
     int32_t* status;
 };
 
-// The exponential and logarithm of base two of the MUFU unit, without the scaling that denormal arguments and results would take
-// (decays and their logarithms that small make no difference to a sum in fp32).
+// The exponential of base two of the MUFU unit, without the scaling that denormal arguments and results would take (decays that small make
+// no difference to a sum in fp32).
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 constexpr float LOG2E = 1.4426950408889634f;
 
 // two values at a time where there are two
@@ -60,30 +59,40 @@ template <int V> __device__ __forceinline__ void mul_v(float* d, const float* a,
         d[0] = a[0] * b[0];
 }
 
-// Decays of V tokens' values g, and with REST also d logsigmoid(z) / dz = sigmoid(-z).  16-bit types: one MUFU instruction for a log-gate, three
-// for a raw logit (and one for REST), right to about 2^-21; fp32: the exact functions.
-template <typename T, bool LOGITS, bool REST, int V> __device__ __forceinline__ void decays(const float* g, float inv_norm, float* a, float* rest) {
+// log2(1 + e) = e P(e) for e of 0 to 1, P fitted to the least relative error: 1.4e-6 with 7 terms (16-bit types), 2e-7 with 9 (fp32).  Relative,
+// because a long memory is a small e: the logarithm of the MUFU unit is right to 2^-22 absolute, which at a logit of 9 is 1e-3 of the rate at
+// which the state decays.  It takes as long (the unit is as busy as the multiply-adds: 16 x 4096 x 768 bf16 61 / 95 us with it, 60 / 96 with P).
+template <typename T, int W> __device__ __forceinline__ void log2_1p(float* y, const float* e) {
+    constexpr int N = sizeof(T) == 4 ? 9 : 7;
+    const float c[N] = {1.44269323f, -0.721159458f, 0.477668375f, -0.339089006f, 0.215284511f, -0.0957975239f, 0.0204011761f};
+    const float d[9] = {1.44269502f, -0.721340179f, 0.480692953f, -0.358408481f, 0.275641412f, -0.197118953f, 0.112856172f, -0.0425670482f, 0.00754917832f};
+    float q[W];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (sizeof(T) == 4) {
-            a[v] = expf(LOGITS ? log_sigmoid(g[v]) * inv_norm : g[v]);
-            if (LOGITS && REST) rest[v] = 1.f / (1.f + expf(g[v]));
-        } else if (!LOGITS) {
-            a[v] = ex2(g[v] * LOG2E);
-        }
+    for (int w = 0; w < W; ++w) q[w] = sizeof(T) == 4 ? d[N - 1] : c[N - 1];
+#pragma unroll
+    for (int k = N - 2; k >= 0; --k) {
+        const float ck[2] = {sizeof(T) == 4 ? d[k] : c[k], sizeof(T) == 4 ? d[k] : c[k]};
+        fma_v<W>(q, q, e, ck);
     }
-    if constexpr (sizeof(T) == 2 && LOGITS) {
+    mul_v<W>(y, q, e);
+}
+
+// Decays of V tokens' values g, and with REST also d logsigmoid(z) / dz = sigmoid(-z): one MUFU instruction for a log-gate (fp32: the exact
+// function), two for a raw logit and one for REST.
+template <typename T, bool LOGITS, bool REST, int V> __device__ __forceinline__ void decays(const float* g, float inv_norm, float* a, float* rest) {
+    if constexpr (!LOGITS) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) a[v] = sizeof(T) == 4 ? expf(g[v]) : ex2(g[v] * LOG2E);
+    } else {
         constexpr int W = V > 1 ? 2 : 1;
-        const float l2e[2] = {LOG2E, LOG2E}, one[2] = {1.f, 1.f}, minus[2] = {-1.f, -1.f}, inv[2] = {inv_norm, inv_norm};
+        const float l2e[2] = {LOG2E, LOG2E}, minus[2] = {-1.f, -1.f}, inv[2] = {inv_norm, inv_norm};
 #pragma unroll
         for (int v = 0; v < V; v += W) {
             float z[W], e[W], t[W];
             mul_v<W>(z, g + v, l2e);
 #pragma unroll
-            for (int w = 0; w < W; ++w) e[w] = ex2(-fabsf(z[w]));
-            fma_v<W>(e, e, one, one);
-#pragma unroll
-            for (int w = 0; w < W; ++w) { e[w] = lg2(e[w]); t[w] = fminf(z[w], 0.f); }
+            for (int w = 0; w < W; ++w) { e[w] = ex2(-fabsf(z[w])); t[w] = fminf(z[w], 0.f); }
+            log2_1p<T, W>(e, e);
             fma_v<W>(t, e, minus, t);                            // log2 of the sigmoid: min(z, 0) - log2(1 + 2^-|z|)
             mul_v<W>(e, t, inv);
 #pragma unroll
