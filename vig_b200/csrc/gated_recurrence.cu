@@ -7,7 +7,8 @@
 // backward reads h_{t-1} as it was rounded, so that x is not read again.
 // Bound by memory where sequences are many (3 tensors forward: x, g in, h out; 5 backward: g, h, dh in, dx, dg out), and by the MUFU unit
 // beside it: a raw logit is two of its instructions (three backward) and seven multiply-adds, half of its rate at the copy bandwidth.  16 x 4096 x 768 bf16
-// from raw logits: forward 62 us (4.9 TB/s), backward 91 us (5.5 TB/s); 1 x 16384 x 768, 48 strips on 384 CTAs, 24 us.
+// from raw logits: forward 60 us (5.0 TB/s), backward 93 us (5.4 TB/s); 16 x 2048 x 768 fp32 51 and 81 us (5.9
+// and 6.2 TB/s); 1 x 16384 x 768 bf16, 48 strips on 384 CTAs, 24 us.
 // Three forms, by the rule in rec_launch: rows of 16-byte pieces through shared memory (rec_tile_kernel), rows of any alignment through
 // registers (rec_strip_kernel), few tokens a thread at a time (rec_few_kernel).
 #include <type_traits>
