@@ -390,10 +390,22 @@ VIG_API int vig_gated_recurrence_fwd(const void* x, const void* g, const float* 
                                      int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,
                                      float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream);
 /* Its gradients: from g, the output h, h0 (NULL as in the forward), d_h and d_final (optional, fp32 [B, D]): d_x and d_g ([B, L, D] contiguous;
- * d_g with respect to what g holds) and d_h0 (optional, fp32 [B, D]). */
+ * d_g with respect to what g holds) and d_h0 (optional, fp32 [B, D]).  In 16 bits d_g is taken at h as it was rounded; the two entries behind this
+ * one take it at the states. */
 VIG_API int vig_gated_recurrence_bwd(const void* g, const void* h, const float* h0, const void* d_h, const float* d_final, void* d_x, void* d_g, float* d_h0,
                                      int B, int L, int D, const int64_t* strides_g, const int64_t* strides_h, const int64_t* strides_dh,
                                      float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream);
+
+/* Forward and gradients of a training step in 16 bits (VIG_ERR_DTYPE for fp32, whose h is the states).  The forward also writes `states`,
+ * vig_gated_recurrence_states_bytes of fp32 on 16 bytes (0 bytes, and NULL, for up to eight tokens); the gradients are taken from x and these in the place of h, so
+ * that no rounding of h is in d_g.  Everything else as above. */
+VIG_API size_t vig_gated_recurrence_states_bytes(int B, int L, int D);
+VIG_API int vig_gated_recurrence_train_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final, float* states,
+                                           int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,
+                                           float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream);
+VIG_API int vig_gated_recurrence_train_bwd(const void* g, const void* x, const float* states, const float* h0, const void* d_h, const float* d_final, void* d_x, void* d_g,
+                                           float* d_h0, int B, int L, int D, const int64_t* strides_g, const int64_t* strides_x, const int64_t* strides_dh,
+                                           float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream);
 
 /*
  * Optional residual add and RMSNorm with 8-bit rows out: s = x (+ residual), y = s * rsqrt(mean(s^2) + eps) * w, and for every group of

@@ -63,6 +63,9 @@ _SIGNATURES = {
     "vig_stem_conv_ln_fwd": (c_int, [c_void_p] * 6 + [c_int] * 5 + [c_float, c_int, c_int, c_void_p, c_void_p]),
     "vig_gated_recurrence_fwd": (c_int, [c_void_p] * 3 + [c_int64] + [c_void_p] * 2 + [c_int64] + [c_int] * 3 + [_P64] * 3 + [c_float, c_int, c_int, c_void_p, c_void_p]),
     "vig_gated_recurrence_bwd": (c_int, [c_void_p] * 8 + [c_int] * 3 + [_P64] * 3 + [c_float, c_int, c_int, c_void_p, c_void_p]),
+    "vig_gated_recurrence_states_bytes": (c_size_t, [c_int] * 3),
+    "vig_gated_recurrence_train_fwd": (c_int, [c_void_p] * 3 + [c_int64] + [c_void_p] * 2 + [c_int64, c_void_p] + [c_int] * 3 + [_P64] * 3 + [c_float, c_int, c_int, c_void_p, c_void_p]),
+    "vig_gated_recurrence_train_bwd": (c_int, [c_void_p] * 9 + [c_int] * 3 + [_P64] * 3 + [c_float, c_int, c_int, c_void_p, c_void_p]),
     "vig_add_rmsnorm_8bit_fwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p, c_int] + [c_void_p] * 3 + [c_int64, c_int, c_int, c_float, c_int, c_int, c_void_p]),
     "vig_add_rmsnorm_train_fwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p, c_int] + [c_void_p] * 2 + [c_int64, c_int, c_float, c_int, c_void_p]),
     "vig_add_rmsnorm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int]),

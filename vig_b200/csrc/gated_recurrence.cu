@@ -3,14 +3,17 @@
 //
 // a_t = exp(g_t) from log-gates, or sigmoid(z_t)^(1/n) = exp(logsigmoid(z_t)/n) from raw logits z with n = gate_logit_normalizer.
 // Gradients: u_t = a_t (dh_t + u_{t+1}), the same recurrence from the other end;  dx_t = dh_t + u_{t+1},  dg_t = u_t h_{t-1},
-// dz_t = dg_t (1 - sigmoid(z_t)) / n,  dh_{-1} = u_0.  States, decays and sums are fp32; h is rounded once, to x's type, and the
-// backward reads h_{t-1} as it was rounded, so that x is not read again.
+// dz_t = dg_t (1 - sigmoid(z_t)) / n,  dh_{-1} = u_0.  States, decays and sums are fp32; h is rounded once, to x's type.  The h_{t-1} of
+// the gate gradients: fp32 calls read h.  In 16 bits the forward of a training step leaves the fp32 state in front of every eight tokens
+// (counted from the end of its scan, half a byte a value), and the backward reads x and walks each eight of them again: h as it was rounded
+// costs the gate gradient a third of its precision (2.3e-3 from 64 bits in bf16 instead of 1.7e-3, fp16 2.9e-4 instead of 2.1e-4).
 // Bound by memory where sequences are many (3 tensors forward: x, g in, h out; 5 backward: g, h, dh in, dx, dg out), and by the MUFU unit
 // beside it: a raw logit is two of its instructions (three backward) and seven multiply-adds, half of its rate at the copy bandwidth.  16 x 4096 x 768 bf16
 // from raw logits: forward 60 us (5.0 TB/s), backward 93 us (5.4 TB/s); 16 x 2048 x 768 fp32 51 and 81 us (5.9
 // and 6.2 TB/s); 1 x 16384 x 768 bf16, 48 strips on 384 CTAs, 24 us.
 // Three forms, by the rule in rec_launch: rows of 16-byte pieces through shared memory (rec_tile_kernel), rows of any alignment through
 // registers (rec_strip_kernel), few tokens a thread at a time (rec_few_kernel).
+#include <string.h>
 #include <type_traits>
 #include "tc_common.cuh"
 
@@ -18,7 +21,9 @@ namespace vig {
 
 struct RecParams {
     const void *x, *g;              // backward: x is dh
-    const void* h_in;               // backward: the forward's h
+    const void* h_in;               // backward: the forward's h; with `walk` its x
+    float* states;                  // [B][(L - 1) / 8][D]: state in front of eight tokens, the scan's last eight (but none in front of its first)
+    int keep, walk;                 // forward: write them; backward: h_{t-1} from them and x instead of from h
     const float* s0;                // state that enters the scan: the initial state; backward: d(final)
     const float* h0;                // backward: the forward's initial state
     void* out;                      // h; backward: dx
@@ -30,7 +35,10 @@ struct RecParams {
     float inv_norm;                 // > 0: g holds raw logits
     int from_end;                   // the scan at hand starts at token L-1
     int32_t* status;
+    // Eight tokens that share a state are counted in the order of the backward: tokens 8 j to 8 j + 7 from the end of the forward's scan.
+    __host__ __device__ int64_t groups() const { return (L - 1) / 8; }
 };
+constexpr int GROUP = 8;
 
 // The exponential of base two of the MUFU unit, without the scaling that denormal arguments and results would take (decays that small make
 // no difference to a sum in fp32).
@@ -108,11 +116,14 @@ template <typename T, bool LOGITS, bool REST, int V> __device__ __forceinline__ 
 }
 
 // ---------------------------------------------------------------------------------------------------
-// Few tokens: a thread owns V channels (one, or 16 bytes of them) and walks their tokens, the loads of up to four tokens under way together.
+// Few tokens: a thread owns V channels (one, or 16 bytes of them; the backward of 16 bits 4, for it holds eight tokens' decays and states) and
+// walks their tokens, the loads of up to four or eight tokens under way together.
+template <typename T, bool BWD> constexpr int few_v = (BWD && sizeof(T) == 2 ? 4 : 16) / (int)sizeof(T);
 template <typename T, int V> struct Few {
-    T e[V];
+    alignas(V * sizeof(T)) T e[V];
     __device__ void load(const T* p) {
-        if constexpr (V > 1) *(uint4*)e = *(const uint4*)p;
+        if constexpr (V * sizeof(T) == 16) *(uint4*)e = *(const uint4*)p;
+        else if constexpr (V > 1) *(uint32_t*)e = *(const uint32_t*)p;
         else e[0] = *p;
     }
     __device__ void get(float* f) const {
@@ -123,12 +134,15 @@ template <typename T, int V> struct Few {
         Few o;
 #pragma unroll
         for (int v = 0; v < V; ++v) o.e[v] = DType<T>::from_f(f[v]);
-        if constexpr (V > 1) *(uint4*)p = *(const uint4*)o.e;
+        if constexpr (V * sizeof(T) == 16) *(uint4*)p = *(const uint4*)o.e;
+        else if constexpr (V > 1) *(uint32_t*)p = *(const uint32_t*)o.e;
         else *p = o.e[0];
     }
 };
 template <int V> __device__ __forceinline__ void state_in(float* s, const float* p) {
-    if constexpr (V > 1) {
+    if constexpr (V == 2) {
+        *(float2*)s = *(const float2*)p;
+    } else if constexpr (V > 1) {
 #pragma unroll
         for (int v = 0; v < V; v += 4) *(float4*)(s + v) = *(const float4*)(p + v);
     } else {
@@ -136,7 +150,9 @@ template <int V> __device__ __forceinline__ void state_in(float* s, const float*
     }
 }
 template <int V> __device__ __forceinline__ void state_out(float* p, const float* s) {
-    if constexpr (V > 1) {
+    if constexpr (V == 2) {
+        *(float2*)p = *(const float2*)s;
+    } else if constexpr (V > 1) {
 #pragma unroll
         for (int v = 0; v < V; v += 4) *(float4*)(p + v) = *(const float4*)(s + v);
     } else {
@@ -144,9 +160,10 @@ template <int V> __device__ __forceinline__ void state_out(float* p, const float
     }
 }
 
-template <typename T, bool LOGITS, bool BWD, int V>
+template <typename T, bool LOGITS, bool BWD, bool KEEP, int V>
 __global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
-    constexpr int U = 4;
+    constexpr bool WALKS = BWD && sizeof(T) == 2;
+    constexpr int U = WALKS ? GROUP : 4;
     const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
     const int per = p.D / V;
     if (i >= (int64_t)p.B * per) return;
@@ -157,10 +174,11 @@ __global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
     T* out = (T*)p.out + b * p.so[0] + d;
     T* outg = BWD ? (T*)p.out_g + b * p.sog[0] + d : nullptr;
     auto at = [&](int k) { return (int64_t)(p.from_end ? p.L - 1 - k : k); };
-    float s[V];
+    alignas(4 * V) float s[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) s[v] = 0.f;
     if (p.s0) state_in<V>(s, p.s0 + b * p.ld_s0 + d);
+    const int next = WALKS && p.walk ? 0 : 1;      // token of h_in that belongs to a token
     for (int k0 = 0; k0 < p.L; k0 += U) {
         Few<T, V> xr[U], gr[U], hr[BWD ? U : 1];
 #pragma unroll
@@ -168,38 +186,77 @@ __global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
             if (k0 + u < p.L) {
                 xr[u].load(x + at(k0 + u) * p.sx[1]);
                 gr[u].load(g + at(k0 + u) * p.sg[1]);
-                if (BWD && k0 + u + 1 < p.L) hr[u].load(hin + at(k0 + u + 1) * p.sh[1]);
+                if (BWD && k0 + u + next < p.L) hr[u].load(hin + at(k0 + u + next) * p.sh[1]);
             }
         }
+        if constexpr (WALKS) {
+            const int left = p.L - k0;
+            float a[U][V], rest[U][V], before[U][V], h[V];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (k0 + u >= p.L) break;
-            float xf[V], gf[V], a[V], rest[V];
-            xr[u].get(xf);
-            gr[u].get(gf);
-            decays<T, LOGITS, BWD, V>(gf, p.inv_norm, a, rest);
-            if (!BWD) {
+            for (int v = 0; v < V; ++v) h[v] = 0.f;
+            if (left > U && p.walk) state_in<V>(h, p.states + ((int64_t)b * p.groups() + k0 / U) * p.D + d);
+            else if (left <= U && p.h0) state_in<V>(h, p.h0 + (int64_t)b * p.D + d);
 #pragma unroll
-                for (int v = 0; v < V; ++v) s[v] = fmaf(a[v], s[v], xf[v]);
-                Few<T, V>::store(out + at(k0 + u) * p.so[1], s);
-            } else {
-                float hb[V], og[V];
-                if (k0 + u + 1 < p.L) {
-                    hr[u].get(hb);
-                } else {
+            for (int u = U - 1; u >= 0; --u) {
+                if (u >= left) continue;
+                float gf[V], hf[V];
+                gr[u].get(gf);
+                decays<T, LOGITS, BWD, V>(gf, p.inv_norm, a[u], rest[u]);
+                hr[u].get(hf);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) hb[v] = 0.f;
-                    if (p.h0) state_in<V>(hb, p.h0 + (int64_t)b * p.D + d);
+                for (int v = 0; v < V; ++v) {
+                    before[u][v] = p.walk || u + 1 == left ? h[v] : hf[v];
+                    h[v] = fmaf(a[u][v], h[v], hf[v]);                     // (used where hf is x)
                 }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (u >= left) break;
+                float xf[V], og[V];
+                xr[u].get(xf);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     xf[v] += s[v];
-                    s[v] = a[v] * xf[v];
-                    og[v] = s[v] * hb[v];
-                    if (LOGITS) og[v] *= p.inv_norm * rest[v];
+                    s[v] = a[u][v] * xf[v];
+                    og[v] = s[v] * before[u][v];
+                    if (LOGITS) og[v] *= p.inv_norm * rest[u][v];
                 }
                 Few<T, V>::store(out + at(k0 + u) * p.so[1], xf);
                 Few<T, V>::store(outg + at(k0 + u) * p.sog[1], og);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k0 + u >= p.L) break;
+                float xf[V], gf[V], a[V], rest[V];
+                xr[u].get(xf);
+                gr[u].get(gf);
+                decays<T, LOGITS, BWD, V>(gf, p.inv_norm, a, rest);
+                if (!BWD) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) s[v] = fmaf(a[v], s[v], xf[v]);
+                    Few<T, V>::store(out + at(k0 + u) * p.so[1], s);
+                    const int behind = p.L - 1 - (k0 + u);         // tokens of the scan behind this one
+                    if (KEEP && behind && behind % GROUP == 0) state_out<V>(p.states + ((int64_t)b * p.groups() + behind / GROUP - 1) * p.D + d, s);
+                } else {
+                    float hb[V], og[V];
+                    if (k0 + u + 1 < p.L) {
+                        hr[u].get(hb);
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) hb[v] = 0.f;
+                        if (p.h0) state_in<V>(hb, p.h0 + (int64_t)b * p.D + d);
+                    }
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        xf[v] += s[v];
+                        s[v] = a[v] * xf[v];
+                        og[v] = s[v] * hb[v];
+                        if (LOGITS) og[v] *= p.inv_norm * rest[v];
+                    }
+                    Few<T, V>::store(out + at(k0 + u) * p.so[1], xf);
+                    Few<T, V>::store(outg + at(k0 + u) * p.sog[1], og);
+                }
             }
         }
     }
@@ -244,7 +301,7 @@ constexpr int RC = 8;                 // CTAs of a cluster of this kernel, at mo
 // The product of decays of a stretch of tokens, kept finite: 0 times it stays 0.  (Were a decay NaN, the stretch's contribution is NaN.)
 __device__ __forceinline__ float finite(float a) { return fminf(a, 3.4028235e38f); }
 
-template <typename T, bool LOGITS, bool BWD, int RUN>
+template <typename T, bool LOGITS, bool BWD, bool KEEP, int RUN>
 __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p) {
     constexpr int V = 1;
     using R = typename Raw<T, V>::type;
@@ -281,22 +338,29 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
         carry[v] = live && p.s0 ? p.s0[b * p.ld_s0 + d + v] : 0.f;
         first[v] = BWD && live && p.h0 ? p.h0[(int64_t)b * p.D + d + v] : 0.f;
     }
+    constexpr bool WALKS = BWD && sizeof(T) == 2;
+    static_assert(!BWD || RUN == GROUP, "a thread's tokens share a state");
+    float* const kept = KEEP || (WALKS && p.walk) ? p.states + (int64_t)b * p.groups() * p.D + d : nullptr;
+    const int keeps = (p.L - 1) % GROUP;           // KEEP: which of eight tokens leave their state
+    const int next = WALKS && p.walk ? 0 : 1;      // token of h_in that belongs to a token
     R xn[RUN], gn[RUN], hn[BWD ? RUN : 1];
+    float sn[V] = {};
     auto fetch = [&](int k0) {
         if (!live) return;
         char *px = to(x, k0), *pg = to(g, k0), *ph = to(hin, k0);
+        if (WALKS && p.walk && k0 + RUN < p.L) sn[0] = kept[(int64_t)(k0 / GROUP) * p.D];
         if (k0 + RUN < p.L) {
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
                 xn[i] = *cell(px, x, i);
                 gn[i] = *cell(pg, g, i);
-                if (BWD) hn[i] = *cell(ph, hin, i + 1);
+                if (BWD) hn[i] = *cell(ph, hin, i + next);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
                 if (k0 + i < p.L) { xn[i] = *cell(px, x, i); gn[i] = *cell(pg, g, i); }
-                if (BWD && k0 + i + 1 < p.L) hn[i] = *cell(ph, hin, i + 1);
+                if (BWD && k0 + i + next < p.L) hn[i] = *cell(ph, hin, i + next);
             }
         }
     };
@@ -306,8 +370,8 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
     for (int base = 0, buf = 0; base < p.L; base += per, buf ^= 1) {
         if (ctas > 1 && threadIdx.x == 0) tc::mbar_expect_tx(bar + 8 * buf, ctas * 32 * (uint32_t)sizeof(Pair));
         const int k0 = base + mine, left = live ? p.L - k0 : 0;        // tokens behind the last one leave the state as it is
-        float a[RUN][V], rest[BWD && LOGITS ? RUN : 1][V], A[V], H[V];
-        R xr[RUN], hr[BWD ? RUN : 1];
+        float a[RUN][V], rest[BWD && LOGITS ? RUN : 1][V], A[V], H[V], before[BWD ? RUN : 1][V];
+        R xr[RUN];
 #pragma unroll
         for (int v = 0; v < V; ++v) { A[v] = 1.f; H[v] = 0.f; }
         auto local = [&](auto whole) {
@@ -323,7 +387,7 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
                 }
                 xr[i] = xn[i];
                 if (BWD) {
-                    hr[i] = hn[i];
+                    Raw<T, V>::get(hn[i], before[i]);
 #pragma unroll
                     for (int v = 0; v < V; ++v) H[v] += xf[v];
                     mul_v<V>(H, a[i], H);
@@ -334,6 +398,23 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
             }
         };
         if (left >= RUN) local(std::true_type()); else local(std::false_type());
+        if constexpr (BWD) {
+            // the states ahead of the tokens in the forward's order
+            if (WALKS && p.walk) {
+                float h = left > RUN ? sn[0] : first[0];
+#pragma unroll
+                for (int i = RUN - 1; i >= 0; --i) {
+                    if (i < left) {
+                        const float xi = before[i][0];
+                        before[i][0] = h;
+                        h = fmaf(a[i][0], h, xi);
+                    }
+                }
+            } else if (left <= RUN) {
+#pragma unroll
+                for (int i = 0; i < RUN; ++i) if (i + 1 == left) before[i][0] = first[0];
+            }
+        }
         if (base + per < p.L) fetch(k0 + per);
         Pair me;
 #pragma unroll
@@ -404,17 +485,13 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
                 if (!BWD) {
                     fma_v<V>(s, a[i], s, xf);
                     *cell(po, out, i) = Raw<T, V>::put(s);
+                    if (KEEP && i % GROUP == keeps && (decltype(whole)::value || i + 1 < left)) kept[(int64_t)((p.L - 1 - k0 - i) / GROUP - 1) * p.D] = s[0];
                 } else {
-                    float hf[V];
-                    Raw<T, V>::get(hr[i], hf);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        if (!decltype(whole)::value && i + 1 >= left) hf[v] = first[v];
-                        o[v] = xf[v] + s[v];
-                    }
+                    for (int v = 0; v < V; ++v) o[v] = xf[v] + s[v];
                     mul_v<V>(s, a[i], o);
                     *cell(po, out, i) = Raw<T, V>::put(o);
-                    mul_v<V>(o, s, hf);
+                    mul_v<V>(o, s, before[i]);
                     if (LOGITS) {
 #pragma unroll
                         for (int v = 0; v < V; ++v) o[v] *= p.inv_norm * rest[i][v];
@@ -460,7 +537,7 @@ template <bool BWD, int LPC> constexpr int tile_smem = TW * tile_stages * tile_w
 // ... and of what its warps, or its cluster's CTAs, tell one another (a pair is 8 bytes a channel)
 template <int LPC, int V> int tile_words(int ctas) { return ctas == 1 ? TW * LPC * V * 4 : 2 * (TW + ctas) * LPC * V * 8; }
 
-template <typename T, bool LOGITS, bool BWD, int LPC>
+template <typename T, bool LOGITS, bool BWD, bool KEEP, int LPC>
 __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p) {
     constexpr int V = 4 / (int)sizeof(T), RUN = tile_run<BWD>, NC = 32 / LPC, ROW = LPC * 4, PIECES = ROW / 16, NT = BWD ? 3 : 2;
     constexpr int CHUNK = tile_chunk<LPC, RUN>;
@@ -494,16 +571,19 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
     const bool piece = d0 + pc * (16 / (int)sizeof(T)) < p.D;
     const int pd = piece ? d0 + pc * (16 / (int)sizeof(T)) : 0;
     const Walk src[3] = {walk(p.x, p.sx, pd), walk(p.g, p.sg, pd), BWD ? walk(p.h_in, p.sh, pd) : Walk{}};
+    constexpr bool WALKS = BWD && sizeof(T) == 2;
+    static_assert(!BWD || RUN == GROUP, "a thread's tokens share a state");
+    const int next = WALKS && p.walk ? 0 : 1;      // token of h_in that belongs to a token
     const uint32_t slot = ring + (r0 / RUN) * CHUNK + (r0 % RUN) * ROW + pc * 16;
     constexpr int HOP = 32 / PIECES, AHEAD = HOP / RUN * CHUNK + HOP % RUN * ROW;      // rows from one copy of a lane to its next, and how far that is
     static_assert(HOP % RUN == 0 || RUN % HOP == 0, "a lane's rows are evenly spaced, or lie in one chunk");
     auto bring = [&](int base, int stage) {
         const int k0 = base + first_of_warp;
-        if (k0 + NC * RUN + (BWD ? 1 : 0) <= p.L) {
+        if (k0 + NC * RUN + (BWD ? next : 0) <= p.L) {
             if (piece) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const char* from = src[n].base + (int64_t)(k0 + r0 + (n == 2 ? 1 : 0)) * src[n].step;
+                    const char* from = src[n].base + (int64_t)(k0 + r0 + (n == 2 ? next : 0)) * src[n].step;
 #pragma unroll
                     for (int r = 0; r < NC * RUN / HOP; ++r)
                         copy_16(slot + stage * tile_warp<BWD, LPC> + n * NC * CHUNK + (HOP >= RUN ? r * AHEAD : r / (RUN / HOP) * CHUNK + r % (RUN / HOP) * AHEAD),
@@ -514,7 +594,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 for (int r = 0; r < NC * RUN / HOP; ++r) {
-                    const int row = r * HOP + r0, k = k0 + row + (n == 2 ? 1 : 0);
+                    const int row = r * HOP + r0, k = k0 + row + (n == 2 ? next : 0);
                     if (k < p.L)
                         copy_16(ring + pc * 16 + stage * tile_warp<BWD, LPC> + n * NC * CHUNK + (row / RUN) * CHUNK + (row % RUN) * ROW, src[n].base + (int64_t)k * src[n].step);
                 }
@@ -531,10 +611,27 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
         carry[v] = live && p.s0 ? p.s0[b * p.ld_s0 + d + v] : 0.f;
         first[v] = BWD && live && p.h0 ? p.h0[(int64_t)b * p.D + d + v] : 0.f;
     }
+    float* const kept = KEEP || (WALKS && p.walk) ? p.states + (int64_t)b * p.groups() * p.D + d : nullptr;
+    const int keeps = (p.L - 1) % GROUP;           // KEEP: which of eight tokens leave their state
+    float sn[V] = {};                              // state in front of the thread's tokens, a step ahead
+    auto state_of = [&](int k0) {
+        if (WALKS && p.walk && live && k0 + RUN < p.L) {
+            const float* from = kept + (int64_t)(k0 / GROUP) * p.D;
+            if constexpr (V == 2) *(float2*)sn = *(const float2*)from;
+            else sn[0] = *from;
+        }
+    };
+    state_of(mine);
     uint32_t phase = 0;
     float a[RUN][V], rest[BWD && LOGITS ? RUN : 1][V], A[V], H[V], s[V];
-    const uint8_t* const mine_of_ring = tiles + wid * tile_stages * tile_warp<BWD, LPC> + q * CHUNK + l * 4;
-    auto cell = [&](int stage, int n, int i) { return *(const R*)(mine_of_ring + stage * tile_warp<BWD, LPC> + n * NC * CHUNK + i * ROW); };
+    uint8_t* const mine_of_ring = tiles + wid * tile_stages * tile_warp<BWD, LPC> + q * CHUNK + l * 4;
+    auto place = [&](int stage, int n, int i) { return (uint32_t*)(mine_of_ring + stage * tile_warp<BWD, LPC> + n * NC * CHUNK + i * ROW); };
+    auto cell = [&](int stage, int n, int i) {
+        const uint32_t word = *place(stage, n, i);
+        R r;
+        memcpy(&r, &word, 4);
+        return r;
+    };
     // token i of a step: its decay, and the chunk's pair up to it
     auto enter = [&](int stage, int i, bool in) {
         float gf[V], xf[V];
@@ -553,19 +650,58 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
         }
         mul_v<V>(A, A, a[i]);
     };
+    // 16 bits: the states ahead of the tokens in the forward's order, in the places of what has been used of them (the gate, and h or x)
+    auto before = [&](int stage, int i, int v) { return place(stage, v ? 1 : 2, i); };
+    auto states = [&](int stage, int left) {
+        float h[V], f[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = left > RUN ? sn[v] : first[v];
+        if (p.walk && left >= RUN) {
+            R xs[RUN];
+#pragma unroll
+            for (int i = RUN - 1; i >= 0; --i) xs[i] = cell(stage, 2, i);
+#pragma unroll
+            for (int i = RUN - 1; i >= 0; --i) {
+                Raw<T, V>::get(xs[i], f);
+#pragma unroll
+                for (int v = 0; v < V; ++v) *before(stage, i, v) = __float_as_uint(h[v]);
+                fma_v<V>(h, a[i], h, f);
+            }
+        } else {
+#pragma unroll
+            for (int i = RUN - 1; i >= 0; --i) {
+                if (i >= left) continue;
+                Raw<T, V>::get(cell(stage, 2, i), f);
+                const bool known = p.walk || i + 1 == left;
+#pragma unroll
+                for (int v = 0; v < V; ++v) *before(stage, i, v) = __float_as_uint(known ? h[v] : f[v]);
+                fma_v<V>(h, a[i], h, f);
+            }
+        }
+    };
     // token i of a step: its outputs from the state ahead of it
-    auto leave = [&](int stage, int i, char* po, char* pog, bool last) {
+    auto leave = [&](int stage, int i, char* po, char* pog, bool last, float* keep) {
         float xf[V], o[V];
         Raw<T, V>::get(cell(stage, 0, i), xf);
         if (!BWD) {
             fma_v<V>(s, a[i], s, xf);
             *(R*)(po + (int64_t)i * out.step) = Raw<T, V>::put(s);
+            if (KEEP && i % GROUP == keeps && !last) {
+                float* to = keep - (int64_t)(i / GROUP) * p.D;
+                if constexpr (V == 2) *(float2*)to = make_float2(s[0], s[1]);
+                else *to = s[0];
+            }
         } else {
             float hf[V];
-            Raw<T, V>::get(cell(stage, 2, i), hf);
-            if (last) {
+            if constexpr (WALKS) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) hf[v] = first[v];
+                for (int v = 0; v < V; ++v) hf[v] = __uint_as_float(*before(stage, i, v));
+            } else {
+                Raw<T, V>::get(cell(stage, 2, i), hf);
+                if (last) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) hf[v] = first[v];
+                }
             }
             add_v<V>(o, xf, s);
             mul_v<V>(s, a[i], o);
@@ -657,6 +793,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
                                      ::"r"(at), "r"(__float_as_uint(me.a[0])), "r"(__float_as_uint(me.h[0])), "r"(count) : "memory");
                 }
             if (base) bring(base + (tile_stages - 1) * per, stage ? stage - 1 : tile_stages - 1);      // what the step before has read, while totals are under way
+            if constexpr (WALKS) states(stage, left);
             wait(bar + 8 * buf, (phase >> buf) & 1);
             phase ^= 1u << buf;
 #pragma unroll
@@ -674,6 +811,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
             for (int v = 0; v < V; ++v) s[v] = fmaf(pa[v], s[v], ph[v]);
         } else {
             // from warp to warp, round and round: no barrier, so the warps stay apart and one's arithmetic runs under another's waiting
+            if constexpr (WALKS) states(stage, left);
             if (base || wid) {
                 wait(bar + 8 * wid, (phase >> 2) & 1);
                 phase ^= 4;
@@ -695,6 +833,8 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
         }
         if (LPC < 32) fma_v<V>(s, ea, s, eh);
         char *po = (char*)out.base + (int64_t)k0 * out.step, *pog = (char*)outg.base + (int64_t)k0 * outg.step;
+        float* const keep = kept + (int64_t)((p.L - 1 - k0 - keeps) / GROUP - 1) * p.D;         // where the first token to leave its state does
+        state_of(k0 + per);
         const int ahead = stage + 1 < tile_stages ? stage + 1 : 0;
         const bool more = base + per < p.L;
         asm volatile("cp.async.wait_group %0;" ::"n"(tile_stages - 2) : "memory");
@@ -705,13 +845,13 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
             // multiply-adds and stores (one after the other, the warps of an SM fall into step and leave it idle)
 #pragma unroll
             for (int i = 0; i < RUN; ++i) {
-                leave(stage, i, po, pog, false);
+                leave(stage, i, po, pog, false, keep);
                 enter(ahead, i, true);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < RUN; ++i)
-                if (i < left) leave(stage, i, po, pog, i + 1 == left);
+                if (i < left) leave(stage, i, po, pog, i + 1 == left, keep);
             if (more) {
 #pragma unroll
                 for (int i = 0; i < RUN; ++i) enter(ahead, i, i < left - per);
@@ -754,7 +894,7 @@ static int rec_clusters(void (*kernel)(RecParams), const RecParams& p, int64_t s
 }
 
 // Whether this device places clusters of 16 of a kernel: more than is promised, so it is asked once.
-template <typename T, bool LOGITS, bool BWD, int LPC> bool places_16() {
+template <typename T, bool LOGITS, bool BWD, bool KEEP, int LPC> bool places_16() {
     static std::atomic<int> known[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
@@ -763,7 +903,7 @@ template <typename T, bool LOGITS, bool BWD, int LPC> bool places_16() {
         cudaLaunchConfig_t cfg;
         cudaLaunchAttribute attr;
         int n = 0;
-        auto kernel = rec_tile_kernel<T, LOGITS, BWD, LPC>;
+        auto kernel = rec_tile_kernel<T, LOGITS, BWD, KEEP, LPC>;
         const bool yes = rec_config(cfg, attr, kernel, 1, 16, TW, tile_smem<BWD, LPC> + tile_words<LPC, 4 / (int)sizeof(T)>(16), nullptr) == cudaSuccess && cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
         if (!yes) cudaGetLastError();
         known[dev].store(k = yes ? 1 : 2, std::memory_order_relaxed);
@@ -779,16 +919,16 @@ static int rec_ctas(int64_t strips, int L, int step, int64_t want) {
     return c;
 }
 
-template <typename T, bool LOGITS, bool BWD>
+template <typename T, bool LOGITS, bool BWD, bool KEEP>
 int rec_strips(const RecParams& p, cudaStream_t s) {
     constexpr int RUN = BWD ? 8 : 16;
     const int64_t strips = (int64_t)p.B * ((p.D + 31) / 32);
-    return rec_clusters(rec_strip_kernel<T, LOGITS, BWD, RUN>, p, strips, rec_ctas(strips, p.L, RW * RUN, device_sms()), RW, 0, s);
+    return rec_clusters(rec_strip_kernel<T, LOGITS, BWD, KEEP, RUN>, p, strips, rec_ctas(strips, p.L, RW * RUN, device_sms()), RW, 0, s);
 }
 
-template <typename T, bool LOGITS, bool BWD, int LPC>
+template <typename T, bool LOGITS, bool BWD, bool KEEP, int LPC>
 int rec_tiles(const RecParams& p, int64_t strips, int c, cudaStream_t s) {
-    return rec_clusters(rec_tile_kernel<T, LOGITS, BWD, LPC>, p, strips, c, TW, tile_smem<BWD, LPC> + tile_words<LPC, 4 / (int)sizeof(T)>(c), s);
+    return rec_clusters(rec_tile_kernel<T, LOGITS, BWD, KEEP, LPC>, p, strips, c, TW, tile_smem<BWD, LPC> + tile_words<LPC, 4 / (int)sizeof(T)>(c), s);
 }
 
 // Whether a step over all three or five tensors is a 32-bit number of bytes
@@ -804,24 +944,24 @@ template <typename T> bool in_pieces(const RecParams& p, bool bwd) {
     return p.D * sizeof(T) % 16 == 0 && fits(p.x, p.sx) && fits(p.g, p.sg) && fits(p.out, p.so) && (!bwd || (fits(p.h_in, p.sh) && fits(p.out_g, p.sog)));
 }
 
-template <typename T, bool LOGITS, bool BWD>
+template <typename T, bool LOGITS, bool BWD, bool KEEP = false>
 int rec_launch(const RecParams& p, cudaStream_t s) {
     const bool pieces = in_pieces<T>(p, BWD);
     // A strip's CTA is made for 64 tokens and more: below 16 a thread that walks them is as fast (8 x 768 channels, 15 tokens: 3.7 us, 16 in strips
     // 4.8), and below 48 where the strips are more than find room at once (256 x 1024 channels, 16 tokens: 29 us in strips, 9 this way).
     const int64_t wide = (int64_t)p.B * ((p.D * (int64_t)sizeof(T) + 127) / 128);
     if (p.L < (wide >= 4 * device_sms() ? 48 : 16) || !short_steps(p, BWD)) {
-        // 16 bytes a thread once there are threads enough for every SM
-        constexpr int V = 16 / (int)sizeof(T);
+        // several channels a thread once there are threads enough for every SM
+        constexpr int V = few_v<T, BWD>;
         const int64_t n = (int64_t)p.B * p.D;
         auto state = [](const float* q, int64_t ld) { return (uintptr_t)q % 16 == 0 && ld % 4 == 0; };
         if (pieces && n / V >= 256ll * device_sms() && state(p.s0, p.ld_s0) && state(p.s_end, p.ld_end) && state(p.h0, 0))
-            rec_few_kernel<T, LOGITS, BWD, V><<<(unsigned)((n / V + 127) / 128), 128, 0, s>>>(p);
+            rec_few_kernel<T, LOGITS, BWD, KEEP, V><<<(unsigned)((n / V + 127) / 128), 128, 0, s>>>(p);
         else
-            rec_few_kernel<T, LOGITS, BWD, 1><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
+            rec_few_kernel<T, LOGITS, BWD, KEEP, 1><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
         return (int)cudaGetLastError();
     }
-    if (!pieces) return rec_strips<T, LOGITS, BWD>(p, s);
+    if (!pieces) return rec_strips<T, LOGITS, BWD, KEEP>(p, s);
     // Width of the strips and CTAs of a cluster.  Four CTAs find room on an SM.  Best is the widest strip of which there are enough by
     // themselves, 6/10 of the room (a cluster's meetings cost: 16 x 4096 x 768 bf16, forward, 62 us with 32 channels and one CTA, 66 with 64 and
     // two); else the widest that reaches that in clusters (4 x 4096 x 384, forward / backward: 12.8 / 17.8 us with 32 channels and eight CTAs,
@@ -843,16 +983,20 @@ int rec_launch(const RecParams& p, cudaStream_t s) {
         lpc = 8;
         c = ctas(8);
         // twice as many where they still find room at once (1 x 65536 x 192: 50 / 82 us with eight, 37 / 58 with sixteen)
-        if (c == 8 && 16 * strips(8) <= room && 8ll * TW * 4 * tile_run<BWD> < p.L && places_16<T, LOGITS, BWD, 8>()) c = 16;
+        if (c == 8 && 16 * strips(8) <= room && 8ll * TW * 4 * tile_run<BWD> < p.L && places_16<T, LOGITS, BWD, KEEP, 8>()) c = 16;
     }
     switch (lpc) {
-        case 32: return rec_tiles<T, LOGITS, BWD, 32>(p, strips(32), c, s);
-        case 16: return rec_tiles<T, LOGITS, BWD, 16>(p, strips(16), c, s);
-        default: return rec_tiles<T, LOGITS, BWD, 8>(p, strips(8), c, s);
+        case 32: return rec_tiles<T, LOGITS, BWD, KEEP, 32>(p, strips(32), c, s);
+        case 16: return rec_tiles<T, LOGITS, BWD, KEEP, 16>(p, strips(16), c, s);
+        default: return rec_tiles<T, LOGITS, BWD, KEEP, 8>(p, strips(8), c, s);
     }
 }
 
 template <bool BWD> int rec_dispatch(const RecParams& p, int dtype, cudaStream_t s) {
+    if constexpr (!BWD) if (p.keep) {
+        if (dtype == VIG_DTYPE_BF16) return p.inv_norm > 0.f ? rec_launch<__nv_bfloat16, true, false, true>(p, s) : rec_launch<__nv_bfloat16, false, false, true>(p, s);
+        return p.inv_norm > 0.f ? rec_launch<__half, true, false, true>(p, s) : rec_launch<__half, false, false, true>(p, s);
+    }
     switch (dtype) {
         case VIG_DTYPE_F32: return p.inv_norm > 0.f ? rec_launch<float, true, BWD>(p, s) : rec_launch<float, false, BWD>(p, s);
         case VIG_DTYPE_BF16: return p.inv_norm > 0.f ? rec_launch<__nv_bfloat16, true, BWD>(p, s) : rec_launch<__nv_bfloat16, false, BWD>(p, s);
@@ -875,7 +1019,7 @@ static int rec_empty(const float* s0, int64_t ld0, float* s_end, int64_t ld_end,
     if (!s_end || !n) return VIG_OK;
     RecParams p{};
     p.s0 = s0; p.ld_s0 = ld0; p.s_end = s_end; p.ld_end = ld_end; p.B = B; p.D = D;
-    rec_few_kernel<float, false, false, 1><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
+    rec_few_kernel<float, false, false, false, 1><<<(unsigned)((n + 127) / 128), 128, 0, s>>>(p);
     return (int)cudaGetLastError();
 }
 
@@ -888,14 +1032,27 @@ static void two(int64_t* dst, const int64_t* src, int L, int D) {
 
 using namespace vig;
 
-extern "C" int vig_gated_recurrence_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final,
-                                        int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,
-                                        float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
+extern "C" size_t vig_gated_recurrence_states_bytes(int B, int L, int D) {
+    return B > 0 && L > GROUP && D > 0 ? (size_t)B * ((L - 1) / GROUP) * D * sizeof(float) : 0;
+}
+
+// what a training step of 16-bit tensors is asked beside: room for its states, which several channels of a thread store together
+static int rec_states_check(const float* states, int B, int L, int D, int dtype) {
+    if (dtype == VIG_DTYPE_F32) return VIG_ERR_DTYPE;
+    if (!vig_gated_recurrence_states_bytes(B, L, D)) return VIG_OK;
+    return !states ? VIG_ERR_NULL : (uintptr_t)states % 16 ? VIG_ERR_ALIGN : VIG_OK;
+}
+
+static int rec_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final, float* states, bool keep,
+                   int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,
+                   float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
     if (const int e = rec_check(B, L, D, gate_logit_normalizer, dtype)) return e;
     if (B > 1 && ((h0 && ld_h0 < 0) || (h_final && ld_final < D))) return VIG_ERR_ARG;
     if (!B || !D || !L) return rec_empty(h0, ld_h0, h_final, ld_final, B, D, (cudaStream_t)stream);
     if (!x || !g || !h) return VIG_ERR_NULL;
+    if (keep) if (const int e = rec_states_check(states, B, L, D, dtype)) return e;
     RecParams p{};
+    p.states = states; p.keep = keep && L > GROUP;
     p.x = x; p.g = g; p.s0 = h0; p.ld_s0 = ld_h0; p.out = h; p.s_end = h_final; p.ld_end = ld_final;
     two(p.sx, strides_x, L, D); two(p.sg, strides_g, L, D); two(p.so, strides_h, L, D);
     p.B = B; p.L = L; p.D = D;
@@ -905,13 +1062,15 @@ extern "C" int vig_gated_recurrence_fwd(const void* x, const void* g, const floa
     return rec_dispatch<false>(p, dtype, (cudaStream_t)stream);
 }
 
-extern "C" int vig_gated_recurrence_bwd(const void* g, const void* h, const float* h0, const void* d_h, const float* d_final, void* d_x, void* d_g, float* d_h0,
-                                        int B, int L, int D, const int64_t* strides_g, const int64_t* strides_h, const int64_t* strides_dh,
-                                        float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
+static int rec_bwd(const void* g, const void* h, const float* states, bool walk, const float* h0, const void* d_h, const float* d_final, void* d_x, void* d_g,
+                   float* d_h0, int B, int L, int D, const int64_t* strides_g, const int64_t* strides_h, const int64_t* strides_dh,
+                   float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
     if (const int e = rec_check(B, L, D, gate_logit_normalizer, dtype)) return e;
     if (!B || !D || !L) return rec_empty(d_final, D, d_h0, D, B, D, (cudaStream_t)stream);
     if (!g || !h || !d_h || !d_x || !d_g) return VIG_ERR_NULL;
+    if (walk) if (const int e = rec_states_check(states, B, L, D, dtype)) return e;
     RecParams p{};
+    p.states = const_cast<float*>(states); p.walk = walk;
     p.x = d_h; p.g = g; p.h_in = h; p.h0 = h0; p.s0 = d_final; p.ld_s0 = D; p.out = d_x; p.out_g = d_g; p.s_end = d_h0; p.ld_end = D;
     two(p.sx, strides_dh, L, D); two(p.sg, strides_g, L, D); two(p.sh, strides_h, L, D); two(p.so, nullptr, L, D); two(p.sog, nullptr, L, D);
     p.B = B; p.L = L; p.D = D;
@@ -919,4 +1078,28 @@ extern "C" int vig_gated_recurrence_bwd(const void* g, const void* h, const floa
     p.from_end = reverse == 0;
     p.status = status_dev;
     return rec_dispatch<true>(p, dtype, (cudaStream_t)stream);
+}
+
+extern "C" int vig_gated_recurrence_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final,
+                                        int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,
+                                        float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
+    return rec_fwd(x, g, h0, ld_h0, h, h_final, ld_final, nullptr, false, B, L, D, strides_x, strides_g, strides_h, gate_logit_normalizer, reverse, dtype, status_dev, stream);
+}
+
+extern "C" int vig_gated_recurrence_bwd(const void* g, const void* h, const float* h0, const void* d_h, const float* d_final, void* d_x, void* d_g, float* d_h0,
+                                        int B, int L, int D, const int64_t* strides_g, const int64_t* strides_h, const int64_t* strides_dh,
+                                        float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
+    return rec_bwd(g, h, nullptr, false, h0, d_h, d_final, d_x, d_g, d_h0, B, L, D, strides_g, strides_h, strides_dh, gate_logit_normalizer, reverse, dtype, status_dev, stream);
+}
+
+extern "C" int vig_gated_recurrence_train_fwd(const void* x, const void* g, const float* h0, int64_t ld_h0, void* h, float* h_final, int64_t ld_final, float* states,
+                                              int B, int L, int D, const int64_t* strides_x, const int64_t* strides_g, const int64_t* strides_h,
+                                              float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
+    return rec_fwd(x, g, h0, ld_h0, h, h_final, ld_final, states, true, B, L, D, strides_x, strides_g, strides_h, gate_logit_normalizer, reverse, dtype, status_dev, stream);
+}
+
+extern "C" int vig_gated_recurrence_train_bwd(const void* g, const void* x, const float* states, const float* h0, const void* d_h, const float* d_final, void* d_x, void* d_g,
+                                              float* d_h0, int B, int L, int D, const int64_t* strides_g, const int64_t* strides_x, const int64_t* strides_dh,
+                                              float gate_logit_normalizer, int reverse, int dtype, int32_t* status_dev, void* stream) {
+    return rec_bwd(g, x, states, true, h0, d_h, d_final, d_x, d_g, d_h0, B, L, D, strides_g, strides_x, strides_dh, gate_logit_normalizer, reverse, dtype, status_dev, stream);
 }

@@ -19,7 +19,7 @@ namespace py = pybind11;
     X(vig_stem_fold_fwd) X(vig_stem_unfold_fwd) X(vig_stem_conv_ln_fwd)                   \
     X(vig_stem_conv_ln_supported) X(vig_swiglu_fwd) X(vig_add_layernorm_fwd) X(vig_chain_launches) X(vig_token_mean_fwd) X(vig_embed_conv_ln_fwd) X(vig_linear_pair_preferred) X(vig_linear_pair_fwd) X(vig_conv_proj_preferred) X(vig_conv_proj_fwd) X(vig_block_tail_preferred) X(vig_block_tail_fwd) \
     X(vig_gated_recurrence_fwd) X(vig_gated_recurrence_bwd) X(vig_add_rmsnorm_8bit_fwd) X(vig_add_rmsnorm_train_fwd) X(vig_add_rmsnorm_bwd) \
-    X(vig_add_rmsnorm_bwd_workspace_bytes) X(vig_adamw_step)
+    X(vig_add_rmsnorm_bwd_workspace_bytes) X(vig_adamw_step) X(vig_gated_recurrence_states_bytes) X(vig_gated_recurrence_train_fwd) X(vig_gated_recurrence_train_bwd)
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
     VIG_HOST_API(X)

@@ -78,9 +78,14 @@ void check_rec(const Tensor& x, const Tensor& g, int dim, double norm) {
     want(x.size(0) * x.size(-1) < (1ll << 31) && x.size(-1) < (1ll << 28) && (dim == 2 || x.size(1) < (1ll << 30)), "B * D must be below 2^31, D below 2^28 and L below 2^30");
 }
 
-void rec_forward(const Tensor& x, const Tensor& g, const Tensor& h0, const Tensor& h, const Tensor& fin, bool reverse, double norm) {
+// `states` (16 bits, for a backward): what the gate gradient takes h_{t-1} from
+void rec_forward(const Tensor& x, const Tensor& g, const Tensor& h0, const Tensor& h, const Tensor& fin, bool reverse, double norm, const Tensor& states = {}) {
     const S2 sx(x), sg(g), sh(h);
-    ok(api.vig_gated_recurrence_fwd(ptr(x), ptr(g), (const float*)ptr(h0), h0.defined() ? h0.stride(0) : 0, ptr(h), (float*)ptr(fin), fin.defined() ? fin.stride(0) : 0,
+    if (states.defined())
+        ok(api.vig_gated_recurrence_train_fwd(ptr(x), ptr(g), (const float*)ptr(h0), h0.defined() ? h0.stride(0) : 0, ptr(h), (float*)ptr(fin), fin.defined() ? fin.stride(0) : 0,
+                                              (float*)ptr(states), (int)x.size(0), (int)x.size(1), (int)x.size(2), sx.s, sg.s, sh.s, (float)norm, reverse, dtype_code(x),
+                                              status_ptr(x.get_device()), stream()), "vig_gated_recurrence_train_fwd");
+    else ok(api.vig_gated_recurrence_fwd(ptr(x), ptr(g), (const float*)ptr(h0), h0.defined() ? h0.stride(0) : 0, ptr(h), (float*)ptr(fin), fin.defined() ? fin.stride(0) : 0,
                                     (int)x.size(0), (int)x.size(1), (int)x.size(2), sx.s, sg.s, sh.s, (float)norm, reverse, dtype_code(x), status_ptr(x.get_device()), stream()),
        "vig_gated_recurrence_fwd");
 }
@@ -91,8 +96,11 @@ struct Rec : torch::autograd::Function<Rec> {
         const Tensor h0 = get(h0_), h = fresh(x.sizes(), x);
         Tensor fin;
         if (want_final) fin = fresh({x.size(0), x.size(2)}, x, at::kFloat);
-        rec_forward(x, g, h0, h, fin, reverse, norm);
-        ctx->save_for_backward({g, h, h0});
+        Tensor states;
+        if (x.scalar_type() != at::kFloat)
+            states = fresh({(int64_t)(api.vig_gated_recurrence_states_bytes((int)x.size(0), (int)x.size(1), (int)x.size(2)) / sizeof(float))}, x, at::kFloat);
+        rec_forward(x, g, h0, h, fin, reverse, norm, states);
+        ctx->save_for_backward({g, states.defined() ? x : h, h0, states});
         ctx->saved_data["reverse"] = reverse;
         ctx->saved_data["norm"] = norm;
         variable_list out{h};
@@ -102,7 +110,8 @@ struct Rec : torch::autograd::Function<Rec> {
     static variable_list backward(AutogradContext* ctx, variable_list d) {
         const auto saved = ctx->get_saved_variables();
         once(d, saved);
-        const Tensor g = rows(saved[0]), h = rows(saved[1]), h0 = saved[2].defined() ? saved[2].contiguous() : saved[2];
+        // h, or x where there are states
+        const Tensor g = rows(saved[0]), h = rows(saved[1]), h0 = saved[2].defined() ? saved[2].contiguous() : saved[2], states = saved[3];
         c10::cuda::CUDAGuard dev(g.device());
         const Tensor dh = d[0].defined() ? rows(d[0]) : at::zeros(h.sizes(), h.options());
         const Tensor df = d.size() > 1 && d[1].defined() ? d[1].contiguous() : Tensor();
@@ -110,7 +119,11 @@ struct Rec : torch::autograd::Function<Rec> {
         Tensor d0;
         if (h0.defined()) d0 = fresh(h0.sizes(), h0);
         const S2 sg(g), sh(h), sd(dh);
-        ok(api.vig_gated_recurrence_bwd(ptr(g), ptr(h), (const float*)ptr(h0), ptr(dh), (const float*)ptr(df), ptr(dx), ptr(dg), (float*)ptr(d0), (int)h.size(0),
+        if (states.defined())
+            ok(api.vig_gated_recurrence_train_bwd(ptr(g), ptr(h), (const float*)ptr(states), (const float*)ptr(h0), ptr(dh), (const float*)ptr(df), ptr(dx), ptr(dg), (float*)ptr(d0),
+                                                  (int)h.size(0), (int)h.size(1), (int)h.size(2), sg.s, sh.s, sd.s, (float)ctx->saved_data["norm"].toDouble(),
+                                                  ctx->saved_data["reverse"].toBool(), dtype_code(h), status_ptr(h.get_device()), stream()), "vig_gated_recurrence_train_bwd");
+        else ok(api.vig_gated_recurrence_bwd(ptr(g), ptr(h), (const float*)ptr(h0), ptr(dh), (const float*)ptr(df), ptr(dx), ptr(dg), (float*)ptr(d0), (int)h.size(0),
                                         (int)h.size(1), (int)h.size(2), sg.s, sh.s, sd.s, (float)ctx->saved_data["norm"].toDouble(),
                                         ctx->saved_data["reverse"].toBool(), dtype_code(h), status_ptr(h.get_device()), stream()), "vig_gated_recurrence_bwd");
         return {dx, dg, d0, Tensor(), Tensor(), Tensor()};

@@ -667,7 +667,8 @@ def gated_recurrence(x, g, initial_state=None, output_final_state=False, *, reve
     ``x``, ``g``: ``[B, L, D]`` of one dtype, any strides with a contiguous last dimension.  ``initial_state``: fp32 ``[B, D]``.  Returns
     ``(h, final_state)``, ``h`` in ``x``'s dtype, ``final_state`` fp32 or None.  States and sums are fp32.  Log-gates may be ``-inf`` (the
     state starts anew at that token) and may be positive as long as products of decays over up to 4096 tokens stay in fp32's range.
-    Differentiable in ``x``, ``g`` and ``initial_state``, through both results; the backward reads ``h`` as it was rounded."""
+    Differentiable in ``x``, ``g`` and ``initial_state``, through both results; gate gradients are taken at the fp32 states, not at ``h`` as it was
+    rounded (in 16 bits the backward reads ``x`` and a state for every eight tokens)."""
     args = (x, g, initial_state, output_final_state, reverse, gate_logit_normalizer)
     res = _lib.host().gated_recurrence(*args)
     if res is None:                         # the device's first call
