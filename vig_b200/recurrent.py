@@ -29,20 +29,29 @@ class GatedRecurrence(nn.Module):
 
     @torch.no_grad()
     def quantize(self):
-        """Lays out the input projection for ``step`` as e4m3 codes with a scale per output channel; weights that change later need another call."""
+        """From now on ``step`` takes its input projection in 8 bits: e4m3 codes with a scale per output channel, laid out here and again at the first step
+        behind a change of the weights (an optimizer's step, ``load_state_dict``, ``to``)."""
         if self.d_model % 16 or 3 * self.d_inner % 16:
             raise ValueError(f"8-bit products want widths of whole 16s; got {self.d_model} and {self.d_inner}")
-        w = self.in_proj.weight.float()
-        scale = (w.abs().amax(1) / 448.0).clamp_min(torch.finfo(torch.float32).tiny)
-        self._in_8bit = ((w / scale[:, None]).to(torch.float8_e4m3fn), scale)
+        self._codes()
         return self
+
+    def _codes(self):
+        """The codes and scales of the weights as they are: kept by their version, as the layouts of ``GatedLinearAttention``."""
+        w = self.in_proj.weight
+        key = (w.dtype, w.device, w.data_ptr(), None if w.is_inference() else w._version)
+        if self._in_8bit is None or self._in_8bit[0] != key:
+            w = w.float()
+            scale = (w.abs().amax(1) / 448.0).clamp_min(torch.finfo(torch.float32).tiny)
+            self._in_8bit = (key, (w / scale[:, None]).to(torch.float8_e4m3fn), scale)
+        return self._in_8bit[1:]
 
     @torch.no_grad()
     def step(self, hidden, residual, state):
         """One token: ``hidden``, ``residual`` ``[B, d_model]`` (``residual`` may be None), ``state`` fp32 ``[B, d_inner]``, updated in place.
         Returns ``(output, residual)``."""
         if self._in_8bit is not None:
-            w, w_scale = self._in_8bit
+            w, w_scale = self._codes()
             q, scale, residual = ops.add_rmsnorm_8bit(hidden, self.norm.weight, residual, self.norm.eps, prenorm=True)
             z = torch._scaled_mm(q, w.t(), scale_a=scale, scale_b=w_scale[None], out_dtype=torch.bfloat16).to(hidden.dtype)
         else:
