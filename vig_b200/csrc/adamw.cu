@@ -7,7 +7,7 @@
 // uses m and v before they are rounded.
 // Bound by memory: p, g, m, v in, p, m, v out -- 28 bytes a value in full precision, 16 (and two scales in 256 values) with 16-bit weights, a
 // full-precision copy of them and states in 8 bits.  21 M fp32 values in 168 tensors 94 us (6.4 TB/s), 85 M with 16-bit weights and 8-bit states
-// 225 us (6.1 TB/s), 0.9 M in 28 tensors 8 us.
+// 233 us (5.9 TB/s), 0.9 M in 28 tensors 8 us.
 #include <cuda_fp8.h>
 #include <algorithm>
 #include "common.cuh"
@@ -53,15 +53,20 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float x)
 __device__ __forceinline__ float from_e4m3(uint8_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
 __device__ __forceinline__ uint8_t to_e4m3(float x) { return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
 
-// One value: gradient, states and weight in, states and weight out; returns the root of the new v.  Written so that every path rounds alike.
-__device__ __forceinline__ float adam_value(const AdamScalars& tab, float g, float& m, float& v, float& p) {
+// One value, in two steps: states from the gradient, then the weight; the second returns the root of the new v.  Written so that every path rounds alike.
+__device__ __forceinline__ void adam_moments(const AdamScalars& tab, float g, float& m, float& v) {
     m = fmaf(tab.b1, m, __fmul_rn(tab.c1, g));
     v = fmaf(tab.b2, v, __fmul_rn(tab.c2, __fmul_rn(g, g)));
-    // root and quotient of the MUFU unit, each right to 2^-23 or so of itself: the step is off by that much of itself, the weight by far less.
-    // (A v below the smallest normal number has the root 0: beside eps it makes no difference.)  The exact forms cost four times the
-    // instructions and bound the 8-bit states: 85 M values 270 us with them.
+}
+// Root and quotient of the MUFU unit, each right to 2^-23 or so of itself: the step is off by that much of itself, the weight by far less.
+// The exact forms cost four times the instructions and bound the 8-bit states: 85 M values 270 us with them.  The unit takes a v below the
+// smallest normal number for 0, but without eps, or with one as small, m is divided by its root alone: SMALL takes such a v times 2^64.
+constexpr float SMALLEST = 1.17549435e-38f;
+template <bool SMALL> __device__ __forceinline__ float adam_weight(const AdamScalars& tab, float m, float v, float& p) {
+    const bool small = SMALL && v < SMALLEST;
     float root;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(small ? v * 0x1p64f : v));
+    if (small) root *= 0x1p-32f;
     p = fmaf(p, tab.keep, -__fdividef(__fmul_rn(tab.rate, m), fmaf(root, tab.root, tab.eps)));
     return root;
 }
@@ -158,11 +163,23 @@ __device__ __forceinline__ void adam_whole(const AdamScalars& tab, const AdamTen
                 const float root = __fmul_rn(v[j][k], sv);
                 v[j][k] = __fmul_rn(root, root);
             }
-            const float root = adam_value(tab, __fmul_rn(g[k], gs), m[j][k], v[j][k], w[k]);
-            if (EIGHT) {
-                v[j][k] = root;
+            adam_moments(tab, __fmul_rn(g[k], gs), m[j][k], v[j][k]);
+        }
+        // one branch for four values: 85 M values with 8-bit states 233 us; 254 with a select in each, 225 without either
+        float root[4];
+        if (fminf(fminf(v[j][0], v[j][1]), fminf(v[j][2], v[j][3])) < SMALLEST) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) root[k] = adam_weight<true>(tab, m[j][k], v[j][k], w[k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) root[k] = adam_weight<false>(tab, m[j][k], v[j][k], w[k]);
+        }
+        if (EIGHT) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[j][k] = root[k];
                 top_m = max(top_m, bits_of(m[j][k]));
-                top_v = max(top_v, bits_of(root));
+                top_v = max(top_v, bits_of(root[k]));
             }
         }
         if (t.master) Four<float>::store(t.master, i, w);
@@ -203,7 +220,8 @@ __device__ __noinline__ void adam_any(const AdamScalars& tab, const AdamTensor& 
                 v[j] = ((const float*)t.v)[i];
             }
             float p = t.master ? t.master[i] : load_as(t.p, i, t.pt);
-            const float root = adam_value(tab, __fmul_rn(load_as(t.g, i, t.gt), gs), m[j], v[j], p);
+            adam_moments(tab, __fmul_rn(load_as(t.g, i, t.gt), gs), m[j], v[j]);
+            const float root = adam_weight<true>(tab, m[j], v[j], p);
             if (t.master) t.master[i] = p;
             store_as(t.p, i, t.pt, p);
             if (eight) {
