@@ -192,6 +192,8 @@ std::tuple<Tensor, Tensor, Tensor> add_rmsnorm_8bit(const Tensor& x_, const Tens
     const int64_t N = x_.size(-1);
     want(group == 0 || group == N || ((group == 32 || group == 64 || group == 128) && N % group == 0), "group must be None, or 32, 64 or 128 and divide N");
     want(eps >= 0, "eps must not be negative");
+    // (without a row there is no gradient to lose)
+    if (x_.numel() && wants_grad({&x_, &w, &res0})) not_implemented("add_rmsnorm_8bit has no gradient: use add_rmsnorm_train, or torch.no_grad()");
     c10::cuda::CUDAGuard dev(x_.device());
     const Tensor x = as_rows(x_), res = res0.defined() ? as_rows(res0) : res0;
     auto sizes = x_.sizes().vec();

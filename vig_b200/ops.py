@@ -688,7 +688,8 @@ def add_rmsnorm_8bit(x, weight, residual=None, eps=1e-6, dtype=torch.float8_e4m3
 
     ``q`` (``float8_e4m3fn`` or ``int8``, ``x``'s shape) times ``scales`` (fp32 ``[..., N / group]``; ``group`` None: one scale a row) is the
     normed row; ``scales = max|y| / 448`` (or 127), 0 where all of a group is zero.  ``group``: 32, 64 or 128.  Any N, any row strides.
-    ``weight`` in ``x``'s dtype or fp32.  The norm is taken from the fp32 sum.  No gradient."""
+    ``weight`` in ``x``'s dtype or fp32.  The norm is taken from the fp32 sum.  No gradient: inputs that require one are refused outside
+    ``torch.no_grad()``."""
     try:
         out = OUT_8BIT[dtype]
     except KeyError:
