@@ -43,8 +43,14 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     for (const Tensor* t : ts) if (t->defined() && t->requires_grad()) return true;
     return false;
 }
+// a dual tensor of forward mode, which need not require a gradient: its tangent would be dropped
+void no_tangents(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->defined() && t->_fw_grad(0).defined()) not_implemented("forward-mode gradients are not implemented");
+}
 // runs on a thread of the autograd engine, without Python's lock: a torch error, no Python one
 void once(const variable_list& ds, const variable_list& saved) {
+    for (const Tensor& t : ds) TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "forward-mode gradients are not implemented");
     if (!at::GradMode::is_enabled()) return;
     for (const auto* list : {&ds, &saved})
         for (const Tensor& t : *list) TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t.requires_grad(), "gradients of these gradients are not implemented");
@@ -136,6 +142,7 @@ std::optional<std::pair<Tensor, OptT>> gated_recurrence(const Tensor& x, const T
     if (!status_known(x.get_device())) return std::nullopt;
     const Tensor h0 = get(h0_);
     if (h0.defined()) check_state(h0, x, "initial_state");
+    no_tangents({&x, &g, &h0});
     c10::cuda::CUDAGuard dev(x.device());
     if (wants_grad({&x, &g, &h0})) {
         const auto out = Rec::apply(x, g, h0_, want_final, reverse, norm);
@@ -152,6 +159,7 @@ Tensor gated_recurrence_step(const Tensor& x, const Tensor& g, const Tensor& sta
     check_rec(x, g, 2, norm);
     check_state(state, x, "state");
     want(state.size(0) <= 1 || state.stride(0) >= state.size(1), "the rows of state must not overlap: it is updated in place");
+    no_tangents({&x, &g, &state});
     if (wants_grad({&x, &g, &state})) not_implemented("gated_recurrence_step updates its state in place and has no gradient: use gated_recurrence, or torch.no_grad()");
     c10::cuda::CUDAGuard dev(x.device());
     state.unsafeGetTensorImpl()->bump_version();
@@ -192,6 +200,7 @@ std::tuple<Tensor, Tensor, Tensor> add_rmsnorm_8bit(const Tensor& x_, const Tens
     const int64_t N = x_.size(-1);
     want(group == 0 || group == N || ((group == 32 || group == 64 || group == 128) && N % group == 0), "group must be None, or 32, 64 or 128 and divide N");
     want(eps >= 0, "eps must not be negative");
+    no_tangents({&x_, &w, &res0});
     // (without a row there is no gradient to lose)
     if (x_.numel() && wants_grad({&x_, &w, &res0})) not_implemented("add_rmsnorm_8bit has no gradient: use add_rmsnorm_train, or torch.no_grad()");
     c10::cuda::CUDAGuard dev(x_.device());
@@ -255,6 +264,7 @@ std::pair<Tensor, Tensor> add_rmsnorm_train(const Tensor& x, const Tensor& w, co
     const Tensor res = get(res_);
     check_norm(x, w, res);
     want(eps >= 0, "eps must not be negative");
+    no_tangents({&x, &w, &res});
     c10::cuda::CUDAGuard dev(x.device());
     if (wants_grad({&x, &w, &res})) {
         const auto out = Norm::apply(x, w, res_, eps);
@@ -270,6 +280,7 @@ std::pair<Tensor, Tensor> add_rmsnorm_backward(const Tensor& dy, const Tensor& r
     check_norm(r, w, dr);
     check_norm(r, w, res);
     want(eps >= 0, "eps must not be negative");
+    no_tangents({&dy, &r, &w, &dr, &res});
     c10::cuda::CUDAGuard dev(r.device());
     return norm_backward(dy, r, res, w, dr, eps);
 }
