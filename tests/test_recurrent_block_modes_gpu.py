@@ -54,3 +54,42 @@ def test_8_bit_weights_are_laid_out_once():
     assert block._codes()[0] is codes
     twin = copy.deepcopy(block)
     assert all(torch.equal(a, b) for a, b in zip(served(twin, x), served(block, x)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autocast(dtype):
+    """Three blocks in fp32 under autocast: outputs and gradients of the fp32 run within what 16-bit products and recurrences round (a handful of units
+    a block), the residual stream in fp32; and served, with and without 8-bit products."""
+    torch.manual_seed(0)
+    blocks = torch.nn.ModuleList([vig_b200.GatedRecurrence(64) for _ in range(3)]).cuda()
+    x = torch.randn(2, 40, 64, device="cuda")
+    unit = 2.0 ** (-8 if dtype == torch.bfloat16 else -11)
+
+    def run():
+        h, residual, finals = x, None, []
+        for b in blocks:
+            h, residual, final = b(h, residual, None, True)
+            finals.append(final)
+        return h, residual, finals
+
+    want = run()
+    w = torch.randn_like(x)
+    grads = torch.autograd.grad(((want[0] + want[1]) * w).sum(), list(blocks.parameters()))
+    with torch.autocast("cuda", dtype):
+        h, residual, finals = run()
+    assert h.dtype == dtype and residual.dtype == torch.float32 and all(f.dtype == torch.float32 for f in finals)
+    far = lambda a, b: float((a.float() - b).norm() / b.norm())  # noqa: E731
+    assert far(h + residual, want[0] + want[1]) < 3 * 8 * unit
+    got = torch.autograd.grad(((h + residual) * w).sum(), list(blocks.parameters()))
+    assert all(a.dtype == torch.float32 and far(a, b) < 3 * 16 * unit for a, b in zip(got, grads))
+    for eight in (False, True):
+        if eight:
+            for b in blocks:
+                b.quantize()
+        with torch.no_grad(), torch.autocast("cuda", dtype):
+            states = [torch.zeros(2, 64, device="cuda") for _ in blocks]
+            for t in range(40):
+                h, residual = x[:, t], None
+                for b, s in zip(blocks, states):
+                    h, residual = b.step(h, residual, s)
+        assert far(h + residual, (want[0] + want[1])[:, -1].detach()) < (0.1 if eight else 3 * 8 * unit)

@@ -21,11 +21,17 @@ class GatedRecurrence(nn.Module):
 
     def forward(self, hidden, residual=None, state=None, output_final_state=False):
         """``hidden`` ``[B, L, d_model]`` and the residual stream (None: it begins with ``hidden``); ``state``: fp32 ``[B, d_inner]`` of the tokens
-        before.  Returns ``(output, residual, final_state)``; differentiable."""
+        before.  Returns ``(output, residual, final_state)``; differentiable.  A residual stream in fp32 takes 16-bit branches,
+        as they come out of a block under ``torch.autocast``."""
+        hidden = self._widened(hidden, residual)
         y, residual = ops.add_rmsnorm_train(hidden, self.norm.weight, residual, self.norm.eps)
         x, g, o = self.in_proj(y).chunk(3, -1)
         h, final = ops.gated_recurrence(x, g, state, output_final_state, gate_logit_normalizer=self.gate_logit_normalizer)
         return self.out_proj(h * F.silu(o)), residual, final
+
+    @staticmethod
+    def _widened(hidden, residual):
+        return hidden if residual is None or residual.dtype != torch.float32 else hidden.float()
 
     @torch.no_grad()
     def quantize(self):
@@ -50,6 +56,7 @@ class GatedRecurrence(nn.Module):
     def step(self, hidden, residual, state):
         """One token: ``hidden``, ``residual`` ``[B, d_model]`` (``residual`` may be None), ``state`` fp32 ``[B, d_inner]``, updated in place.
         Returns ``(output, residual)``."""
+        hidden = self._widened(hidden, residual)
         if self._in_8bit is not None:
             w, w_scale = self._codes()
             q, scale, residual = ops.add_rmsnorm_8bit(hidden, self.norm.weight, residual, self.norm.eps, prenorm=True)
