@@ -160,24 +160,16 @@ template <int V> __device__ __forceinline__ void state_out(float* p, const float
     }
 }
 
-template <typename T, bool LOGITS, bool BWD, bool KEEP, int V>
-__global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
+// V channels of a sequence from the state s, token by token
+template <typename T, bool LOGITS, bool BWD, bool KEEP, int V> __device__ __forceinline__ void rec_walk(const RecParams& p, int b, int d, float* s) {
     constexpr bool WALKS = BWD && sizeof(T) == 2;
     constexpr int U = WALKS ? GROUP : 4;
-    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    const int per = p.D / V;
-    if (i >= (int64_t)p.B * per) return;
-    const int b = (int)(i / per), d = (int)(i % per) * V;
     const T* x = (const T*)p.x + b * p.sx[0] + d;
     const T* g = (const T*)p.g + b * p.sg[0] + d;
     const T* hin = BWD ? (const T*)p.h_in + b * p.sh[0] + d : nullptr;
     T* out = (T*)p.out + b * p.so[0] + d;
     T* outg = BWD ? (T*)p.out_g + b * p.sog[0] + d : nullptr;
     auto at = [&](int k) { return (int64_t)(p.from_end ? p.L - 1 - k : k); };
-    alignas(4 * V) float s[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = 0.f;
-    if (p.s0) state_in<V>(s, p.s0 + b * p.ld_s0 + d);
     const int next = WALKS && p.walk ? 0 : 1;      // token of h_in that belongs to a token
     for (int k0 = 0; k0 < p.L; k0 += U) {
         Few<T, V> xr[U], gr[U], hr[BWD ? U : 1];
@@ -263,6 +255,26 @@ __global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
     if (p.s_end) state_out<V>(p.s_end + b * p.ld_end + d, s);
 }
 
+template <typename T, bool LOGITS, bool BWD, bool KEEP, int V>
+__global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
+    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    const int per = p.D / V;
+    if (i >= (int64_t)p.B * per) return;
+    const int b = (int)(i / per), d = (int)(i % per) * V;
+    alignas(4 * V) float s[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = 0.f;
+    if (p.s0) state_in<V>(s, p.s0 + b * p.ld_s0 + d);
+    rec_walk<T, LOGITS, BWD, KEEP, V>(p, b, d, s);
+}
+
+// Long sequences are joined from stretches of tokens, and a stretch's product of decays can be 0 in fp32 where none of them is: an infinite state would
+// become NaN over it.  A CTA that met an infinite state (which costs a maximum a step to know) walks that channel again when it is done, by one thread.
+template <typename T, bool LOGITS, bool BWD, bool KEEP> __device__ __noinline__ void rec_again(const RecParams& p, int b, int d, float s) {
+    rec_walk<T, LOGITS, BWD, KEEP, 1>(p, b, d, &s);
+}
+constexpr float INFINITE = __builtin_huge_valf();
+
 // ---------------------------------------------------------------------------------------------------
 // Rows of any alignment.  A cluster of CTAs owns a strip of 32 channels of one sequence and walks it in steps of (CTAs x 8 warps x RUN)
 // tokens.  A warp's lanes are channels, a thread holds RUN consecutive tokens of its channel in registers.  In a step every
@@ -302,13 +314,15 @@ constexpr int RC = 8;                 // CTAs of a cluster of this kernel, at mo
 __device__ __forceinline__ float finite(float a) { return fminf(a, 3.4028235e38f); }
 
 template <typename T, bool LOGITS, bool BWD, bool KEEP, int RUN>
-__global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p) {
+__global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const __grid_constant__ RecParams p) {
     constexpr int V = 1;
     using R = typename Raw<T, V>::type;
     struct alignas(8 * V) Pair { float a[V], h[V]; };                 // product of decays and contribution of a stretch of tokens
     __shared__ Pair own[2][RW][32];                // of each warp's tokens
     __shared__ Pair all[2][RC][32];                // of each CTA's
     __shared__ uint64_t landed[2];                 // counts the bytes of `all`
+    __shared__ float begun[32];                    // the state that entered, and whether one was infinite: for a CTA that walks again
+    __shared__ bool met[32];
     const uint32_t rank = tc::cluster_rank(), ctas = tc::cluster_size(), bar = tc::smem_u32(landed);
     if (ctas > 1) {
         if (threadIdx.x == 0) {
@@ -343,6 +357,8 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
     float* const kept = KEEP || (WALKS && p.walk) ? p.states + (int64_t)b * p.groups() * p.D + d : nullptr;
     const int keeps = (p.L - 1) % GROUP;           // KEEP: which of eight tokens leave their state
     const int next = WALKS && p.walk ? 0 : 1;      // token of h_in that belongs to a token
+    if (wid == 0) { begun[lane] = carry[0]; met[lane] = false; }
+    float most = 0.f;                              // the largest magnitude of a state or a contribution
     R xn[RUN], gn[RUN], hn[BWD ? RUN : 1];
     float sn[V] = {};
     auto fetch = [&](int k0) {
@@ -475,6 +491,7 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
                 }
             }
         }
+        most = fmaxf(most, fmaxf(fabsf(s[0]), fabsf(H[0])));
         char *po = to(out, k0), *pog = to(outg, k0);
         auto outputs = [&](auto whole) {
 #pragma unroll
@@ -508,10 +525,14 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const RecParams p
         }
     }
     // no CTA leaves while another may still write to it (one that gave up waiting)
+    __syncthreads();                               // (the marks are clear)
+    if (most == INFINITE) met[lane] = true;
+    __syncthreads();
     if (ctas > 1) {
-        asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-        asm volatile("barrier.cluster.wait;" ::: "memory");
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     }
+    if (wid == 0 && live && met[lane]) rec_again<T, LOGITS, BWD, KEEP>(p, b, d, begun[lane]);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -538,12 +559,14 @@ template <bool BWD, int LPC> constexpr int tile_smem = TW * tile_stages * tile_w
 template <int LPC, int V> int tile_words(int ctas) { return ctas == 1 ? TW * LPC * V * 4 : 2 * (TW + ctas) * LPC * V * 8; }
 
 template <typename T, bool LOGITS, bool BWD, bool KEEP, int LPC>
-__global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p) {
+__global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const __grid_constant__ RecParams p) {
     constexpr int V = 4 / (int)sizeof(T), RUN = tile_run<BWD>, NC = 32 / LPC, ROW = LPC * 4, PIECES = ROW / 16, NT = BWD ? 3 : 2;
     constexpr int CHUNK = tile_chunk<LPC, RUN>;
     using R = typename Raw<T, V>::type;
     struct alignas(8 * V) Pair { float a[V], h[V]; };
     extern __shared__ __align__(128) uint8_t tiles[];
+    __shared__ float begun[LPC * V];               // the state that entered, and whether one was infinite: for a CTA that walks again
+    __shared__ bool met[LPC * V];
     __shared__ uint64_t landed[TW];                // one CTA: one a warp, its mail is there; several: 0 and 1 count the bytes of `all`
     const uint32_t rank = tc::cluster_rank(), ctas = tc::cluster_size(), bar = tc::smem_u32(landed);
     // behind the tiles, one CTA: the state ahead of each warp's tokens, from the warp before; several: the pair of each warp's tokens and of each
@@ -622,6 +645,11 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
         }
     };
     state_of(mine);
+    if (threadIdx.x < LPC) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) { begun[l * V + v] = carry[v]; met[l * V + v] = false; }
+    }
+    float most[V] = {};                            // the largest magnitude of a state or a contribution
     uint32_t phase = 0;
     float a[RUN][V], rest[BWD && LOGITS ? RUN : 1][V], A[V], H[V], s[V];
     uint8_t* const mine_of_ring = tiles + wid * tile_stages * tile_warp<BWD, LPC> + q * CHUNK + l * 4;
@@ -832,6 +860,8 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
             }
         }
         if (LPC < 32) fma_v<V>(s, ea, s, eh);
+#pragma unroll
+        for (int v = 0; v < V; ++v) most[v] = fmaxf(most[v], fmaxf(fabsf(s[v]), fabsf(H[v])));
         char *po = (char*)out.base + (int64_t)k0 * out.step, *pog = (char*)outg.base + (int64_t)k0 * outg.step;
         float* const keep = kept + (int64_t)((p.L - 1 - k0 - keeps) / GROUP - 1) * p.D;         // where the first token to leave its state does
         state_of(k0 + per);
@@ -867,10 +897,15 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const RecParams p)
         stage = ahead;
     }
     // no CTA leaves while another may still write to it (one that gave up waiting)
+    __syncthreads();                               // (the marks are clear)
+#pragma unroll
+    for (int v = 0; v < V; ++v) if (most[v] == INFINITE) met[l * V + v] = true;
+    __syncthreads();
     if (ctas > 1) {
-        asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-        asm volatile("barrier.cluster.wait;" ::: "memory");
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     }
+    if (threadIdx.x < LPC * V && d0 + threadIdx.x < p.D && met[threadIdx.x]) rec_again<T, LOGITS, BWD, KEEP>(p, b, d0 + (int)threadIdx.x, begun[threadIdx.x]);
 }
 
 static cudaError_t rec_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, void (*kernel)(RecParams), int64_t strips, int c, int warps, size_t smem, cudaStream_t s) {
