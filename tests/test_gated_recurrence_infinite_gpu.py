@@ -57,3 +57,28 @@ def test_infinite_initial_state():
     g[:, 1000] = float("-inf")
     h, final = vig_b200.gated_recurrence(x, g, h0, True)
     assert torch.isposinf(h[:, :1000]).all() and torch.isnan(h[:, 1000:]).all() and torch.isnan(final).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,D", [(2, 200, 64), (1, 3000, 33), (64, 400, 768)])
+def test_what_is_finite_keeps_its_bits(B, L, D, dtype):
+    """An infinity changes nothing ahead of itself and in no other channel, forward and in the gradients."""
+    gen = torch.Generator(device="cuda").manual_seed(L)
+    x, d_h = (torch.randn(B, L, D, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    g = (-torch.rand(B, L, D, generator=gen, device="cuda")).to(dtype)
+
+    def run(x, d_h):
+        leaf = [x.clone().requires_grad_(True), g.clone().requires_grad_(True)]
+        h, final = vig_b200.gated_recurrence(*leaf, None, True)
+        return (h.detach(), final.detach(), *torch.autograd.grad(h, leaf, d_h))
+
+    h, final, dx, dg = run(x, d_h)
+    n = L // 2
+    x2, d2 = x.clone(), d_h.clone()
+    x2[:, n, 5], d2[:, n, 9] = float("inf"), float("-inf")
+    h2, final2, dx2, dg2 = run(x2, d2)
+    assert torch.isposinf(h2[:, n:, 5]).all() and torch.isposinf(final2[:, 5]).all() and torch.isneginf(dx2[:, :n + 1, 9]).all()
+    assert not torch.isfinite(dg2[:, n + 1:, 5]).any() and not torch.isfinite(dg2[:, 1:n + 1, 9]).any()
+    h2[:, n:, 5], final2[:, 5], dx2[:, :n + 1, 9] = h[:, n:, 5], final[:, 5], dx[:, :n + 1, 9]
+    dg2[:, n + 1:, 5], dg2[:, :n + 1, 9] = dg[:, n + 1:, 5], dg[:, :n + 1, 9]
+    assert all(torch.equal(a, b) for a, b in zip((h2, final2, dx2, dg2), (h, final, dx, dg)))

@@ -160,8 +160,9 @@ template <int V> __device__ __forceinline__ void state_out(float* p, const float
     }
 }
 
-// V channels of a sequence from the state s, token by token
-template <typename T, bool LOGITS, bool BWD, bool KEEP, int V> __device__ __forceinline__ void rec_walk(const RecParams& p, int b, int d, float* s) {
+// V channels of a sequence from the state s, token by token.  AGAIN: only what is not finite is written, the rest is there.
+template <typename T, bool LOGITS, bool BWD, bool KEEP, int V, bool AGAIN = false> __device__ __forceinline__ void rec_walk(const RecParams& p, int b, int d, float* s) {
+    auto writes = [](float value) { return !AGAIN || !(fabsf(value) <= 3.4028235e38f); };
     constexpr bool WALKS = BWD && sizeof(T) == 2;
     constexpr int U = WALKS ? GROUP : 4;
     const T* x = (const T*)p.x + b * p.sx[0] + d;
@@ -213,8 +214,10 @@ template <typename T, bool LOGITS, bool BWD, bool KEEP, int V> __device__ __forc
                     og[v] = s[v] * before[u][v];
                     if (LOGITS) og[v] *= p.inv_norm * rest[u][v];
                 }
-                Few<T, V>::store(out + at(k0 + u) * p.so[1], xf);
-                Few<T, V>::store(outg + at(k0 + u) * p.sog[1], og);
+                if (writes(xf[0])) {
+                    Few<T, V>::store(out + at(k0 + u) * p.so[1], xf);
+                    Few<T, V>::store(outg + at(k0 + u) * p.sog[1], og);
+                }
             }
         } else {
 #pragma unroll
@@ -227,6 +230,7 @@ template <typename T, bool LOGITS, bool BWD, bool KEEP, int V> __device__ __forc
                 if (!BWD) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) s[v] = fmaf(a[v], s[v], xf[v]);
+                    if (!writes(s[0])) continue;
                     Few<T, V>::store(out + at(k0 + u) * p.so[1], s);
                     const int behind = p.L - 1 - (k0 + u);         // tokens of the scan behind this one
                     if (KEEP && behind && behind % GROUP == 0) state_out<V>(p.states + ((int64_t)b * p.groups() + behind / GROUP - 1) * p.D + d, s);
@@ -246,13 +250,14 @@ template <typename T, bool LOGITS, bool BWD, bool KEEP, int V> __device__ __forc
                         og[v] = s[v] * hb[v];
                         if (LOGITS) og[v] *= p.inv_norm * rest[v];
                     }
+                    if (!writes(xf[0])) continue;
                     Few<T, V>::store(out + at(k0 + u) * p.so[1], xf);
                     Few<T, V>::store(outg + at(k0 + u) * p.sog[1], og);
                 }
             }
         }
     }
-    if (p.s_end) state_out<V>(p.s_end + b * p.ld_end + d, s);
+    if (p.s_end && writes(s[0])) state_out<V>(p.s_end + b * p.ld_end + d, s);
 }
 
 template <typename T, bool LOGITS, bool BWD, bool KEEP, int V>
@@ -269,9 +274,10 @@ __global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
 }
 
 // Long sequences are joined from stretches of tokens, and a stretch's product of decays can be 0 in fp32 where none of them is: an infinite state would
-// become NaN over it.  A CTA that met an infinite state (which costs a maximum a step to know) walks that channel again when it is done, by one thread.
+// become NaN over it.  A CTA that met an infinite state (which costs a maximum a step to know) walks that channel again when it is done, by one
+// thread.  (Ahead of its infinity nothing changes: a state that is no number, or infinite, stays so.)
 template <typename T, bool LOGITS, bool BWD, bool KEEP> __device__ __noinline__ void rec_again(const RecParams& p, int b, int d, float s) {
-    rec_walk<T, LOGITS, BWD, KEEP, 1>(p, b, d, &s);
+    rec_walk<T, LOGITS, BWD, KEEP, 1, true>(p, b, d, &s);
 }
 constexpr float INFINITE = __builtin_huge_valf();
 
