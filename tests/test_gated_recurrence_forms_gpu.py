@@ -178,3 +178,17 @@ def test_states_refusals():
     bwd = lambda states, dtype=1: lib.vig_gated_recurrence_train_bwd(p(x), p(x), states, None, p(x), None, p(x), p(x), None, 1, 20, 8, None, None, None, 0.0, 0, dtype, None, _lib.stream_ptr())  # noqa: E731
     for call in (fwd, bwd):
         assert call(None) == -1 and call(st.data_ptr() + 4) == -4 and call(st.data_ptr(), 0) == -3
+
+
+@pytest.mark.parametrize("B,L,D,dtype", [(3, 1, 64, 1), (2, 9, 100, 2), (1, 20000, 96, 1), (2, 5000, 97, 2), (4, 1101, 384, 1), (40, 300, 768, 0), (3, 700, 96, 0)])
+@pytest.mark.parametrize("reverse", [0, 1])
+def test_c_state_in_place(B, L, D, dtype, reverse):
+    """The final state where the initial one was, over one CTA and over clusters of which one writes it: the bits of two buffers."""
+    from vig_b200 import _lib
+    lib, p = _lib.lib(), _lib.ptr
+    t = (torch.float32, torch.bfloat16, torch.float16)[dtype]
+    x, g, _, h0, _ = make(B, L, D, t, 1.0, seed=L)
+    h, h2, final, state = torch.empty_like(x), torch.empty_like(x), torch.empty_like(h0), h0.clone()
+    for out, s0, s1 in ((h, h0, final), (h2, state, state)):
+        assert lib.vig_gated_recurrence_fwd(p(x), p(g), p(s0), D, p(out), p(s1), D, B, L, D, None, None, None, 1.0, reverse, dtype, None, _lib.stream_ptr()) == 0
+    assert torch.equal(h, h2) and torch.equal(final, state) and not torch.equal(final, h0)

@@ -336,7 +336,6 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const __grid_cons
             tc::mbar_init(bar + 8, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
-        asm volatile("barrier.cluster.arrive.release;" ::: "memory");       // I run; waited for before the first CTA's memory is written
     }
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
     const int strips = (p.D + 32 * V - 1) / (32 * V);
@@ -442,6 +441,8 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const __grid_cons
 #pragma unroll
         for (int v = 0; v < V; ++v) { me.a[v] = finite(A[v]); me.h[v] = H[v]; }
         own[buf][wid][lane] = me;
+        // I run, and have read the state that enters: waited for before a CTA's memory is written, and so before the final state is, which may lie there
+        if (ctas > 1 && base == 0) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
         __syncthreads();
         float s[V];
         if (ctas > 1) {
@@ -581,7 +582,6 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const __grid_const
     Pair (*own)[TW][LPC] = (Pair (*)[TW][LPC])(tiles + tile_smem<BWD, LPC>), *all = (Pair*)(own + 2);
     if (threadIdx.x < TW) tc::mbar_init(bar + 8 * threadIdx.x, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (ctas > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");       // I run; waited for before the first CTA's memory is written
     __syncthreads();
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, q = lane / LPC, l = lane % LPC;
     const int strips = (p.D + LPC * V - 1) / (LPC * V);
@@ -800,6 +800,8 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const __grid_const
                 for (int v = 0; v < V; ++v) { me.a[v] = A[v]; me.h[v] = H[v]; }
                 own[buf][wid][l] = me;
             }
+            // I run, and have read the state that enters: waited for before a CTA's memory is written, and so before the final state is, which may lie there
+            if (base == 0) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
             __syncthreads();
             // joined: the tokens of the CTA ahead of this warp's; and all of them
             float pa[V], ph[V];
