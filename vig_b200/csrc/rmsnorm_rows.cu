@@ -39,7 +39,7 @@ struct NormBwdParams {
 template <int OUT> __device__ __forceinline__ float out_top() { return OUT == VIG_OUT_INT8 ? 127.f : 448.f; }
 
 template <int OUT> __device__ __forceinline__ uint8_t code_of(float v) {
-    if (OUT == VIG_OUT_INT8) return (uint8_t)(int8_t)__float2int_rn(fminf(fmaxf(v, -127.f), 127.f));
+    if (OUT == VIG_OUT_INT8) return (uint8_t)(int8_t)__float2int_rn(v);          // 127 at most, by the scale; 0 for a NaN
     return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
 }
 
