@@ -192,3 +192,18 @@ def test_c_state_in_place(B, L, D, dtype, reverse):
     for out, s0, s1 in ((h, h0, final), (h2, state, state)):
         assert lib.vig_gated_recurrence_fwd(p(x), p(g), p(s0), D, p(out), p(s1), D, B, L, D, None, None, None, 1.0, reverse, dtype, None, _lib.stream_ptr()) == 0
     assert torch.equal(h, h2) and torch.equal(final, state) and not torch.equal(final, h0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("norm", [1.0, 16.0])
+def test_long_memories(norm, dtype):
+    """Logits of 7 to 10: states that decay by 1e-4 a token and less.  The logarithm is right to a part in 10^6 of itself, and a decay is rounded to 2^-25
+    at random: some 1e-5 of the state over 6000 tokens.  A logarithm right to 2^-22 absolute would be off by 1e-3."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(1, 6000, 64, generator=gen, device="cuda").to(dtype)
+    z = (8.5 + 0.5 * torch.randn(1, 6000, 64, generator=gen, device="cuda")).to(dtype)
+    _, final = vig_b200.gated_recurrence(x, z, None, True, gate_logit_normalizer=norm)
+    a, s = decay(z.double(), norm), torch.zeros(1, 64, dtype=torch.float64, device="cuda")
+    for t in range(6000):
+        s = a[:, t] * s + x[:, t].double()
+    assert float((final.double() - s).norm() / s.norm()) < 1e-4
