@@ -220,6 +220,7 @@ template <typename T, bool LOGITS, bool BWD, bool KEEP, int V, bool AGAIN = fals
                 }
             }
         } else {
+            const int due = (p.L - 1 - k0) % GROUP;        // the token that leaves its state
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (k0 + u >= p.L) break;
@@ -232,8 +233,7 @@ template <typename T, bool LOGITS, bool BWD, bool KEEP, int V, bool AGAIN = fals
                     for (int v = 0; v < V; ++v) s[v] = fmaf(a[v], s[v], xf[v]);
                     if (!writes(s[0])) continue;
                     Few<T, V>::store(out + at(k0 + u) * p.so[1], s);
-                    const int behind = p.L - 1 - (k0 + u);         // tokens of the scan behind this one
-                    if (KEEP && behind && behind % GROUP == 0) state_out<V>(p.states + ((int64_t)b * p.groups() + behind / GROUP - 1) * p.D + d, s);
+                    if (KEEP && u == due && k0 + u + 1 < p.L) state_out<V>(p.states + ((int64_t)b * p.groups() + (p.L - 1 - k0) / GROUP - 1) * p.D + d, s);
                 } else {
                     float hb[V], og[V];
                     if (k0 + u + 1 < p.L) {
