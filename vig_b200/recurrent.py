@@ -42,6 +42,13 @@ class GatedRecurrence(nn.Module):
         self._codes()
         return self
 
+    def _apply(self, *args, **kwargs):
+        # moved or cast: laid out again at the next step, even where the weights come to lie at the old place
+        module = super()._apply(*args, **kwargs)
+        if self._in_8bit is not None:
+            self._in_8bit = (None, *self._in_8bit[1:])
+        return module
+
     def _codes(self):
         """The codes and scales of the weights as they are: kept by their version, as the layouts of ``GatedLinearAttention``."""
         w = self.in_proj.weight
