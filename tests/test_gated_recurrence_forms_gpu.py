@@ -81,8 +81,9 @@ FORMS = [
     (24, 300, 1024, torch.float16, 32, 32),
     (48, 300, 1000, torch.bfloat16, 32, 16),         # backward in halves
     (16, 301, 768, torch.bfloat16, 16, 16),          # strips of 16 lanes, one CTA, several steps
-    (24, 300, 768, torch.float16, 16, 32),           # backward: clusters of two
-    (17, 300, 1024, torch.bfloat16, 16, 32),
+    (24, 300, 768, torch.float16, 16, 16),
+    (17, 300, 1024, torch.bfloat16, 16, 16),
+    (12, 300, 768, torch.float32, 16, 32),           # backward: clusters of two
     (8, 701, 384, torch.bfloat16, 32, 32),           # clusters of eight
     (4, 1101, 384, torch.float16, 16, 16),
     (1, 3001, 192, torch.bfloat16, 8, 8),            # clusters of eight or sixteen, several steps

@@ -8,9 +8,10 @@
 // (counted from the end of its scan, half a byte a value), and the backward reads x and walks each eight of them again: h as it was rounded
 // costs the gate gradient a third of its precision (2.3e-3 from 64 bits in bf16 instead of 1.7e-3, fp16 2.9e-4 instead of 2.1e-4).
 // Bound by memory where sequences are many (3 tensors forward: x, g in, h out; 5 backward: g, h, dh in, dx, dg out), and by the MUFU unit
-// beside it: a raw logit is two of its instructions (three backward) and seven multiply-adds, half of its rate at the copy bandwidth.  16 x 4096 x 768 bf16
-// from raw logits: forward 60 us (5.0 TB/s), backward 93 us (5.4 TB/s); 16 x 2048 x 768 fp32 51 and 81 us (5.9
-// and 6.2 TB/s); 1 x 16384 x 768 bf16, 48 strips on 384 CTAs, 24 us.
+// beside it: a raw logit is two of its instructions (three backward) and seven multiply-adds, half of its rate at the copy bandwidth.  Calls on other
+// inputs and outputs than the last, 16 x 4096 x 768 bf16 from raw logits: forward 62 us (4.9 TB/s), 66 with states, backward 111 us (4.8 TB/s), 74 and 121
+// in a loop of seconds, where the power limit takes a tenth of the clock; 16 x 2048 x 768 fp32 54 and 87 us (5.6 and 5.8 TB/s); 1 x 16384 x 768 bf16, 48
+// strips on 384 CTAs, 29 and 47 us.
 // Three forms, by the rule in rec_launch: rows of 16-byte pieces through shared memory (rec_tile_kernel), rows of any alignment through
 // registers (rec_strip_kernel), few tokens a thread at a time (rec_few_kernel).
 #include <string.h>
@@ -552,6 +553,7 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const __grid_cons
 //   decays of the next step under the outputs of this one                             67                       28
 //   the state handed from warp to warp, no barrier                                    62                       28
 //   four CTAs of four warps an SM, requests under the exchange                        62 (backward 103 -> 91)  24
+//   (graph replays on the same buffers; backward from h.  States and x in its place: 91 -> 108)
 // Also tried: every warp adding up all pairs behind flags instead of the hand-over (the warps then keep step: 71), 32 tokens a thread
 // (1 x 16384 x 768 26), prefetch hints on the copies (no difference).
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
@@ -1006,26 +1008,27 @@ int rec_launch(const RecParams& p, cudaStream_t s) {
     }
     if (!pieces) return rec_strips<T, LOGITS, BWD, KEEP>(p, s);
     // Width of the strips and CTAs of a cluster.  Four CTAs find room on an SM.  Best is the widest strip of which there are enough by
-    // themselves, 6/10 of the room (a cluster's meetings cost: 16 x 4096 x 768 bf16, forward, 62 us with 32 channels and one CTA, 66 with 64 and
-    // two); else the widest that reaches that in clusters (4 x 4096 x 384, forward / backward: 12.8 / 17.8 us with 32 channels and eight CTAs,
-    // 13.6 / 19.2 with 16 and four); else the narrowest (1 x 16384 x 768: 25 / 38 us with 16 channels, 31 / 48 with 32).  The backward writes two
-    // tensors, and half rows of them cost once many are under way (24 x 4096 x 768: 203 us with 32 channels, 131 with 64 and two CTAs, 148 with
-    // one; 16 x 4096 x 768: 93 with 32 channels, 104 with 64 and two): strips of 64 channels from 35/100 of the room, narrower ones by themselves
-    // from 45/100.
-    const int64_t room = 4 * device_sms(), joined = room * 60 / 100, alone = BWD ? room * 45 / 100 : joined, whole_rows = BWD ? room * 35 / 100 : joined;
+    // themselves, 6/10 of the room (a cluster's meetings cost: 16 x 4096 x 768 bf16, forward, 64 us with 32 channels and one CTA, 72 with 64 and
+    // two); else the widest that reaches that in clusters (4 x 4096 x 384, forward: 16.7 us with 32 channels and eight CTAs, 18.5 with 16 and
+    // four); else the narrowest (1 x 16384 x 768, forward / backward: 29 / 47 us with 16 channels, 35 / 61 with 32).  The backward takes
+    // narrower strips by themselves from 45/100 (16 x 2048 x 768: 61 us with 32 channels, 67 with 64 and two CTAs, 84 with one; 24 x 4096 x 768: 143, 158
+    // and 175).  In fp32 its two tensors' half rows cost once many are under way (12 x 4096 x 768: 202 us with 16 channels, 153 with 32 and two
+    // CTAs): whole rows of 128 bytes from 35/100 of the room.
+    const int64_t room = 4 * device_sms(), joined = room * 60 / 100, alone = BWD ? room * 45 / 100 : joined;
+    const int64_t whole_rows = BWD && sizeof(T) == 4 ? room * 35 / 100 : joined;
     auto strips = [&](int lpc) { const int w = lpc * (4 / (int)sizeof(T)); return (int64_t)p.B * ((p.D + w - 1) / w); };
     auto ctas = [&](int lpc) { return rec_ctas(strips(lpc), p.L, TW * (32 / lpc) * tile_run<BWD>, joined); };
     int lpc = 0, c = 1;
     if (strips(32) >= whole_rows) { lpc = 32; c = ctas(32); }
-    // a few more than find room at once would make a second round of their own: in halves (56 x 1024 x 768, 672 strips of 64 channels: backward 89
-    // us, 79 with 32; 50 x 2048 x 768, 600 strips: forward 98, 88)
+    // a few more than find room at once would make a second round of their own: in halves (56 x 1024 x 768, 672 strips of 64 channels: backward 105
+    // us, 94 with 32; 50 x 2048 x 768, 600 strips: forward 102, 93)
     if (strips(32) > room && strips(32) * 10 <= room * (BWD ? 15 : 11)) { lpc = 16; c = 1; }
     for (int w = 16; w >= 8 && !lpc; w /= 2) if (strips(w) >= alone) lpc = w;
     for (int w = 32; w >= 8 && !lpc; w /= 2) if (strips(w) * ctas(w) >= joined) { lpc = w; c = ctas(w); }
     if (!lpc) {
         lpc = 8;
         c = ctas(8);
-        // twice as many where they still find room at once (1 x 65536 x 192: 50 / 82 us with eight, 37 / 58 with sixteen)
+        // twice as many where they still find room at once (1 x 65536 x 192: 53 / 100 us with eight, 41 / 73 with sixteen)
         if (c == 8 && 16 * strips(8) <= room && 8ll * TW * 4 * tile_run<BWD> < p.L && places_16<T, LOGITS, BWD, KEEP, 8>()) c = 16;
     }
     switch (lpc) {
