@@ -6,9 +6,11 @@
 // round(y/s); where all of y is zero (or s below the smallest normal number), s and the codes are 0, and a NaN makes s NaN.  y is never rounded to 16 bits on the way.
 // Backward, with t = w dy and xh = r rstd:  dr = rstd (t - xh mean(t xh)) + d_r,  dw = sum over rows of dy xh; rstd is computed again from r.
 // In 16 bits the backward takes the sum from x and the residual again: r as it was rounded would be one tensor instead of two (8 in all instead
-// of 9, backward 68 us instead of 86), but its roundings stand in dw beside dw's own, 2.5e-3 from 64 bits instead of 1.8e-3 in bf16.
-// Bound by memory: x, residual in, r and one byte a value out; backward dy, r, d_r in, dr out.  131072 x 768 bf16 to e4m3 114 us (6.2 TB/s);
-// 262144 x 192 bf16 forward 65 us (6.2 TB/s), backward 86 us (5.8 TB/s); one row of 768 2.5 us, a launch.
+// of 9, backward 68 us instead of 86 in graph replays), but its roundings stand in dw beside dw's own, 2.5e-3 from 64 bits instead of 1.8e-3 in bf16.
+// Bound by memory: x, residual in, r and one byte a value out; backward dy, x, residual, d_r in, dr out.  Calls on other inputs and outputs than the
+// last: 131072 x 768 bf16 to e4m3 117 us (6.0 TB/s); 262144 x 192 bf16 forward 67 us (6.0 TB/s), backward 89 us (5.7 TB/s); one row of 768 2.6 us, a
+// launch.  Rows off 16 bytes are read and written a value at a time: 32768 x 767 87 / 122 / 145 us, 768 35 / 37 / 51; rows wider than a CTA's
+// registers (norm_any_kernel, 4096 x 20000) 279 / 307 / 768 us, 0.3 of the bandwidth forward and 0.16 backward.
 #include <cuda_fp8.h>
 #include "common.cuh"
 
