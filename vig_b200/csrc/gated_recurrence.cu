@@ -161,17 +161,24 @@ template <int V> __device__ __forceinline__ void state_out(float* p, const float
     }
 }
 
-// V channels of a sequence from the state s, token by token.  AGAIN: only what is not finite is written, the rest is there.
-template <typename T, bool LOGITS, bool BWD, bool KEEP, int V, bool AGAIN = false> __device__ __forceinline__ void rec_walk(const RecParams& p, int b, int d, float* s) {
-    auto writes = [](float value) { return !AGAIN || !(fabsf(value) <= 3.4028235e38f); };
+template <typename T, bool LOGITS, bool BWD, bool KEEP, int V>
+__global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
     constexpr bool WALKS = BWD && sizeof(T) == 2;
     constexpr int U = WALKS ? GROUP : 4;
+    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
+    const int per = p.D / V;
+    if (i >= (int64_t)p.B * per) return;
+    const int b = (int)(i / per), d = (int)(i % per) * V;
     const T* x = (const T*)p.x + b * p.sx[0] + d;
     const T* g = (const T*)p.g + b * p.sg[0] + d;
     const T* hin = BWD ? (const T*)p.h_in + b * p.sh[0] + d : nullptr;
     T* out = (T*)p.out + b * p.so[0] + d;
     T* outg = BWD ? (T*)p.out_g + b * p.sog[0] + d : nullptr;
     auto at = [&](int k) { return (int64_t)(p.from_end ? p.L - 1 - k : k); };
+    alignas(4 * V) float s[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = 0.f;
+    if (p.s0) state_in<V>(s, p.s0 + b * p.ld_s0 + d);
     const int next = WALKS && p.walk ? 0 : 1;      // token of h_in that belongs to a token
     for (int k0 = 0; k0 < p.L; k0 += U) {
         Few<T, V> xr[U], gr[U], hr[BWD ? U : 1];
@@ -215,10 +222,8 @@ template <typename T, bool LOGITS, bool BWD, bool KEEP, int V, bool AGAIN = fals
                     og[v] = s[v] * before[u][v];
                     if (LOGITS) og[v] *= p.inv_norm * rest[u][v];
                 }
-                if (writes(xf[0])) {
-                    Few<T, V>::store(out + at(k0 + u) * p.so[1], xf);
-                    Few<T, V>::store(outg + at(k0 + u) * p.sog[1], og);
-                }
+                Few<T, V>::store(out + at(k0 + u) * p.so[1], xf);
+                Few<T, V>::store(outg + at(k0 + u) * p.sog[1], og);
             }
         } else {
             const int due = (p.L - 1 - k0) % GROUP;        // the token that leaves its state
@@ -232,7 +237,6 @@ template <typename T, bool LOGITS, bool BWD, bool KEEP, int V, bool AGAIN = fals
                 if (!BWD) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) s[v] = fmaf(a[v], s[v], xf[v]);
-                    if (!writes(s[0])) continue;
                     Few<T, V>::store(out + at(k0 + u) * p.so[1], s);
                     if (KEEP && u == due && k0 + u + 1 < p.L) state_out<V>(p.states + ((int64_t)b * p.groups() + (p.L - 1 - k0) / GROUP - 1) * p.D + d, s);
                 } else {
@@ -251,36 +255,15 @@ template <typename T, bool LOGITS, bool BWD, bool KEEP, int V, bool AGAIN = fals
                         og[v] = s[v] * hb[v];
                         if (LOGITS) og[v] *= p.inv_norm * rest[v];
                     }
-                    if (!writes(xf[0])) continue;
                     Few<T, V>::store(out + at(k0 + u) * p.so[1], xf);
                     Few<T, V>::store(outg + at(k0 + u) * p.sog[1], og);
                 }
             }
         }
     }
-    if (p.s_end && writes(s[0])) state_out<V>(p.s_end + b * p.ld_end + d, s);
+    if (p.s_end) state_out<V>(p.s_end + b * p.ld_end + d, s);
 }
 
-template <typename T, bool LOGITS, bool BWD, bool KEEP, int V>
-__global__ void __launch_bounds__(128) rec_few_kernel(const RecParams p) {
-    const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
-    const int per = p.D / V;
-    if (i >= (int64_t)p.B * per) return;
-    const int b = (int)(i / per), d = (int)(i % per) * V;
-    alignas(4 * V) float s[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = 0.f;
-    if (p.s0) state_in<V>(s, p.s0 + b * p.ld_s0 + d);
-    rec_walk<T, LOGITS, BWD, KEEP, V>(p, b, d, s);
-}
-
-// Long sequences are joined from stretches of tokens, and a stretch's product of decays can be 0 in fp32 where none of them is: an infinite state would
-// become NaN over it.  A CTA that met an infinite state (which costs a maximum a step to know) walks that channel again when it is done, by one
-// thread.  (Ahead of its infinity nothing changes: a state that is no number, or infinite, stays so.)
-template <typename T, bool LOGITS, bool BWD, bool KEEP> __device__ __noinline__ void rec_again(const RecParams& p, int b, int d, float s) {
-    rec_walk<T, LOGITS, BWD, KEEP, 1, true>(p, b, d, &s);
-}
-constexpr float INFINITE = __builtin_huge_valf();
 
 // ---------------------------------------------------------------------------------------------------
 // Rows of any alignment.  A cluster of CTAs owns a strip of 32 channels of one sequence and walks it in steps of (CTAs x 8 warps x RUN)
@@ -320,6 +303,84 @@ constexpr int RC = 8;                 // CTAs of a cluster of this kernel, at mo
 // The product of decays of a stretch of tokens, kept finite: 0 times it stays 0.  (Were a decay NaN, the stretch's contribution is NaN.)
 __device__ __forceinline__ float finite(float a) { return fminf(a, 3.4028235e38f); }
 
+// A stretch's product of decays can be 0 in fp32 where none of them is, and an infinite state would become NaN over it.  A CTA that met one (which
+// costs a maximum a step to know) tells its cluster, and when all are done the warps go over such channels again, 32 tokens to a scan in which a product of
+// 0 without a decay of 0 is -0 and leaves an infinite state as it is.  What is not finite is written, the rest keeps its bits.  (16 x 4096 x 768 bf16
+// with an infinity in one channel of each sequence 0.32 ms, in all 2.9.  Telling the zeros apart in every join instead: 62 / 111 -> 66 / 125 us without any.)
+constexpr float INFINITE = __builtin_huge_valf();
+__device__ __forceinline__ float times(float a, float b) {
+    const float c = finite(a * b);
+    return c == 0.f ? (__float_as_uint(a) == 0 || __float_as_uint(b) == 0 ? 0.f : -0.f) : c;
+}
+__device__ __forceinline__ float behind(float a, float s, float h) {
+    return __float_as_uint(a) == 0x80000000u && fabsf(s) == INFINITE ? s + h : fmaf(a, s, h);
+}
+__device__ __forceinline__ void mark(uint32_t* word, uint32_t ctas) {
+    const uint32_t at = tc::smem_u32(word);
+    for (uint32_t r = 0; r < ctas; ++r) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::map_rank(at, r)), "r"(1u) : "memory");
+}
+template <typename T, bool LOGITS, bool BWD, bool KEEP> __device__ __noinline__ void rec_again(const RecParams& p, int b, int d, float s) {
+    constexpr uint32_t ALL = 0xffffffffu;
+    const int lane = threadIdx.x & 31;
+    const bool walk = BWD && sizeof(T) == 2 && p.walk;
+    auto at = [&](const void* q, const int64_t* st, int k) { return (T*)q + b * st[0] + (int64_t)(p.from_end ? p.L - 1 - k : k) * st[1] + d; };
+    auto get = [&](const void* q, const int64_t* st, int k) { return k < p.L ? DType<T>::to_f(*at(q, st, k)) : 0.f; };
+    float xn = get(p.x, p.sx, lane), gn = get(p.g, p.sg, lane), hn = BWD ? get(p.h_in, p.sh, lane + (walk ? 0 : 1)) : 0.f;
+    for (int k0 = 0; k0 < p.L; k0 += 32) {
+        const int k = k0 + lane;
+        const bool in = k < p.L;
+        const float x = xn, g = gn, hin = hn;
+        if (k0 + 32 < p.L) {
+            xn = get(p.x, p.sx, k + 32);
+            gn = get(p.g, p.sg, k + 32);
+            if (BWD) hn = get(p.h_in, p.sh, k + 32 + (walk ? 0 : 1));
+        }
+        float a, rest = 1.f;
+        decays<T, LOGITS, BWD, 1>(&g, p.inv_norm, &a, &rest);
+        if (!in) a = 1.f;
+        float A = a, H = BWD ? a * x : x;
+#pragma unroll
+        for (int off = 1; off < 32; off *= 2) {
+            const float oa = __shfl_up_sync(ALL, A, off), oh = __shfl_up_sync(ALL, H, off);
+            if (lane >= off) {
+                H = behind(A, oh, H);
+                A = times(A, oa);
+            }
+        }
+        const float state = behind(A, s, H);
+        float before = __shfl_up_sync(ALL, state, 1);
+        if (lane == 0) before = s;
+        s = __shfl_sync(ALL, state, 31);
+        auto odd = [](float value) { return !(fabsf(value) <= 3.4028235e38f); };
+        if (!BWD) {
+            if (in && odd(state)) {
+                *at(p.out, p.so, k) = DType<T>::from_f(state);
+                const int later = p.L - 1 - k;
+                if (KEEP && later && later % GROUP == 0) p.states[((int64_t)b * p.groups() + later / GROUP - 1) * p.D + d] = state;
+            }
+        } else {
+            float hb = hin;
+            if (walk) {
+                const int left = p.L - (k & ~(GROUP - 1));
+                float h = left > GROUP ? p.states[((int64_t)b * p.groups() + k / GROUP) * p.D + d] : left > 0 && p.h0 ? p.h0[(int64_t)b * p.D + d] : 0.f;
+#pragma unroll
+                for (int i = GROUP - 1; i >= 0; --i) {
+                    if ((lane & (GROUP - 1)) == i) hb = h;
+                    h = fmaf(__shfl_sync(ALL, a, i, GROUP), h, __shfl_sync(ALL, hin, i, GROUP));
+                }
+            } else if (k == p.L - 1) {
+                hb = p.h0 ? p.h0[(int64_t)b * p.D + d] : 0.f;
+            }
+            const float dx = x + before;
+            if (in && odd(dx)) {
+                *at(p.out, p.so, k) = DType<T>::from_f(dx);
+                *at(p.out_g, p.sog, k) = DType<T>::from_f(LOGITS ? state * hb * p.inv_norm * rest : state * hb);
+            }
+        }
+    }
+    if (p.s_end && lane == 0 && !(fabsf(s) <= 3.4028235e38f)) p.s_end[b * p.ld_end + d] = s;
+}
+
 template <typename T, bool LOGITS, bool BWD, bool KEEP, int RUN>
 __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const __grid_constant__ RecParams p) {
     constexpr int V = 1;
@@ -329,7 +390,7 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const __grid_cons
     __shared__ Pair all[2][RC][32];                // of each CTA's
     __shared__ uint64_t landed[2];                 // counts the bytes of `all`
     __shared__ float begun[32];                    // the state that entered, and whether one was infinite: for a CTA that walks again
-    __shared__ bool met[32];
+    __shared__ uint32_t met[32];
     const uint32_t rank = tc::cluster_rank(), ctas = tc::cluster_size(), bar = tc::smem_u32(landed);
     if (ctas > 1) {
         if (threadIdx.x == 0) {
@@ -363,7 +424,7 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const __grid_cons
     float* const kept = KEEP || (WALKS && p.walk) ? p.states + (int64_t)b * p.groups() * p.D + d : nullptr;
     const int keeps = (p.L - 1) % GROUP;           // KEEP: which of eight tokens leave their state
     const int next = WALKS && p.walk ? 0 : 1;      // token of h_in that belongs to a token
-    if (wid == 0) { begun[lane] = carry[0]; met[lane] = false; }
+    if (wid == 0) { begun[lane] = carry[0]; met[lane] = 0; }
     float most = 0.f;                              // the largest magnitude of a state or a contribution
     R xn[RUN], gn[RUN], hn[BWD ? RUN : 1];
     float sn[V] = {};
@@ -532,15 +593,14 @@ __global__ void __launch_bounds__(RW * 32, 2) rec_strip_kernel(const __grid_cons
             for (int v = 0; v < V; ++v) p.s_end[b * p.ld_end + d + v] = s[v];
         }
     }
-    // no CTA leaves while another may still write to it (one that gave up waiting)
-    __syncthreads();                               // (the marks are clear)
-    if (most == INFINITE) met[lane] = true;
-    __syncthreads();
+    // no CTA leaves while another may still write to it (one that gave up waiting; marks), and what another has written is there
+    if (most == INFINITE) mark(met + lane, ctas);
+    if (ctas == 1) __syncthreads();
     if (ctas > 1) {
         asm volatile("barrier.cluster.arrive.release;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     }
-    if (wid == 0 && live && met[lane]) rec_again<T, LOGITS, BWD, KEEP>(p, b, d, begun[lane]);
+    for (int c = wid * (int)ctas + (int)rank; c < 32; c += RW * (int)ctas) if (met[c]) rec_again<T, LOGITS, BWD, KEEP>(p, b, d - lane + c, begun[c]);
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -575,7 +635,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const __grid_const
     struct alignas(8 * V) Pair { float a[V], h[V]; };
     extern __shared__ __align__(128) uint8_t tiles[];
     __shared__ float begun[LPC * V];               // the state that entered, and whether one was infinite: for a CTA that walks again
-    __shared__ bool met[LPC * V];
+    __shared__ uint32_t met[LPC * V];
     __shared__ uint64_t landed[TW];                // one CTA: one a warp, its mail is there; several: 0 and 1 count the bytes of `all`
     const uint32_t rank = tc::cluster_rank(), ctas = tc::cluster_size(), bar = tc::smem_u32(landed);
     // behind the tiles, one CTA: the state ahead of each warp's tokens, from the warp before; several: the pair of each warp's tokens and of each
@@ -583,6 +643,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const __grid_const
     float (*mail)[LPC][V] = (float (*)[LPC][V])(tiles + tile_smem<BWD, LPC>);
     Pair (*own)[TW][LPC] = (Pair (*)[TW][LPC])(tiles + tile_smem<BWD, LPC>), *all = (Pair*)(own + 2);
     if (threadIdx.x < TW) tc::mbar_init(bar + 8 * threadIdx.x, 1);
+    if (threadIdx.x < LPC * V) met[threadIdx.x] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     __syncthreads();
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, q = lane / LPC, l = lane % LPC;
@@ -655,7 +716,7 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const __grid_const
     state_of(mine);
     if (threadIdx.x < LPC) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) { begun[l * V + v] = carry[v]; met[l * V + v] = false; }
+        for (int v = 0; v < V; ++v) begun[l * V + v] = carry[v];
     }
     float most[V] = {};                            // the largest magnitude of a state or a contribution
     uint32_t phase = 0;
@@ -906,16 +967,15 @@ __global__ void __launch_bounds__(TW * 32, 4) rec_tile_kernel(const __grid_const
         if (ctas == 1) bring(base + tile_stages * per, stage);
         stage = ahead;
     }
-    // no CTA leaves while another may still write to it (one that gave up waiting)
-    __syncthreads();                               // (the marks are clear)
+    // no CTA leaves while another may still write to it (one that gave up waiting; marks), and what another has written is there
 #pragma unroll
-    for (int v = 0; v < V; ++v) if (most[v] == INFINITE) met[l * V + v] = true;
-    __syncthreads();
+    for (int v = 0; v < V; ++v) if (most[v] == INFINITE) mark(met + l * V + v, ctas);
+    if (ctas == 1) __syncthreads();
     if (ctas > 1) {
         asm volatile("barrier.cluster.arrive.release;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     }
-    if (threadIdx.x < LPC * V && d0 + threadIdx.x < p.D && met[threadIdx.x]) rec_again<T, LOGITS, BWD, KEEP>(p, b, d0 + (int)threadIdx.x, begun[threadIdx.x]);
+    for (int c = wid * (int)ctas + (int)rank; c < LPC * V; c += TW * (int)ctas) if (met[c]) rec_again<T, LOGITS, BWD, KEEP>(p, b, d0 + c, begun[c]);
 }
 
 static cudaError_t rec_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute& attr, void (*kernel)(RecParams), int64_t strips, int c, int warps, size_t smem, cudaStream_t s) {
