@@ -208,3 +208,23 @@ def test_long_memories(norm, dtype):
     for t in range(6000):
         s = a[:, t] * s + x[:, t].double()
     assert float((final.double() - s).norm() / s.norm()) < 1e-4
+
+
+@pytest.mark.parametrize("D,reverse", [(1024, False), (1001, True)])
+def test_gradients_beyond_32_bits(D, reverse):
+    """Tensors of more than 2^31 values: gradients at both ends against calls on those ends alone.  4000 tokens forget what is beyond them; both calls then
+    round values that agree to 1e-6."""
+    L, n = 2_200_000, 3000
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    x, g, d = (torch.empty(1, L, D, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(3))
+    kw = dict(gate_logit_normalizer=1.0, reverse=reverse)
+
+    def grads(part):
+        leaf = [t[:, part].detach().requires_grad_(True) for t in (x, g)]
+        return torch.autograd.grad(vig_b200.gated_recurrence(*leaf, **kw)[0], leaf, d[:, part])
+
+    whole = grads(slice(None))
+    for end, keep in ((slice(0, n + 4000), slice(0, n)), (slice(L - n - 4000, L), slice(4000, n + 4000))):
+        for got, want in zip(whole, grads(end)):
+            got, want = got[:, end][:, keep].float(), want[:, keep].float()
+            assert ((got - want).abs() <= 2 * UNIT[torch.bfloat16] * want.abs() + 1e-5).all()
