@@ -93,3 +93,24 @@ def test_autocast(dtype):
                 for b, s in zip(blocks, states):
                     h, residual = b.step(h, residual, s)
         assert far(h + residual, (want[0] + want[1])[:, -1].detach()) < (0.1 if eight else 3 * 8 * unit)
+
+
+def test_only_16_bits_are_widened():
+    block, r = build(dtype=torch.float32), torch.randn(2, 5, 64, device="cuda")
+    with pytest.raises(TypeError):
+        block(r.double(), r)
+    with pytest.raises(TypeError):
+        block(r, r.bfloat16())
+
+
+def test_weights_of_inference_mode():
+    """They have no version: quantize() takes them as they are then."""
+    with torch.inference_mode():
+        block, x = build().quantize(), torch.randn(4, 64, device="cuda").bfloat16()
+        before = served(block, x)
+        block.in_proj.weight.mul_(2)
+        after = served(block.quantize(), x)
+        assert not torch.equal(after[2], before[2])
+        fresh = build(seed=3)
+        fresh.load_state_dict(block.state_dict())
+        assert all(torch.equal(a, b) for a, b in zip(after, served(fresh.quantize(), x)))

@@ -7,7 +7,7 @@
 // the gate gradients: fp32 calls read h.  In 16 bits the forward of a training step leaves the fp32 state in front of every eight tokens
 // (counted from the end of its scan, half a byte a value), and the backward reads x and walks each eight of them again: h as it was rounded
 // costs the gate gradient a third of its precision (2.3e-3 from 64 bits in bf16 instead of 1.7e-3, fp16 2.9e-4 instead of 2.1e-4).
-// Bound by memory where sequences are many (3 tensors forward: x, g in, h out; 5 backward: g, h, dh in, dx, dg out), and by the MUFU unit
+// Bound by memory where sequences are many (3 tensors forward: x, g in, h out; 5 backward: g, dh, h or x in, dx, dg out), and by the MUFU unit
 // beside it: a raw logit is two of its instructions (three backward) and seven multiply-adds, half of its rate at the copy bandwidth.  Calls on other
 // inputs and outputs than the last, 16 x 4096 x 768 bf16 from raw logits: forward 62 us (4.9 TB/s), 66 with states, backward 111 us (4.8 TB/s), 74 and 121
 // in a loop of seconds, where the power limit takes a tenth of the clock; 16 x 2048 x 768 fp32 54 and 87 us (5.6 and 5.8 TB/s); 1 x 16384 x 768 bf16, 48
@@ -71,7 +71,7 @@ template <int V> __device__ __forceinline__ void mul_v(float* d, const float* a,
 
 // log2(1 + e) = e P(e) for e of 0 to 1, P fitted to the least relative error: 1.4e-6 with 7 terms (16-bit types), 2e-7 with 9 (fp32).  Relative,
 // because a long memory is a small e: the logarithm of the MUFU unit is right to 2^-22 absolute, which at a logit of 9 is 1e-3 of the rate at
-// which the state decays.  It takes as long (the unit is as busy as the multiply-adds: 16 x 4096 x 768 bf16 61 / 95 us with it, 60 / 96 with P).
+// which the state decays.  It takes as long (the unit is as busy as the multiply-adds: 16 x 4096 x 768 bf16 61 / 95 us with it, 60 / 96 with P, replays, backward from h).
 template <typename T, int W> __device__ __forceinline__ void log2_1p(float* y, const float* e) {
     constexpr int N = sizeof(T) == 4 ? 9 : 7;
     const float c[N] = {1.44269323f, -0.721159458f, 0.477668375f, -0.339089006f, 0.215284511f, -0.0957975239f, 0.0204011761f};

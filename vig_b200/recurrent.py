@@ -31,14 +31,16 @@ class GatedRecurrence(nn.Module):
 
     @staticmethod
     def _widened(hidden, residual):
-        return hidden if residual is None or residual.dtype != torch.float32 else hidden.float()
+        return hidden.float() if residual is not None and residual.dtype == torch.float32 and hidden.dtype in (torch.bfloat16, torch.float16) else hidden
 
     @torch.no_grad()
     def quantize(self):
         """From now on ``step`` takes its input projection in 8 bits: e4m3 codes with a scale per output channel, laid out here and again at the first step
-        behind a change of the weights (an optimizer's step, ``load_state_dict``, ``to``)."""
+        behind a change of the weights (an optimizer's step, ``load_state_dict``, ``to``).  Weights made in inference mode have no version: they want
+        another call when they change."""
         if self.d_model % 16 or 3 * self.d_inner % 16:
             raise ValueError(f"8-bit products want widths of whole 16s; got {self.d_model} and {self.d_inner}")
+        self._in_8bit = None
         self._codes()
         return self
 
