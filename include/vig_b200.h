@@ -440,6 +440,87 @@ VIG_API int vig_adamw_step(int count, void* const* params, const void* const* gr
                            const int* param_dtypes, const int* grad_dtypes, int64_t step, double lr, double beta1, double beta2, double eps,
                            double weight_decay, const float* grad_scale, const float* found_inf, void* stream);
 
+/* ---- blocks with a selective state space ---------------------------------------------------------------------------------------------- */
+/*
+ * Selective scan: delta = softplus(dt + dt_bias) (softplus 0: dt + dt_bias), h_t[d,n] = exp(delta_t[d] A[d,n]) h_{t-1}[d,n] + delta_t[d] u_t[d] b_t[n],
+ * y_t[d] = (sum_n c_t[n] h_t[d,n] + skip[d] u_t[d]) silu(z_t[d]).  All pointers are device pointers; optional ones are NULL.
+ *   u, dt, z (optional), y, d_y: [B, L, D] of dtype, unit stride over D, element strides (b, l).  b, c: [B, L, G, N] of dtype, unit stride over N,
+ *   strides (b, l, g); channel d reads group d / (D / G), D % G == 0, 1 <= N <= 128.  A: fp32 [D, N] contiguous.  skip, dt_bias (optional): [D] of
+ *   skip_dtype, bias_dtype (dtype or fp32).  lengths (optional): int32 [B], tokens of a sequence that count (taken into 0..L): behind them y
+ *   and gradients are zeros and states stay.  h0 (optional), h_final (optional): fp32 [B, D, N], sequences ld_h0 / ld_final apart, channels N apart;
+ *   h_final may be h0.  Any alignment.  B * D < 2^31, D < 2^28, L < 2^30.
+ * vig_selective_scan_fwd: y and h_final; with `states` (vig_selective_scan_states_bytes) also the states that enter every 64th token, for a backward.
+ * vig_selective_scan_bwd: from the inputs, these states, d_y and d_final (optional, fp32 [B, D, N] contiguous): d_u, d_dt, d_z [B, L, D] and d_b,
+ *   d_c [B, L, G, N] of dtype, d_A fp32 [D, N], d_skip, d_bias (optional) [D] of their types, d_h0 (optional) fp32 [B, D, N], all contiguous.  Sums over
+ *   channels, tokens and sequences are fp32 in a fixed order.
+ * vig_selective_scan_step: L = 1; h_final is the state, updated in place (h0 and lengths are not looked at).
+ */
+typedef struct vig_selective_scan_args {
+    int32_t B, L, D, N, G, dtype, skip_dtype, bias_dtype, softplus, reserved;
+    const void *u, *dt, *z, *b, *c;
+    const float* A;
+    const void *skip, *dt_bias;
+    const int32_t* lengths;
+    const float* h0;
+    int64_t ld_h0;
+    void* y;
+    float* h_final;
+    int64_t ld_final;
+    float* states;
+    int64_t s_u[2], s_dt[2], s_z[2], s_y[2], s_b[3], s_c[3];
+    const void* d_y;
+    int64_t s_dy[2];
+    const float* d_final;
+    void *d_u, *d_dt, *d_z, *d_b, *d_c;
+    float* d_A;
+    void *d_skip, *d_bias;
+    float* d_h0;
+    void* workspace;
+    size_t workspace_bytes;
+} vig_selective_scan_args;
+VIG_API size_t vig_selective_scan_states_bytes(int B, int L, int D, int N);
+VIG_API int vig_selective_scan_fwd(const vig_selective_scan_args* args, void* stream);
+VIG_API size_t vig_selective_scan_bwd_workspace_bytes(int B, int L, int D, int N, int G);
+VIG_API int vig_selective_scan_bwd(const vig_selective_scan_args* args, void* stream);
+VIG_API int vig_selective_scan_step(const vig_selective_scan_args* args, void* stream);
+
+/*
+ * Causal convolution over few tokens, a channel at a time: pre_t[d] = bias[d] + sum_k w[d,k] x_{t-K+1+k}[d], y = silu(pre) (silu 0: pre); 1 <= K <= 8.
+ * x, y: [B, L, D], unit stride over D, element strides (b, l); w: [D, K] contiguous, bias (optional): [D], both of w_dtype (dtype or fp32).  What stands in
+ * front of the first token is the state: [B, K-1, D] of dtype, strides (b, row), its last row the token just before (NULL: zeros).  state_out
+ * (optional, may not overlap x or the state): the last K-1 tokens in the same form.  lengths as above.  B * D < 2^31, D < 2^28, L < 2^30.
+ * Backward: d_x [B, L, D] contiguous, d_w [D, K] and d_bias (optional) of w_dtype, d_state (optional) [B, K-1, D] contiguous, from d_y and
+ * d_state_out (optional, [B, K-1, D] contiguous).  Step: x, y [B, D] with row strides; the state is moved on in place.
+ */
+VIG_API int vig_causal_conv_fwd(const void* x, const void* w, int w_dtype, const void* bias, const void* state, void* y, void* state_out, const int32_t* lengths,
+                                int B, int L, int D, int K, const int64_t* strides_x, const int64_t* strides_y, const int64_t* strides_state,
+                                const int64_t* strides_state_out, int silu, int dtype, void* stream);
+VIG_API size_t vig_causal_conv_bwd_workspace_bytes(int B, int L, int D, int K);
+VIG_API int vig_causal_conv_bwd(const void* x, const void* w, int w_dtype, const void* bias, const void* state, const void* d_y, const void* d_state_out,
+                                const int32_t* lengths, void* d_x, void* d_w, void* d_bias, void* d_state, int B, int L, int D, int K, const int64_t* strides_x,
+                                const int64_t* strides_state, const int64_t* strides_dy, int silu, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+VIG_API int vig_causal_conv_step(const void* x, int64_t ldx, void* state, const int64_t* strides_state, const void* w, int w_dtype, const void* bias, void* y, int64_t ldy,
+                                 int B, int D, int K, int silu, int dtype, void* stream);
+
+/*
+ * Optional residual add and LayerNorm, as a trained norm has it: r = x (+ residual), y = (r - mean(r)) / sqrt(var(r) + eps) * w + bias, taken from the
+ * fp32 sum; w, bias (optional): [N] of w_dtype (the rows' dtype or fp32).  Arguments as in vig_add_rmsnorm_train_fwd / vig_add_rmsnorm_bwd; d_bias (optional) [N].
+ */
+VIG_API int vig_add_layernorm_train_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* w, const void* bias, int w_dtype, void* y,
+                                        void* residual_out, int64_t rows, int N, float eps, int dtype, void* stream);
+VIG_API size_t vig_add_layernorm_bwd_workspace_bytes(int64_t rows, int N);
+VIG_API int vig_add_layernorm_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* w, int w_dtype,
+                                  const void* d_r, int64_t ld_dr, void* dx, void* dw, void* d_bias, int64_t rows, int N, float eps, int dtype, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/*
+ * Product of 8-bit integers: y[m, n] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + bias[n], summed in 32-bit integers (K <= 131072, so that no sum
+ * overflows), scaled in fp32, rounded once to dtype.  x: int8 [M, K] with row stride ldx; w: int8 [N, K] with row stride ldw; x_scales [M], w_scales [N]: fp32;
+ * bias (optional): [N] of dtype; y: [M, N] with row stride ldy.  Any sizes and alignment.  status_dev: optional int32, bit 0 = a bounded wait ran out.
+ */
+VIG_API int vig_linear_int8_fwd(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw, const float* w_scales, const void* bias, void* y,
+                                int64_t ldy, int64_t M, int N, int K, int dtype, int32_t* status_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -71,6 +71,19 @@ _SIGNATURES = {
     "vig_add_rmsnorm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int]),
     "vig_add_rmsnorm_bwd": (c_int, [c_void_p, c_int64] * 3 + [c_void_p, c_int] + [c_void_p, c_int64] + [c_void_p] * 2 + [c_int64, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
     "vig_adamw_step": (c_int, [c_int] + [POINTER(c_void_p)] * 7 + [_P64] + [POINTER(c_int)] * 2 + [c_int64] + [c_double] * 5 + [c_void_p] * 3),
+    "vig_selective_scan_states_bytes": (c_size_t, [c_int] * 4),
+    "vig_selective_scan_fwd": (c_int, [c_void_p] * 2),
+    "vig_selective_scan_bwd_workspace_bytes": (c_size_t, [c_int] * 5),
+    "vig_selective_scan_bwd": (c_int, [c_void_p] * 2),
+    "vig_selective_scan_step": (c_int, [c_void_p] * 2),
+    "vig_causal_conv_fwd": (c_int, [c_void_p] * 2 + [c_int] + [c_void_p] * 5 + [c_int] * 4 + [_P64] * 4 + [c_int] * 2 + [c_void_p]),
+    "vig_causal_conv_bwd_workspace_bytes": (c_size_t, [c_int] * 4),
+    "vig_causal_conv_bwd": (c_int, [c_void_p] * 2 + [c_int] + [c_void_p] * 9 + [c_int] * 4 + [_P64] * 3 + [c_int] * 2 + [c_void_p, c_size_t, c_void_p]),
+    "vig_causal_conv_step": (c_int, [c_void_p, c_int64, c_void_p, _P64, c_void_p, c_int, c_void_p, c_void_p, c_int64] + [c_int] * 5 + [c_void_p]),
+    "vig_add_layernorm_train_fwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p] * 2 + [c_int] + [c_void_p] * 2 + [c_int64, c_int, c_float, c_int, c_void_p]),
+    "vig_add_layernorm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "vig_add_layernorm_bwd": (c_int, [c_void_p, c_int64] * 3 + [c_void_p, c_int] + [c_void_p, c_int64] + [c_void_p] * 3 + [c_int64, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "vig_linear_int8_fwd": (c_int, [c_void_p, c_int64, c_void_p] * 2 + [c_void_p] * 2 + [c_int64] * 2 + [c_int] * 3 + [c_void_p] * 2),
     "vig_swiglu_fwd": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int64, c_int64, c_int, c_void_p]),
 }
 EXPORTS = tuple(_SIGNATURES)

@@ -19,7 +19,10 @@ namespace py = pybind11;
     X(vig_stem_fold_fwd) X(vig_stem_unfold_fwd) X(vig_stem_conv_ln_fwd)                   \
     X(vig_stem_conv_ln_supported) X(vig_swiglu_fwd) X(vig_add_layernorm_fwd) X(vig_chain_launches) X(vig_token_mean_fwd) X(vig_embed_conv_ln_fwd) X(vig_linear_pair_preferred) X(vig_linear_pair_fwd) X(vig_conv_proj_preferred) X(vig_conv_proj_fwd) X(vig_block_tail_preferred) X(vig_block_tail_fwd) \
     X(vig_gated_recurrence_fwd) X(vig_gated_recurrence_bwd) X(vig_add_rmsnorm_8bit_fwd) X(vig_add_rmsnorm_train_fwd) X(vig_add_rmsnorm_bwd) \
-    X(vig_add_rmsnorm_bwd_workspace_bytes) X(vig_adamw_step) X(vig_gated_recurrence_states_bytes) X(vig_gated_recurrence_train_fwd) X(vig_gated_recurrence_train_bwd)
+    X(vig_add_rmsnorm_bwd_workspace_bytes) X(vig_adamw_step) X(vig_gated_recurrence_states_bytes) X(vig_gated_recurrence_train_fwd) X(vig_gated_recurrence_train_bwd) \
+    X(vig_selective_scan_states_bytes) X(vig_selective_scan_fwd) X(vig_selective_scan_bwd_workspace_bytes) X(vig_selective_scan_bwd) X(vig_selective_scan_step) \
+    X(vig_causal_conv_fwd) X(vig_causal_conv_bwd_workspace_bytes) X(vig_causal_conv_bwd) X(vig_causal_conv_step) X(vig_add_layernorm_train_fwd) \
+    X(vig_add_layernorm_bwd_workspace_bytes) X(vig_add_layernorm_bwd) X(vig_linear_int8_fwd)
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
     VIG_HOST_API(X)
@@ -56,5 +59,6 @@ void bi_gla_into(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
 
 void bind_model(py::module_& m);
 void bind_train(py::module_& m);
+void bind_state_space(py::module_& m);
 
 }  // namespace vig_host

@@ -166,4 +166,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("scan", &scan);
     bind_model(m);
     bind_train(m);
+    bind_state_space(m);
 }

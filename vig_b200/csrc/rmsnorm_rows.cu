@@ -12,7 +12,7 @@
 // launch.  Rows off 16 bytes are read and written a value at a time: 32768 x 767 87 / 122 / 145 us, 768 35 / 37 / 51; rows wider than a CTA's
 // registers (norm_any_kernel, 4096 x 20000) 279 / 307 / 768 us, 0.3 of the bandwidth forward and 0.16 backward.
 #include <cuda_fp8.h>
-#include "common.cuh"
+#include "norm_rows.cuh"
 
 namespace vig {
 
@@ -52,35 +52,6 @@ template <int OUT> __device__ __forceinline__ float scale_of(float top, float* i
     if (s < 1.17549435e-38f) s = 0.f;                            // its reciprocal is no number of this type
     *inv = s > 0.f ? 1.f / s : s;
     return s;
-}
-
-template <typename T> __device__ __forceinline__ float weight_at(const void* w, int i, int w_f32) {
-    return w_f32 ? ((const float*)w)[i] : DType<T>::to_f(((const T*)w)[i]);
-}
-
-constexpr int NT = 256;
-
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-#pragma unroll
-    for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) v += sh[i];
-    return v;
-}
-
-__device__ __forceinline__ float block_top(float v, float* sh) {
-    uint32_t u = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v)));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = __uint_as_float(u);
-    __syncthreads();
-    u = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) u = max(u, __float_as_uint(sh[i]));
-    return __uint_as_float(u);
 }
 
 // Rows too wide for the registers of a CTA (more than 16384 values of 16 bits, 8192 of fp32): a CTA takes a row a value at a time, and reads
@@ -164,9 +135,6 @@ __global__ void __launch_bounds__(NT) norm_bwd_any_kernel(const NormBwdParams p)
     }
 }
 
-// dw = the CTAs' shares, added in a fixed order: 32 channels x 32 warps
-constexpr int DW = 32;
-
 template <typename T>
 __global__ void __launch_bounds__(DW * 32) norm_dw_kernel(const NormBwdParams p) {
     __shared__ float sh[DW][32];
@@ -192,62 +160,6 @@ __global__ void __launch_bounds__(DW * 32) norm_dw_kernel(const NormBwdParams p)
 // row is in flight while it works on one.  Everything about a row that needs the other threads -- the sum of squares and max|r w| --
 // comes out of one reading and one reduction.  TPR below 32: a warp takes several rows; above: a CTA takes one.  Rows that are no whole
 // vectors, or do not begin on 16 bytes, are read and written a value at a time in the same arrangement: the same bits come out.
-template <typename T> __device__ __forceinline__ void take(Vec16<T>& v, const T* row, int vi, int N, int whole) {
-    constexpr int V = DType<T>::VEC;
-    if (whole) {
-        v.load(row + vi * V);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v.e[i] = vi * V + i < N ? row[vi * V + i] : DType<T>::from_f(0.f);
-    }
-}
-template <typename T> __device__ __forceinline__ void give(const Vec16<T>& v, T* row, int vi, int N, int whole) {
-    constexpr int V = DType<T>::VEC;
-    if (whole) {
-        v.store(row + vi * V);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) if (vi * V + i < N) row[vi * V + i] = v.e[i];
-    }
-}
-template <typename T> __device__ __forceinline__ void weights_of(const void* w, int w_f32, int vi, int N, int whole, float* f) {
-    constexpr int V = DType<T>::VEC;
-    if (w_f32) {
-        Vec16<float> v[V / 4];
-#pragma unroll
-        for (int i = 0; i < V / 4; ++i) {
-            take<float>(v[i], (const float*)w, vi * (V / 4) + i, N, whole);
-            v[i].to_float(f + 4 * i);
-        }
-    } else {
-        Vec16<T> v;
-        take<T>(v, (const T*)w, vi, N, whole);
-        v.to_float(f);
-    }
-}
-
-__device__ __forceinline__ float top_of(float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }
-
-// a summed and b summed (or, MAX, its largest value by bits) over the TPR threads of a row
-template <int TPR, bool MAX> __device__ __forceinline__ void over_row(float& a, float& b, float (*sh)[2], int& buf) {
-#pragma unroll
-    for (int m = (TPR < 32 ? TPR : 32) / 2; m; m >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, m);
-        const float o = __shfl_xor_sync(0xffffffffu, b, m);
-        b = MAX ? top_of(b, o) : b + o;
-    }
-    if (TPR > 32) {
-        constexpr int W = TPR / 32;
-        float (*s)[2] = sh + buf * W;                            // two buffers in turn, so that one barrier a reduction is enough
-        buf ^= 1;
-        if ((threadIdx.x & 31) == 0) { s[threadIdx.x >> 5][0] = a; s[threadIdx.x >> 5][1] = b; }
-        __syncthreads();
-        a = s[0][0]; b = s[0][1];
-#pragma unroll
-        for (int i = 1; i < W; ++i) { a += s[i][0]; b = MAX ? top_of(b, s[i][1]) : b + s[i][1]; }
-    }
-}
-
 template <int OUT, int V> __device__ __forceinline__ void store_codes(uint8_t* row, int vi, int N, int whole, const float* t, float rstd, float inv) {
     // y first: rstd times the scale's reciprocal may be out of range where neither is
     uint32_t word[V / 4];
@@ -273,8 +185,6 @@ template <int OUT, int V> __device__ __forceinline__ void store_codes(uint8_t* r
         *(uint32_t*)q = word[0];
     }
 }
-
-template <int TPR> constexpr int norm_threads = TPR > 128 ? TPR : 128;
 
 template <typename T, int OUT, int TPR, int VPT>
 __global__ void __launch_bounds__(norm_threads<TPR>) norm_rows_kernel(const NormParams p) {
@@ -496,21 +406,6 @@ __global__ void __launch_bounds__(norm_bwd_threads<TPR>, norm_bwd_ctas<TPR, VPT 
         }
     }
 }
-
-// CTAs of the backward, whose shares of dw the workspace holds: at most four an SM
-static int norm_blocks(int64_t rows) {
-    const int64_t most = (int64_t)device_sms() * 4;
-    return (int)(rows < most ? rows : most);
-}
-
-// threads a row of nv vectors: a power of two of which three or four vectors a thread make the row (fewer where a group or a warp wants more)
-static int threads_a_row(int nv, int least) {
-    int tpr = least;
-    while (tpr * 4 < nv) tpr *= 2;
-    return tpr;
-}
-
-static bool on_16(const void* q, int64_t ld, int size) { return (uintptr_t)q % 16 == 0 && ld * size % 16 == 0; }
 
 template <typename T, int OUT, int TPR> int norm_rows_launch(const NormParams& p, int nv, cudaStream_t s) {
     constexpr int THREADS = norm_threads<TPR>, RPB = THREADS / TPR;

@@ -1,0 +1,207 @@
+// What the forward and the backward of the selective scan share: how a CTA's tile of tokens lies in shared memory, how its lanes divide it, and
+// the scan of a warp's runs.
+//
+// A CTA has WARPS warps and CT = WARPS * CPW channels of one sequence and goes over its tokens in tiles of 64.  A warp takes one of its channels
+// at a time: lane = 4 * run + part, a run being 8 tokens and a part S of the NB = 4 S states that are gone over together.  So the work of a
+// channel and tile is 8 x S products a lane, two values to an instruction (f32x2); the eight runs are joined by a scan over the lanes, and no
+// warp waits for another one within a tile.  Maps (B and C, the same for all channels of a group) stay in registers over a warp's channels.
+#pragma once
+#include "tc_common.cuh"
+
+namespace vig {
+namespace scan {
+
+using namespace tc;
+
+constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 64, RUN = 8, PARTS = 4;
+constexpr unsigned ALL = 0xffffffffu;
+
+// where the row of token t of a tile lies: eight lanes that read token j of their runs read eight neighbouring rows
+__device__ __forceinline__ int row_of(int t) { return (t % RUN) * RUN + t / RUN; }
+
+template <typename T> __device__ __forceinline__ float param_at(const void* p, int i, int f32) { return f32 ? ((const float*)p)[i] : DType<T>::to_f(((const T*)p)[i]); }
+
+// max(x, 0) + log(1 + exp(-|x|)); log1p, because a step of 1e-4 has to keep its own precision
+template <typename T> __device__ __forceinline__ float softplus(float x) {
+    const float e = sizeof(T) == 4 ? expf(-fabsf(x)) : __expf(-fabsf(x));
+    return fmaxf(x, 0.f) + log1pf(e);
+}
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy8(void* dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy4(void* dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// NC values from global into shared memory, where they begin on their own size: `wide` of them in a piece (what pointers and strides allow), or
+// one at a time; values from `have` on are zeros
+template <typename T, int NC> __device__ __forceinline__ void fetch(T* dst, const T* src, int have, int piece_bytes) {
+    constexpr int BYTES = NC * (int)sizeof(T);
+    if (have >= NC && piece_bytes >= 4) {
+        if (BYTES % 16 == 0 && piece_bytes >= 16) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) copy16((char*)dst + 16 * i, (const char*)src + 16 * i);
+            return;
+        }
+        if (BYTES % 8 == 0 && piece_bytes >= 8) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 8; ++i) copy8((char*)dst + 8 * i, (const char*)src + 8 * i);
+            return;
+        }
+        if (BYTES % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 4; ++i) copy4((char*)dst + 4 * i, (const char*)src + 4 * i);
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) dst[i] = i < have ? src[i] : DType<T>::from_f(0.f);
+}
+
+// NC values out of registers, as far as they exist
+template <typename T, int NC> __device__ __forceinline__ void put(T* dst, const float* v, int have, int piece_bytes) {
+    T e[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) e[i] = DType<T>::from_f(v[i]);
+    constexpr int BYTES = NC * (int)sizeof(T);
+    if (have >= NC) {
+        if (BYTES % 16 == 0 && piece_bytes >= 16) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) { uint4 w; memcpy(&w, (const char*)e + 16 * i, 16); ((uint4*)dst)[i] = w; }
+            return;
+        }
+        if (BYTES % 8 == 0 && piece_bytes >= 8) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 8; ++i) { uint2 w; memcpy(&w, (const char*)e + 8 * i, 8); ((uint2*)dst)[i] = w; }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) if (i < have) dst[i] = e[i];
+}
+
+// One value for each of 8 tokens and 4 parts, summed over the parts; part p keeps tokens 2 p and 2 p + 1
+__device__ __forceinline__ float2 over_parts(const float* v, int part) {
+    float w[4];
+    const bool hi = part & 2, odd = part & 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (hi ? v[4 + i] : v[i]) + __shfl_xor_sync(ALL, hi ? v[i] : v[4 + i], 2);
+    float2 r;
+    r.x = (odd ? w[2] : w[0]) + __shfl_xor_sync(ALL, odd ? w[0] : w[2], 1);
+    r.y = (odd ? w[3] : w[1]) + __shfl_xor_sync(ALL, odd ? w[1] : w[3], 1);
+    return r;
+}
+
+__device__ __forceinline__ F2 f2_shfl_up(F2 v, int lanes) { return f2_make(__shfl_up_sync(ALL, f2_lo(v), lanes), __shfl_up_sync(ALL, f2_hi(v), lanes)); }
+__device__ __forceinline__ F2 f2_shfl_down(F2 v, int lanes) { return f2_make(__shfl_down_sync(ALL, f2_lo(v), lanes), __shfl_down_sync(ALL, f2_hi(v), lanes)); }
+__device__ __forceinline__ F2 f2_shfl(F2 v, int lane) { return f2_make(__shfl_sync(ALL, f2_lo(v), lane), __shfl_sync(ALL, f2_hi(v), lane)); }
+
+// decays of a run, exp(delta A) with A in log2 units
+template <int S> __device__ __forceinline__ void decays(F2 (*a)[S / 2], const float* delta, const F2* A2) {
+#pragma unroll
+    for (int j = 0; j < RUN; ++j)
+#pragma unroll
+        for (int s = 0; s < S / 2; ++s) {
+            const F2 x = f2_mul(f2_make(delta[j], delta[j]), A2[s]);
+            a[j][s] = f2_make(ex2(f2_lo(x)), ex2(f2_hi(x)));
+        }
+}
+
+// The state that enters each lane's run, h = a h + x B over the tile; h0: the state that enters the tile.  A run's own sum E (run 0's on top of h0)
+// and the product P of its decays are joined over the lanes by doubling.  An infinite state times a product that has left the type's range
+// would be a NaN where the recurrence token by token keeps the infinity: with a sum that is not finite the runs follow one another.
+template <int S> __device__ __forceinline__ void entering(F2* in, const F2* h0, const F2 (*a)[S / 2], const F2 (*b)[S / 2], const float* x, int run, int lane) {
+    F2 P[S / 2], E[S / 2];
+#pragma unroll
+    for (int s = 0; s < S / 2; ++s) { P[s] = a[0][s]; E[s] = run == 0 ? h0[s] : 0ull; }
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+        const F2 xj = f2_make(x[j], x[j]);
+#pragma unroll
+        for (int s = 0; s < S / 2; ++s) {
+            E[s] = f2_fma(a[j][s], E[s], f2_mul(xj, b[j][s]));
+            if (j) P[s] = f2_mul(P[s], a[j][s]);
+        }
+    }
+    F2 probe = 0ull;                                             // 0, or NaN
+#pragma unroll
+    for (int s = 0; s < S / 2; ++s) probe = f2_fma(E[s], 0ull, probe);
+    if (__any_sync(ALL, !(f2_lo(probe) + f2_hi(probe) == 0.f))) {
+        F2 now[S / 2];
+#pragma unroll
+        for (int s = 0; s < S / 2; ++s) now[s] = h0[s];
+#pragma unroll 1
+        for (int r = 0; r < RUN; ++r) {
+            F2 end[S / 2];
+#pragma unroll
+            for (int s = 0; s < S / 2; ++s) { if (run == r) in[s] = now[s]; end[s] = now[s]; }
+#pragma unroll
+            for (int j = 0; j < RUN; ++j)
+#pragma unroll
+                for (int s = 0; s < S / 2; ++s) end[s] = f2_fma(a[j][s], end[s], f2_mul(f2_make(x[j], x[j]), b[j][s]));
+#pragma unroll
+            for (int s = 0; s < S / 2; ++s) now[s] = f2_shfl(end[s], r * PARTS + lane % PARTS);
+        }
+        return;
+    }
+#pragma unroll
+    for (int d = 1; d < RUN; d *= 2) {
+#pragma unroll
+        for (int s = 0; s < S / 2; ++s) {
+            const F2 e = f2_shfl_up(E[s], d * PARTS);
+            E[s] = f2_fma(P[s], run >= d ? e : 0ull, E[s]);
+            if (2 * d < RUN) P[s] = f2_mul(P[s], f2_shfl_up(P[s], d * PARTS));
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < S / 2; ++s) {
+        const F2 e = f2_shfl_up(E[s], PARTS);
+        in[s] = run == 0 ? h0[s] : e;
+    }
+}
+
+// S values of a row in shared memory, as pairs
+template <typename T, int S> __device__ __forceinline__ void pairs(F2* out, const T* row) {
+    T e[S];
+    if constexpr (S * sizeof(T) == 16) { const uint4 w = *(const uint4*)row; memcpy(e, &w, 16); }
+    else if constexpr (S * sizeof(T) == 8) { const uint2 w = *(const uint2*)row; memcpy(e, &w, 8); }
+    else { const uint32_t w = *(const uint32_t*)row; memcpy(e, &w, 4); }
+#pragma unroll
+    for (int s = 0; s < S / 2; ++s) out[s] = f2_make(DType<T>::to_f(e[2 * s]), DType<T>::to_f(e[2 * s + 1]));
+}
+
+struct Params {
+    const void *u, *dt, *z, *b, *c, *skip, *bias, *dy;
+    const float *A, *h0, *d_final;
+    const int32_t* lengths;
+    void *y, *d_u, *d_dt, *d_z;
+    float *h_final, *states, *d_h0;
+    float *part_b, *part_c, *part_A, *part_skip, *part_bias;     // shares of the gradients that are sums: [channel tiles of a group][B, L, G, N], [B][D, N], [B][D]
+    int64_t s_u[2], s_dt[2], s_z[2], s_y[2], s_dy[2], s_b[3], s_c[3], ld_h0, ld_final;
+    int B, L, D, N, G, skip_f32, bias_f32, softplus;
+    int tiles, ctiles;                                           // tiles of tokens; CTAs of a group's channels
+    int piece, piece_maps, piece_state;                          // bytes of a copy that pointers and strides allow: rows, maps, states
+};
+
+// a length is a number from 0 to L, whatever the caller's memory holds
+__device__ __forceinline__ int length_of(const Params& p, int b) { return p.lengths ? min(max(p.lengths[b], 0), p.L) : p.L; }
+
+// [64 tokens][Npad] of a map of this tile; tokens from `len` on and states from N on are zeros
+template <typename T> __device__ __forceinline__ void fetch_map(T* dst, const T* src, int64_t stride, int t0, int len, int N, int Npad, int piece) {
+    if (piece >= 16) {
+        const int n16 = Npad * (int)sizeof(T) / 16, have = N * (int)sizeof(T) / 16;
+        for (int i = threadIdx.x; i < TILE * n16; i += THREADS) {
+            const int t = i / n16, k = i - t * n16;
+            char* to = (char*)(dst + row_of(t) * Npad) + 16 * k;
+            if (t0 + t < len && k < have) copy16(to, (const char*)(src + (t0 + t) * stride) + 16 * k);
+            else *(uint4*)to = make_uint4(0u, 0u, 0u, 0u);
+        }
+    } else {
+        for (int i = threadIdx.x; i < TILE * Npad; i += THREADS) {
+            const int t = i / Npad, n = i - t * Npad;
+            dst[row_of(t) * Npad + n] = t0 + t < len && n < N ? src[(t0 + t) * stride + n] : DType<T>::from_f(0.f);
+        }
+    }
+}
+
+}  // namespace scan
+}  // namespace vig
