@@ -445,7 +445,7 @@ VIG_API int vig_adamw_step(int count, void* const* params, const void* const* gr
  * Selective scan: delta = softplus(dt + dt_bias) (softplus 0: dt + dt_bias), h_t[d,n] = exp(delta_t[d] A[d,n]) h_{t-1}[d,n] + delta_t[d] u_t[d] b_t[n],
  * y_t[d] = (sum_n c_t[n] h_t[d,n] + skip[d] u_t[d]) silu(z_t[d]).  All pointers are device pointers; optional ones are NULL.
  *   u, dt, z (optional), y, d_y: [B, L, D] of dtype, unit stride over D, element strides (b, l).  b, c: [B, L, G, N] of dtype, unit stride over N,
- *   strides (b, l, g); channel d reads group d / (D / G), D % G == 0, 1 <= N <= 128.  A: fp32 [D, N] contiguous.  skip, dt_bias (optional): [D] of
+ *   strides (b, l, g); channel d reads group d / (D / G), D % G == 0, 1 <= N <= 64.  A: fp32 [D, N] contiguous.  skip, dt_bias (optional): [D] of
  *   skip_dtype, bias_dtype (dtype or fp32).  lengths (optional): int32 [B], tokens of a sequence that count (taken into 0..L): behind them y
  *   and gradients are zeros and states stay.  h0 (optional), h_final (optional): fp32 [B, D, N], sequences ld_h0 / ld_final apart, channels N apart;
  *   h_final may be h0.  Any alignment.  B * D < 2^31, D < 2^28, L < 2^30.
@@ -454,6 +454,7 @@ VIG_API int vig_adamw_step(int count, void* const* params, const void* const* gr
  *   d_c [B, L, G, N] of dtype, d_A fp32 [D, N], d_skip, d_bias (optional) [D] of their types, d_h0 (optional) fp32 [B, D, N], all contiguous.  Sums over
  *   channels, tokens and sequences are fp32 in a fixed order.
  * vig_selective_scan_step: L = 1; h_final is the state, updated in place (h0 and lengths are not looked at).
+ * status: optional int32 on the device, bit 0 = a bounded wait ran out.
  */
 typedef struct vig_selective_scan_args {
     int32_t B, L, D, N, G, dtype, skip_dtype, bias_dtype, softplus, reserved;
@@ -477,6 +478,7 @@ typedef struct vig_selective_scan_args {
     float* d_h0;
     void* workspace;
     size_t workspace_bytes;
+    int32_t* status;
 } vig_selective_scan_args;
 VIG_API size_t vig_selective_scan_states_bytes(int B, int L, int D, int N);
 VIG_API int vig_selective_scan_fwd(const vig_selective_scan_args* args, void* stream);

@@ -68,7 +68,7 @@ void check_scan(const Scan& s, int dim) {
     want_type(s.A.scalar_type() == at::kFloat, "A must be float32");
     want(s.A.dim() == 2 && s.A.size(0) == D && s.A.is_contiguous(), "A must be a contiguous [D, N] tensor; got " + shape_of(s.A));
     const int64_t N = s.A.size(1);
-    want(N >= 1 && N <= 128, "1 to 128 states a channel are supported; got " + std::to_string(N));
+    want(N >= 1 && N <= 64, "1 to 64 states a channel are supported; got " + std::to_string(N));
     for (const auto& [t, name] : {std::pair<const Tensor*, const char*>{&s.B, "B"}, {&s.C, "C"}}) {
         same_device(*t, u, name);
         want_type(t->scalar_type() == u.scalar_type(), std::string(name) + " must have u's dtype");
@@ -102,6 +102,7 @@ vig_selective_scan_args scan_args(const Scan& s, bool softplus) {
     rows(a.s_u, s.u); rows(a.s_dt, s.dt); rows(a.s_z, s.z);
     const auto maps = [&](int64_t* to, const Tensor& t) { rows(to, t); to[2] = t.dim() == dim + 1 ? t.stride(dim - 1) : 0; };
     maps(a.s_b, s.B); maps(a.s_c, s.C);
+    a.status = status_ptr(s.u.get_device());
     return a;
 }
 
@@ -161,20 +162,22 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
     }
 };
 
-std::pair<Tensor, OptT> selective_scan(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const OptT& D, const OptT& z, const OptT& bias,
+// nullopt: the device's error word has to be registered first
+std::optional<std::pair<Tensor, OptT>> selective_scan(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const OptT& D, const OptT& z, const OptT& bias,
                                        const OptT& h0, bool want_final, bool softplus, const OptT& lengths) {
     Scan s{u, dt, A, B, C, get(D), get(z), get(bias), get(h0), Tensor()};
     check_scan(s, 3);
+    if (!status_known(u.get_device())) return std::nullopt;
     if (s.h0.defined()) check_states(s.h0, s, "initial_state");
     no_tangents({&u, &dt, &A, &B, &C, &s.D, &s.z, &s.bias, &s.h0});
     c10::cuda::CUDAGuard dev(u.device());
     s.lengths = lengths_of(lengths, u);
     if (wants_grad({&u, &dt, &A, &B, &C, &s.D, &s.z, &s.bias, &s.h0})) {
         const auto out = ScanNode::apply(u, dt, A, B, C, D, z, bias, h0, s.lengths.defined() ? OptT(s.lengths) : OptT(), want_final, softplus);
-        return {out[0], want_final ? OptT(out[1]) : OptT()};
+        return std::make_pair(out[0], want_final ? OptT(out[1]) : OptT());
     }
     const auto [y, fin] = scan_forward(s, want_final, softplus, nullptr);
-    return {y, want_final ? OptT(fin) : OptT()};
+    return std::make_pair(y, want_final ? OptT(fin) : OptT());
 }
 
 Tensor selective_scan_step(const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Tensor& state, const OptT& D, const OptT& z, const OptT& bias,

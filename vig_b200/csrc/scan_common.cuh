@@ -1,10 +1,11 @@
-// What the forward and the backward of the selective scan share: how a CTA's tile of tokens lies in shared memory, how its lanes divide it, and
-// the scan of a warp's runs.
+// What the forward and the backward of the selective scan share: how the lanes of a warp divide a tile of tokens, and how states go from tile to tile.
 //
-// A CTA has WARPS warps and CT = WARPS * CPW channels of one sequence and goes over its tokens in tiles of 64.  A warp takes one of its channels
-// at a time: lane = 4 * run + part, a run being 8 tokens and a part S of the NB = 4 S states that are gone over together.  So the work of a
-// channel and tile is 8 x S products a lane, two values to an instruction (f32x2); the eight runs are joined by a scan over the lanes, and no
-// warp waits for another one within a tile.  Maps (B and C, the same for all channels of a group) stay in registers over a warp's channels.
+// A CTA has CT neighbouring channels of one sequence, and each of its warps a tile of 64 tokens at a time: warp w tiles w, w + W, w + 2 W, ...  Within a tile a
+// warp takes one channel after the other: lane = 4 * run + part, a run being 8 tokens and a part S of the NB = 4 S states that are gone over together.  So
+// the work of a channel and tile is 8 x S products a lane, two values to an instruction (f32x2); the eight runs are joined by a scan over the lanes.
+// The state that enters a tile comes from the warp of the tile before through shared memory (`carry`): everything that does not depend on it is done before it
+// is waited for, and what the next warp needs is sent on before the outputs are computed.  Warps meet nowhere else: while one waits for its rows,
+// others compute.  The maps (B and C, the same for all channels of a group) are read once for a tile.
 #pragma once
 #include "tc_common.cuh"
 
@@ -13,7 +14,7 @@ namespace scan {
 
 using namespace tc;
 
-constexpr int WARPS = 4, THREADS = 32 * WARPS, TILE = 64, RUN = 8, PARTS = 4;
+constexpr int TILE = 64, RUN = 8, PARTS = 4;
 constexpr unsigned ALL = 0xffffffffu;
 
 // where the row of token t of a tile lies: eight lanes that read token j of their runs read eight neighbouring rows
@@ -21,59 +22,76 @@ __device__ __forceinline__ int row_of(int t) { return (t % RUN) * RUN + t / RUN;
 
 template <typename T> __device__ __forceinline__ float param_at(const void* p, int i, int f32) { return f32 ? ((const float*)p)[i] : DType<T>::to_f(((const T*)p)[i]); }
 
-// max(x, 0) + log(1 + exp(-|x|)); log1p, because a step of 1e-4 has to keep its own precision
-template <typename T> __device__ __forceinline__ float softplus(float x) {
-    const float e = sizeof(T) == 4 ? expf(-fabsf(x)) : __expf(-fabsf(x));
-    return fmaxf(x, 0.f) + log1pf(e);
+// Of a pair of values, max(x, 0) + log(1 + e), e = exp(-|x|): a step of 1e-4 has to keep its own precision, so log(1 + e) is e times a polynomial of least
+// relative error on [0, 1] (3e-8, by exchange; 1.7e-7 with fp32 arithmetic).
+template <typename T> __device__ __forceinline__ F2 softplus(F2 x) {
+    const float lo = f2_lo(x), hi = f2_hi(x);
+    const F2 e = sizeof(T) == 4 ? f2_make(expf(-fabsf(lo)), expf(-fabsf(hi))) : f2_make(ex2(-fabsf(lo) * LOG2E), ex2(-fabsf(hi) * LOG2E));
+    constexpr float c[] = {0.99999994f, -0.499994934f, 0.333190978f, -0.24842982f, 0.191060066f, -0.136632457f, 0.0782259554f, -0.0295052417f, 0.00523269456f};
+    F2 s = f2_make(c[8], c[8]);
+#pragma unroll
+    for (int i = 7; i >= 0; --i) s = f2_fma(s, e, f2_make(c[i], c[i]));
+    return f2_fma(s, e, f2_make(fmaxf(lo, 0.f), fmaxf(hi, 0.f)));
 }
+__device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-x * LOG2E)); }
 
 __device__ __forceinline__ void copy16(void* dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy8(void* dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(void* dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// NC values from global into shared memory, where they begin on their own size: `wide` of them in a piece (what pointers and strides allow), or
-// one at a time; values from `have` on are zeros
-template <typename T, int NC> __device__ __forceinline__ void fetch(T* dst, const T* src, int have, int piece_bytes) {
+// NC values of a row into shared memory of the lane's own: in pieces of what pointers and strides allow, or one at a time; values from `have` on are zeros
+template <typename T, int NC> __device__ __forceinline__ void fetch(T* dst, const T* src, int have, int piece) {
     constexpr int BYTES = NC * (int)sizeof(T);
-    if (have >= NC && piece_bytes >= 4) {
-        if (BYTES % 16 == 0 && piece_bytes >= 16) {
+    if (have >= NC && piece >= 8) {
+        if (BYTES % 16 == 0 && piece >= 16) {
 #pragma unroll
             for (int i = 0; i < BYTES / 16; ++i) copy16((char*)dst + 16 * i, (const char*)src + 16 * i);
-            return;
-        }
-        if (BYTES % 8 == 0 && piece_bytes >= 8) {
+        } else {
 #pragma unroll
             for (int i = 0; i < BYTES / 8; ++i) copy8((char*)dst + 8 * i, (const char*)src + 8 * i);
-            return;
         }
-        if (BYTES % 4 == 0) {
-#pragma unroll
-            for (int i = 0; i < BYTES / 4; ++i) copy4((char*)dst + 4 * i, (const char*)src + 4 * i);
-            return;
-        }
+        return;
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) dst[i] = i < have ? src[i] : DType<T>::from_f(0.f);
 }
 
+// the same into registers, from either memory
+template <typename T, int NC> __device__ __forceinline__ void read(float* f, const T* src, int have, int piece) {
+    constexpr int BYTES = NC * (int)sizeof(T);
+    T e[NC];
+    if (have >= NC && piece >= 8) {
+        if (BYTES % 16 == 0 && piece >= 16) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) { const uint4 w = ((const uint4*)src)[i]; memcpy((char*)e + 16 * i, &w, 16); }
+        } else {
+#pragma unroll
+            for (int i = 0; i < BYTES / 8; ++i) { const uint2 w = ((const uint2*)src)[i]; memcpy((char*)e + 8 * i, &w, 8); }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) e[i] = i < have ? src[i] : DType<T>::from_f(0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) f[i] = DType<T>::to_f(e[i]);
+}
+
 // NC values out of registers, as far as they exist
-template <typename T, int NC> __device__ __forceinline__ void put(T* dst, const float* v, int have, int piece_bytes) {
+template <typename T, int NC> __device__ __forceinline__ void put(T* dst, const float* v, int have, int piece) {
     T e[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) e[i] = DType<T>::from_f(v[i]);
     constexpr int BYTES = NC * (int)sizeof(T);
-    if (have >= NC) {
-        if (BYTES % 16 == 0 && piece_bytes >= 16) {
+    if (have >= NC && piece >= 8) {
+        if (BYTES % 16 == 0 && piece >= 16) {
 #pragma unroll
             for (int i = 0; i < BYTES / 16; ++i) { uint4 w; memcpy(&w, (const char*)e + 16 * i, 16); ((uint4*)dst)[i] = w; }
-            return;
-        }
-        if (BYTES % 8 == 0 && piece_bytes >= 8) {
+        } else {
 #pragma unroll
             for (int i = 0; i < BYTES / 8; ++i) { uint2 w; memcpy(&w, (const char*)e + 8 * i, 8); ((uint2*)dst)[i] = w; }
-            return;
         }
+        return;
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) if (i < have) dst[i] = e[i];
@@ -106,25 +124,27 @@ template <int S> __device__ __forceinline__ void decays(F2 (*a)[S / 2], const fl
         }
 }
 
-// The state that enters each lane's run, h = a h + x B over the tile; h0: the state that enters the tile.  A run's own sum E (run 0's on top of h0)
-// and the product P of its decays are joined over the lanes by doubling.  An infinite state times a product that has left the type's range
-// would be a NaN where the recurrence token by token keeps the infinity: with a sum that is not finite the runs follow one another.
-template <int S> __device__ __forceinline__ void entering(F2* in, const F2* h0, const F2 (*a)[S / 2], const F2 (*b)[S / 2], const float* x, int run, int lane) {
-    F2 P[S / 2], E[S / 2];
-#pragma unroll
-    for (int s = 0; s < S / 2; ++s) { P[s] = a[0][s]; E[s] = run == 0 ? h0[s] : 0ull; }
+// A run's own sum E of h = a h + x B, from nothing, and the product P of its decays
+template <int S> __device__ __forceinline__ void own_sum(F2* P, F2* E, const F2 (*a)[S / 2], const F2 (*b)[S / 2], const float* x) {
 #pragma unroll
     for (int j = 0; j < RUN; ++j) {
         const F2 xj = f2_make(x[j], x[j]);
 #pragma unroll
         for (int s = 0; s < S / 2; ++s) {
-            E[s] = f2_fma(a[j][s], E[s], f2_mul(xj, b[j][s]));
-            if (j) P[s] = f2_mul(P[s], a[j][s]);
+            const F2 in = f2_mul(xj, b[j][s]);
+            E[s] = j ? f2_fma(a[j][s], E[s], in) : in;
+            P[s] = j ? f2_mul(P[s], a[j][s]) : a[j][s];
         }
     }
+}
+
+// The state that enters each lane's run, from the runs' own sums and the state h0 that enters the tile; E of the last run becomes what leaves the tile.  Runs
+// are joined over the lanes by doubling.  An infinite state times a product that has left the type's range would be a NaN where the recurrence token by
+// token keeps the infinity: with a sum that is not finite the runs follow one another.
+template <int S> __device__ __forceinline__ void entering(F2* in, F2* E, F2* P, const F2* h0, const F2 (*a)[S / 2], const F2 (*b)[S / 2], const float* x, int run, int part) {
     F2 probe = 0ull;                                             // 0, or NaN
 #pragma unroll
-    for (int s = 0; s < S / 2; ++s) probe = f2_fma(E[s], 0ull, probe);
+    for (int s = 0; s < S / 2; ++s) probe = f2_fma(h0[s], 0ull, f2_fma(E[s], 0ull, probe));
     if (__any_sync(ALL, !(f2_lo(probe) + f2_hi(probe) == 0.f))) {
         F2 now[S / 2];
 #pragma unroll
@@ -139,10 +159,14 @@ template <int S> __device__ __forceinline__ void entering(F2* in, const F2* h0, 
 #pragma unroll
                 for (int s = 0; s < S / 2; ++s) end[s] = f2_fma(a[j][s], end[s], f2_mul(f2_make(x[j], x[j]), b[j][s]));
 #pragma unroll
-            for (int s = 0; s < S / 2; ++s) now[s] = f2_shfl(end[s], r * PARTS + lane % PARTS);
+            for (int s = 0; s < S / 2; ++s) now[s] = f2_shfl(end[s], r * PARTS + part);
         }
+#pragma unroll
+        for (int s = 0; s < S / 2; ++s) E[s] = now[s];
         return;
     }
+#pragma unroll
+    for (int s = 0; s < S / 2; ++s) E[s] = f2_fma(P[s], run == 0 ? h0[s] : 0ull, E[s]);
 #pragma unroll
     for (int d = 1; d < RUN; d *= 2) {
 #pragma unroll
@@ -158,6 +182,30 @@ template <int S> __device__ __forceinline__ void entering(F2* in, const F2* h0, 
         in[s] = run == 0 ? h0[s] : e;
     }
 }
+
+// What a tile's warp leaves for the warp of the next one: the flag counts the tiles that are through.  A wait is bounded; one that runs out raises the status and
+// the CTA's flag, after which nobody waits any more.
+struct Handover {
+    volatile int* given_up;
+    int32_t* status;
+    __device__ __forceinline__ void await(const uint32_t* flag, uint32_t want) const {
+        const uint32_t addr = smem_u32(flag);
+        uint32_t got;
+#pragma unroll 1
+        for (uint32_t i = 0;; ++i) {
+            asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(got) : "r"(addr) : "memory");
+            if (__all_sync(ALL, got == want)) return;
+            if (i >= (1u << 21) || __any_sync(ALL, *given_up)) break;
+            if (i > 8) __nanosleep(32);
+        }
+        *given_up = 1;
+        if (status && (threadIdx.x & 31) == 0) atomicOr(status, 1);
+    }
+    __device__ __forceinline__ void pass(uint32_t* flag, uint32_t value) const {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(flag)), "r"(value) : "memory");
+    }
+};
 
 // S values of a row in shared memory, as pairs
 template <typename T, int S> __device__ __forceinline__ void pairs(F2* out, const T* row) {
@@ -178,6 +226,7 @@ struct Params {
     float *part_b, *part_c, *part_A, *part_skip, *part_bias;     // shares of the gradients that are sums: [channel tiles of a group][B, L, G, N], [B][D, N], [B][D]
     int64_t s_u[2], s_dt[2], s_z[2], s_y[2], s_dy[2], s_b[3], s_c[3], ld_h0, ld_final;
     int B, L, D, N, G, skip_f32, bias_f32, softplus;
+    int32_t* status;
     int tiles, ctiles;                                           // tiles of tokens; CTAs of a group's channels
     int piece, piece_maps, piece_state;                          // bytes of a copy that pointers and strides allow: rows, maps, states
 };
@@ -185,21 +234,22 @@ struct Params {
 // a length is a number from 0 to L, whatever the caller's memory holds
 __device__ __forceinline__ int length_of(const Params& p, int b) { return p.lengths ? min(max(p.lengths[b], 0), p.L) : p.L; }
 
-// [64 tokens][Npad] of a map of this tile; tokens from `len` on and states from N on are zeros
-template <typename T> __device__ __forceinline__ void fetch_map(T* dst, const T* src, int64_t stride, int t0, int len, int N, int Npad, int piece) {
+// [64 tokens][Npad] of a map of this tile, by a warp; tokens from `len` on and states from N on are zeros
+template <typename T> __device__ __forceinline__ void fetch_map(T* dst, const T* src, int64_t stride, int64_t t0, int len, int N, int Npad, int piece, int lane) {
     if (piece >= 16) {
         const int n16 = Npad * (int)sizeof(T) / 16, have = N * (int)sizeof(T) / 16;
-        for (int i = threadIdx.x; i < TILE * n16; i += THREADS) {
-            const int t = i / n16, k = i - t * n16;
-            char* to = (char*)(dst + row_of(t) * Npad) + 16 * k;
-            if (t0 + t < len && k < have) copy16(to, (const char*)(src + (t0 + t) * stride) + 16 * k);
-            else *(uint4*)to = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int t = lane; t < TILE; t += 32) {
+            char* to = (char*)(dst + row_of(t) * Npad);
+            const char* from = (const char*)(src + (t0 + t) * stride);
+            for (int k = 0; k < n16; ++k) {
+                if (t0 + t < len && k < have) copy16(to + 16 * k, from + 16 * k);
+                else *(uint4*)(to + 16 * k) = make_uint4(0u, 0u, 0u, 0u);
+            }
         }
     } else {
-        for (int i = threadIdx.x; i < TILE * Npad; i += THREADS) {
-            const int t = i / Npad, n = i - t * Npad;
-            dst[row_of(t) * Npad + n] = t0 + t < len && n < N ? src[(t0 + t) * stride + n] : DType<T>::from_f(0.f);
-        }
+        for (int t = lane; t < TILE; t += 32)
+            for (int n = 0; n < Npad; ++n) dst[row_of(t) * Npad + n] = t0 + t < len && n < N ? src[(t0 + t) * stride + n] : DType<T>::from_f(0.f);
     }
 }
 

@@ -4,117 +4,130 @@
 //   y_t[d] = (sum_n C_t[n] h_t[d, n] + D[d] u_t[d]) silu(z_t[d]).
 //
 // Every (token, channel, state) costs an exponential and three multiply-adds, every (token, channel) three 16-bit values in and one out: with 16
-// states the exponentials bound it (MUFU, 16 a cycle and SM), not memory.  So each is taken once: a CTA walks its channels' tokens in tiles, and
-// within a tile a warp's lanes divide tokens and states (scan_common.cuh) and join their runs by a scan over the lanes, where two passes over
+// states the exponentials bound it (MUFU, 16 a cycle and SM), not memory.  So each is taken once: the warps of a CTA take tiles of the same channels'
+// tokens in turn and hand the state from tile to tile, within a tile a warp's lanes divide tokens and states (scan_common.cuh); two passes over
 // independent chunks would take every exponential twice.
 #include "scan_common.cuh"
 
 namespace vig {
 using namespace scan;
 
-template <typename T, int S, int CPW> struct FwdSmem {
-    static constexpr int NC = 2 * CPW, CT = WARPS * CPW;         // channels of a thread ahead of and behind the scan, of the CTA
-    static constexpr int SLOT = NC * (int)sizeof(T), ROWS = 3 * THREADS * SLOT;
-    static __host__ __device__ int padded(int N) { return (N + 4 * S - 1) / (4 * S) * (4 * S); }
-    static int bytes(int N) { return 2 * ROWS + 4 * TILE * padded(N) * (int)sizeof(T) + 3 * CT * TILE * 4 + 2 * CT * padded(N) * 4; }
+// Shared memory: for every warp the rows of u, dt and z, the maps, and steps and inputs a channel at a time; for the CTA A, the states between tiles and
+// their flags, bias and skip.
+template <typename T, int S, int CT> struct FwdSmem {
+    static constexpr int NB = 4 * S, ROWS = TILE * CT * (int)sizeof(T);
+    static __host__ __device__ int padded(int N) { return (N + NB - 1) / NB * NB; }
+    static __host__ __device__ int warp_bytes(int N) {
+        const int Np = padded(N);
+        return 3 * ROWS + 2 * TILE * Np * (int)sizeof(T) + (Np > NB ? 3 : 2) * CT * TILE * 4;
+    }
+    static int bytes(int N, int W) { return W * warp_bytes(N) + (2 * CT * padded(N) + CT * padded(N) / NB + 2 * CT + 4) * 4; }
 };
 
-template <typename T, int S, int CPW>
-__global__ void __launch_bounds__(THREADS, 3) scan_fwd_kernel(const Params p) {
-    using M = FwdSmem<T, S, CPW>;
-    constexpr int NC = M::NC, CT = M::CT, NB = 4 * S;
+template <typename T, int S, int CT, int W>
+__global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kernel(const Params p) {
+    using M = FwdSmem<T, S, CT>;
+    constexpr int NB = M::NB, THREADS = 32 * W;
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, run = lane / PARTS, part = lane % PARTS;
     const int Npad = M::padded(p.N), Dg = p.D / p.G;
     const int ct = blockIdx.x % p.ctiles, g = blockIdx.x / p.ctiles % p.G, b = blockIdx.x / p.ctiles / p.G;
-    const int c0 = ct * CT, have = min(CT, Dg - c0), d0 = g * Dg + c0;            // channels of the CTA, the first one's index
+    const int c0 = ct * CT, have = min(CT, Dg - c0), d = g * Dg + c0;             // channels of the CTA, the first one's index
     const int len = length_of(p, b), ntiles = (len + TILE - 1) / TILE;
-    T* const slots = (T*)smem;
-    T* const maps = (T*)(smem + 2 * M::ROWS);
-    float* const delta = (float*)(maps + 4 * TILE * Npad);
-    float* const x = delta + CT * TILE;
-    float* const ys = x + CT * TILE;
-    float* const sA = ys + CT * TILE;
-    float* const sh = sA + CT * Npad;
+    char* const mine = smem + warp * M::warp_bytes(p.N);
+    T *const ru = (T*)mine, *const rdt = ru + TILE * CT, *const rz = rdt + TILE * CT, *const mB = rz + TILE * CT, *const mC = mB + TILE * Npad;
+    float *const delta = (float*)(mC + TILE * Npad), *const x = delta + CT * TILE;
+    float* const ys = Npad > NB ? x + CT * TILE : delta;         // with one block of states a channel's steps are done with when its sums are there
+    float *const sA = (float*)(smem + W * M::warp_bytes(p.N)), *const carry = sA + CT * Npad, *const bias = carry + CT * Npad, *const skip = bias + CT;
+    uint32_t* const flags = (uint32_t*)(skip + CT);
+    int* const given_up = (int*)(flags + CT * Npad / NB);
+    const Handover hand{given_up, p.status};
 
-    // ahead of and behind the scan a thread has one token and NC channels
-    const int t = tid % TILE, cl = tid / TILE * NC, mine = min(max(have - cl, 0), NC), d = d0 + cl;
-    float bias[NC], skip[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        bias[i] = p.bias && i < mine ? param_at<T>(p.bias, d + i, p.bias_f32) : 0.f;
-        skip[i] = p.skip && i < mine ? param_at<T>(p.skip, d + i, p.skip_f32) : 0.f;
-    }
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
-        sA[i] = in ? p.A[(int64_t)(d0 + c) * p.N + n] * LOG2E : 0.f;
-        sh[i] = in && p.h0 ? p.h0[b * p.ld_h0 + (int64_t)(d0 + c) * p.N + n] : 0.f;
+        sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] * LOG2E : 0.f;
+        carry[i] = in && p.h0 ? p.h0[b * p.ld_h0 + (int64_t)(d + c) * p.N + n] : 0.f;
     }
+    for (int i = tid; i < CT; i += THREADS) {
+        bias[i] = p.bias && i < have ? param_at<T>(p.bias, d + i, p.bias_f32) : 0.f;
+        skip[i] = p.skip && i < have ? param_at<T>(p.skip, d + i, p.skip_f32) : 0.f;
+    }
+    for (int i = tid; i < CT * Npad / NB; i += THREADS) flags[i] = 0;
+    if (tid == 0) *given_up = 0;
+    __syncthreads();
     const T *u = (const T*)p.u + b * p.s_u[0] + d, *dt = (const T*)p.dt + b * p.s_dt[0] + d, *z = p.z ? (const T*)p.z + b * p.s_z[0] + d : nullptr;
-    const T *mb = (const T*)p.b + b * p.s_b[0] + g * p.s_b[2], *mc = (const T*)p.c + b * p.s_c[0] + g * p.s_c[2];
+    const T *gB = (const T*)p.b + b * p.s_b[0] + g * p.s_b[2], *gC = (const T*)p.c + b * p.s_c[0] + g * p.s_c[2];
     T* const y = (T*)p.y + b * p.s_y[0] + d;
-    auto slot = [&](int buf, int k) { return slots + ((buf * 3 + k) * THREADS + tid) * NC; };
-    auto map = [&](int buf, int k) { return maps + (buf * 2 + k) * TILE * Npad; };
-    auto bring = [&](int tile, int buf) {
-        const int64_t at = (int64_t)tile * TILE + t;
-        if (at < len) {
-            fetch<T, NC>(slot(buf, 0), u + at * p.s_u[1], mine, p.piece);
-            fetch<T, NC>(slot(buf, 1), dt + at * p.s_dt[1], mine, p.piece);
-            if (z) fetch<T, NC>(slot(buf, 2), z + at * p.s_z[1], mine, p.piece);
-        }
-        fetch_map<T>(map(buf, 0), mb, p.s_b[1], tile * TILE, len, p.N, Npad, p.piece_maps);
-        fetch_map<T>(map(buf, 1), mc, p.s_c[1], tile * TILE, len, p.N, Npad, p.piece_maps);
-    };
-    if (ntiles) bring(0, 0);
 
-    for (int tile = 0; tile < ntiles; ++tile) {
-        const int buf = tile & 1, at = tile * TILE + t;
-        copies_done();
-        __syncthreads();                                         // the tile's maps are there; nobody is left in the tile before
-        if (tile + 1 < ntiles) bring(tile + 1, buf ^ 1);
+    for (int tile = warp; tile < ntiles; tile += W) {
+        const int64_t t0 = (int64_t)tile * TILE;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            float dl = 0.f, xi = 0.f;                            // behind the end a token changes nothing
-            if (at < len && i < mine) {
-                dl = DType<T>::to_f(slot(buf, 1)[i]) + bias[i];
-                if (p.softplus) dl = softplus<T>(dl);
-                xi = dl * DType<T>::to_f(slot(buf, 0)[i]);
+        for (int t = lane; t < TILE; t += 32) {
+            if (t0 + t < len) {
+                fetch<T, CT>(rdt + t * CT, dt + (t0 + t) * p.s_dt[1], have, p.piece);
+                fetch<T, CT>(ru + t * CT, u + (t0 + t) * p.s_u[1], have, p.piece);
+                if (z) fetch<T, CT>(rz + t * CT, z + (t0 + t) * p.s_z[1], have, p.piece);
             }
-            delta[(cl + i) * TILE + t] = dl;
-            x[(cl + i) * TILE + t] = xi;
         }
-        __syncthreads();
+        fetch_map<T>(mB, gB, p.s_b[1], t0, len, p.N, Npad, p.piece_maps, lane);
+        fetch_map<T>(mC, gC, p.s_c[1], t0, len, p.N, Npad, p.piece_maps, lane);
+        copies_done();
+        __syncwarp();
+#pragma unroll 1
+        for (int t = lane; t < TILE; t += 32) {
+            const bool in = t0 + t < len;                        // behind the end a token changes nothing
+            float uf[CT], df[CT];
+            read<T, CT>(uf, ru + t * CT, CT, 16);
+            read<T, CT>(df, rdt + t * CT, CT, 16);
+#pragma unroll
+            for (int c = 0; c < CT; c += 2) {
+                F2 dl = f2_add(f2_make(df[c], df[c + 1]), *(const F2*)(bias + c));
+                if (p.softplus) dl = softplus<T>(dl);
+                const F2 xi = f2_mul(dl, f2_make(uf[c], uf[c + 1]));
+                delta[c * TILE + t] = in ? f2_lo(dl) : 0.f;
+                delta[(c + 1) * TILE + t] = in ? f2_hi(dl) : 0.f;
+                x[c * TILE + t] = in ? f2_lo(xi) : 0.f;
+                x[(c + 1) * TILE + t] = in ? f2_hi(xi) : 0.f;
+            }
+        }
+        __syncwarp();
 
         for (int n0 = 0; n0 < Npad; n0 += NB) {
             F2 B[RUN][S / 2], C[RUN][S / 2];
 #pragma unroll
             for (int j = 0; j < RUN; ++j) {
                 const int at = (j * RUN + run) * Npad + n0 + part * S;
-                pairs<T, S>(B[j], map(buf, 0) + at);
-                pairs<T, S>(C[j], map(buf, 1) + at);
+                pairs<T, S>(B[j], mB + at);
+                pairs<T, S>(C[j], mC + at);
             }
 #pragma unroll 1
-            for (int ci = 0; ci < CPW; ++ci) {
-                const int c = warp * CPW + ci;
-                if (c >= have) break;
-                float* const h_at = sh + c * Npad + n0 + part * S;
-                F2 A2[S / 2], h0[S / 2], h[S / 2];
+            for (int c = 0; c < have; ++c) {
+                float* const h_at = carry + c * Npad + n0 + part * S;
+                uint32_t* const flag = flags + n0 / NB * CT + c;
+                F2 A2[S / 2], a[RUN][S / 2], P[S / 2], E[S / 2], h0[S / 2], h[S / 2];
                 pairs<float, S>(A2, sA + c * Npad + n0 + part * S);
-                pairs<float, S>(h0, h_at);
-                if (p.states && run == 0) {
-                    float* to = p.states + (((int64_t)b * p.tiles + tile) * p.D + d0 + c) * p.N + n0 + part * S;
-#pragma unroll
-                    for (int s = 0; s < S; ++s) if (n0 + part * S + s < p.N) to[s] = s & 1 ? f2_hi(h0[s / 2]) : f2_lo(h0[s / 2]);
-                }
                 float dl[RUN], xr[RUN], yv[RUN];
                 *(float4*)dl = *(const float4*)(delta + c * TILE + run * RUN);
                 *(float4*)(dl + 4) = *(const float4*)(delta + c * TILE + run * RUN + 4);
                 *(float4*)xr = *(const float4*)(x + c * TILE + run * RUN);
                 *(float4*)(xr + 4) = *(const float4*)(x + c * TILE + run * RUN + 4);
-                F2 a[RUN][S / 2];
                 decays<S>(a, dl, A2);
-                entering<S>(h, h0, a, B, xr, run, lane);
+                own_sum<S>(P, E, a, B, xr);
+                hand.await(flag, (uint32_t)tile);
+                pairs<float, S>(h0, h_at);
+                entering<S>(h, E, P, h0, a, B, xr, run, part);
+                __syncwarp();
+                if (run == RUN - 1) {
+#pragma unroll
+                    for (int s = 0; s < S / 2; ++s) *(F2*)(h_at + 2 * s) = E[s];
+                }
+                hand.pass(flag, (uint32_t)tile + 1);
+                if (p.states && run == 0) {
+                    float* to = p.states + (((int64_t)b * p.tiles + tile) * p.D + d + c) * p.N + n0 + part * S;
+#pragma unroll
+                    for (int s = 0; s < S; ++s) if (n0 + part * S + s < p.N) to[s] = s & 1 ? f2_hi(h0[s / 2]) : f2_lo(h0[s / 2]);
+                }
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
                     const F2 xj = f2_make(xr[j], xr[j]);
@@ -130,39 +143,35 @@ __global__ void __launch_bounds__(THREADS, 3) scan_fwd_kernel(const Params p) {
                 float2* const ya = (float2*)(ys + c * TILE + run * RUN + part * 2);
                 if (n0) { const float2 was = *ya; got.x += was.x; got.y += was.y; }
                 *ya = got;
-                __syncwarp();
-                if (run == RUN - 1) {
-#pragma unroll
-                    for (int s = 0; s < S / 2; ++s) *(F2*)(h_at + 2 * s) = h[s];
-                }
-                __syncwarp();
             }
         }
-        __syncthreads();
-        if (at < len && mine) {
-            float out[NC];
+        __syncwarp();
+#pragma unroll 1
+        for (int t = lane; t < TILE; t += 32) {
+            if (t0 + t >= len) break;
+            float uf[CT], out[CT];
+            read<T, CT>(uf, ru + t * CT, CT, 16);
 #pragma unroll
-            for (int i = 0; i < NC; ++i) {
-                if (i < mine) {
-                    out[i] = fmaf(skip[i], DType<T>::to_f(slot(buf, 0)[i]), ys[(cl + i) * TILE + t]);
-                    if (z) { const float v = DType<T>::to_f(slot(buf, 2)[i]); out[i] *= v * sigmoidf_(v); }
-                } else {
-                    out[i] = 0.f;
-                }
+            for (int c = 0; c < CT; ++c) out[c] = fmaf(skip[c], uf[c], ys[c * TILE + t]);
+            if (z) {
+                read<T, CT>(uf, rz + t * CT, CT, 16);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) out[c] *= uf[c] * sigmoid(uf[c]);
             }
-            put<T, NC>(y + at * p.s_y[1], out, mine, p.piece);
+            put<T, CT>(y + (t0 + t) * p.s_y[1], out, have, p.piece);
         }
+        __syncwarp();
     }
     // behind the end the outputs are zeros
-    for (int64_t at = (int64_t)len + t; at < p.L; at += TILE) {
-        const float out[NC] = {};
-        if (mine) put<T, NC>(y + at * p.s_y[1], out, mine, p.piece);
+    for (int64_t at = (int64_t)len + tid; at < p.L; at += THREADS) {
+        const float out[CT] = {};
+        put<T, CT>(y + at * p.s_y[1], out, have, p.piece);
     }
     if (p.h_final) {
         __syncthreads();
         for (int i = tid; i < CT * Npad; i += THREADS) {
             const int c = i / Npad, n = i - c * Npad;
-            if (c < have && n < p.N) p.h_final[b * p.ld_final + (int64_t)(d0 + c) * p.N + n] = sh[i];
+            if (c < have && n < p.N) p.h_final[b * p.ld_final + (int64_t)(d + c) * p.N + n] = carry[i];
         }
     }
 }
@@ -170,293 +179,337 @@ __global__ void __launch_bounds__(THREADS, 3) scan_fwd_kernel(const Params p) {
 // Backward, from the states that enter each tile (the forward wrote them) and the tiles from the last to the first.  With g_t = dL/dh_t,
 //   g_t = C_t dy_t + a_{t+1} g_{t+1},  dC_t = sum_d h_t dy_t,  dB_t = sum_d g_t delta_t u_t,  du_t = delta_t sum_n g_t B_t + D dy_t,
 //   ddelta_t = sum_n g_t (a_t h_{t-1} A + u_t B_t),  dA = sum g_t a_t h_{t-1} delta_t,
-// dy being d_out silu(z).  A lane keeps the decays and states of its run; the maps' gradients add up in registers over the warp's channels, then
-// over the CTA's warps, and the shares of CTAs, of sequences and of tokens are added in a fixed order by sum_kernel.
-template <typename T, int S, int CPW> struct BwdSmem {
-    static constexpr int NC = 2 * CPW, CT = WARPS * CPW, NB = 4 * S;
-    static constexpr int SLOT = NC * (int)sizeof(T), ROWS = 4 * THREADS * SLOT;
-    static __host__ __device__ int padded(int N) { return (N + NB - 1) / NB * NB; }
-    static int bytes(int N) {
-        const int Np = padded(N);
-        return 2 * ROWS + 4 * TILE * Np * (int)sizeof(T) + 6 * CT * TILE * 4 + 4 * CT * Np * 4 + 8 * CT * Np * 4 + WARPS * TILE * NB * 2 * 4 + 2 * NC * THREADS * 4;
-    }
+// dy being d_out silu(z).  What goes from tile to tile is a_t g_t of a tile's first token.  A lane keeps the decays and states of its run; the maps and the sums
+// of their gradients over the CTA's channels, 64 values a lane and state block, are kept in tensor memory, where each lane has a row of its own: registers
+// have no room for them, and in shared memory every access would take four turns.  The shares of CTAs, sequences and warps are added in a fixed order by
+// sum_kernel.
+constexpr int BS = 2, BNB = PARTS * BS, BCT = 16, BW = 4, BTHREADS = 32 * BW;     // states of a lane, of a block; channels and warps of a CTA
+
+struct BwdSmem {
+    static __host__ __device__ int padded(int N) { return (N + BNB - 1) / BNB * BNB; }
+    static __host__ __device__ int warp_floats(int N) { return 4 * BCT * TILE + 2 * BCT * padded(N); }
+    static int bytes(int N) { return (BW * warp_floats(N) + 2 * BCT * padded(N) + BCT * padded(N) / BNB + 2 * BCT + 2 * BW * BCT + 8) * 4; }
 };
+// columns of tensor memory: a power of two, 32 at least
+static __host__ __device__ int bwd_columns(int N) {
+    int c = 64;
+    while (c < BwdSmem::padded(N) / BNB * 64) c *= 2;
+    return c;
+}
 
-template <typename T, int S, int CPW>
-__global__ void __launch_bounds__(THREADS, 2) scan_bwd_kernel(const Params p) {
-    using M = BwdSmem<T, S, CPW>;
-    constexpr int NC = M::NC, CT = M::CT, NB = M::NB;
-    extern __shared__ __align__(16) char smem[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, run = lane / PARTS, part = lane % PARTS;
-    const int Npad = M::padded(p.N), Dg = p.D / p.G;
-    const int ct = blockIdx.x % p.ctiles, g = blockIdx.x / p.ctiles % p.G, b = blockIdx.x / p.ctiles / p.G;
-    const int c0 = ct * CT, have = min(CT, Dg - c0), d0 = g * Dg + c0;
-    const int len = length_of(p, b), ntiles = (len + TILE - 1) / TILE;
-    T* const slots = (T*)smem;
-    T* const maps = (T*)(smem + 2 * M::ROWS);
-    float* const delta = (float*)(maps + 4 * TILE * Npad);
-    float* const x = delta + CT * TILE;
-    float* const dys = x + CT * TILE;
-    float* const ys = dys + CT * TILE;                           // sum C h,
-    float* const gb = ys + CT * TILE;                            // sum g B,
-    float* const ga = gb + CT * TILE;                            // sum g a h A
-    float* const sA = ga + CT * TILE;
-    float* const sq = sA + CT * Npad;                            // a g of the token behind the tile
-    float* const sh = sq + CT * Npad;                            // states that enter the tile, two buffers
-    float* const dA = sh + 2 * CT * Npad;                        // a lane's share of dA: [channel][state block][lane][S]
-    float* const shares = dA + 8 * CT * Npad;            // a warp's dB and dC: [dB, dC][warp][token][NB]
-    float* const tok = shares + WARPS * TILE * NB * 2;           // a thread's shares of dD and dbias: [2 NC][thread]
-
-    const int t = tid % TILE, cl = tid / TILE * NC, mine = min(max(have - cl, 0), NC), d = d0 + cl;
-    float bias[NC], skip[NC];
+// NC values a lane summed over the lanes: lane i has the sum of value i / (32 / NC)
+template <int NC> __device__ __forceinline__ float over_lanes(float* v, int lane) {
+    int bit = 16;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        bias[i] = p.bias && i < mine ? param_at<T>(p.bias, d + i, p.bias_f32) : 0.f;
-        skip[i] = p.skip && i < mine ? param_at<T>(p.skip, d + i, p.skip_f32) : 0.f;
-        tok[i * THREADS + tid] = 0.f;
-        tok[(NC + i) * THREADS + tid] = 0.f;
+    for (int n = NC / 2; n; n /= 2, bit /= 2) {
+        const bool up = lane & bit;
+#pragma unroll
+        for (int i = 0; i < NC / 2; ++i)
+            if (i < n) v[i] = (up ? v[i + n] : v[i]) + __shfl_xor_sync(ALL, up ? v[i] : v[i + n], bit);
+    }
+    float r = v[0];
+#pragma unroll
+    for (; bit; bit /= 2) r += __shfl_xor_sync(ALL, r, bit);
+    return r;
+}
+
+// values out of tensor memory are there: nothing that takes them is moved ahead of the wait
+__device__ __forceinline__ void pinned(float* v) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+        asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
+}
+__device__ __forceinline__ void landed(float* v) { tc_wait_ld(); pinned(v); }
+__device__ __forceinline__ void landed(float* v, float* w) { tc_wait_ld(); pinned(v); pinned(w); }
+
+template <typename T>
+__global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
+    constexpr int S = BS, NB = BNB, CT = BCT, W = BW, THREADS = BTHREADS;
+    extern __shared__ __align__(16) char smem[];
+    __shared__ uint32_t tmem_slot;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, run = lane / PARTS, part = lane % PARTS;
+    const int Npad = BwdSmem::padded(p.N), Dg = p.D / p.G, columns = bwd_columns(p.N);
+    const int ct = blockIdx.x % p.ctiles, g = blockIdx.x / p.ctiles % p.G, b = blockIdx.x / p.ctiles / p.G;
+    const int c0 = ct * CT, have = min(CT, Dg - c0), d = g * Dg + c0;
+    const int len = length_of(p, b), ntiles = (len + TILE - 1) / TILE;
+    float *const delta = (float*)smem + warp * BwdSmem::warp_floats(p.N), *const x = delta + CT * TILE, *const dys = x + CT * TILE, *const ys = dys + CT * TILE;
+    float *const st = ys + CT * TILE, *const dA = st + CT * Npad;          // states that enter the tile; the warp's share of dA
+    float *const gb = x, *const ga = dys;                        // sum g B, sum g a h A: where a channel's inputs are done with
+    float *const sA = (float*)smem + W * BwdSmem::warp_floats(p.N), *const carry = sA + CT * Npad, *const bias = carry + CT * Npad, *const skip = bias + CT;
+    float* const shares = skip + CT;                             // the warps' shares of dD and dbias
+    uint32_t* const flags = (uint32_t*)(shares + 2 * W * CT);
+    int* const given_up = (int*)(flags + CT * Npad / NB);
+    const Handover hand{given_up, p.status};
+
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
-        sA[i] = in ? p.A[(int64_t)(d0 + c) * p.N + n] : 0.f;
-        sq[i] = in && p.d_final ? p.d_final[((int64_t)b * p.D + d0 + c) * p.N + n] : 0.f;
+        sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] : 0.f;
+        carry[i] = in && p.d_final ? p.d_final[((int64_t)b * p.D + d + c) * p.N + n] : 0.f;
     }
-    for (int i = tid; i < CT * Npad * 8; i += THREADS) dA[i] = 0.f;
+    for (int i = lane; i < 2 * CT * Npad; i += 32) st[i] = 0.f;
+    for (int i = tid; i < CT; i += THREADS) {
+        bias[i] = p.bias && i < have ? param_at<T>(p.bias, d + i, p.bias_f32) : 0.f;
+        skip[i] = p.skip && i < have ? param_at<T>(p.skip, d + i, p.skip_f32) : 0.f;
+    }
+    for (int i = tid; i < CT * Npad / NB; i += THREADS) flags[i] = 0;
+    if (tid == 0) *given_up = 0;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot + ((uint32_t)(32 * warp) << 16);      // [state block][B, C, dB, dC][8 tokens x 2 states]
     const T *u = (const T*)p.u + b * p.s_u[0] + d, *dt = (const T*)p.dt + b * p.s_dt[0] + d, *z = p.z ? (const T*)p.z + b * p.s_z[0] + d : nullptr;
     const T* dy = (const T*)p.dy + b * p.s_dy[0] + d;
-    const T *mb = (const T*)p.b + b * p.s_b[0] + g * p.s_b[2], *mc = (const T*)p.c + b * p.s_c[0] + g * p.s_c[2];
-    auto slot = [&](int buf, int k) { return slots + ((buf * 4 + k) * THREADS + tid) * NC; };
-    auto map = [&](int buf, int k) { return maps + (buf * 2 + k) * TILE * Npad; };
-    auto bring = [&](int tile, int buf) {
-        const int64_t at = (int64_t)tile * TILE + t;
-        if (at < len) {
-            fetch<T, NC>(slot(buf, 0), u + at * p.s_u[1], mine, p.piece);
-            fetch<T, NC>(slot(buf, 1), dt + at * p.s_dt[1], mine, p.piece);
-            if (z) fetch<T, NC>(slot(buf, 2), z + at * p.s_z[1], mine, p.piece);
-            fetch<T, NC>(slot(buf, 3), dy + at * p.s_dy[1], mine, p.piece);
-        }
-        fetch_map<T>(map(buf, 0), mb, p.s_b[1], tile * TILE, len, p.N, Npad, p.piece_maps);
-        fetch_map<T>(map(buf, 1), mc, p.s_c[1], tile * TILE, len, p.N, Npad, p.piece_maps);
-        const float* st = p.states + (((int64_t)b * p.tiles + tile) * p.D + d0) * p.N;
-        for (int i = tid; i < CT * Npad; i += THREADS) {
-            const int c = i / Npad, n = i - c * Npad;
-            float* to = sh + buf * CT * Npad + i;
-            if (c < have && n < p.N) copy4(to, st + c * p.N + n);
-            else *to = 0.f;
-        }
-    };
-    if (ntiles) bring(ntiles - 1, (ntiles - 1) & 1);
+    const T *gB = (const T*)p.b + b * p.s_b[0] + g * p.s_b[2], *gC = (const T*)p.c + b * p.s_c[0] + g * p.s_c[2];
+    float sum_skip = 0.f, sum_bias = 0.f;                        // of channel lane / 2
 
-    for (int tile = ntiles - 1; tile >= 0; --tile) {
-        const int buf = tile & 1, at = tile * TILE + t;
-        copies_done();
-        __syncthreads();
-        if (tile) bring(tile - 1, buf ^ 1);
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            float dl = 0.f, xi = 0.f, di = 0.f;
-            if (at < len && i < mine) {
-                dl = DType<T>::to_f(slot(buf, 1)[i]) + bias[i];
-                if (p.softplus) dl = softplus<T>(dl);
-                xi = dl * DType<T>::to_f(slot(buf, 0)[i]);
-                di = DType<T>::to_f(slot(buf, 3)[i]);
-                if (z) { const float v = DType<T>::to_f(slot(buf, 2)[i]); di *= v * sigmoidf_(v); }
-            }
-            delta[(cl + i) * TILE + t] = dl;
-            x[(cl + i) * TILE + t] = xi;
-            dys[(cl + i) * TILE + t] = di;
-        }
-        __syncthreads();
-
+    for (int back = warp; back < ntiles; back += W) {
+        const int tile = ntiles - 1 - back;
+        const int64_t t0 = (int64_t)tile * TILE;
+        const float* from = p.states + (((int64_t)b * p.tiles + tile) * p.D + d) * p.N;
+        for (int i = lane; i < have * p.N; i += 32) copy4(st + (p.N == Npad ? i : i / p.N * Npad + i % p.N), from + i);
         for (int n0 = 0; n0 < Npad; n0 += NB) {
-            F2 B[RUN][S / 2], C[RUN][S / 2], dB[RUN][S / 2], dC[RUN][S / 2];
+            float mb[RUN * S], mc[RUN * S];
 #pragma unroll
             for (int j = 0; j < RUN; ++j) {
-                const int at = (j * RUN + run) * Npad + n0 + part * S;
-                pairs<T, S>(B[j], map(buf, 0) + at);
-                pairs<T, S>(C[j], map(buf, 1) + at);
+                const int64_t at = t0 + run * RUN + j;
 #pragma unroll
-                for (int s = 0; s < S / 2; ++s) { dB[j][s] = 0ull; dC[j][s] = 0ull; }
-            }
-#pragma unroll 1
-            for (int ci = 0; ci < CPW; ++ci) {
-                const int c = warp * CPW + ci;
-                if (c >= have) break;
-                const int at = c * Npad + n0 + part * S;
-                F2 A[S / 2], A2[S / 2], h0[S / 2], h[RUN + 1][S / 2], a[RUN][S / 2];
-                pairs<float, S>(A, sA + at);
-                pairs<float, S>(h0, sh + buf * CT * Npad + at);
-#pragma unroll
-                for (int s = 0; s < S / 2; ++s) A2[s] = f2_mul(A[s], f2_make(LOG2E, LOG2E));
-                float dl[RUN], xr[RUN], dr[RUN], sums[RUN];
-#pragma unroll
-                for (int k = 0; k < RUN; k += 4) {
-                    *(float4*)(dl + k) = *(const float4*)(delta + c * TILE + run * RUN + k);
-                    *(float4*)(xr + k) = *(const float4*)(x + c * TILE + run * RUN + k);
-                    *(float4*)(dr + k) = *(const float4*)(dys + c * TILE + run * RUN + k);
+                for (int s = 0; s < S; ++s) {
+                    const int n = n0 + part * S + s;
+                    const bool in = at < len && n < p.N;
+                    mb[j * S + s] = in ? DType<T>::to_f(gB[at * p.s_b[1] + n]) : 0.f;
+                    mc[j * S + s] = in ? DType<T>::to_f(gC[at * p.s_c[1] + n]) : 0.f;
                 }
+            }
+            tc_st16(tmem + n0 / NB * 64, (const uint32_t*)mb);
+            tc_st16(tmem + n0 / NB * 64 + 16, (const uint32_t*)mc);
+        }
+        tc_wait_st();
+#pragma unroll 1
+        for (int t = lane; t < TILE; t += 32) {
+            const bool in = t0 + t < len;
+            const int64_t at = in ? t0 + t : t0;
+            float uf[CT], df[CT], gf[CT];
+            read<T, CT>(uf, u + at * p.s_u[1], have, p.piece);
+            read<T, CT>(df, dt + at * p.s_dt[1], have, p.piece);
+            read<T, CT>(gf, dy + at * p.s_dy[1], have, p.piece);
+#pragma unroll
+            for (int c = 0; c < CT; c += 2) {
+                F2 dl = f2_add(f2_make(df[c], df[c + 1]), *(const F2*)(bias + c));
+                if (p.softplus) dl = softplus<T>(dl);
+                const F2 xi = f2_mul(dl, f2_make(uf[c], uf[c + 1]));
+                delta[c * TILE + t] = in ? f2_lo(dl) : 0.f;
+                delta[(c + 1) * TILE + t] = in ? f2_hi(dl) : 0.f;
+                x[c * TILE + t] = in ? f2_lo(xi) : 0.f;
+                x[(c + 1) * TILE + t] = in ? f2_hi(xi) : 0.f;
+            }
+            if (z) {
+                read<T, CT>(uf, z + at * p.s_z[1], have, p.piece);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) gf[c] *= uf[c] * sigmoid(uf[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c) dys[c * TILE + t] = in ? gf[c] : 0.f;
+        }
+        copies_done();
+        __syncwarp();
+
+#pragma unroll 1
+        for (int c = 0; c < have; ++c) {
+            float dl[RUN], xr[RUN], dr[RUN];
+#pragma unroll
+            for (int k = 0; k < RUN; k += 4) {
+                *(float4*)(dl + k) = *(const float4*)(delta + c * TILE + run * RUN + k);
+                *(float4*)(xr + k) = *(const float4*)(x + c * TILE + run * RUN + k);
+                *(float4*)(dr + k) = *(const float4*)(dys + c * TILE + run * RUN + k);
+            }
+            F2 s_y[RUN], s_b[RUN], s_a[RUN];                     // what is summed over the states
+#pragma unroll
+            for (int j = 0; j < RUN; ++j) s_y[j] = s_b[j] = s_a[j] = 0ull;
+#pragma unroll 1
+            for (int n0 = 0; n0 < Npad; n0 += NB) {
+                const int at = c * Npad + n0 + part * S;
+                const uint32_t col = tmem + n0 / NB * 64;
+                float mb[RUN * S], mc[RUN * S], md[RUN * S];
+                tc_ld16(col, mb);
+                tc_ld16(col + 16, mc);
+                F2 A[1], A2[1], P[1], E[1], h0[1], h[RUN + 1][1], a[RUN][1], B[RUN][1];
+                pairs<float, S>(A, sA + at);
+                pairs<float, S>(h0, st + at);
+                A2[0] = f2_mul(A[0], f2_make(LOG2E, LOG2E));
                 decays<S>(a, dl, A2);
-                entering<S>(h[0], h0, a, B, xr, run, lane);
+                landed(mb, mc);
+#pragma unroll
+                for (int j = 0; j < RUN; ++j) B[j][0] = f2_make(mb[2 * j], mb[2 * j + 1]);
+                if (c) tc_ld16(col + 48, md);
+                own_sum<S>(P, E, a, B, xr);
+                F2 Pb = P[0], Q = 0ull;
+#pragma unroll
+                for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), f2_make(dr[j], dr[j]), Q));
+                entering<S>(h[0], E, P, h0, a, B, xr, run, part);
+                if (c) landed(md);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
-                    const F2 xj = f2_make(xr[j], xr[j]), dj = f2_make(dr[j], dr[j]);
-                    F2 sum = 0ull;
-#pragma unroll
-                    for (int s = 0; s < S / 2; ++s) {
-                        h[j + 1][s] = f2_fma(a[j][s], h[j][s], f2_mul(xj, B[j][s]));
-                        sum = s ? f2_fma(C[j][s], h[j + 1][s], sum) : f2_mul(C[j][s], h[j + 1][s]);
-                        dC[j][s] = f2_fma(h[j + 1][s], dj, dC[j][s]);
-                    }
-                    sums[j] = f2_lo(sum) + f2_hi(sum);
+                    h[j + 1][0] = f2_fma(a[j][0], h[j][0], f2_mul(f2_make(xr[j], xr[j]), B[j][0]));
+                    s_y[j] = f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), h[j + 1][0], s_y[j]);
+                    const F2 add = f2_fma(h[j + 1][0], f2_make(dr[j], dr[j]), c ? f2_make(md[2 * j], md[2 * j + 1]) : 0ull);
+                    md[2 * j] = f2_lo(add);
+                    md[2 * j + 1] = f2_hi(add);
                 }
-                const int to = c * TILE + run * RUN + part * 2;
-                auto leave = [&](float* into) {
-                    float2 got = over_parts(sums, part);
-                    if (n0) { const float2 was = *(const float2*)(into + to); got.x += was.x; got.y += was.y; }
-                    *(float2*)(into + to) = got;
-                };
-                if (z) leave(ys);
+                tc_st16(col + 48, (const uint32_t*)md);
                 // from the other end: q_t = a_t g_t is what token t - 1 gets
-                F2 P[S / 2], Q[S / 2], q0[S / 2];
-                pairs<float, S>(q0, sq + at);
+                uint32_t* const flag = flags + n0 / NB * CT + c;
+                float* const q_at = carry + at;
+                F2 q0[1];
+                hand.await(flag, (uint32_t)back);
+                pairs<float, S>(q0, q_at);
+                Q = f2_fma(Pb, run == RUN - 1 ? q0[0] : 0ull, Q);
 #pragma unroll
-                for (int s = 0; s < S / 2; ++s) { Q[s] = run == RUN - 1 ? q0[s] : 0ull; P[s] = a[0][s]; }
-#pragma unroll
-                for (int j = RUN - 1; j >= 0; --j)
-#pragma unroll
-                    for (int s = 0; s < S / 2; ++s) {
-                        Q[s] = f2_mul(a[j][s], f2_fma(C[j][s], f2_make(dr[j], dr[j]), Q[s]));
-                        if (j) P[s] = f2_mul(P[s], a[j][s]);
-                    }
-#pragma unroll
-                for (int k = 1; k < RUN; k *= 2)
-#pragma unroll
-                    for (int s = 0; s < S / 2; ++s) {
-                        const F2 e = f2_shfl_down(Q[s], k * PARTS);
-                        Q[s] = f2_fma(P[s], run + k < RUN ? e : 0ull, Q[s]);
-                        if (2 * k < RUN) P[s] = f2_mul(P[s], f2_shfl_down(P[s], k * PARTS));
-                    }
-#pragma unroll
-                for (int s = 0; s < S / 2; ++s) {
-                    const F2 e = f2_shfl_down(Q[s], PARTS);
-                    Q[s] = run == RUN - 1 ? q0[s] : e;
+                for (int k = 1; k < RUN; k *= 2) {
+                    const F2 e = f2_shfl_down(Q, k * PARTS);
+                    Q = f2_fma(Pb, run + k < RUN ? e : 0ull, Q);
+                    if (2 * k < RUN) Pb = f2_mul(Pb, f2_shfl_down(Pb, k * PARTS));
                 }
-                float sums_a[RUN];
-                F2 dAs[S / 2];
-                float* const dA_at = dA + ((c * (Npad / NB) + n0 / NB) * 32 + lane) * S;
-                pairs<float, S>(dAs, dA_at);
+                __syncwarp();
+                if (run == 0) *(F2*)q_at = Q;
+                hand.pass(flag, (uint32_t)back + 1);
+                {
+                    const F2 e = f2_shfl_down(Q, PARTS);
+                    Q = run == RUN - 1 ? q0[0] : e;
+                }
+                if (c) { tc_ld16(col + 32, md); landed(md); }
+                F2 dAs = 0ull;
 #pragma unroll
                 for (int j = RUN - 1; j >= 0; --j) {
-                    const F2 xj = f2_make(xr[j], xr[j]), dj = f2_make(dr[j], dr[j]), lj = f2_make(dl[j], dl[j]);
-                    F2 sb = 0ull, sa = 0ull;
-#pragma unroll
-                    for (int s = 0; s < S / 2; ++s) {
-                        const F2 gr = f2_fma(C[j][s], dj, Q[s]);
-                        sb = s ? f2_fma(gr, B[j][s], sb) : f2_mul(gr, B[j][s]);
-                        dB[j][s] = f2_fma(gr, xj, dB[j][s]);
-                        Q[s] = f2_mul(a[j][s], gr);
-                        const F2 f = f2_mul(Q[s], h[j][s]);
-                        sa = s ? f2_fma(f, A[s], sa) : f2_mul(f, A[s]);
-                        dAs[s] = f2_fma(f, lj, dAs[s]);
-                    }
-                    sums[j] = f2_lo(sb) + f2_hi(sb);
-                    sums_a[j] = f2_lo(sa) + f2_hi(sa);
+                    const F2 gr = f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), f2_make(dr[j], dr[j]), Q);
+                    s_b[j] = f2_fma(gr, B[j][0], s_b[j]);
+                    const F2 add = f2_fma(gr, f2_make(xr[j], xr[j]), c ? f2_make(md[2 * j], md[2 * j + 1]) : 0ull);
+                    md[2 * j] = f2_lo(add);
+                    md[2 * j + 1] = f2_hi(add);
+                    Q = f2_mul(a[j][0], gr);
+                    const F2 f = f2_mul(Q, h[j][0]);
+                    s_a[j] = f2_fma(f, A[0], s_a[j]);
+                    dAs = f2_fma(f, f2_make(dl[j], dl[j]), dAs);
                 }
-                leave(gb);
-#pragma unroll
-                for (int j = 0; j < RUN; ++j) sums[j] = sums_a[j];
-                leave(ga);
-#pragma unroll
-                for (int s = 0; s < S / 2; ++s) *(F2*)(dA_at + 2 * s) = dAs[s];
-                __syncwarp();
-                if (run == 0) {
-#pragma unroll
-                    for (int s = 0; s < S / 2; ++s) *(F2*)(sq + at + 2 * s) = Q[s];
-                }
-                __syncwarp();
+                tc_st16(col + 32, (const uint32_t*)md);
+                // dA over the runs: a lane of an even run keeps the first state's sum, of an odd one the second's
+                const bool odd = run & 1;
+                float v = (odd ? f2_hi(dAs) : f2_lo(dAs)) + __shfl_xor_sync(ALL, odd ? f2_lo(dAs) : f2_hi(dAs), PARTS);
+                v += __shfl_xor_sync(ALL, v, 2 * PARTS);
+                v += __shfl_xor_sync(ALL, v, 4 * PARTS);
+                if (run < 2) dA[at + run] += v;
+                tc_wait_st();
             }
-            // the warps' shares of the maps' gradients, added and left for sum_kernel
-            if (n0) __syncthreads();
+            float v[RUN];
+            const int to = c * TILE + run * RUN + part * 2;
+            if (z) {
 #pragma unroll
-            for (int j = 0; j < RUN; ++j)
+                for (int j = 0; j < RUN; ++j) v[j] = f2_lo(s_y[j]) + f2_hi(s_y[j]);
+                *(float2*)(ys + to) = over_parts(v, part);
+            }
 #pragma unroll
-                for (int s = 0; s < S / 2; ++s) {
-                    const int at = (run * RUN + j) * NB + part * S + 2 * s;
-                    *(F2*)(shares + warp * TILE * NB + at) = dB[j][s];
-                    *(F2*)(shares + (WARPS + warp) * TILE * NB + at) = dC[j][s];
-                }
-            __syncthreads();
-            for (int i = tid; i < 2 * TILE * NB; i += THREADS) {
-                const int which = i / (TILE * NB), k = i - which * TILE * NB, tt = k / NB, n = n0 + k % NB;
-                if (tile * TILE + tt < len && n < p.N) {
-                    float v = 0.f;
+            for (int j = 0; j < RUN; ++j) v[j] = f2_lo(s_b[j]) + f2_hi(s_b[j]);
+            *(float2*)(gb + to) = over_parts(v, part);
 #pragma unroll
-                    for (int w = 0; w < WARPS; ++w) v += shares[(which * WARPS + w) * TILE * NB + k];
-                    float* out = which ? p.part_c : p.part_b;
-                    out[((((int64_t)ct * p.B + b) * p.L + tile * TILE + tt) * p.G + g) * p.N + n] = v;
-                }
+            for (int j = 0; j < RUN; ++j) v[j] = f2_lo(s_a[j]) + f2_hi(s_a[j]);
+            *(float2*)(ga + to) = over_parts(v, part);
+        }
+        __syncwarp();
+        // the tile's maps have their gradients from this CTA's channels
+        for (int n0 = 0; n0 < Npad; n0 += NB) {
+            float mb[RUN * S], mc[RUN * S];
+            tc_ld16(tmem + n0 / NB * 64 + 32, mb);
+            tc_ld16(tmem + n0 / NB * 64 + 48, mc);
+            landed(mb, mc);
+#pragma unroll
+            for (int j = 0; j < RUN; ++j) {
+                const int64_t at = t0 + run * RUN + j;
+                const int64_t to = ((((int64_t)ct * p.B + b) * p.L + at) * p.G + g) * p.N + n0 + part * S;
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+                    if (at < len && n0 + part * S + s < p.N) { p.part_b[to + s] = mb[j * S + s]; p.part_c[to + s] = mc[j * S + s]; }
             }
         }
-        // (the barrier ahead of the sums stands between the warps' sums over states and this)
-        if (at < len && mine) {
-            float du[NC], dd[NC], dz[NC];
+        float keep_skip[CT], keep_bias[CT];
 #pragma unroll
-            for (int i = 0; i < NC; ++i) {
-                du[i] = dd[i] = dz[i] = 0.f;
-                if (i < mine) {
-                    const int k = (cl + i) * TILE + t;
-                    const float ui = DType<T>::to_f(slot(buf, 0)[i]);
-                    du[i] = fmaf(gb[k], delta[k], skip[i] * dys[k]);
-                    dd[i] = fmaf(gb[k], ui, ga[k]);
-                    if (p.softplus) dd[i] *= sigmoidf_(DType<T>::to_f(slot(buf, 1)[i]) + bias[i]);
-                    if (z) {
-                        const float v = DType<T>::to_f(slot(buf, 2)[i]), s = sigmoidf_(v);
-                        dz[i] = DType<T>::to_f(slot(buf, 3)[i]) * fmaf(skip[i], ui, ys[k]) * s * fmaf(v, 1.f - s, 1.f);
-                    }
-                    tok[i * THREADS + tid] = fmaf(dys[k], ui, tok[i * THREADS + tid]);
-                    tok[(NC + i) * THREADS + tid] += dd[i];
+        for (int c = 0; c < CT; ++c) keep_skip[c] = keep_bias[c] = 0.f;
+#pragma unroll 1
+        for (int t = lane; t < TILE; t += 32) {
+            if (t0 + t >= len) break;
+            const int64_t at = t0 + t, row = ((int64_t)b * p.L + at) * p.D + d;
+            float uf[CT], gf[CT], zf[CT], out[CT];
+            read<T, CT>(uf, u + at * p.s_u[1], have, p.piece);
+            read<T, CT>(gf, dy + at * p.s_dy[1], have, p.piece);
+            if (z) {
+                read<T, CT>(zf, z + at * p.s_z[1], have, p.piece);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const float s = sigmoid(zf[c]);
+                    out[c] = gf[c] * fmaf(skip[c], uf[c], ys[c * TILE + t]) * s * fmaf(zf[c], 1.f - s, 1.f);
+                    gf[c] *= zf[c] * s;
                 }
+                put<T, CT>((T*)p.d_z + row, out, have, p.piece);
             }
-            const int64_t row = ((int64_t)b * p.L + at) * p.D + d;
-            put<T, NC>((T*)p.d_u + row, du, mine, p.piece);
-            put<T, NC>((T*)p.d_dt + row, dd, mine, p.piece);
-            if (z) put<T, NC>((T*)p.d_z + row, dz, mine, p.piece);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                out[c] = fmaf(gb[c * TILE + t], delta[c * TILE + t], skip[c] * gf[c]);
+                keep_skip[c] = fmaf(gf[c], uf[c], keep_skip[c]);
+            }
+            put<T, CT>((T*)p.d_u + row, out, have, p.piece);
+            if (p.softplus) read<T, CT>(zf, dt + at * p.s_dt[1], have, p.piece);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                out[c] = fmaf(gb[c * TILE + t], uf[c], ga[c * TILE + t]);
+                if (p.softplus) out[c] *= sigmoid(zf[c] + bias[c]);
+                keep_bias[c] += out[c];
+            }
+            put<T, CT>((T*)p.d_dt + row, out, have, p.piece);
         }
+        __syncwarp();
+        sum_skip += over_lanes<CT>(keep_skip, lane);
+        sum_bias += over_lanes<CT>(keep_bias, lane);
     }
     // behind the end all gradients are zeros
-    for (int64_t at = (int64_t)len + t; at < p.L; at += TILE) {
-        const float none[NC] = {};
+    for (int64_t at = (int64_t)len + tid; at < p.L; at += THREADS) {
+        const float none[CT] = {};
         const int64_t row = ((int64_t)b * p.L + at) * p.D + d;
-        if (mine) {
-            put<T, NC>((T*)p.d_u + row, none, mine, p.piece);
-            put<T, NC>((T*)p.d_dt + row, none, mine, p.piece);
-            if (z) put<T, NC>((T*)p.d_z + row, none, mine, p.piece);
-        }
+        put<T, CT>((T*)p.d_u + row, none, have, p.piece);
+        put<T, CT>((T*)p.d_dt + row, none, have, p.piece);
+        if (z) put<T, CT>((T*)p.d_z + row, none, have, p.piece);
     }
     for (int64_t i = (int64_t)len * p.N + tid; i < (int64_t)p.L * p.N; i += THREADS) {
         const int64_t at = ((((int64_t)ct * p.B + b) * p.L + i / p.N) * p.G + g) * p.N + i % p.N;
         p.part_b[at] = 0.f;
         p.part_c[at] = 0.f;
     }
+    if (!(lane & 1)) { shares[warp * CT + lane / 2] = sum_skip; shares[(W + warp) * CT + lane / 2] = sum_bias; }
+    tc_fence_before();
     __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"(columns) : "memory");
+    }
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         if (c < have && n < p.N) {
             float v = 0.f;
-            const float* from = dA + ((c * (Npad / NB) + n / NB) * 32 + n % NB / S) * S + n % S;
-            for (int r = 0; r < RUN; ++r) v += from[r * PARTS * S];
-            const int64_t at = ((int64_t)b * p.D + d0 + c) * p.N + n;
+#pragma unroll
+            for (int w = 0; w < W; ++w) v += dA[(w - warp) * BwdSmem::warp_floats(p.N) + i];
+            const int64_t at = ((int64_t)b * p.D + d + c) * p.N + n;
             p.part_A[at] = v;
-            if (p.d_h0) p.d_h0[at] = sq[i];
+            if (p.d_h0) p.d_h0[at] = carry[i];
         }
     }
     if (tid < have) {
-        const float *from = tok + tid % NC * THREADS + tid / NC * TILE, *from2 = from + NC * THREADS;
         float v = 0.f, v2 = 0.f;
-        for (int k = 0; k < TILE; ++k) { v += from[k]; v2 += from2[k]; }
-        if (p.part_skip) p.part_skip[(int64_t)b * p.D + d0 + tid] = v;
-        if (p.part_bias) p.part_bias[(int64_t)b * p.D + d0 + tid] = v2;
+#pragma unroll
+        for (int w = 0; w < W; ++w) { v += shares[w * CT + tid]; v2 += shares[(W + w) * CT + tid]; }
+        p.part_skip[(int64_t)b * p.D + d + tid] = v;
+        p.part_bias[(int64_t)b * p.D + d + tid] = v2;
     }
 }
 
@@ -499,7 +552,7 @@ template <typename T> __global__ void __launch_bounds__(128) scan_step_kernel(co
     const float u = DType<T>::to_f(((const T*)p.u)[b * p.s_u + d]), zv = p.z ? DType<T>::to_f(((const T*)p.z)[b * p.s_z + d]) : 0.f;
     float dl = DType<T>::to_f(((const T*)p.dt)[b * p.s_dt + d]) + (p.bias ? param_at<T>(p.bias, d, p.bias_f32) : 0.f);
     const float skip = p.skip ? param_at<T>(p.skip, d, p.skip_f32) : 0.f;
-    if (p.softplus) dl = softplus<T>(dl);
+    if (p.softplus) dl = f2_lo(softplus<T>(f2_make(dl, dl)));
     const float x = dl * u;
     float y = 0.f;
     for (int n0 = part * 4; n0 < p.N; n0 += 16) {
@@ -534,7 +587,7 @@ template <typename T> __global__ void __launch_bounds__(128) scan_step_kernel(co
     y += __shfl_xor_sync(ALL, y, 1);
     if (in && part == 0) {
         y = fmaf(skip, u, y);
-        if (p.z) y *= zv * sigmoidf_(zv);
+        if (p.z) y *= zv * sigmoid(zv);
         ((T*)p.y)[b * p.s_y + d] = DType<T>::from_f(y);
     }
 }
@@ -545,40 +598,37 @@ static void narrow(int& piece, const void* ptr, const int64_t* strides, int coun
     piece = min(piece, piece_of((int64_t)(uintptr_t)ptr));
     for (int i = 0; i < count; ++i) piece = min(piece, piece_of(strides[i] * size));
 }
-template <int CT> void place(Params& p) { p.ctiles = (p.D / p.G + CT - 1) / CT; }
-
-template <typename T, int S, int CPW> int fwd_launch(Params& p, cudaStream_t s) {
-    place<WARPS * CPW>(p);
+template <typename T, int S, int CT, int W> int fwd_launch(Params& p, cudaStream_t s) {
+    p.ctiles = (p.D / p.G + CT - 1) / CT;
     const int64_t grid = (int64_t)p.B * p.G * p.ctiles;
-    const int smem = FwdSmem<T, S, CPW>::bytes(p.N);
+    const int smem = FwdSmem<T, S, CT>::bytes(p.N, W);
     if (grid >= (1ll << 31)) return VIG_ERR_SHAPE;
-    if (const cudaError_t e = ensure_smem_attr((const void*)scan_fwd_kernel<T, S, CPW>, smem)) return (int)e;
-    scan_fwd_kernel<T, S, CPW><<<(unsigned)grid, THREADS, smem, s>>>(p);
+    if (const cudaError_t e = ensure_smem_attr((const void*)scan_fwd_kernel<T, S, CT, W>, smem)) return (int)e;
+    scan_fwd_kernel<T, S, CT, W><<<(unsigned)grid, 32 * W, smem, s>>>(p);
     return (int)cudaGetLastError();
 }
-template <typename T, int S, int CPW> int bwd_launch(Params& p, cudaStream_t s) {
-    place<WARPS * CPW>(p);
+template <typename T> int bwd_launch(Params& p, cudaStream_t s) {
     const int64_t grid = (int64_t)p.B * p.G * p.ctiles;
-    const int smem = BwdSmem<T, S, CPW>::bytes(p.N);
+    const int smem = BwdSmem::bytes(p.N);
     if (grid >= (1ll << 31)) return VIG_ERR_SHAPE;
-    if (const cudaError_t e = ensure_smem_attr((const void*)scan_bwd_kernel<T, S, CPW>, smem)) return (int)e;
-    scan_bwd_kernel<T, S, CPW><<<(unsigned)grid, THREADS, smem, s>>>(p);
+    if (const cudaError_t e = ensure_smem_attr((const void*)scan_bwd_kernel<T>, smem)) return (int)e;
+    scan_bwd_kernel<T><<<(unsigned)grid, BTHREADS, smem, s>>>(p);
     return (int)cudaGetLastError();
 }
-
-// channels of a CTA of the backward: fewer where the maps of many states need the room
-constexpr int bwd_ct(int N) { return N <= 64 ? 4 * WARPS : WARPS; }
 
 template <typename T> int fwd_pick(Params& p, cudaStream_t s) {
-    return p.N <= 8 ? fwd_launch<T, 2, 4>(p, s) : fwd_launch<T, 4, 4>(p, s);
+    // sixteen channels a CTA where that fills the device, else four
+    const int64_t wide = (int64_t)p.B * p.G * ((p.D / p.G + 15) / 16);
+    const bool few = wide < 2 * device_sms();
+    if (p.N <= 8) return few ? fwd_launch<T, 2, 4, 4>(p, s) : fwd_launch<T, 2, 16, 4>(p, s);
+    return few ? fwd_launch<T, 4, 4, 4>(p, s) : fwd_launch<T, 4, 16, 4>(p, s);
 }
-template <typename T> int bwd_pick(Params& p, cudaStream_t s) { return p.N <= 64 ? bwd_launch<T, 2, 4>(p, s) : bwd_launch<T, 2, 1>(p, s); }
 
 static int check(const vig_selective_scan_args* a, bool grads) {
     if (!a) return VIG_ERR_NULL;
     const auto type_ok = [&](int t) { return t == a->dtype || t == VIG_DTYPE_F32; };
     if (a->dtype < VIG_DTYPE_F32 || a->dtype > VIG_DTYPE_F16 || (a->skip && !type_ok(a->skip_dtype)) || (a->dt_bias && !type_ok(a->bias_dtype))) return VIG_ERR_DTYPE;
-    if (a->B < 0 || a->L < 0 || a->D < 0 || a->N < 1 || a->N > 128 || a->G < 1 || a->D % a->G) return VIG_ERR_SHAPE;
+    if (a->B < 0 || a->L < 0 || a->D < 0 || a->N < 1 || a->N > 64 || a->G < 1 || a->D % a->G) return VIG_ERR_SHAPE;
     if ((int64_t)a->B * a->D >= (1ll << 31) || a->D >= (1 << 28) || a->L >= (1 << 30)) return VIG_ERR_SHAPE;
     if (!a->B || !a->D) return VIG_OK;
     if (!a->A || (a->L && (!a->u || !a->dt || !a->b || !a->c || (!grads && !a->y)))) return VIG_ERR_NULL;
@@ -597,6 +647,7 @@ static Params params_of(const vig_selective_scan_args* a, bool grads) {
     p.B = a->B; p.L = a->L; p.D = a->D; p.N = a->N; p.G = a->G; p.softplus = a->softplus;
     p.skip_f32 = a->skip_dtype == VIG_DTYPE_F32; p.bias_f32 = a->bias_dtype == VIG_DTYPE_F32;
     p.tiles = (p.L + TILE - 1) / TILE;
+    p.status = a->status;
     const int size = a->dtype == VIG_DTYPE_F32 ? 4 : 2;
     p.piece = p.piece_maps = 16;
     narrow(p.piece, p.u, p.s_u, 2, size); narrow(p.piece, p.dt, p.s_dt, 2, size); narrow(p.piece, p.z, p.s_z, 2, size);
@@ -633,7 +684,7 @@ extern "C" int vig_selective_scan_fwd(const vig_selective_scan_args* a, void* st
 
 extern "C" size_t vig_selective_scan_bwd_workspace_bytes(int B, int L, int D, int N, int G) {
     if (B <= 0 || L < 0 || D <= 0 || N <= 0 || G <= 0) return 0;
-    const size_t ctiles = (D / G + bwd_ct(N) - 1) / bwd_ct(N);
+    const size_t ctiles = (D / G + BCT - 1) / BCT;
     return sizeof(float) * (2 * ctiles * B * L * G * N + (size_t)B * D * (N + 2));
 }
 
@@ -643,7 +694,7 @@ extern "C" int vig_selective_scan_bwd(const vig_selective_scan_args* a, void* st
     if (!a->workspace || a->workspace_bytes < vig_selective_scan_bwd_workspace_bytes(a->B, a->L, a->D, a->N, a->G)) return VIG_ERR_WORKSPACE;
     const cudaStream_t s = (cudaStream_t)stream;
     Params p = params_of(a, true);
-    p.ctiles = (p.D / p.G + bwd_ct(p.N) - 1) / bwd_ct(p.N);
+    p.ctiles = (p.D / p.G + BCT - 1) / BCT;
     const int64_t maps = (int64_t)p.B * p.L * p.G * p.N, rows = (int64_t)p.B * p.D;
     p.part_b = (float*)a->workspace;
     p.part_c = p.part_b + p.ctiles * maps;
@@ -652,9 +703,9 @@ extern "C" int vig_selective_scan_bwd(const vig_selective_scan_args* a, void* st
     p.part_bias = p.part_skip + rows;
     int e;
     switch (a->dtype) {
-        case VIG_DTYPE_F32: e = bwd_pick<float>(p, s); break;
-        case VIG_DTYPE_BF16: e = bwd_pick<__nv_bfloat16>(p, s); break;
-        default: e = bwd_pick<__half>(p, s); break;
+        case VIG_DTYPE_F32: e = bwd_launch<float>(p, s); break;
+        case VIG_DTYPE_BF16: e = bwd_launch<__nv_bfloat16>(p, s); break;
+        default: e = bwd_launch<__half>(p, s); break;
     }
     if (e) return e;
     SumJobs jobs{};

@@ -738,12 +738,17 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=N
     ``h_t[d, n] = exp(delta_t[d] A[d, n]) h_{t-1}[d, n] + delta_t[d] u_t[d] B_t[n]``, ``y_t[d] = (sum_n C_t[n] h_t[d, n] + D[d] u_t[d]) silu(z_t[d])``.
 
     ``u``, ``dt``, ``z`` (optional): ``[B, L, D]`` of one dtype, any strides with a contiguous last dimension.  ``B``, ``C``: ``[B, L, N]``, or ``[B, L, G, N]``
-    for G groups of neighbouring channels, of the same dtype; 1 to 128 states.  ``A``: fp32 ``[D, N]`` (negative, for states that fade).  ``D``, ``dt_bias``
+    for G groups of neighbouring channels, of the same dtype; 1 to 64 states.  ``A``: fp32 ``[D, N]`` (negative, for states that fade).  ``D``, ``dt_bias``
     (optional): ``[D]`` of ``u``'s dtype or fp32.  ``initial_state``: fp32 ``[B, D, N]``.  ``dt_softplus=False``: ``delta = dt + dt_bias``.  ``lengths``: int
     ``[B]``, how many tokens of each sequence count: behind them outputs and gradients are zeros, whatever stands there, and the final state is the one
     behind the last that counts.  Returns ``(y, final_state)``, ``y`` in ``u``'s dtype, ``final_state`` fp32 or None.  Steps, states and sums are fp32.
     Differentiable in every floating input, through both results."""
-    return _lib.host().selective_scan(u, dt, A, B, C, D, z, dt_bias, initial_state, output_final_state, dt_softplus, lengths)
+    args = (u, dt, A, B, C, D, z, dt_bias, initial_state, output_final_state, dt_softplus, lengths)
+    res = _lib.host().selective_scan(*args)
+    if res is None:                         # the device's first call
+        status_word(u.device)
+        res = _lib.host().selective_scan(*args)
+    return res
 
 
 def selective_scan_step(u, dt, A, B, C, state, D=None, z=None, dt_bias=None, *, dt_softplus=True):
