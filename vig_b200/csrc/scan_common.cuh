@@ -5,7 +5,9 @@
 // the work of a channel and tile is 8 x S products a lane, two values to an instruction (f32x2); the eight runs are joined by a scan over the lanes.
 // The state that enters a tile comes from the warp of the tile before through shared memory (`carry`): everything that does not depend on it is done before it
 // is waited for, and what the next warp needs is sent on before the outputs are computed.  Warps meet nowhere else: while one waits for its rows,
-// others compute.  The maps (B and C, the same for all channels of a group) are read once for a tile.
+// others compute.  The maps (B and C, the same for all channels of a group)
+// are read once for a tile and kept in tensor memory, where each lane has a row of its own: registers have no room for them beside a run's decays, and out
+// of shared memory every access would take four turns.
 #pragma once
 #include "tc_common.cuh"
 
@@ -17,47 +19,37 @@ using namespace tc;
 constexpr int TILE = 64, RUN = 8, PARTS = 4;
 constexpr unsigned ALL = 0xffffffffu;
 
-// where the row of token t of a tile lies: eight lanes that read token j of their runs read eight neighbouring rows
-__device__ __forceinline__ int row_of(int t) { return (t % RUN) * RUN + t / RUN; }
-
 template <typename T> __device__ __forceinline__ float param_at(const void* p, int i, int f32) { return f32 ? ((const float*)p)[i] : DType<T>::to_f(((const T*)p)[i]); }
 
+// exp(-|x|) of a pair: what the product with log2(e) loses is put back, or steps of -10 would be 5e-7 off all along a sequence
+__device__ __forceinline__ F2 exp_minus_abs(F2 x) {
+    const F2 ax = x | 0x8000000080000000ull;                     // -|x|
+    const F2 k = f2_make(LOG2E, LOG2E), t = f2_mul(ax, k);
+    const F2 lost = f2_fma(ax, f2_make(1.925963033e-8f, 1.925963033e-8f), f2_fma(ax, k, t ^ 0x8000000080000000ull));
+    const F2 e = f2_make(ex2(f2_lo(t)), ex2(f2_hi(t)));
+    return f2_fma(e, f2_mul(lost, f2_make(LN2, LN2)), e);
+}
 // Of a pair of values, max(x, 0) + log(1 + e), e = exp(-|x|): a step of 1e-4 has to keep its own precision, so log(1 + e) is e times a polynomial of least
-// relative error on [0, 1] (3e-8, by exchange; 1.7e-7 with fp32 arithmetic).
-template <typename T> __device__ __forceinline__ F2 softplus(F2 x) {
-    const float lo = f2_lo(x), hi = f2_hi(x);
-    const F2 e = sizeof(T) == 4 ? f2_make(expf(-fabsf(lo)), expf(-fabsf(hi))) : f2_make(ex2(-fabsf(lo) * LOG2E), ex2(-fabsf(hi) * LOG2E));
-    constexpr float c[] = {0.99999994f, -0.499994934f, 0.333190978f, -0.24842982f, 0.191060066f, -0.136632457f, 0.0782259554f, -0.0295052417f, 0.00523269456f};
-    F2 s = f2_make(c[8], c[8]);
+// relative error on [0, 1] (5e-9, by exchange; 1.4e-7 with fp32 arithmetic).
+__device__ __forceinline__ F2 softplus(F2 x) {
+    const F2 e = exp_minus_abs(x);
+    constexpr float c[] = {1.f, -0.499999017f, 0.333299637f, -0.249541342f, 0.196759388f, -0.153055921f, 0.106036551f, -0.0569595359f, 0.0198514629f, -0.00324402563f};
+    F2 s = f2_make(c[9], c[9]);
 #pragma unroll
-    for (int i = 7; i >= 0; --i) s = f2_fma(s, e, f2_make(c[i], c[i]));
-    return f2_fma(s, e, f2_make(fmaxf(lo, 0.f), fmaxf(hi, 0.f)));
+    for (int i = 8; i >= 0; --i) s = f2_fma(s, e, f2_make(c[i], c[i]));
+    return f2_fma(s, e, f2_make(fmaxf(f2_lo(x), 0.f), fmaxf(f2_hi(x), 0.f)));
+}
+// softplus'(x)
+__device__ __forceinline__ float slope(float x) {
+    const float e = f2_lo(exp_minus_abs(f2_make(x, x))), r = rcp(1.f + e);
+    return x < 0.f ? e * r : r;
 }
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-x * LOG2E)); }
 
-__device__ __forceinline__ void copy16(void* dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
-__device__ __forceinline__ void copy8(void* dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(void* dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// NC values of a row into shared memory of the lane's own: in pieces of what pointers and strides allow, or one at a time; values from `have` on are zeros
-template <typename T, int NC> __device__ __forceinline__ void fetch(T* dst, const T* src, int have, int piece) {
-    constexpr int BYTES = NC * (int)sizeof(T);
-    if (have >= NC && piece >= 8) {
-        if (BYTES % 16 == 0 && piece >= 16) {
-#pragma unroll
-            for (int i = 0; i < BYTES / 16; ++i) copy16((char*)dst + 16 * i, (const char*)src + 16 * i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < BYTES / 8; ++i) copy8((char*)dst + 8 * i, (const char*)src + 8 * i);
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < NC; ++i) dst[i] = i < have ? src[i] : DType<T>::from_f(0.f);
-}
-
-// the same into registers, from either memory
+// NC values of a row into registers: in pieces of what pointers and strides allow, or one at a time; values from `have` on are zeros
 template <typename T, int NC> __device__ __forceinline__ void read(float* f, const T* src, int have, int piece) {
     constexpr int BYTES = NC * (int)sizeof(T);
     T e[NC];
@@ -124,24 +116,21 @@ template <int S> __device__ __forceinline__ void decays(F2 (*a)[S / 2], const fl
         }
 }
 
-// A run's own sum E of h = a h + x B, from nothing, and the product P of its decays
-template <int S> __device__ __forceinline__ void own_sum(F2* P, F2* E, const F2 (*a)[S / 2], const F2 (*b)[S / 2], const float* x) {
+// A run's own sum E of h = a h + b, from nothing, and the product P of its decays
+template <int S> __device__ __forceinline__ void own_sum(F2* P, F2* E, const F2 (*a)[S / 2], const F2 (*b)[S / 2]) {
 #pragma unroll
-    for (int j = 0; j < RUN; ++j) {
-        const F2 xj = f2_make(x[j], x[j]);
+    for (int j = 0; j < RUN; ++j)
 #pragma unroll
         for (int s = 0; s < S / 2; ++s) {
-            const F2 in = f2_mul(xj, b[j][s]);
-            E[s] = j ? f2_fma(a[j][s], E[s], in) : in;
+            E[s] = j ? f2_fma(a[j][s], E[s], b[j][s]) : b[j][s];
             P[s] = j ? f2_mul(P[s], a[j][s]) : a[j][s];
         }
-    }
 }
 
 // The state that enters each lane's run, from the runs' own sums and the state h0 that enters the tile; E of the last run becomes what leaves the tile.  Runs
 // are joined over the lanes by doubling.  An infinite state times a product that has left the type's range would be a NaN where the recurrence token by
 // token keeps the infinity: with a sum that is not finite the runs follow one another.
-template <int S> __device__ __forceinline__ void entering(F2* in, F2* E, F2* P, const F2* h0, const F2 (*a)[S / 2], const F2 (*b)[S / 2], const float* x, int run, int part) {
+template <int S> __device__ __forceinline__ void entering(F2* in, F2* E, F2* P, const F2* h0, const F2 (*a)[S / 2], const F2 (*b)[S / 2], int run, int part) {
     F2 probe = 0ull;                                             // 0, or NaN
 #pragma unroll
     for (int s = 0; s < S / 2; ++s) probe = f2_fma(h0[s], 0ull, f2_fma(E[s], 0ull, probe));
@@ -157,7 +146,7 @@ template <int S> __device__ __forceinline__ void entering(F2* in, F2* E, F2* P, 
 #pragma unroll
             for (int j = 0; j < RUN; ++j)
 #pragma unroll
-                for (int s = 0; s < S / 2; ++s) end[s] = f2_fma(a[j][s], end[s], f2_mul(f2_make(x[j], x[j]), b[j][s]));
+                for (int s = 0; s < S / 2; ++s) end[s] = f2_fma(a[j][s], end[s], b[j][s]);
 #pragma unroll
             for (int s = 0; s < S / 2; ++s) now[s] = f2_shfl(end[s], r * PARTS + part);
         }
@@ -183,29 +172,100 @@ template <int S> __device__ __forceinline__ void entering(F2* in, F2* E, F2* P, 
     }
 }
 
-// What a tile's warp leaves for the warp of the next one: the flag counts the tiles that are through.  A wait is bounded; one that runs out raises the status and
-// the CTA's flag, after which nobody waits any more.
+// What a tile's warp leaves for the warp of the next one, with a word that counts the tiles that are through.  The word is polled: a wait on an mbarrier of shared
+// memory resumes too late for steps of a few hundred cycles (8 x 4096 x 768 2.3 ms for 1.7).  A wait is bounded; one that runs out raises the status
+// and the CTA's flag, after which nobody waits any more.  Lanes leave together, because instructions on tensor memory follow that want the whole warp.
 struct Handover {
     volatile int* given_up;
     int32_t* status;
     __device__ __forceinline__ void await(const uint32_t* flag, uint32_t want) const {
         const uint32_t addr = smem_u32(flag);
-        uint32_t got;
 #pragma unroll 1
         for (uint32_t i = 0;; ++i) {
+            uint32_t got;
             asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(got) : "r"(addr) : "memory");
-            if (__all_sync(ALL, got == want)) return;
-            if (i >= (1u << 21) || __any_sync(ALL, *given_up)) break;
-            if (i > 8) __nanosleep(32);
+            if (got == want) break;
+            if ((i & 63u) == 63u && (i >= (1u << 24) || *given_up)) {
+                *given_up = 1;
+                if (status) atomicOr(status, 1);
+                break;
+            }
         }
-        *given_up = 1;
-        if (status && (threadIdx.x & 31) == 0) atomicOr(status, 1);
+        __syncwarp();
     }
     __device__ __forceinline__ void pass(uint32_t* flag, uint32_t value) const {
         __syncwarp();
         if ((threadIdx.x & 31) == 0) asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(flag)), "r"(value) : "memory");
     }
 };
+
+// Tensor memory, 16 or 32 columns of a lane's own row: the whole warp at once, and nothing that takes the values is moved ahead of the wait
+template <int N> __device__ __forceinline__ void recall(uint32_t from, float* v) {
+    __syncwarp();
+    if constexpr (N == 32) tc_ld32(from, v);
+    else tc_ld16(from, v);
+}
+template <int N> __device__ __forceinline__ void landed(float* v) {
+    __syncwarp();
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+        asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
+}
+template <int N> __device__ __forceinline__ void keep(uint32_t to, const float* v) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; i += 16) tc_st16(to + i, (const uint32_t*)v + i);
+}
+__device__ __forceinline__ void kept() {
+    __syncwarp();
+    tc_wait_st();
+}
+
+__device__ __forceinline__ uint32_t tmem_take(uint32_t* slot, int columns) {
+    __syncwarp();
+    if (threadIdx.x < 32) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    return *slot;
+}
+__device__ __forceinline__ void tmem_give(uint32_t tmem, int columns) {
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    }
+}
+
+// S states of a lane's 8 tokens of a map, out of global memory; tokens from `len` on and states from N on are zeros
+template <typename T, int S> __device__ __forceinline__ void map_of(float* m, const T* src, int64_t stride, int64_t t0, int len, int n, int N, int piece) {
+    constexpr int BYTES = S * (int)sizeof(T);
+    const bool whole = n + S <= N && piece >= BYTES;
+#pragma unroll
+    for (int j = 0; j < RUN; ++j) {
+        const T* from = src + (t0 + j) * stride + n;
+        T e[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) e[s] = DType<T>::from_f(0.f);
+        if (t0 + j < len) {
+            if (whole) {
+                if constexpr (BYTES == 16) { const uint4 w = *(const uint4*)from; memcpy(e, &w, 16); }
+                else if constexpr (BYTES == 8) { const uint2 w = *(const uint2*)from; memcpy(e, &w, 8); }
+                else { const uint32_t w = *(const uint32_t*)from; memcpy(e, &w, 4); }
+            } else {
+#pragma unroll
+                for (int s = 0; s < S; ++s) if (n + s < N) e[s] = from[s];
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) m[j * S + s] = DType<T>::to_f(e[s]);
+    }
+}
 
 // S values of a row in shared memory, as pairs
 template <typename T, int S> __device__ __forceinline__ void pairs(F2* out, const T* row) {
@@ -233,25 +293,6 @@ struct Params {
 
 // a length is a number from 0 to L, whatever the caller's memory holds
 __device__ __forceinline__ int length_of(const Params& p, int b) { return p.lengths ? min(max(p.lengths[b], 0), p.L) : p.L; }
-
-// [64 tokens][Npad] of a map of this tile, by a warp; tokens from `len` on and states from N on are zeros
-template <typename T> __device__ __forceinline__ void fetch_map(T* dst, const T* src, int64_t stride, int64_t t0, int len, int N, int Npad, int piece, int lane) {
-    if (piece >= 16) {
-        const int n16 = Npad * (int)sizeof(T) / 16, have = N * (int)sizeof(T) / 16;
-#pragma unroll
-        for (int t = lane; t < TILE; t += 32) {
-            char* to = (char*)(dst + row_of(t) * Npad);
-            const char* from = (const char*)(src + (t0 + t) * stride);
-            for (int k = 0; k < n16; ++k) {
-                if (t0 + t < len && k < have) copy16(to + 16 * k, from + 16 * k);
-                else *(uint4*)(to + 16 * k) = make_uint4(0u, 0u, 0u, 0u);
-            }
-        }
-    } else {
-        for (int t = lane; t < TILE; t += 32)
-            for (int n = 0; n < Npad; ++n) dst[row_of(t) * Npad + n] = t0 + t < len && n < N ? src[(t0 + t) * stride + n] : DType<T>::from_f(0.f);
-    }
-}
 
 }  // namespace scan
 }  // namespace vig

@@ -12,33 +12,32 @@
 namespace vig {
 using namespace scan;
 
-// Shared memory: for every warp the rows of u, dt and z, the maps, and steps and inputs a channel at a time; for the CTA A, the states between tiles and
-// their flags, bias and skip.
-template <typename T, int S, int CT> struct FwdSmem {
-    static constexpr int NB = 4 * S, ROWS = TILE * CT * (int)sizeof(T);
+// A CTA's shared memory: for every warp steps and inputs a channel at a time; A, the states between tiles and their flags, bias and skip.
+template <int S, int CT> struct FwdSmem {
+    static constexpr int NB = PARTS * S;
     static __host__ __device__ int padded(int N) { return (N + NB - 1) / NB * NB; }
-    static __host__ __device__ int warp_bytes(int N) {
-        const int Np = padded(N);
-        return 3 * ROWS + 2 * TILE * Np * (int)sizeof(T) + (Np > NB ? 3 : 2) * CT * TILE * 4;
-    }
-    static int bytes(int N, int W) { return W * warp_bytes(N) + (2 * CT * padded(N) + CT * padded(N) / NB + 2 * CT + 4) * 4; }
+    static int bytes(int N, int W) { return (W * 2 * CT * TILE + 2 * CT * padded(N) + CT * padded(N) / NB + 2 * CT + 4) * 4; }
 };
-
+// columns of tensor memory: 2 x 8 S for every block of states, a power of two, 32 at least
+template <int S> __host__ __device__ int fwd_columns(int N) {
+    int c = 32;
+    while (c < (N + PARTS * S - 1) / (PARTS * S) * 2 * RUN * S) c *= 2;
+    return c;
+}
 template <typename T, int S, int CT, int W>
-__global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kernel(const Params p) {
-    using M = FwdSmem<T, S, CT>;
-    constexpr int NB = M::NB, THREADS = 32 * W;
-    extern __shared__ __align__(16) char smem[];
+__global__ void __launch_bounds__(32 * W, 16 / W) scan_fwd_kernel(const Params p) {
+    using M = FwdSmem<S, CT>;
+    constexpr int NB = M::NB, THREADS = 32 * W, MAP = RUN * S;
+    extern __shared__ __align__(16) float room[];
+    __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, run = lane / PARTS, part = lane % PARTS;
-    const int Npad = M::padded(p.N), Dg = p.D / p.G;
+    const int Npad = M::padded(p.N), Dg = p.D / p.G, columns = fwd_columns<S>(p.N);
     const int ct = blockIdx.x % p.ctiles, g = blockIdx.x / p.ctiles % p.G, b = blockIdx.x / p.ctiles / p.G;
     const int c0 = ct * CT, have = min(CT, Dg - c0), d = g * Dg + c0;             // channels of the CTA, the first one's index
     const int len = length_of(p, b), ntiles = (len + TILE - 1) / TILE;
-    char* const mine = smem + warp * M::warp_bytes(p.N);
-    T *const ru = (T*)mine, *const rdt = ru + TILE * CT, *const rz = rdt + TILE * CT, *const mB = rz + TILE * CT, *const mC = mB + TILE * Npad;
-    float *const delta = (float*)(mC + TILE * Npad), *const x = delta + CT * TILE;
-    float* const ys = Npad > NB ? x + CT * TILE : delta;         // with one block of states a channel's steps are done with when its sums are there
-    float *const sA = (float*)(smem + W * M::warp_bytes(p.N)), *const carry = sA + CT * Npad, *const bias = carry + CT * Npad, *const skip = bias + CT;
+    float *const delta = room + warp * 2 * CT * TILE, *const x = delta + CT * TILE;
+    float* const ys = delta;                                     // a channel's steps are done with when its sums are there
+    float *const sA = room + W * 2 * CT * TILE, *const carry = sA + CT * Npad, *const bias = carry + CT * Npad, *const skip = bias + CT;
     uint32_t* const flags = (uint32_t*)(skip + CT);
     int* const given_up = (int*)(flags + CT * Npad / NB);
     const Handover hand{given_up, p.status};
@@ -55,35 +54,31 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
     }
     for (int i = tid; i < CT * Npad / NB; i += THREADS) flags[i] = 0;
     if (tid == 0) *given_up = 0;
-    __syncthreads();
+    const uint32_t tmem_base = tmem_take(&tmem_slot, columns), tmem = tmem_base + ((uint32_t)(32 * (warp & 3)) << 16);
     const T *u = (const T*)p.u + b * p.s_u[0] + d, *dt = (const T*)p.dt + b * p.s_dt[0] + d, *z = p.z ? (const T*)p.z + b * p.s_z[0] + d : nullptr;
     const T *gB = (const T*)p.b + b * p.s_b[0] + g * p.s_b[2], *gC = (const T*)p.c + b * p.s_c[0] + g * p.s_c[2];
     T* const y = (T*)p.y + b * p.s_y[0] + d;
 
     for (int tile = warp; tile < ntiles; tile += W) {
         const int64_t t0 = (int64_t)tile * TILE;
-#pragma unroll
-        for (int t = lane; t < TILE; t += 32) {
-            if (t0 + t < len) {
-                fetch<T, CT>(rdt + t * CT, dt + (t0 + t) * p.s_dt[1], have, p.piece);
-                fetch<T, CT>(ru + t * CT, u + (t0 + t) * p.s_u[1], have, p.piece);
-                if (z) fetch<T, CT>(rz + t * CT, z + (t0 + t) * p.s_z[1], have, p.piece);
-            }
+        for (int n0 = 0; n0 < Npad; n0 += NB) {
+            float m[MAP];
+            map_of<T, S>(m, gB, p.s_b[1], t0 + run * RUN, len, n0 + part * S, p.N, p.piece_maps);
+            keep<MAP>(tmem + n0 / NB * 2 * MAP, m);
+            map_of<T, S>(m, gC, p.s_c[1], t0 + run * RUN, len, n0 + part * S, p.N, p.piece_maps);
+            keep<MAP>(tmem + n0 / NB * 2 * MAP + MAP, m);
         }
-        fetch_map<T>(mB, gB, p.s_b[1], t0, len, p.N, Npad, p.piece_maps, lane);
-        fetch_map<T>(mC, gC, p.s_c[1], t0, len, p.N, Npad, p.piece_maps, lane);
-        copies_done();
-        __syncwarp();
 #pragma unroll 1
         for (int t = lane; t < TILE; t += 32) {
             const bool in = t0 + t < len;                        // behind the end a token changes nothing
+            const int64_t at = in ? t0 + t : t0;
             float uf[CT], df[CT];
-            read<T, CT>(uf, ru + t * CT, CT, 16);
-            read<T, CT>(df, rdt + t * CT, CT, 16);
+            read<T, CT>(df, dt + at * p.s_dt[1], have, p.piece);
+            read<T, CT>(uf, u + at * p.s_u[1], have, p.piece);
 #pragma unroll
             for (int c = 0; c < CT; c += 2) {
                 F2 dl = f2_add(f2_make(df[c], df[c + 1]), *(const F2*)(bias + c));
-                if (p.softplus) dl = softplus<T>(dl);
+                if (p.softplus) dl = softplus(dl);
                 const F2 xi = f2_mul(dl, f2_make(uf[c], uf[c + 1]));
                 delta[c * TILE + t] = in ? f2_lo(dl) : 0.f;
                 delta[(c + 1) * TILE + t] = in ? f2_hi(dl) : 0.f;
@@ -91,32 +86,37 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
                 x[(c + 1) * TILE + t] = in ? f2_hi(xi) : 0.f;
             }
         }
+        kept();
         __syncwarp();
 
-        for (int n0 = 0; n0 < Npad; n0 += NB) {
-            F2 B[RUN][S / 2], C[RUN][S / 2];
-#pragma unroll
-            for (int j = 0; j < RUN; ++j) {
-                const int at = (j * RUN + run) * Npad + n0 + part * S;
-                pairs<T, S>(B[j], mB + at);
-                pairs<T, S>(C[j], mC + at);
-            }
 #pragma unroll 1
-            for (int c = 0; c < have; ++c) {
+        for (int c = 0; c < have; ++c) {
+            float yv[RUN];
+#pragma unroll 1
+            for (int n0 = 0; n0 < Npad; n0 += NB) {
                 float* const h_at = carry + c * Npad + n0 + part * S;
                 uint32_t* const flag = flags + n0 / NB * CT + c;
-                F2 A2[S / 2], a[RUN][S / 2], P[S / 2], E[S / 2], h0[S / 2], h[S / 2];
+                const uint32_t col = tmem + n0 / NB * 2 * MAP;
+                float m[MAP], dl[RUN], xr[RUN];
+                recall<MAP>(col, m);
+                F2 A2[S / 2], a[RUN][S / 2], in[RUN][S / 2], P[S / 2], E[S / 2], h0[S / 2], h[S / 2];
                 pairs<float, S>(A2, sA + c * Npad + n0 + part * S);
-                float dl[RUN], xr[RUN], yv[RUN];
-                *(float4*)dl = *(const float4*)(delta + c * TILE + run * RUN);
-                *(float4*)(dl + 4) = *(const float4*)(delta + c * TILE + run * RUN + 4);
-                *(float4*)xr = *(const float4*)(x + c * TILE + run * RUN);
-                *(float4*)(xr + 4) = *(const float4*)(x + c * TILE + run * RUN + 4);
+#pragma unroll
+                for (int k = 0; k < RUN; k += 4) {
+                    *(float4*)(dl + k) = *(const float4*)(delta + c * TILE + run * RUN + k);
+                    *(float4*)(xr + k) = *(const float4*)(x + c * TILE + run * RUN + k);
+                }
                 decays<S>(a, dl, A2);
-                own_sum<S>(P, E, a, B, xr);
+                landed<MAP>(m);
+#pragma unroll
+                for (int j = 0; j < RUN; ++j)
+#pragma unroll
+                    for (int s = 0; s < S / 2; ++s) in[j][s] = f2_mul(f2_make(xr[j], xr[j]), f2_make(m[j * S + 2 * s], m[j * S + 2 * s + 1]));
+                own_sum<S>(P, E, a, in);
+                recall<MAP>(col + MAP, m);
                 hand.await(flag, (uint32_t)tile);
                 pairs<float, S>(h0, h_at);
-                entering<S>(h, E, P, h0, a, B, xr, run, part);
+                entering<S>(h, E, P, h0, a, in, run, part);
                 __syncwarp();
                 if (run == RUN - 1) {
 #pragma unroll
@@ -128,33 +128,32 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
 #pragma unroll
                     for (int s = 0; s < S; ++s) if (n0 + part * S + s < p.N) to[s] = s & 1 ? f2_hi(h0[s / 2]) : f2_lo(h0[s / 2]);
                 }
+                landed<MAP>(m);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
-                    const F2 xj = f2_make(xr[j], xr[j]);
                     F2 sum = 0ull;
 #pragma unroll
                     for (int s = 0; s < S / 2; ++s) {
-                        h[s] = f2_fma(a[j][s], h[s], f2_mul(xj, B[j][s]));
-                        sum = s ? f2_fma(C[j][s], h[s], sum) : f2_mul(C[j][s], h[s]);
+                        const F2 C = f2_make(m[j * S + 2 * s], m[j * S + 2 * s + 1]);
+                        h[s] = f2_fma(a[j][s], h[s], in[j][s]);
+                        sum = s ? f2_fma(C, h[s], sum) : f2_mul(C, h[s]);
                     }
-                    yv[j] = f2_lo(sum) + f2_hi(sum);
+                    const float v = f2_lo(sum) + f2_hi(sum);
+                    yv[j] = n0 ? yv[j] + v : v;
                 }
-                float2 got = over_parts(yv, part);
-                float2* const ya = (float2*)(ys + c * TILE + run * RUN + part * 2);
-                if (n0) { const float2 was = *ya; got.x += was.x; got.y += was.y; }
-                *ya = got;
             }
+            *(float2*)(ys + c * TILE + run * RUN + part * 2) = over_parts(yv, part);
         }
         __syncwarp();
 #pragma unroll 1
         for (int t = lane; t < TILE; t += 32) {
             if (t0 + t >= len) break;
             float uf[CT], out[CT];
-            read<T, CT>(uf, ru + t * CT, CT, 16);
+            read<T, CT>(uf, u + (t0 + t) * p.s_u[1], have, p.piece);
 #pragma unroll
             for (int c = 0; c < CT; ++c) out[c] = fmaf(skip[c], uf[c], ys[c * TILE + t]);
             if (z) {
-                read<T, CT>(uf, rz + t * CT, CT, 16);
+                read<T, CT>(uf, z + (t0 + t) * p.s_z[1], have, p.piece);
 #pragma unroll
                 for (int c = 0; c < CT; ++c) out[c] *= uf[c] * sigmoid(uf[c]);
             }
@@ -167,8 +166,8 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
         const float out[CT] = {};
         put<T, CT>(y + at * p.s_y[1], out, have, p.piece);
     }
+    tmem_give(tmem_base, columns);                               // (a barrier too)
     if (p.h_final) {
-        __syncthreads();
         for (int i = tid; i < CT * Npad; i += THREADS) {
             const int c = i / Npad, n = i - c * Npad;
             if (c < have && n < p.N) p.h_final[b * p.ld_final + (int64_t)(d + c) * p.N + n] = carry[i];
@@ -179,9 +178,8 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
 // Backward, from the states that enter each tile (the forward wrote them) and the tiles from the last to the first.  With g_t = dL/dh_t,
 //   g_t = C_t dy_t + a_{t+1} g_{t+1},  dC_t = sum_d h_t dy_t,  dB_t = sum_d g_t delta_t u_t,  du_t = delta_t sum_n g_t B_t + D dy_t,
 //   ddelta_t = sum_n g_t (a_t h_{t-1} A + u_t B_t),  dA = sum g_t a_t h_{t-1} delta_t,
-// dy being d_out silu(z).  What goes from tile to tile is a_t g_t of a tile's first token.  A lane keeps the decays and states of its run; the maps and the sums
-// of their gradients over the CTA's channels, 64 values a lane and state block, are kept in tensor memory, where each lane has a row of its own: registers
-// have no room for them, and in shared memory every access would take four turns.  The shares of CTAs, sequences and warps are added in a fixed order by
+// dy being d_out silu(z).  What goes from tile to tile is a_t g_t of a tile's first token.  A lane keeps the decays and states of its run in registers; the sums
+// of the maps' gradients over the CTA's channels are in tensor memory beside the maps.  The shares of CTAs, sequences and warps are added in a fixed order by
 // sum_kernel.
 constexpr int BS = 2, BNB = PARTS * BS, BCT = 16, BW = 4, BTHREADS = 32 * BW;     // states of a lane, of a block; channels and warps of a CTA
 
@@ -213,15 +211,6 @@ template <int NC> __device__ __forceinline__ float over_lanes(float* v, int lane
     return r;
 }
 
-// values out of tensor memory are there: nothing that takes them is moved ahead of the wait
-__device__ __forceinline__ void pinned(float* v) {
-#pragma unroll
-    for (int i = 0; i < 16; i += 8)
-        asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
-}
-__device__ __forceinline__ void landed(float* v) { tc_wait_ld(); pinned(v); }
-__device__ __forceinline__ void landed(float* v, float* w) { tc_wait_ld(); pinned(v); pinned(w); }
-
 template <typename T>
 __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
     constexpr int S = BS, NB = BNB, CT = BCT, W = BW, THREADS = BTHREADS;
@@ -241,10 +230,6 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
     int* const given_up = (int*)(flags + CT * Npad / NB);
     const Handover hand{given_up, p.status};
 
-    if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
@@ -258,10 +243,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
     }
     for (int i = tid; i < CT * Npad / NB; i += THREADS) flags[i] = 0;
     if (tid == 0) *given_up = 0;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = tmem_slot + ((uint32_t)(32 * warp) << 16);      // [state block][B, C, dB, dC][8 tokens x 2 states]
+    const uint32_t tmem_base = tmem_take(&tmem_slot, columns), tmem = tmem_base + ((uint32_t)(32 * warp) << 16);      // [state block][B, C, dB, dC][8 tokens x 2 states]
     const T *u = (const T*)p.u + b * p.s_u[0] + d, *dt = (const T*)p.dt + b * p.s_dt[0] + d, *z = p.z ? (const T*)p.z + b * p.s_z[0] + d : nullptr;
     const T* dy = (const T*)p.dy + b * p.s_dy[0] + d;
     const T *gB = (const T*)p.b + b * p.s_b[0] + g * p.s_b[2], *gC = (const T*)p.c + b * p.s_c[0] + g * p.s_c[2];
@@ -274,21 +256,12 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
         for (int i = lane; i < have * p.N; i += 32) copy4(st + (p.N == Npad ? i : i / p.N * Npad + i % p.N), from + i);
         for (int n0 = 0; n0 < Npad; n0 += NB) {
             float mb[RUN * S], mc[RUN * S];
-#pragma unroll
-            for (int j = 0; j < RUN; ++j) {
-                const int64_t at = t0 + run * RUN + j;
-#pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    const int n = n0 + part * S + s;
-                    const bool in = at < len && n < p.N;
-                    mb[j * S + s] = in ? DType<T>::to_f(gB[at * p.s_b[1] + n]) : 0.f;
-                    mc[j * S + s] = in ? DType<T>::to_f(gC[at * p.s_c[1] + n]) : 0.f;
-                }
-            }
-            tc_st16(tmem + n0 / NB * 64, (const uint32_t*)mb);
-            tc_st16(tmem + n0 / NB * 64 + 16, (const uint32_t*)mc);
+            map_of<T, S>(mb, gB, p.s_b[1], t0 + run * RUN, len, n0 + part * S, p.N, p.piece_maps);
+            map_of<T, S>(mc, gC, p.s_c[1], t0 + run * RUN, len, n0 + part * S, p.N, p.piece_maps);
+            keep<16>(tmem + n0 / NB * 64, mb);
+            keep<16>(tmem + n0 / NB * 64 + 16, mc);
         }
-        tc_wait_st();
+        kept();
 #pragma unroll 1
         for (int t = lane; t < TILE; t += 32) {
             const bool in = t0 + t < len;
@@ -300,7 +273,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
 #pragma unroll
             for (int c = 0; c < CT; c += 2) {
                 F2 dl = f2_add(f2_make(df[c], df[c + 1]), *(const F2*)(bias + c));
-                if (p.softplus) dl = softplus<T>(dl);
+                if (p.softplus) dl = softplus(dl);
                 const F2 xi = f2_mul(dl, f2_make(uf[c], uf[c + 1]));
                 delta[c * TILE + t] = in ? f2_lo(dl) : 0.f;
                 delta[(c + 1) * TILE + t] = in ? f2_hi(dl) : 0.f;
@@ -320,13 +293,11 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
 
 #pragma unroll 1
         for (int c = 0; c < have; ++c) {
-            float dl[RUN], xr[RUN], dr[RUN];
-#pragma unroll
-            for (int k = 0; k < RUN; k += 4) {
-                *(float4*)(dl + k) = *(const float4*)(delta + c * TILE + run * RUN + k);
-                *(float4*)(xr + k) = *(const float4*)(x + c * TILE + run * RUN + k);
-                *(float4*)(dr + k) = *(const float4*)(dys + c * TILE + run * RUN + k);
-            }
+            // read again where they are used: registers are what this kernel is short of
+            auto row = [&](float* v, const float* from) {
+                *(float4*)v = *(const float4*)(from + c * TILE + run * RUN);
+                *(float4*)(v + 4) = *(const float4*)(from + c * TILE + run * RUN + 4);
+            };
             F2 s_y[RUN], s_b[RUN], s_a[RUN];                     // what is summed over the states
 #pragma unroll
             for (int j = 0; j < RUN; ++j) s_y[j] = s_b[j] = s_a[j] = 0ull;
@@ -334,33 +305,41 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
             for (int n0 = 0; n0 < Npad; n0 += NB) {
                 const int at = c * Npad + n0 + part * S;
                 const uint32_t col = tmem + n0 / NB * 64;
-                float mb[RUN * S], mc[RUN * S], md[RUN * S];
-                tc_ld16(col, mb);
-                tc_ld16(col + 16, mc);
-                F2 A[1], A2[1], P[1], E[1], h0[1], h[RUN + 1][1], a[RUN][1], B[RUN][1];
+                float mb[RUN * S], mc[RUN * S], md[RUN * S], xr[RUN], dr[RUN];
+                recall<16>(col, mb);
+                recall<16>(col + 16, mc);
+                F2 A[1], P[1], E[1], h0[1], h[RUN + 1][1], a[RUN][1], in[RUN][1], Q = 0ull, Pb;
                 pairs<float, S>(A, sA + at);
-                pairs<float, S>(h0, st + at);
-                A2[0] = f2_mul(A[0], f2_make(LOG2E, LOG2E));
-                decays<S>(a, dl, A2);
-                landed(mb, mc);
+                {
+                    const F2 A2[1] = {f2_mul(A[0], f2_make(LOG2E, LOG2E))};
+                    float dl[RUN];
+                    row(dl, delta);
+                    decays<S>(a, dl, A2);
+                }
+                row(xr, x);
+                row(dr, dys);
+                landed<16>(mb);
+                landed<16>(mc);
+                if (c) recall<16>(col + 48, md);
 #pragma unroll
-                for (int j = 0; j < RUN; ++j) B[j][0] = f2_make(mb[2 * j], mb[2 * j + 1]);
-                if (c) tc_ld16(col + 48, md);
-                own_sum<S>(P, E, a, B, xr);
-                F2 Pb = P[0], Q = 0ull;
+                for (int j = 0; j < RUN; ++j) in[j][0] = f2_mul(f2_make(xr[j], xr[j]), f2_make(mb[2 * j], mb[2 * j + 1]));
+                own_sum<S>(P, E, a, in);
+                Pb = P[0];
 #pragma unroll
                 for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), f2_make(dr[j], dr[j]), Q));
-                entering<S>(h[0], E, P, h0, a, B, xr, run, part);
-                if (c) landed(md);
+                pairs<float, S>(h0, st + at);
+                entering<S>(h[0], E, P, h0, a, in, run, part);
+                if (c) landed<16>(md);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
-                    h[j + 1][0] = f2_fma(a[j][0], h[j][0], f2_mul(f2_make(xr[j], xr[j]), B[j][0]));
+                    h[j + 1][0] = f2_fma(a[j][0], h[j][0], in[j][0]);
                     s_y[j] = f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), h[j + 1][0], s_y[j]);
                     const F2 add = f2_fma(h[j + 1][0], f2_make(dr[j], dr[j]), c ? f2_make(md[2 * j], md[2 * j + 1]) : 0ull);
                     md[2 * j] = f2_lo(add);
                     md[2 * j + 1] = f2_hi(add);
                 }
-                tc_st16(col + 48, (const uint32_t*)md);
+                keep<16>(col + 48, md);
+                if (c) recall<16>(col + 32, md);
                 // from the other end: q_t = a_t g_t is what token t - 1 gets
                 uint32_t* const flag = flags + n0 / NB * CT + c;
                 float* const q_at = carry + at;
@@ -381,12 +360,16 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                     const F2 e = f2_shfl_down(Q, PARTS);
                     Q = run == RUN - 1 ? q0[0] : e;
                 }
-                if (c) { tc_ld16(col + 32, md); landed(md); }
+                float dl[RUN];
+                row(dl, delta);
+                row(xr, x);
+                row(dr, dys);
+                if (c) landed<16>(md);
                 F2 dAs = 0ull;
 #pragma unroll
                 for (int j = RUN - 1; j >= 0; --j) {
                     const F2 gr = f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), f2_make(dr[j], dr[j]), Q);
-                    s_b[j] = f2_fma(gr, B[j][0], s_b[j]);
+                    s_b[j] = f2_fma(gr, f2_make(mb[2 * j], mb[2 * j + 1]), s_b[j]);
                     const F2 add = f2_fma(gr, f2_make(xr[j], xr[j]), c ? f2_make(md[2 * j], md[2 * j + 1]) : 0ull);
                     md[2 * j] = f2_lo(add);
                     md[2 * j + 1] = f2_hi(add);
@@ -395,14 +378,14 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                     s_a[j] = f2_fma(f, A[0], s_a[j]);
                     dAs = f2_fma(f, f2_make(dl[j], dl[j]), dAs);
                 }
-                tc_st16(col + 32, (const uint32_t*)md);
+                keep<16>(col + 32, md);
                 // dA over the runs: a lane of an even run keeps the first state's sum, of an odd one the second's
                 const bool odd = run & 1;
                 float v = (odd ? f2_hi(dAs) : f2_lo(dAs)) + __shfl_xor_sync(ALL, odd ? f2_lo(dAs) : f2_hi(dAs), PARTS);
                 v += __shfl_xor_sync(ALL, v, 2 * PARTS);
                 v += __shfl_xor_sync(ALL, v, 4 * PARTS);
                 if (run < 2) dA[at + run] += v;
-                tc_wait_st();
+                kept();
             }
             float v[RUN];
             const int to = c * TILE + run * RUN + part * 2;
@@ -422,9 +405,10 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
         // the tile's maps have their gradients from this CTA's channels
         for (int n0 = 0; n0 < Npad; n0 += NB) {
             float mb[RUN * S], mc[RUN * S];
-            tc_ld16(tmem + n0 / NB * 64 + 32, mb);
-            tc_ld16(tmem + n0 / NB * 64 + 48, mc);
-            landed(mb, mc);
+            recall<16>(tmem + n0 / NB * 64 + 32, mb);
+            recall<16>(tmem + n0 / NB * 64 + 48, mc);
+            landed<16>(mb);
+            landed<16>(mc);
 #pragma unroll
             for (int j = 0; j < RUN; ++j) {
                 const int64_t at = t0 + run * RUN + j;
@@ -464,7 +448,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
                 out[c] = fmaf(gb[c * TILE + t], uf[c], ga[c * TILE + t]);
-                if (p.softplus) out[c] *= sigmoid(zf[c] + bias[c]);
+                if (p.softplus) out[c] *= slope(zf[c] + bias[c]);
                 keep_bias[c] += out[c];
             }
             put<T, CT>((T*)p.d_dt + row, out, have, p.piece);
@@ -487,12 +471,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
         p.part_c[at] = 0.f;
     }
     if (!(lane & 1)) { shares[warp * CT + lane / 2] = sum_skip; shares[(W + warp) * CT + lane / 2] = sum_bias; }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 0) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"(columns) : "memory");
-    }
+    tmem_give(tmem_base, columns);                               // (a barrier too)
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         if (c < have && n < p.N) {
@@ -552,7 +531,7 @@ template <typename T> __global__ void __launch_bounds__(128) scan_step_kernel(co
     const float u = DType<T>::to_f(((const T*)p.u)[b * p.s_u + d]), zv = p.z ? DType<T>::to_f(((const T*)p.z)[b * p.s_z + d]) : 0.f;
     float dl = DType<T>::to_f(((const T*)p.dt)[b * p.s_dt + d]) + (p.bias ? param_at<T>(p.bias, d, p.bias_f32) : 0.f);
     const float skip = p.skip ? param_at<T>(p.skip, d, p.skip_f32) : 0.f;
-    if (p.softplus) dl = f2_lo(softplus<T>(f2_make(dl, dl)));
+    if (p.softplus) dl = f2_lo(softplus(f2_make(dl, dl)));
     const float x = dl * u;
     float y = 0.f;
     for (int n0 = part * 4; n0 < p.N; n0 += 16) {
@@ -601,7 +580,7 @@ static void narrow(int& piece, const void* ptr, const int64_t* strides, int coun
 template <typename T, int S, int CT, int W> int fwd_launch(Params& p, cudaStream_t s) {
     p.ctiles = (p.D / p.G + CT - 1) / CT;
     const int64_t grid = (int64_t)p.B * p.G * p.ctiles;
-    const int smem = FwdSmem<T, S, CT>::bytes(p.N, W);
+    const int smem = FwdSmem<S, CT>::bytes(p.N, W);
     if (grid >= (1ll << 31)) return VIG_ERR_SHAPE;
     if (const cudaError_t e = ensure_smem_attr((const void*)scan_fwd_kernel<T, S, CT, W>, smem)) return (int)e;
     scan_fwd_kernel<T, S, CT, W><<<(unsigned)grid, 32 * W, smem, s>>>(p);
