@@ -46,8 +46,61 @@ __device__ __forceinline__ float slope(float x) {
 }
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-x * LOG2E)); }
 
+// where the row of token t of a tile's map lies: eight lanes that read token j of their runs read eight neighbouring rows
+__device__ __forceinline__ int row_of(int t) { return (t % RUN) * RUN + t / RUN; }
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
+__device__ __forceinline__ void copy8(void* dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(void* dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory"); }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// NC values of a row into shared memory of the lane's own: in pieces of what pointers and strides allow, or one at a time; values from `have` on are zeros
+template <typename T, int NC> __device__ __forceinline__ void fetch(T* dst, const T* src, int have, int piece) {
+    constexpr int BYTES = NC * (int)sizeof(T);
+    if (have >= NC && piece >= 8) {
+        if (BYTES % 16 == 0 && piece >= 16) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) copy16((char*)dst + 16 * i, (const char*)src + 16 * i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < BYTES / 8; ++i) copy8((char*)dst + 8 * i, (const char*)src + 8 * i);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) dst[i] = i < have ? src[i] : DType<T>::from_f(0.f);
+}
+
+// [64 tokens][Npad] of a map of this tile, by a warp; tokens from `len` on and states from N on are zeros
+template <typename T> __device__ __forceinline__ void fetch_map(T* dst, const T* src, int64_t stride, int64_t t0, int len, int N, int Npad, int piece, int lane) {
+    if (piece >= 16) {
+        const int n16 = Npad * (int)sizeof(T) / 16, have = N * (int)sizeof(T) / 16;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int t = lane + 32 * r;
+            char* to = (char*)(dst + row_of(t) * Npad);
+            const char* from = (const char*)(src + (t0 + t) * stride);
+            for (int k = 0; k < n16; ++k) {
+                if (t0 + t < len && k < have) copy16(to + 16 * k, from + 16 * k);
+                else *(uint4*)(to + 16 * k) = make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+    } else {
+        for (int t = lane; t < TILE; t += 32)
+            for (int n = 0; n < Npad; ++n) dst[row_of(t) * Npad + n] = t0 + t < len && n < N ? src[(t0 + t) * stride + n] : DType<T>::from_f(0.f);
+    }
+}
+
+// a row's words as they lie in shared memory
+template <int WORDS> __device__ __forceinline__ void words(uint32_t* to, const void* from) {
+    if constexpr (WORDS % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < WORDS / 4; ++i) { const uint4 w = ((const uint4*)from)[i]; to[4 * i] = w.x; to[4 * i + 1] = w.y; to[4 * i + 2] = w.z; to[4 * i + 3] = w.w; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS / 2; ++i) { const uint2 w = ((const uint2*)from)[i]; to[2 * i] = w.x; to[2 * i + 1] = w.y; }
+    }
+}
 
 // NC values of a row into registers: in pieces of what pointers and strides allow, or one at a time; values from `have` on are zeros
 template <typename T, int NC> __device__ __forceinline__ void read(float* f, const T* src, int have, int piece) {
@@ -127,49 +180,60 @@ template <int S> __device__ __forceinline__ void own_sum(F2* P, F2* E, const F2 
         }
 }
 
-// The state that enters each lane's run, from the runs' own sums and the state h0 that enters the tile; E of the last run becomes what leaves the tile.  Runs
-// are joined over the lanes by doubling.  An infinite state times a product that has left the type's range would be a NaN where the recurrence token by
-// token keeps the infinity: with a sum that is not finite the runs follow one another.
-template <int S> __device__ __forceinline__ void entering(F2* in, F2* E, F2* P, const F2* h0, const F2 (*a)[S / 2], const F2 (*b)[S / 2], int run, int part) {
+// The states that enter each lane's run, of Q channels, from the runs' own sums and the states h0 that enter the tile; E of the last run becomes what leaves the
+// tile.  Runs are joined over the lanes by doubling.  An infinite state times a product that has left the type's range would be a NaN where the recurrence
+// token by token keeps the infinity: with a sum that is not finite the runs follow one another.
+template <int S, int Q>
+__device__ __forceinline__ void entering(F2 (*in)[S / 2], F2 (*E)[S / 2], F2 (*P)[S / 2], const F2 (*h0)[S / 2], const F2 (*a)[RUN][S / 2], const F2 (*b)[RUN][S / 2], int run, int part) {
     F2 probe = 0ull;                                             // 0, or NaN
 #pragma unroll
-    for (int s = 0; s < S / 2; ++s) probe = f2_fma(h0[s], 0ull, f2_fma(E[s], 0ull, probe));
+    for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int s = 0; s < S / 2; ++s) probe = f2_fma(h0[q][s], 0ull, f2_fma(E[q][s], 0ull, probe));
     if (__any_sync(ALL, !(f2_lo(probe) + f2_hi(probe) == 0.f))) {
-        F2 now[S / 2];
 #pragma unroll
-        for (int s = 0; s < S / 2; ++s) now[s] = h0[s];
+        for (int q = 0; q < Q; ++q) {
+            F2 now[S / 2];
+#pragma unroll
+            for (int s = 0; s < S / 2; ++s) now[s] = h0[q][s];
 #pragma unroll 1
-        for (int r = 0; r < RUN; ++r) {
-            F2 end[S / 2];
+            for (int r = 0; r < RUN; ++r) {
+                F2 end[S / 2];
 #pragma unroll
-            for (int s = 0; s < S / 2; ++s) { if (run == r) in[s] = now[s]; end[s] = now[s]; }
+                for (int s = 0; s < S / 2; ++s) { if (run == r) in[q][s] = now[s]; end[s] = now[s]; }
 #pragma unroll
-            for (int j = 0; j < RUN; ++j)
+                for (int j = 0; j < RUN; ++j)
 #pragma unroll
-                for (int s = 0; s < S / 2; ++s) end[s] = f2_fma(a[j][s], end[s], b[j][s]);
+                    for (int s = 0; s < S / 2; ++s) end[s] = f2_fma(a[q][j][s], end[s], b[q][j][s]);
 #pragma unroll
-            for (int s = 0; s < S / 2; ++s) now[s] = f2_shfl(end[s], r * PARTS + part);
+                for (int s = 0; s < S / 2; ++s) now[s] = f2_shfl(end[s], r * PARTS + part);
+            }
+#pragma unroll
+            for (int s = 0; s < S / 2; ++s) E[q][s] = now[s];
         }
-#pragma unroll
-        for (int s = 0; s < S / 2; ++s) E[s] = now[s];
         return;
     }
 #pragma unroll
-    for (int s = 0; s < S / 2; ++s) E[s] = f2_fma(P[s], run == 0 ? h0[s] : 0ull, E[s]);
+    for (int q = 0; q < Q; ++q)
 #pragma unroll
-    for (int d = 1; d < RUN; d *= 2) {
+        for (int s = 0; s < S / 2; ++s) E[q][s] = f2_fma(P[q][s], run == 0 ? h0[q][s] : 0ull, E[q][s]);
+#pragma unroll
+    for (int d = 1; d < RUN; d *= 2)
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int s = 0; s < S / 2; ++s) {
+                const F2 e = f2_shfl_up(E[q][s], d * PARTS);
+                E[q][s] = f2_fma(P[q][s], run >= d ? e : 0ull, E[q][s]);
+                if (2 * d < RUN) P[q][s] = f2_mul(P[q][s], f2_shfl_up(P[q][s], d * PARTS));
+            }
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
 #pragma unroll
         for (int s = 0; s < S / 2; ++s) {
-            const F2 e = f2_shfl_up(E[s], d * PARTS);
-            E[s] = f2_fma(P[s], run >= d ? e : 0ull, E[s]);
-            if (2 * d < RUN) P[s] = f2_mul(P[s], f2_shfl_up(P[s], d * PARTS));
+            const F2 e = f2_shfl_up(E[q][s], PARTS);
+            in[q][s] = run == 0 ? h0[q][s] : e;
         }
-    }
-#pragma unroll
-    for (int s = 0; s < S / 2; ++s) {
-        const F2 e = f2_shfl_up(E[s], PARTS);
-        in[s] = run == 0 ? h0[s] : e;
-    }
 }
 
 // What a tile's warp leaves for the warp of the next one, with a word that counts the tiles that are through.  The word is polled: a wait on an mbarrier of shared

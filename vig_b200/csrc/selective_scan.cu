@@ -7,37 +7,41 @@
 // states the exponentials bound it (MUFU, 16 a cycle and SM), not memory.  So each is taken once: the warps of a CTA take tiles of the same channels'
 // tokens in turn and hand the state from tile to tile, within a tile a warp's lanes divide tokens and states (scan_common.cuh); two passes over
 // independent chunks would take every exponential twice.
+#include <cstdlib>
 #include "scan_common.cuh"
 
 namespace vig {
 using namespace scan;
 
-// A CTA's shared memory: for every warp steps and inputs a channel at a time; A, the states between tiles and their flags, bias and skip.
-template <int S, int CT> struct FwdSmem {
-    static constexpr int NB = PARTS * S;
+// A CTA's shared memory: for every warp the rows and maps of its next tile, which are under way while it works on one, and steps and inputs a channel at a
+// time; A, the states between tiles and their flags, bias and skip.  Of the tile at hand, u and z wait for the outputs in tensor memory.
+template <typename T, int S, int CT> struct FwdSmem {
+    static constexpr int NB = PARTS * S, ROWS = TILE * CT * (int)sizeof(T);
+    static constexpr int STASH = 2 * CT * (int)sizeof(T) / 4, COLUMNS = 2 * (STASH < 16 ? 16 : STASH);   // words of a row's u and z; of both rows of a lane
     static __host__ __device__ int padded(int N) { return (N + NB - 1) / NB * NB; }
-    static int bytes(int N, int W) { return (W * 2 * CT * TILE + 2 * CT * padded(N) + CT * padded(N) / NB + 2 * CT + 4) * 4; }
+    static __host__ __device__ int warp_bytes(int N) {
+        const int Np = padded(N);
+        return 3 * ROWS + 2 * TILE * Np * (int)sizeof(T) + (Np > NB ? 3 : 2) * CT * TILE * 4;
+    }
+    static int bytes(int N, int W) { return W * warp_bytes(N) + (2 * CT * padded(N) + CT * padded(N) / NB + 2 * CT + 4) * 4; }
 };
-// columns of tensor memory: 2 x 8 S for every block of states, a power of two, 32 at least
-template <int S> __host__ __device__ int fwd_columns(int N) {
-    int c = 32;
-    while (c < (N + PARTS * S - 1) / (PARTS * S) * 2 * RUN * S) c *= 2;
-    return c;
-}
+
 template <typename T, int S, int CT, int W>
-__global__ void __launch_bounds__(32 * W, 16 / W) scan_fwd_kernel(const Params p) {
-    using M = FwdSmem<S, CT>;
-    constexpr int NB = M::NB, THREADS = 32 * W, MAP = RUN * S;
-    extern __shared__ __align__(16) float room[];
+__global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kernel(const Params p) {
+    using M = FwdSmem<T, S, CT>;
+    constexpr int NB = M::NB, THREADS = 32 * W, HALF = M::STASH / 2;
+    extern __shared__ __align__(16) char room[];
     __shared__ uint32_t tmem_slot;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, run = lane / PARTS, part = lane % PARTS;
-    const int Npad = M::padded(p.N), Dg = p.D / p.G, columns = fwd_columns<S>(p.N);
+    const int Npad = M::padded(p.N), Dg = p.D / p.G;
     const int ct = blockIdx.x % p.ctiles, g = blockIdx.x / p.ctiles % p.G, b = blockIdx.x / p.ctiles / p.G;
     const int c0 = ct * CT, have = min(CT, Dg - c0), d = g * Dg + c0;             // channels of the CTA, the first one's index
     const int len = length_of(p, b), ntiles = (len + TILE - 1) / TILE;
-    float *const delta = room + warp * 2 * CT * TILE, *const x = delta + CT * TILE;
-    float* const ys = delta;                                     // a channel's steps are done with when its sums are there
-    float *const sA = room + W * 2 * CT * TILE, *const carry = sA + CT * Npad, *const bias = carry + CT * Npad, *const skip = bias + CT;
+    char* const mine = room + warp * M::warp_bytes(p.N);
+    T *const ru = (T*)mine, *const rdt = ru + TILE * CT, *const rz = rdt + TILE * CT, *const mB = rz + TILE * CT, *const mC = mB + TILE * Npad;
+    float *const delta = (float*)(mC + TILE * Npad), *const x = delta + CT * TILE;
+    float* const ys = Npad > NB ? x + CT * TILE : delta;         // with one block of states a channel's steps are done with when its sums are there
+    float *const sA = (float*)(room + W * M::warp_bytes(p.N)), *const carry = sA + CT * Npad, *const bias = carry + CT * Npad, *const skip = bias + CT;
     uint32_t* const flags = (uint32_t*)(skip + CT);
     int* const given_up = (int*)(flags + CT * Npad / NB);
     const Handover hand{given_up, p.status};
@@ -54,27 +58,42 @@ __global__ void __launch_bounds__(32 * W, 16 / W) scan_fwd_kernel(const Params p
     }
     for (int i = tid; i < CT * Npad / NB; i += THREADS) flags[i] = 0;
     if (tid == 0) *given_up = 0;
-    const uint32_t tmem_base = tmem_take(&tmem_slot, columns), tmem = tmem_base + ((uint32_t)(32 * (warp & 3)) << 16);
+    const uint32_t tmem_base = tmem_take(&tmem_slot, (W > 4 ? 2 : 1) * M::COLUMNS);
+    const uint32_t tmem = tmem_base + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * M::COLUMNS;
     const T *u = (const T*)p.u + b * p.s_u[0] + d, *dt = (const T*)p.dt + b * p.s_dt[0] + d, *z = p.z ? (const T*)p.z + b * p.s_z[0] + d : nullptr;
     const T *gB = (const T*)p.b + b * p.s_b[0] + g * p.s_b[2], *gC = (const T*)p.c + b * p.s_c[0] + g * p.s_c[2];
     T* const y = (T*)p.y + b * p.s_y[0] + d;
+    auto bring = [&](int tile) {
+        const int64_t t0 = (int64_t)tile * TILE;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int t = lane + 32 * r;
+            if (t0 + t < len) {
+                fetch<T, CT>(rdt + t * CT, dt + (t0 + t) * p.s_dt[1], have, p.piece);
+                fetch<T, CT>(ru + t * CT, u + (t0 + t) * p.s_u[1], have, p.piece);
+                if (z) fetch<T, CT>(rz + t * CT, z + (t0 + t) * p.s_z[1], have, p.piece);
+            }
+        }
+        fetch_map<T>(mB, gB, p.s_b[1], t0, len, p.N, Npad, p.piece_maps, lane);
+        fetch_map<T>(mC, gC, p.s_c[1], t0, len, p.N, Npad, p.piece_maps, lane);
+    };
+    if (warp < ntiles) bring(warp);
 
     for (int tile = warp; tile < ntiles; tile += W) {
         const int64_t t0 = (int64_t)tile * TILE;
-        for (int n0 = 0; n0 < Npad; n0 += NB) {
-            float m[MAP];
-            map_of<T, S>(m, gB, p.s_b[1], t0 + run * RUN, len, n0 + part * S, p.N, p.piece_maps);
-            keep<MAP>(tmem + n0 / NB * 2 * MAP, m);
-            map_of<T, S>(m, gC, p.s_c[1], t0 + run * RUN, len, n0 + part * S, p.N, p.piece_maps);
-            keep<MAP>(tmem + n0 / NB * 2 * MAP + MAP, m);
-        }
+        copies_done();
+        __syncwarp();
 #pragma unroll 1
-        for (int t = lane; t < TILE; t += 32) {
+        for (int r = 0; r < 2; ++r) {
+            const int t = lane + 32 * r;
             const bool in = t0 + t < len;                        // behind the end a token changes nothing
-            const int64_t at = in ? t0 + t : t0;
+            alignas(16) uint32_t stash[M::COLUMNS / 2];
+            words<HALF>(stash, ru + t * CT);
+            words<HALF>(stash + HALF, rz + t * CT);
+            keep<M::COLUMNS / 2>(tmem + r * (M::COLUMNS / 2), (const float*)stash);
             float uf[CT], df[CT];
-            read<T, CT>(df, dt + at * p.s_dt[1], have, p.piece);
-            read<T, CT>(uf, u + at * p.s_u[1], have, p.piece);
+            read<T, CT>(uf, ru + t * CT, CT, 16);
+            read<T, CT>(df, rdt + t * CT, CT, 16);
 #pragma unroll
             for (int c = 0; c < CT; c += 2) {
                 F2 dl = f2_add(f2_make(df[c], df[c + 1]), *(const F2*)(bias + c));
@@ -86,78 +105,86 @@ __global__ void __launch_bounds__(32 * W, 16 / W) scan_fwd_kernel(const Params p
                 x[(c + 1) * TILE + t] = in ? f2_hi(xi) : 0.f;
             }
         }
-        kept();
         __syncwarp();
 
+        for (int n0 = 0; n0 < Npad; n0 += NB) {
+            F2 B[RUN][S / 2], C[RUN][S / 2];
+#pragma unroll
+            for (int j = 0; j < RUN; ++j) {
+                const int at = (j * RUN + run) * Npad + n0 + part * S;
+                pairs<T, S>(B[j], mB + at);
+                pairs<T, S>(C[j], mC + at);
+            }
+            __syncwarp();
+            if (n0 + NB >= Npad && tile + W < ntiles) bring(tile + W);       // all of this tile is elsewhere by now
 #pragma unroll 1
-        for (int c = 0; c < have; ++c) {
-            float yv[RUN];
-#pragma unroll 1
-            for (int n0 = 0; n0 < Npad; n0 += NB) {
+            for (int c = 0; c < have; ++c) {
                 float* const h_at = carry + c * Npad + n0 + part * S;
                 uint32_t* const flag = flags + n0 / NB * CT + c;
-                const uint32_t col = tmem + n0 / NB * 2 * MAP;
-                float m[MAP], dl[RUN], xr[RUN];
-                recall<MAP>(col, m);
-                F2 A2[S / 2], a[RUN][S / 2], in[RUN][S / 2], P[S / 2], E[S / 2], h0[S / 2], h[S / 2];
+                F2 A2[S / 2], a[1][RUN][S / 2], in[1][RUN][S / 2], P[1][S / 2], E[1][S / 2], h0[1][S / 2], h[1][S / 2];
                 pairs<float, S>(A2, sA + c * Npad + n0 + part * S);
+                float dl[RUN], xr[RUN], yv[RUN];
 #pragma unroll
                 for (int k = 0; k < RUN; k += 4) {
                     *(float4*)(dl + k) = *(const float4*)(delta + c * TILE + run * RUN + k);
                     *(float4*)(xr + k) = *(const float4*)(x + c * TILE + run * RUN + k);
                 }
-                decays<S>(a, dl, A2);
-                landed<MAP>(m);
+                decays<S>(a[0], dl, A2);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j)
 #pragma unroll
-                    for (int s = 0; s < S / 2; ++s) in[j][s] = f2_mul(f2_make(xr[j], xr[j]), f2_make(m[j * S + 2 * s], m[j * S + 2 * s + 1]));
-                own_sum<S>(P, E, a, in);
-                recall<MAP>(col + MAP, m);
+                    for (int s = 0; s < S / 2; ++s) in[0][j][s] = f2_mul(f2_make(xr[j], xr[j]), B[j][s]);
+                own_sum<S>(P[0], E[0], a[0], in[0]);
                 hand.await(flag, (uint32_t)tile);
-                pairs<float, S>(h0, h_at);
-                entering<S>(h, E, P, h0, a, in, run, part);
+                pairs<float, S>(h0[0], h_at);
+                entering<S, 1>(h, E, P, h0, a, in, run, part);
                 __syncwarp();
                 if (run == RUN - 1) {
 #pragma unroll
-                    for (int s = 0; s < S / 2; ++s) *(F2*)(h_at + 2 * s) = E[s];
+                    for (int s = 0; s < S / 2; ++s) *(F2*)(h_at + 2 * s) = E[0][s];
                 }
                 hand.pass(flag, (uint32_t)tile + 1);
                 if (p.states && run == 0) {
                     float* to = p.states + (((int64_t)b * p.tiles + tile) * p.D + d + c) * p.N + n0 + part * S;
 #pragma unroll
-                    for (int s = 0; s < S; ++s) if (n0 + part * S + s < p.N) to[s] = s & 1 ? f2_hi(h0[s / 2]) : f2_lo(h0[s / 2]);
+                    for (int s = 0; s < S; ++s) if (n0 + part * S + s < p.N) to[s] = s & 1 ? f2_hi(h0[0][s / 2]) : f2_lo(h0[0][s / 2]);
                 }
-                landed<MAP>(m);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
                     F2 sum = 0ull;
 #pragma unroll
                     for (int s = 0; s < S / 2; ++s) {
-                        const F2 C = f2_make(m[j * S + 2 * s], m[j * S + 2 * s + 1]);
-                        h[s] = f2_fma(a[j][s], h[s], in[j][s]);
-                        sum = s ? f2_fma(C, h[s], sum) : f2_mul(C, h[s]);
+                        h[0][s] = f2_fma(a[0][j][s], h[0][s], in[0][j][s]);
+                        sum = s ? f2_fma(C[j][s], h[0][s], sum) : f2_mul(C[j][s], h[0][s]);
                     }
-                    const float v = f2_lo(sum) + f2_hi(sum);
-                    yv[j] = n0 ? yv[j] + v : v;
+                    yv[j] = f2_lo(sum) + f2_hi(sum);
                 }
+                float2 got = over_parts(yv, part);
+                float2* const ya = (float2*)(ys + c * TILE + run * RUN + part * 2);
+                if (n0) { const float2 was = *ya; got.x += was.x; got.y += was.y; }
+                *ya = got;
             }
-            *(float2*)(ys + c * TILE + run * RUN + part * 2) = over_parts(yv, part);
         }
+        kept();
         __syncwarp();
 #pragma unroll 1
-        for (int t = lane; t < TILE; t += 32) {
-            if (t0 + t >= len) break;
-            float uf[CT], out[CT];
-            read<T, CT>(uf, u + (t0 + t) * p.s_u[1], have, p.piece);
+        for (int r = 0; r < 2; ++r) {
+            const int t = lane + 32 * r;
+            alignas(16) uint32_t stash[M::COLUMNS / 2];
+            recall<M::COLUMNS / 2>(tmem + r * (M::COLUMNS / 2), (float*)stash);
+            landed<M::COLUMNS / 2>((float*)stash);
+            if (t0 + t < len) {
+                float uf[CT], out[CT];
+                read<T, CT>(uf, (const T*)stash, CT, 16);
 #pragma unroll
-            for (int c = 0; c < CT; ++c) out[c] = fmaf(skip[c], uf[c], ys[c * TILE + t]);
-            if (z) {
-                read<T, CT>(uf, z + (t0 + t) * p.s_z[1], have, p.piece);
+                for (int c = 0; c < CT; ++c) out[c] = fmaf(skip[c], uf[c], ys[c * TILE + t]);
+                if (z) {
+                    read<T, CT>(uf, (const T*)(stash + HALF), CT, 16);
 #pragma unroll
-                for (int c = 0; c < CT; ++c) out[c] *= uf[c] * sigmoid(uf[c]);
+                    for (int c = 0; c < CT; ++c) out[c] *= uf[c] * sigmoid(uf[c]);
+                }
+                put<T, CT>(y + (t0 + t) * p.s_y[1], out, have, p.piece);
             }
-            put<T, CT>(y + (t0 + t) * p.s_y[1], out, have, p.piece);
         }
         __syncwarp();
     }
@@ -166,7 +193,7 @@ __global__ void __launch_bounds__(32 * W, 16 / W) scan_fwd_kernel(const Params p
         const float out[CT] = {};
         put<T, CT>(y + at * p.s_y[1], out, have, p.piece);
     }
-    tmem_give(tmem_base, columns);                               // (a barrier too)
+    tmem_give(tmem_base, (W > 4 ? 2 : 1) * M::COLUMNS);          // (a barrier too)
     if (p.h_final) {
         for (int i = tid; i < CT * Npad; i += THREADS) {
             const int c = i / Npad, n = i - c * Npad;
@@ -328,7 +355,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
 #pragma unroll
                 for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), f2_make(dr[j], dr[j]), Q));
                 pairs<float, S>(h0, st + at);
-                entering<S>(h[0], E, P, h0, a, in, run, part);
+                entering<S, 1>(&h[0], &E, &P, &h0, &a, &in, run, part);
                 if (c) landed<16>(md);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
@@ -580,7 +607,7 @@ static void narrow(int& piece, const void* ptr, const int64_t* strides, int coun
 template <typename T, int S, int CT, int W> int fwd_launch(Params& p, cudaStream_t s) {
     p.ctiles = (p.D / p.G + CT - 1) / CT;
     const int64_t grid = (int64_t)p.B * p.G * p.ctiles;
-    const int smem = FwdSmem<S, CT>::bytes(p.N, W);
+    const int smem = FwdSmem<T, S, CT>::bytes(p.N, W);
     if (grid >= (1ll << 31)) return VIG_ERR_SHAPE;
     if (const cudaError_t e = ensure_smem_attr((const void*)scan_fwd_kernel<T, S, CT, W>, smem)) return (int)e;
     scan_fwd_kernel<T, S, CT, W><<<(unsigned)grid, 32 * W, smem, s>>>(p);
@@ -595,12 +622,16 @@ template <typename T> int bwd_launch(Params& p, cudaStream_t s) {
     return (int)cudaGetLastError();
 }
 
+template <typename T, int S> int fwd_width(Params& p, int ct, cudaStream_t s) {
+    if (getenv("FWD_CT")) ct = atoi(getenv("FWD_CT"));
+    if (ct == 48) return fwd_launch<T, S, 4, 8>(p, s);
+    if (ct == 46) return fwd_launch<T, S, 4, 6>(p, s);
+    return ct == 4 ? fwd_launch<T, S, 4, 4>(p, s) : ct == 8 ? fwd_launch<T, S, 8, 4>(p, s) : fwd_launch<T, S, 16, 4>(p, s);
+}
 template <typename T> int fwd_pick(Params& p, cudaStream_t s) {
-    // sixteen channels a CTA where that fills the device, else four
     const int64_t wide = (int64_t)p.B * p.G * ((p.D / p.G + 15) / 16);
-    const bool few = wide < 2 * device_sms();
-    if (p.N <= 8) return few ? fwd_launch<T, 2, 4, 4>(p, s) : fwd_launch<T, 2, 16, 4>(p, s);
-    return few ? fwd_launch<T, 4, 4, 4>(p, s) : fwd_launch<T, 4, 16, 4>(p, s);
+    const int ct = wide >= 2 * device_sms() ? 16 : wide >= device_sms() ? 8 : 4;
+    return p.N <= 8 ? fwd_width<T, 2>(p, ct, s) : fwd_width<T, 4>(p, ct, s);
 }
 
 static int check(const vig_selective_scan_args* a, bool grads) {
