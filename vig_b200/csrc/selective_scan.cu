@@ -7,7 +7,6 @@
 // states the exponentials bound it (MUFU, 16 a cycle and SM), not memory.  So each is taken once: the warps of a CTA take tiles of the same channels'
 // tokens in turn and hand the state from tile to tile, within a tile a warp's lanes divide tokens and states (scan_common.cuh); two passes over
 // independent chunks would take every exponential twice.
-#include <cstdlib>
 #include "scan_common.cuh"
 
 namespace vig {
@@ -117,6 +116,7 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
             }
             __syncwarp();
             if (n0 + NB >= Npad && tile + W < ntiles) bring(tile + W);       // all of this tile is elsewhere by now
+            if (!n0 && tile < W) hand.await(flags + have / W, (uint32_t)tile);    // warps begin some channels apart, or each hiccup of one is all the others'
 #pragma unroll 1
             for (int c = 0; c < have; ++c) {
                 float* const h_at = carry + c * Npad + n0 + part * S;
@@ -287,6 +287,10 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
             map_of<T, S>(mc, gC, p.s_c[1], t0 + run * RUN, len, n0 + part * S, p.N, p.piece_maps);
             keep<16>(tmem + n0 / NB * 64, mb);
             keep<16>(tmem + n0 / NB * 64 + 16, mc);
+#pragma unroll
+            for (int k = 0; k < RUN * S; ++k) mb[k] = 0.f;
+            keep<16>(tmem + n0 / NB * 64 + 32, mb);
+            keep<16>(tmem + n0 / NB * 64 + 48, mb);
         }
         kept();
 #pragma unroll 1
@@ -317,6 +321,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
         }
         copies_done();
         __syncwarp();
+// (warps side by side here, not some channels apart as in the forward: they share the instructions that are fetched, 1371 -> 1198 us)
 
 #pragma unroll 1
         for (int c = 0; c < have; ++c) {
@@ -347,7 +352,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 row(dr, dys);
                 landed<16>(mb);
                 landed<16>(mc);
-                if (c) recall<16>(col + 48, md);
+                recall<16>(col + 48, md);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) in[j][0] = f2_mul(f2_make(xr[j], xr[j]), f2_make(mb[2 * j], mb[2 * j + 1]));
                 own_sum<S>(P, E, a, in);
@@ -356,17 +361,17 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), f2_make(dr[j], dr[j]), Q));
                 pairs<float, S>(h0, st + at);
                 entering<S, 1>(&h[0], &E, &P, &h0, &a, &in, run, part);
-                if (c) landed<16>(md);
+                landed<16>(md);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
                     h[j + 1][0] = f2_fma(a[j][0], h[j][0], in[j][0]);
                     s_y[j] = f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), h[j + 1][0], s_y[j]);
-                    const F2 add = f2_fma(h[j + 1][0], f2_make(dr[j], dr[j]), c ? f2_make(md[2 * j], md[2 * j + 1]) : 0ull);
+                    const F2 add = f2_fma(h[j + 1][0], f2_make(dr[j], dr[j]), f2_make(md[2 * j], md[2 * j + 1]));
                     md[2 * j] = f2_lo(add);
                     md[2 * j + 1] = f2_hi(add);
                 }
                 keep<16>(col + 48, md);
-                if (c) recall<16>(col + 32, md);
+                recall<16>(col + 32, md);
                 // from the other end: q_t = a_t g_t is what token t - 1 gets
                 uint32_t* const flag = flags + n0 / NB * CT + c;
                 float* const q_at = carry + at;
@@ -391,13 +396,13 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 row(dl, delta);
                 row(xr, x);
                 row(dr, dys);
-                if (c) landed<16>(md);
+                landed<16>(md);
                 F2 dAs = 0ull;
 #pragma unroll
                 for (int j = RUN - 1; j >= 0; --j) {
                     const F2 gr = f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), f2_make(dr[j], dr[j]), Q);
                     s_b[j] = f2_fma(gr, f2_make(mb[2 * j], mb[2 * j + 1]), s_b[j]);
-                    const F2 add = f2_fma(gr, f2_make(xr[j], xr[j]), c ? f2_make(md[2 * j], md[2 * j + 1]) : 0ull);
+                    const F2 add = f2_fma(gr, f2_make(xr[j], xr[j]), f2_make(md[2 * j], md[2 * j + 1]));
                     md[2 * j] = f2_lo(add);
                     md[2 * j + 1] = f2_hi(add);
                     Q = f2_mul(a[j][0], gr);
@@ -622,16 +627,12 @@ template <typename T> int bwd_launch(Params& p, cudaStream_t s) {
     return (int)cudaGetLastError();
 }
 
-template <typename T, int S> int fwd_width(Params& p, int ct, cudaStream_t s) {
-    if (getenv("FWD_CT")) ct = atoi(getenv("FWD_CT"));
-    if (ct == 48) return fwd_launch<T, S, 4, 8>(p, s);
-    if (ct == 46) return fwd_launch<T, S, 4, 6>(p, s);
-    return ct == 4 ? fwd_launch<T, S, 4, 4>(p, s) : ct == 8 ? fwd_launch<T, S, 8, 4>(p, s) : fwd_launch<T, S, 16, 4>(p, s);
-}
-template <typename T> int fwd_pick(Params& p, cudaStream_t s) {
+// Sixteen channels a CTA where that gives every SM two CTAs, else eight, or four with more warps along the tokens (a warp by itself takes 5 cycles an
+// instruction: 1 x 16384 x 768 1004 / 531 / 303 us; 16 x 4096 x 768 711 / 705 / 817).
+template <typename T, int S> int fwd_width(Params& p, cudaStream_t s) {
     const int64_t wide = (int64_t)p.B * p.G * ((p.D / p.G + 15) / 16);
-    const int ct = wide >= 2 * device_sms() ? 16 : wide >= device_sms() ? 8 : 4;
-    return p.N <= 8 ? fwd_width<T, 2>(p, ct, s) : fwd_width<T, 4>(p, ct, s);
+    if (wide >= 2 * device_sms()) return fwd_launch<T, S, 16, 4>(p, s);
+    return wide >= device_sms() ? fwd_launch<T, S, 8, 4>(p, s) : fwd_launch<T, S, 4, 6>(p, s);
 }
 
 static int check(const vig_selective_scan_args* a, bool grads) {
@@ -686,9 +687,9 @@ extern "C" int vig_selective_scan_fwd(const vig_selective_scan_args* a, void* st
     if (!a->B || !a->D) return VIG_OK;
     Params p = params_of(a, false);
     switch (a->dtype) {
-        case VIG_DTYPE_F32: return fwd_pick<float>(p, (cudaStream_t)stream);
-        case VIG_DTYPE_BF16: return fwd_pick<__nv_bfloat16>(p, (cudaStream_t)stream);
-        default: return fwd_pick<__half>(p, (cudaStream_t)stream);
+        case VIG_DTYPE_F32: return p.N <= 8 ? fwd_width<float, 2>(p, (cudaStream_t)stream) : fwd_width<float, 4>(p, (cudaStream_t)stream);
+        case VIG_DTYPE_BF16: return p.N <= 8 ? fwd_width<__nv_bfloat16, 2>(p, (cudaStream_t)stream) : fwd_width<__nv_bfloat16, 4>(p, (cudaStream_t)stream);
+        default: return p.N <= 8 ? fwd_width<__half, 2>(p, (cudaStream_t)stream) : fwd_width<__half, 4>(p, (cudaStream_t)stream);
     }
 }
 
