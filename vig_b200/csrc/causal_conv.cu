@@ -16,7 +16,7 @@ struct ConvParams {
     float* partial;                                              // backward: [block][K + 1][D]
     const int32_t* lengths;
     int64_t s_x[2], s_y[2], s_st[2], s_out[2], s_dy[2];
-    int B, L, D, w_f32, silu, run, runs, blocks;
+    int B, L, D, w_f32, w_whole, silu, run, runs, blocks;
 };
 
 __device__ __forceinline__ int length_of(const ConvParams& p, int b) { return p.lengths ? min(max(p.lengths[b], 0), p.L) : p.L; }
@@ -47,6 +47,38 @@ template <typename T, int V> struct Piece {
 
 template <typename T> __device__ __forceinline__ float weight(const void* w, int64_t i, int f32) { return f32 ? ((const float*)w)[i] : DType<T>::to_f(((const T*)w)[i]); }
 
+// the taps and biases of V neighbouring channels: whole pieces of 16 bytes where the channels are, since they lie one behind the other
+template <typename T, typename W, int K, int V> __device__ __forceinline__ void taps_of(const W* w, const W* bias, int d, int whole, float (*f)[V], float* b) {
+    W e[V * K], c[V];
+    constexpr bool PIECES = V * (int)sizeof(W) % 16 == 0;
+    if (PIECES && whole) {
+        const uint4* from = (const uint4*)(w + (int64_t)d * K);
+#pragma unroll
+        for (int i = 0; i < V * K * (int)sizeof(W) / 16; ++i) { const uint4 v = __ldg(from + i); memcpy((char*)e + 16 * i, &v, 16); }
+        if (bias) {
+#pragma unroll
+            for (int i = 0; i < V * (int)sizeof(W) / 16; ++i) { const uint4 v = __ldg((const uint4*)(bias + d) + i); memcpy((char*)c + 16 * i, &v, 16); }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V * K; ++i) e[i] = w[(int64_t)d * K + i];
+        if (bias) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) c[v] = bias[d + v];
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        b[v] = bias ? DType<W>::to_f(c[v]) : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) f[k][v] = DType<W>::to_f(e[v * K + k]);
+    }
+}
+template <typename T, int K, int V> __device__ __forceinline__ void taps(const ConvParams& p, int d, float (*f)[V], float* b) {
+    if (p.w_f32) taps_of<T, float, K, V>((const float*)p.w, (const float*)p.bias, d, p.w_whole, f, b);
+    else taps_of<T, T, K, V>((const T*)p.w, (const T*)p.bias, d, p.w_whole, f, b);
+}
+
 // token t of channels d..d+V-1: out of the state in front of the first, zeros from the end on
 template <typename T, int K, int V> __device__ __forceinline__ Piece<T, V> token(const ConvParams& p, int b, int64_t t, int len, int d) {
     Piece<T, V> v;
@@ -70,12 +102,7 @@ template <typename T, int K, int V> __global__ void __launch_bounds__(256) conv_
     const int d = (int)(i % nv) * V, r = (int)(i / nv % p.runs), b = (int)(i / nv / p.runs), len = length_of(p, b);
     const int64_t t0 = (int64_t)r * p.run, t1 = min((int64_t)p.L, t0 + p.run);
     float w[K][V], bias[V], win[K][V];                           // win[k]: token t - K + 1 + k
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        bias[v] = p.bias ? weight<T>(p.bias, d + v, p.w_f32) : 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) w[k][v] = weight<T>(p.w, (int64_t)(d + v) * K + k, p.w_f32);
-    }
+    taps<T, K, V>(p, d, w, bias);
 #pragma unroll
     for (int k = 1; k < K; ++k) {
         const Piece<T, V> x = token<T, K, V>(p, b, t0 - K + k, len, d);
@@ -123,12 +150,12 @@ template <typename T, int K, int V> __global__ void __launch_bounds__(256) conv_
     const bool in = vec < nv;
     const int d = (in ? vec : 0) * V;
     float w[K][V], bias[V], dw[K][V], db[V];
+    taps<T, K, V>(p, d, w, bias);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        bias[v] = p.bias ? weight<T>(p.bias, d + v, p.w_f32) : 0.f;
         db[v] = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) { w[k][v] = weight<T>(p.w, (int64_t)(d + v) * K + k, p.w_f32); dw[k][v] = 0.f; }
+        for (int k = 0; k < K; ++k) dw[k][v] = 0.f;
     }
     const int64_t all = (int64_t)p.B * p.runs;
     for (int64_t i = (int64_t)blockIdx.y * 8 + row; i < all && in; i += (int64_t)gridDim.y * 8) {
@@ -342,7 +369,7 @@ extern "C" int vig_causal_conv_fwd(const void* x, const void* w, int w_dtype, co
     ConvParams p{};
     p.x = x; p.w = w; p.bias = bias; p.state = K > 1 ? state : nullptr; p.y = y; p.state_out = K > 1 ? state_out : nullptr; p.lengths = lengths;
     strides(p.s_x, strides_x, L, D); strides(p.s_y, strides_y, L, D); strides(p.s_st, strides_state, K - 1, D); strides(p.s_out, strides_state_out, K - 1, D);
-    p.B = B; p.L = L; p.D = D; p.w_f32 = w_dtype == VIG_DTYPE_F32; p.silu = silu;
+    p.B = B; p.L = L; p.D = D; p.w_f32 = w_dtype == VIG_DTYPE_F32; p.w_whole = ((uintptr_t)w | (uintptr_t)bias) % 16 == 0; p.silu = silu;
     return by_type<FWD>(p, K, dtype, (cudaStream_t)stream);
 }
 
@@ -361,7 +388,7 @@ extern "C" int vig_causal_conv_bwd(const void* x, const void* w, int w_dtype, co
     p.x = x; p.w = w; p.bias = bias; p.state = K > 1 ? state : nullptr; p.dy = d_y; p.d_out = K > 1 ? d_state_out : nullptr; p.lengths = lengths;
     p.dx = d_x; p.dw = d_w; p.dbias = d_bias; p.d_state = K > 1 ? d_state : nullptr; p.partial = (float*)workspace;
     strides(p.s_x, strides_x, L, D); strides(p.s_st, strides_state, K - 1, D); strides(p.s_dy, strides_dy, L, D);
-    p.B = B; p.L = L; p.D = D; p.w_f32 = w_dtype == VIG_DTYPE_F32; p.silu = silu;
+    p.B = B; p.L = L; p.D = D; p.w_f32 = w_dtype == VIG_DTYPE_F32; p.w_whole = ((uintptr_t)w | (uintptr_t)bias) % 16 == 0; p.silu = silu;
     p.blocks = bwd_blocks(B, L, D);
     return by_type<BWD>(p, K, dtype, (cudaStream_t)stream);
 }

@@ -311,6 +311,8 @@ struct MapKey {
     }
 };
 
+constexpr int MAP_BYTES = 16;            // beside the dtype codes: a map of 8-bit values
+
 inline bool encode_cached(CUtensorMap* m, const MapKey& key) {
     constexpr int SLOTS = 1024;
     struct Slot { bool used; MapKey key; CUtensorMap map; };
@@ -326,7 +328,9 @@ inline bool encode_cached(CUtensorMap* m, const MapKey& key) {
     cuuint32_t box[4], estr[4] = {1, 1, 1, 1};
     for (int i = 0; i < 4; ++i) { dims[i] = key.dims[i]; box[i] = key.box[i]; }
     for (int i = 0; i < 3; ++i) strides[i] = key.strides[i];
-    CUresult r = fn(m, key.dtype == VIG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)key.rank,
+    const CUtensorMapDataType type = key.dtype == MAP_BYTES ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : key.dtype == VIG_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : key.dtype == VIG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUresult r = fn(m, type, (cuuint32_t)key.rank,
                     const_cast<void*>(key.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                     key.swizzle == 2 ? CU_TENSOR_MAP_SWIZZLE_64B : key.swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
