@@ -3,7 +3,8 @@
 //
 // Bound by memory: x in, y out; backward x and dy in, dx out.  A thread walks a run of tokens of a few neighbouring channels and keeps the
 // window in registers, so that each value is read once and, at the border of two runs, K - 1 times more out of the cache.
-#include "common.cuh"
+#include <type_traits>
+#include "tc_common.cuh"
 
 namespace vig {
 namespace {
@@ -26,6 +27,7 @@ template <typename T, int V> struct Piece {
     __device__ void load(const T* q) {
         if constexpr (V * sizeof(T) == 16) { const uint4 w = *(const uint4*)q; memcpy(e, &w, 16); }
         else if constexpr (V * sizeof(T) == 8) { const uint2 w = *(const uint2*)q; memcpy(e, &w, 8); }
+        else if constexpr (V * sizeof(T) == 4) { const uint32_t w = *(const uint32_t*)q; memcpy(e, &w, 4); }
         else {
 #pragma unroll
             for (int i = 0; i < V; ++i) e[i] = q[i];
@@ -34,6 +36,7 @@ template <typename T, int V> struct Piece {
     __device__ void store(T* q) const {
         if constexpr (V * sizeof(T) == 16) { uint4 w; memcpy(&w, e, 16); *(uint4*)q = w; }
         else if constexpr (V * sizeof(T) == 8) { uint2 w; memcpy(&w, e, 8); *(uint2*)q = w; }
+        else if constexpr (V * sizeof(T) == 4) { uint32_t w; memcpy(&w, e, 4); *(uint32_t*)q = w; }
         else {
 #pragma unroll
             for (int i = 0; i < V; ++i) q[i] = e[i];
@@ -79,6 +82,8 @@ template <typename T, int K, int V> __device__ __forceinline__ void taps(const C
     else taps_of<T, T, K, V>((const T*)p.w, (const T*)p.bias, d, p.w_whole, f, b);
 }
 
+__device__ __forceinline__ float sigmoid_of(float x) { return tc::rcp(1.f + tc::ex2(-x * tc::LOG2E)); }
+
 // token t of channels d..d+V-1: out of the state in front of the first, zeros from the end on
 template <typename T, int K, int V> __device__ __forceinline__ Piece<T, V> token(const ConvParams& p, int b, int64_t t, int len, int d) {
     Piece<T, V> v;
@@ -93,47 +98,89 @@ template <typename T, int K, int V> __device__ __forceinline__ Piece<T, V> token
     return v;
 }
 
-constexpr int AHEAD = 8;                                         // tokens that a thread has under way
+// Tokens come in blocks of U: the window X holds the K - 1 before a block and the block itself, so that every index is known to the compiler and nothing is moved
+// but K - 1 values a block.  Blocks to come are on their way to shared memory, STAGES of them, every thread's values into slots of its own: registers
+// would hold one and leave room for half the threads (16384 x 768 38 us, training 16 x 4096 x 768 362).  Single values of 16 bits, which no asynchronous copy
+// takes, go through registers.
+constexpr int STAGES = 4;
 
-template <typename T, int K, int V> __global__ void __launch_bounds__(256) conv_fwd_kernel(const ConvParams p) {
+template <typename T, int V, int U, int ROWS, int THREADS> struct Ahead {
+    static constexpr int BYTES = V * (int)sizeof(T);
+    static constexpr bool ASYNC = BYTES >= 4;
+    static constexpr int ROOM = ASYNC ? STAGES * ROWS * U * THREADS * BYTES : 0;
+    char* slots;                                                 // the thread's
+    __device__ __forceinline__ char* slot(int stage, int row, int j) const { return slots + ((stage * ROWS + row) * U + j) * THREADS * BYTES; }
+    __device__ __forceinline__ void bring(int stage, int row, int j, const T* from, bool there) const {
+        if constexpr (ASYNC) {
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot(stage, row, j));
+            const int bytes = there ? BYTES : 0;                 // the rest of the slot becomes zeros
+            if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+            else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+            else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+        }
+    }
+    __device__ __forceinline__ void done() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory"); }
+    __device__ __forceinline__ void take(int stage, int row, int j, const T* from, bool there, float* f) const {
+        Piece<T, V> v;
+        if constexpr (ASYNC) v.load((const T*)slot(stage, row, j));
+        else if (there) v.load(from);
+        else v.zero();
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = DType<T>::to_f(v.e[e]);
+    }
+};
+
+template <typename T, int K, int V, int U> __global__ void __launch_bounds__(256) conv_fwd_kernel(const ConvParams p) {
+    extern __shared__ __align__(16) char ring[];
+    const Ahead<T, V, U, 1, 256> ahead{ring + threadIdx.x * V * (int)sizeof(T)};
     const int nv = p.D / V;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)p.B * p.runs * nv;
     if (i >= all) return;
     const int d = (int)(i % nv) * V, r = (int)(i / nv % p.runs), b = (int)(i / nv / p.runs), len = length_of(p, b);
-    const int64_t t0 = (int64_t)r * p.run, t1 = min((int64_t)p.L, t0 + p.run);
-    float w[K][V], bias[V], win[K][V];                           // win[k]: token t - K + 1 + k
+    const int t0 = r * p.run, t1 = min(p.L, t0 + p.run), stop = min(t1, len);
+    const T* const x = (const T*)p.x + b * p.s_x[0] + d;
+    T* const y = (T*)p.y + b * p.s_y[0] + d;
+    const int64_t sx = p.s_x[1], sy = p.s_y[1];
+    auto bring = [&](int t, int stage) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) ahead.bring(stage, 0, j, t + j < stop ? x + (t + j) * sx : x, t + j < stop);
+        ahead.done();
+    };
+#pragma unroll
+    for (int k = 0; k < STAGES; ++k) bring(t0 + k * U, k);
+    float w[K][V], bias[V], X[K - 1 + U][V];
     taps<T, K, V>(p, d, w, bias);
 #pragma unroll
-    for (int k = 1; k < K; ++k) {
-        const Piece<T, V> x = token<T, K, V>(p, b, t0 - K + k, len, d);
+    for (int k = 0; k < K - 1; ++k) {
+        const Piece<T, V> v = token<T, K, V>(p, b, (int64_t)t0 - (K - 1) + k, len, d);
 #pragma unroll
-        for (int v = 0; v < V; ++v) win[k][v] = DType<T>::to_f(x.e[v]);
+        for (int e = 0; e < V; ++e) X[k][e] = DType<T>::to_f(v.e[e]);
     }
-    T* const y = (T*)p.y + b * p.s_y[0] + d;
-    for (int64_t t = t0; t < t1; t += AHEAD) {
-        Piece<T, V> x[AHEAD];
+    int stage = 0;
+    for (int t = t0; t < t1; t += U, stage = stage + 1 < STAGES ? stage + 1 : 0) {
+        ahead.wait();
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            if (t + j < min(t1, (int64_t)len)) x[j].load((const T*)p.x + b * p.s_x[0] + (t + j) * p.s_x[1] + d);
-            else x[j].zero();
-        }
+        for (int j = 0; j < U; ++j) ahead.take(stage, 0, j, x + (t + j) * sx, t + j < stop, X[K - 1 + j]);
+        bring(t + STAGES * U, stage);
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
+        for (int j = 0; j < U; ++j) {
             if (t + j >= t1) break;
             Piece<T, V> out;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
+            for (int e = 0; e < V; ++e) {
+                float s = bias[e];
 #pragma unroll
-                for (int k = 0; k + 1 < K; ++k) win[k][v] = win[k + 1][v];
-                win[K - 1][v] = DType<T>::to_f(x[j].e[v]);
-                float s = bias[v];
-#pragma unroll
-                for (int k = 0; k < K; ++k) s = fmaf(w[k][v], win[k][v], s);
-                if (p.silu) s *= sigmoidf_(s);
-                out.e[v] = DType<T>::from_f(t + j < len ? s : 0.f);
+                for (int k = 0; k < K; ++k) s = fmaf(w[k][e], X[j + k][e], s);
+                if (p.silu) s *= sigmoid_of(s);
+                out.e[e] = DType<T>::from_f(t + j < len ? s : 0.f);
             }
-            out.store(y + (t + j) * p.s_y[1]);
+            out.store(y + (t + j) * sy);
         }
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) X[k][e] = X[U + k][e];
     }
     if (p.state_out && r == p.runs - 1) {
 #pragma unroll
@@ -141,10 +188,14 @@ template <typename T, int K, int V> __global__ void __launch_bounds__(256) conv_
     }
 }
 
-// A block takes 32 V channels and walks runs of tokens, eight at a time; its threads' shares of dw and dbias stay in registers, are added in shared memory
-// and left for conv_sum_kernel.  Where a gradient of the state is wanted, a sequence's first run begins K - 1 tokens ahead of it.
-template <typename T, int K, int V> __global__ void __launch_bounds__(256) conv_bwd_kernel(const ConvParams p) {
-    __shared__ float sh[8][32 * V];
+// A block of threads takes 32 V channels and walks runs of tokens, ROWS at a time; its threads' shares of dw and dbias stay in registers, are added in shared memory
+// and left for conv_sum_kernel.  Where a gradient of the state is wanted, a sequence's first run begins K - 1 tokens ahead of it.  A run's last tokens
+// want dpre of the K - 1 behind it; blocks of U tokens all inside run and sequence go without the questions that this and the ends ask.
+constexpr int ROWS = 8;
+
+template <typename T, int K, int V, int U> __global__ void __launch_bounds__(32 * ROWS, 2) conv_bwd_kernel(const ConvParams p) {
+    extern __shared__ __align__(16) char ring[];                 // at the end [ROWS][32 V] shares
+    const Ahead<T, V, U, 2, 32 * ROWS> ahead{ring + (threadIdx.y * 32 + threadIdx.x) * V * (int)sizeof(T)};
     const int lane = threadIdx.x, row = threadIdx.y, nv = p.D / V;
     const int vec = blockIdx.x * 32 + lane;
     const bool in = vec < nv;
@@ -152,81 +203,119 @@ template <typename T, int K, int V> __global__ void __launch_bounds__(256) conv_
     float w[K][V], bias[V], dw[K][V], db[V];
     taps<T, K, V>(p, d, w, bias);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        db[v] = 0.f;
+    for (int e = 0; e < V; ++e) {
+        db[e] = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) dw[k][v] = 0.f;
+        for (int k = 0; k < K; ++k) dw[k][e] = 0.f;
     }
     const int64_t all = (int64_t)p.B * p.runs;
-    for (int64_t i = (int64_t)blockIdx.y * 8 + row; i < all && in; i += (int64_t)gridDim.y * 8) {
+    for (int64_t i = (int64_t)blockIdx.y * ROWS + row; i < all && in; i += (int64_t)gridDim.y * ROWS) {
         const int r = (int)(i % p.runs), b = (int)(i / p.runs), len = length_of(p, b);
-        const int64_t first = (int64_t)r * p.run, t1 = min((int64_t)p.L, first + p.run), t0 = r == 0 && p.d_state ? -(K - 1) : first;
-        float win[K][V], dp[K][V];                               // dp[k]: dpre of token t - K + 1 + k
+        const int first = r * p.run, t1 = min(p.L, first + p.run), t0 = r == 0 && p.d_state ? -(K - 1) : first, end = t1 + K - 1;
+        const int calm = min(t1, len) - (p.d_out ? K - 1 : 0);   // up to where a block asks nothing
+        const T *const x = (const T*)p.x + b * p.s_x[0] + d, *const dy = (const T*)p.dy + b * p.s_dy[0] + d;
+        const T* const st = p.state ? (const T*)p.state + b * p.s_st[0] + d : nullptr;
+        T* const dx = (T*)p.dx + (int64_t)b * p.L * p.D + d;
+        const int64_t sx = p.s_x[1], sd = p.s_dy[1], ss = p.s_st[1];
+        float X[K - 1 + U][V], P[K - 1 + U][V];                  // tokens; their dpre
+        // where token t is, and whether it is there at all
+        auto place = [&](int t, bool& there) {
+            there = t < 0 ? st && t >= -(K - 1) : t < len;
+            return !there ? x : t < 0 ? st + (t + K - 1) * ss : x + t * sx;
+        };
+        auto bring = [&](int t, int stage) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const Piece<T, V> x = token<T, K, V>(p, b, t0 - K + k, len, d);
-#pragma unroll
-            for (int v = 0; v < V; ++v) { win[k][v] = DType<T>::to_f(x.e[v]); dp[k][v] = 0.f; }
-        }
-        for (int64_t t = t0; t < t1 + K - 1; t += 4) {
-            Piece<T, V> xs[4], ds[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                xs[j] = token<T, K, V>(p, b, t + j, len, d);
-                if (t + j >= 0 && t + j < len) ds[j].load((const T*)p.dy + b * p.s_dy[0] + (t + j) * p.s_dy[1] + d);
-                else ds[j].zero();
+            for (int j = 0; j < U; ++j) {
+                bool there;
+                const T* from = place(t + j, there);
+                there = there && t + j < end;
+                ahead.bring(stage, 0, j, there ? from : x, there);
+                const bool inside = t + j >= 0 && t + j < len && t + j < end;
+                ahead.bring(stage, 1, j, inside ? dy + (t + j) * sd : dy, inside);
             }
+            ahead.done();
+        };
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t tj = t + j, to = tj - (K - 1);     // the window of token `to` is complete with tj
-                if (tj >= t1 + K - 1) break;
-                const bool own = tj >= first && tj < t1;         // whose share of dw is this run's
+        for (int k = 0; k < STAGES; ++k) bring(t0 + k * U, k);
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) {
+            const Piece<T, V> v = token<T, K, V>(p, b, (int64_t)t0 - (K - 1) + k, len, d);
+#pragma unroll
+            for (int e = 0; e < V; ++e) { X[k][e] = DType<T>::to_f(v.e[e]); P[k][e] = 0.f; }
+        }
+        auto block = [&](int t, auto quiet) {
+            constexpr bool Q = decltype(quiet)::value;
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const int tj = t + j;
+                    float s = bias[e];
+#pragma unroll
+                    for (int k = 0; k < K; ++k) s = fmaf(w[k][e], X[j + k][e], s);
+                    const float sg = sigmoid_of(s), own = P[K - 1 + j][e], act = own * sg * fmaf(s, 1.f - sg, 1.f);
+                    float g = p.silu ? act : own;
+                    if (!Q && (tj < 0 || tj >= len)) g = 0.f;
+                    P[K - 1 + j][e] = g;
+                    if (Q || (tj >= first && tj < t1)) {         // whose share of dw is this run's
+                        db[e] += g;
+#pragma unroll
+                        for (int k = 0; k < K; ++k) dw[k][e] = fmaf(g, X[j + k][e], dw[k][e]);
+                    }
+                }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int to = t + j - (K - 1);                  // the window of token `to` is complete with t + j
+                if (to < t0 || (!Q && to >= t1)) continue;
                 Piece<T, V> out;
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-#pragma unroll
-                    for (int k = 0; k + 1 < K; ++k) { win[k][v] = win[k + 1][v]; dp[k][v] = dp[k + 1][v]; }
-                    win[K - 1][v] = DType<T>::to_f(xs[j].e[v]);
-                    float g = DType<T>::to_f(ds[j].e[v]);
-                    if (p.silu) {
-                        float s = bias[v];
-#pragma unroll
-                        for (int k = 0; k < K; ++k) s = fmaf(w[k][v], win[k][v], s);
-                        const float sg = sigmoidf_(s);
-                        g = tj >= 0 && tj < len ? g * sg * fmaf(s, 1.f - sg, 1.f) : 0.f;
-                    }
-                    dp[K - 1][v] = g;
-                    if (own) {
-                        db[v] += g;
-#pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][v] = fmaf(g, win[k][v], dw[k][v]);
-                    }
+                for (int e = 0; e < V; ++e) {
                     float o = 0.f;
 #pragma unroll
-                    for (int k = 0; k < K; ++k) o = fmaf(w[K - 1 - k][v], dp[k][v], o);
-                    // what the state handed on gives back: its row k is token len - (K - 1) + k
-                    if (p.d_out && to >= len - (K - 1) && to < len) o += DType<T>::to_f(((const T*)p.d_out)[((int64_t)b * (K - 1) + (to - len + K - 1)) * p.D + d + v]);
-                    out.e[v] = DType<T>::from_f(to < len ? o : 0.f);
+                    for (int k = 0; k < K; ++k) o = fmaf(w[K - 1 - k][e], P[j + k][e], o);
+                    if (!Q) {
+                        // what the state handed on gives back: its row k is token len - (K - 1) + k
+                        if (p.d_out && to >= len - (K - 1) && to < len) o += DType<T>::to_f(((const T*)p.d_out)[((int64_t)b * (K - 1) + (to - len + K - 1)) * p.D + d + e]);
+                        if (to >= len) o = 0.f;
+                    }
+                    out.e[e] = DType<T>::from_f(o);
                 }
-                if (to >= t0) {
-                    if (to >= 0) out.store((T*)p.dx + ((int64_t)b * p.L + to) * p.D + d);
-                    else out.store((T*)p.d_state + ((int64_t)b * (K - 1) + to + K - 1) * p.D + d);
-                }
+                if (Q || to >= 0) out.store(dx + (int64_t)to * p.D);
+                else out.store((T*)p.d_state + ((int64_t)b * (K - 1) + to + K - 1) * p.D + d);
             }
+        };
+        int stage = 0;
+        for (int t = t0; t < end; t += U, stage = stage + 1 < STAGES ? stage + 1 : 0) {
+            ahead.wait();
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                bool there = true;
+                const T* from = Ahead<T, V, U, 2, 32 * ROWS>::ASYNC ? x : place(t + j, there);
+                ahead.take(stage, 0, j, from, there, X[K - 1 + j]);
+                ahead.take(stage, 1, j, dy + (t + j) * sd, t + j >= 0 && t + j < len, P[K - 1 + j]);
+            }
+            bring(t + STAGES * U, stage);
+            if (t >= K - 1 && t + U <= calm) block(t, std::true_type{});
+            else block(t, std::false_type{});
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) { X[k][e] = X[U + k][e]; P[k][e] = P[U + k][e]; }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    // shares of the block's eight rows of threads
+    // shares of the block's rows of threads
+    float (*const sh)[32 * V] = (float (*)[32 * V])ring;
 #pragma unroll
     for (int k = 0; k <= K; ++k) {
         __syncthreads();
 #pragma unroll
-        for (int v = 0; v < V; ++v) sh[row][lane * V + v] = k < K ? dw[k < K ? k : 0][v] : db[v];
+        for (int e = 0; e < V; ++e) sh[row][lane * V + e] = k < K ? dw[k < K ? k : 0][e] : db[e];
         __syncthreads();
-        const int c = row * 32 + lane;
-        if (c < 32 * V && blockIdx.x * 32 * V + c < p.D) {
+        for (int c = row * 32 + lane; c < 32 * V && blockIdx.x * 32 * V + c < p.D; c += 32 * ROWS) {
             float s = 0.f;
 #pragma unroll
-            for (int r = 0; r < 8; ++r) s += sh[r][c];
+            for (int r = 0; r < ROWS; ++r) s += sh[r][c];
             p.partial[((int64_t)blockIdx.y * (K + 1) + k) * p.D + blockIdx.x * 32 * V + c] = s;
         }
     }
@@ -264,7 +353,7 @@ template <typename T, int K> __global__ void __launch_bounds__(128) conv_step_ke
     float s = p.bias ? weight<T>(p.bias, d, p.w_f32) : 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) s = fmaf(weight<T>(p.w, (int64_t)d * K + k, p.w_f32), DType<T>::to_f(row[k]), s);
-    if (p.silu) s *= sigmoidf_(s);
+    if (p.silu) s *= sigmoid_of(s);
     ((T*)p.y)[b * p.s_y[0] + d] = DType<T>::from_f(s);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) st[k * p.s_out[1]] = row[k + 1];
@@ -278,41 +367,46 @@ bool aligned(const void* q, const int64_t* s, int count, int bytes, int size) {
 }
 
 template <typename T, int K> int fwd_launch(ConvParams& p, cudaStream_t s) {
-    constexpr int V = 16 / sizeof(T);
-    const int size = (int)sizeof(T);
-    const bool whole = p.D % V == 0 && aligned(p.x, p.s_x, 2, 16, size) && aligned(p.y, p.s_y, 2, 16, size) && aligned(p.state, p.s_st, 2, 16, size) &&
-                       aligned(p.state_out, p.s_out, 2, 16, size);
+    constexpr int V = 4, U = 4;
+    const int size = (int)sizeof(T), bytes = V * size;
+    const bool whole = p.D % V == 0 && aligned(p.x, p.s_x, 2, bytes, size) && aligned(p.y, p.s_y, 2, bytes, size) && aligned(p.state, p.s_st, 2, bytes, size) &&
+                       aligned(p.state_out, p.s_out, 2, bytes, size);
     const int64_t nv = whole ? p.D / V : p.D;
-    // runs of 32 tokens, or shorter ones down to 8 where that would be less than 512 threads an SM
-    p.run = 32;
-    while (p.run > AHEAD && (int64_t)p.B * ((p.L + p.run - 1) / p.run) * nv < (int64_t)device_sms() * 512) p.run /= 2;
+    // runs of 64 tokens, or shorter ones down to a block where that would be less than 1024 threads an SM
+    p.run = 64;
+    while (p.run > U && (int64_t)p.B * ((p.L + p.run - 1) / p.run) * nv < (int64_t)device_sms() * 1024) p.run /= 2;
     p.runs = p.L ? (p.L + p.run - 1) / p.run : 1;
     const int64_t grid = ((int64_t)p.B * p.runs * nv + 255) / 256;
     if (grid >= (1ll << 31)) return VIG_ERR_SHAPE;
-    if (whole) conv_fwd_kernel<T, K, V><<<(unsigned)grid, 256, 0, s>>>(p);
-    else conv_fwd_kernel<T, K, 1><<<(unsigned)grid, 256, 0, s>>>(p);
+    const auto kernel = whole ? conv_fwd_kernel<T, K, V, U> : conv_fwd_kernel<T, K, 1, U>;
+    const int smem = whole ? Ahead<T, V, U, 1, 256>::ROOM : Ahead<T, 1, U, 1, 256>::ROOM;
+    if (const cudaError_t e = tc::ensure_smem_attr((const void*)kernel, smem)) return (int)e;
+    kernel<<<(unsigned)grid, 256, smem, s>>>(p);
     return (int)cudaGetLastError();
 }
 
 // blocks of the backward along the tokens, whose shares the workspace holds
 int bwd_blocks(int64_t B, int64_t L, int D) {
-    const int64_t most = ((int64_t)device_sms() * 6 + (D + 127) / 128 - 1) / ((D + 127) / 128), runs = B * (L / 8 + 1);
+    const int64_t cols = (D + 127) / 128, most = ((int64_t)device_sms() * 4 + cols - 1) / cols, runs = B * (L / 8 + 1);
     return (int)(runs < most ? runs : most);
 }
 
 template <typename T, int K> int bwd_launch(ConvParams& p, cudaStream_t s) {
-    constexpr int V = 4;
+    constexpr int V = K <= 4 ? 4 : 2, U = 4;
     const int size = (int)sizeof(T), bytes = V * size;
     const int64_t rows[1] = {p.D};
     const bool whole = p.D % V == 0 && aligned(p.x, p.s_x, 2, bytes, size) && aligned(p.dy, p.s_dy, 2, bytes, size) && aligned(p.state, p.s_st, 2, bytes, size) &&
                        aligned(p.dx, rows, 1, bytes, size) && aligned(p.d_state, rows, 1, bytes, size);
     const int width = whole ? 32 * V : 32, cols = (p.D + width - 1) / width;
     p.run = 64;
-    while (p.run > 8 && (int64_t)p.B * ((p.L + p.run - 1) / p.run) < 8ll * p.blocks) p.run /= 2;
+    while (p.run > 8 && (int64_t)p.B * ((p.L + p.run - 1) / p.run) < (int64_t)ROWS * p.blocks) p.run /= 2;
     p.runs = p.L ? (p.L + p.run - 1) / p.run : 1;
-    const dim3 grid(cols, p.blocks), block(32, 8);
-    if (whole) conv_bwd_kernel<T, K, V><<<grid, block, 0, s>>>(p);
-    else conv_bwd_kernel<T, K, 1><<<grid, block, 0, s>>>(p);
+    const dim3 grid(cols, p.blocks), block(32, ROWS);
+    const auto kernel = whole ? conv_bwd_kernel<T, K, V, U> : conv_bwd_kernel<T, K, 1, U>;
+    constexpr int shares = ROWS * 32 * 4;                        // a channel's
+    const int smem = whole ? max(Ahead<T, V, U, 2, 32 * ROWS>::ROOM, V * shares) : max(Ahead<T, 1, U, 2, 32 * ROWS>::ROOM, shares);
+    if (const cudaError_t e = tc::ensure_smem_attr((const void*)kernel, smem)) return (int)e;
+    kernel<<<grid, block, smem, s>>>(p);
     if (const cudaError_t e = cudaGetLastError()) return (int)e;
     return (int)launch_next(conv_sum_kernel<T, K>, dim3((p.D + 31) / 32, K + 1), block, 0, s, p);
 }
