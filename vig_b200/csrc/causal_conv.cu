@@ -366,15 +366,20 @@ bool aligned(const void* q, const int64_t* s, int count, int bytes, int size) {
     return true;
 }
 
+// tokens of a run where a sequence has about `runs` of them: whole blocks, two at least
+template <int U> int run_of(int L, int64_t runs) {
+    const int64_t run = runs > 0 ? (L + runs - 1) / runs : L;
+    return (int)(run <= 2 * U ? 2 * U : (run + U - 1) / U * U);
+}
+
 template <typename T, int K> int fwd_launch(ConvParams& p, cudaStream_t s) {
     constexpr int V = 4, U = 4;
     const int size = (int)sizeof(T), bytes = V * size;
     const bool whole = p.D % V == 0 && aligned(p.x, p.s_x, 2, bytes, size) && aligned(p.y, p.s_y, 2, bytes, size) && aligned(p.state, p.s_st, 2, bytes, size) &&
                        aligned(p.state_out, p.s_out, 2, bytes, size);
     const int64_t nv = whole ? p.D / V : p.D;
-    // runs of 64 tokens, or shorter ones down to a block where that would be less than 1024 threads an SM
-    p.run = 64;
-    while (p.run > U && (int64_t)p.B * ((p.L + p.run - 1) / p.run) * nv < (int64_t)device_sms() * 1024) p.run /= 2;
+    // runs as long as they may be where every thread that finds room has one: each begins with taps, a window and a wait
+    p.run = run_of<U>(p.L, (int64_t)device_sms() * 768 / (p.B * nv));
     p.runs = p.L ? (p.L + p.run - 1) / p.run : 1;
     const int64_t grid = ((int64_t)p.B * p.runs * nv + 255) / 256;
     if (grid >= (1ll << 31)) return VIG_ERR_SHAPE;
@@ -398,8 +403,7 @@ template <typename T, int K> int bwd_launch(ConvParams& p, cudaStream_t s) {
     const bool whole = p.D % V == 0 && aligned(p.x, p.s_x, 2, bytes, size) && aligned(p.dy, p.s_dy, 2, bytes, size) && aligned(p.state, p.s_st, 2, bytes, size) &&
                        aligned(p.dx, rows, 1, bytes, size) && aligned(p.d_state, rows, 1, bytes, size);
     const int width = whole ? 32 * V : 32, cols = (p.D + width - 1) / width;
-    p.run = 64;
-    while (p.run > 8 && (int64_t)p.B * ((p.L + p.run - 1) / p.run) < (int64_t)ROWS * p.blocks) p.run /= 2;
+    p.run = run_of<U>(p.L, (int64_t)ROWS * p.blocks / p.B);
     p.runs = p.L ? (p.L + p.run - 1) / p.run : 1;
     const dim3 grid(cols, p.blocks), block(32, ROWS);
     const auto kernel = whole ? conv_bwd_kernel<T, K, V, U> : conv_bwd_kernel<T, K, 1, U>;

@@ -97,6 +97,22 @@ template <typename T> __global__ void __launch_bounds__(DW * 32) layer_dw_kernel
     }
 }
 
+// a summed over the TPR threads of a row
+template <int TPR> __device__ __forceinline__ void over_row(float& a, float (*sh)[2], int& buf) {
+#pragma unroll
+    for (int m = (TPR < 32 ? TPR : 32) / 2; m; m >>= 1) a += __shfl_xor_sync(0xffffffffu, a, m);
+    if (TPR > 32) {
+        constexpr int W = TPR / 32;
+        float (*s)[2] = sh + buf * W;
+        buf ^= 1;
+        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5][0] = a;
+        __syncthreads();
+        a = s[0][0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) a += s[i][0];
+    }
+}
+
 // TPR threads share a row, VPT vectors of 16 bytes each, as in the RMS norm's kernels.
 template <typename T, int TPR, int VPT> __global__ void __launch_bounds__(norm_threads<TPR>) layer_rows_kernel(const LayerParams p) {
     constexpr int V = DType<T>::VEC, THREADS = norm_threads<TPR>, RPB = THREADS / TPR;
@@ -135,7 +151,7 @@ template <typename T, int TPR, int VPT> __global__ void __launch_bounds__(norm_t
     // a CTA's threads leave together: all of them take part in every reduction
     for (int64_t first = (int64_t)blockIdx.x * RPB; first < p.rows; first += hop, row += hop) {
         const bool in = row < p.rows;
-        float v[VPT][V], s = 0.f, ss = 0.f, none = 0.f;
+        float v[VPT][V], s = 0.f, ss = 0.f;
 #pragma unroll
         for (int m = 0; m < VPT; ++m) {
             const int vi = t + m * TPR;
@@ -153,7 +169,7 @@ template <typename T, int TPR, int VPT> __global__ void __launch_bounds__(norm_t
             }
         }
         fetch(row + hop);
-        over_row<TPR, false>(s, none, sh, buf);
+        over_row<TPR>(s, sh, buf);
         const float mean = s / (float)p.N;
 #pragma unroll
         for (int m = 0; m < VPT; ++m) {
@@ -166,7 +182,7 @@ template <typename T, int TPR, int VPT> __global__ void __launch_bounds__(norm_t
                 }
             }
         }
-        over_row<TPR, false>(ss, none, sh, buf);
+        over_row<TPR>(ss, sh, buf);
         const float rstd = 1.f / sqrtf(ss / (float)p.N + p.eps);
 #pragma unroll
         for (int m = 0; m < VPT; ++m) {
@@ -348,7 +364,8 @@ template <typename T> int layer_launch(LayerParams p, cudaStream_t s) {
     constexpr int V = DType<T>::VEC;
     const int size = (int)sizeof(T), nv = (p.N + V - 1) / V;
     p.whole = p.N % V == 0 && on_16(p.x, p.ldx, size) && (!p.res || on_16(p.res, p.ldr, size)) && on_16(p.w, 0, 1) && on_16(p.bias, 0, 1) && on_16(p.y, 0, 1) && on_16(p.r, 0, 1);
-    switch (threads_a_row(nv, 8)) {
+    switch (threads_a_row(nv, 4)) {
+        case 4: return layer_rows_launch<T, 4>(p, nv, s);
         case 8: return layer_rows_launch<T, 8>(p, nv, s);
         case 16: return layer_rows_launch<T, 16>(p, nv, s);
         case 32: return layer_rows_launch<T, 32>(p, nv, s);
@@ -390,7 +407,8 @@ template <typename T> int layer_bwd_launch(LayerBwdParams p, cudaStream_t s) {
               on_16(p.dx, 0, 1) && on_16(p.partial, 0, 1);
     const int nv = (p.N + V - 1) / V;
     int e;
-    switch (threads_a_row(nv, 8)) {
+    switch (threads_a_row(nv, 4)) {
+        case 4: e = layer_bwd_rows_launch<T, 4>(p, nv, s); break;
         case 8: e = layer_bwd_rows_launch<T, 8>(p, nv, s); break;
         case 16: e = layer_bwd_rows_launch<T, 16>(p, nv, s); break;
         case 32: e = layer_bwd_rows_launch<T, 32>(p, nv, s); break;
