@@ -8,5 +8,6 @@ from .modules import RMSNorm, GatedLinearAttention, GLAMLP, GLABlock  # noqa: F4
 from .vig import ViG, build_vig  # noqa: F401
 from .hier import HierViG, GLA2D, VSSBlock  # noqa: F401
 from .recurrent import GatedRecurrence  # noqa: F401
+from .state_space import SelectiveStateSpace  # noqa: F401
 from .optim import AdamW  # noqa: F401
 from . import native  # noqa: F401  (imported here so that it knows the operators as they are before anyone wraps them)

@@ -631,8 +631,10 @@ template <typename T> int bwd_launch(Params& p, cudaStream_t s) {
 // instruction: 1 x 16384 x 768 1004 / 531 / 303 us; 16 x 4096 x 768 711 / 705 / 817).
 template <typename T, int S> int fwd_width(Params& p, cudaStream_t s) {
     const int64_t wide = (int64_t)p.B * p.G * ((p.D / p.G + 15) / 16);
-    if (wide >= 2 * device_sms()) return fwd_launch<T, S, 16, 4>(p, s);
-    return wide >= device_sms() ? fwd_launch<T, S, 8, 4>(p, s) : fwd_launch<T, S, 4, 6>(p, s);
+    const auto fits = [&](int bytes) { return bytes <= 227 * 1024; };      // (maps of many states in fp32)
+    if (wide >= 2 * device_sms() && fits(FwdSmem<T, S, 16>::bytes(p.N, 4))) return fwd_launch<T, S, 16, 4>(p, s);
+    if (wide >= device_sms() || !fits(FwdSmem<T, S, 4>::bytes(p.N, 6))) return fwd_launch<T, S, 8, 4>(p, s);
+    return fwd_launch<T, S, 4, 6>(p, s);
 }
 
 static int check(const vig_selective_scan_args* a, bool grads) {
@@ -643,7 +645,7 @@ static int check(const vig_selective_scan_args* a, bool grads) {
     if ((int64_t)a->B * a->D >= (1ll << 31) || a->D >= (1 << 28) || a->L >= (1 << 30)) return VIG_ERR_SHAPE;
     if (!a->B || !a->D) return VIG_OK;
     if (!a->A || (a->L && (!a->u || !a->dt || !a->b || !a->c || (!grads && !a->y)))) return VIG_ERR_NULL;
-    if (grads && (!a->d_b || !a->d_c || !a->d_A || (a->L && (!a->states || !a->d_y || !a->d_u || !a->d_dt || (a->z && !a->d_z))))) return VIG_ERR_NULL;
+    if (grads && (!a->d_A || (a->L && (!a->d_b || !a->d_c || !a->states || !a->d_y || !a->d_u || !a->d_dt || (a->z && !a->d_z))))) return VIG_ERR_NULL;
     return VIG_OK;
 }
 

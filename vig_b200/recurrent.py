@@ -17,7 +17,7 @@ class GatedRecurrence(nn.Module):
         self.norm = RMSNorm(d_model, eps=eps)
         self.in_proj = nn.Linear(d_model, 3 * self.d_inner, bias=False)
         self.out_proj = nn.Linear(self.d_inner, d_model, bias=False)
-        self._in_8bit = None
+        self._in_8bit, self._type_8bit = None, torch.float8_e4m3fn
 
     def forward(self, hidden, residual=None, state=None, output_final_state=False):
         """``hidden`` ``[B, L, d_model]`` and the residual stream (None: it begins with ``hidden``); ``state``: fp32 ``[B, d_inner]`` of the tokens
@@ -34,13 +34,15 @@ class GatedRecurrence(nn.Module):
         return hidden.float() if residual is not None and residual.dtype == torch.float32 and hidden.dtype in (torch.bfloat16, torch.float16) else hidden
 
     @torch.no_grad()
-    def quantize(self):
-        """From now on ``step`` takes its input projection in 8 bits: e4m3 codes with a scale per output channel, laid out here and again at the first step
-        behind a change of the weights (an optimizer's step, ``load_state_dict``, ``to``).  Weights made in inference mode have no version: they want
-        another call when they change."""
+    def quantize(self, dtype=torch.float8_e4m3fn):
+        """From now on ``step`` takes its input projection in 8 bits: e4m3 codes, or with ``torch.int8`` integers (whose products are summed exactly by
+        ``ops.linear_int8``), with a scale per output channel, laid out here and again at the first step behind a change of the weights (an optimizer's step,
+        ``load_state_dict``, ``to``).  Weights made in inference mode have no version: they want another call when they change."""
+        if dtype not in ops.OUT_8BIT:
+            raise TypeError(f"unsupported 8-bit dtype {dtype}; expected float8_e4m3fn or int8")
         if self.d_model % 16 or 3 * self.d_inner % 16:
             raise ValueError(f"8-bit products want widths of whole 16s; got {self.d_model} and {self.d_inner}")
-        self._in_8bit = None
+        self._in_8bit, self._type_8bit = None, dtype
         self._codes()
         return self
 
@@ -57,8 +59,10 @@ class GatedRecurrence(nn.Module):
         key = (w.dtype, w.device, w.data_ptr(), None if w.is_inference() else w._version)
         if self._in_8bit is None or self._in_8bit[0] != key:
             w = w.float()
-            scale = (w.abs().amax(1) / 448.0).clamp_min(torch.finfo(torch.float32).tiny)
-            self._in_8bit = (key, (w / scale[:, None]).to(torch.float8_e4m3fn), scale)
+            whole = self._type_8bit == torch.int8
+            scale = (w.abs().amax(1) / (127.0 if whole else 448.0)).clamp_min(torch.finfo(torch.float32).tiny)
+            codes = w / scale[:, None]
+            self._in_8bit = (key, (codes.round() if whole else codes).to(self._type_8bit), scale)
         return self._in_8bit[1:]
 
     @torch.no_grad()
@@ -68,8 +72,11 @@ class GatedRecurrence(nn.Module):
         hidden = self._widened(hidden, residual)
         if self._in_8bit is not None:
             w, w_scale = self._codes()
-            q, scale, residual = ops.add_rmsnorm_8bit(hidden, self.norm.weight, residual, self.norm.eps, prenorm=True)
-            z = torch._scaled_mm(q, w.t(), scale_a=scale, scale_b=w_scale[None], out_dtype=torch.bfloat16).to(hidden.dtype)
+            q, scale, residual = ops.add_rmsnorm_8bit(hidden, self.norm.weight, residual, self.norm.eps, dtype=self._type_8bit, prenorm=True)
+            if self._type_8bit == torch.int8:
+                z = ops.linear_int8(q, scale, w, w_scale, dtype=hidden.dtype)
+            else:
+                z = torch._scaled_mm(q, w.t(), scale_a=scale, scale_b=w_scale[None], out_dtype=torch.bfloat16).to(hidden.dtype)
         else:
             y, residual = ops.add_rmsnorm_train(hidden, self.norm.weight, residual, self.norm.eps)
             z = self.in_proj(y)
