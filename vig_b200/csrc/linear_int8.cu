@@ -29,9 +29,10 @@ template <typename T> __device__ __forceinline__ float bias_at(const void* bias,
 // ---------------------------------------------------------------------------------------------------
 // Pairs.  Roles, rings and the two forms (streaming; W's columns stationary) as in gemm_pair.cu.
 constexpr int I8_BK = 128, I8_A = 128 * I8_BK, I8_B = 128 * I8_BK;       // one CTA's k box of x: its 128 rows; of W: its half of 256
-constexpr int I8_EPI = 16, I8_THREADS = 64 + 32 * I8_EPI, I8_MAX_ST = 8, I8_BARS = 8 * (2 * I8_MAX_ST + 5);
-template <typename T> constexpr int i8_box = 32 * 32 * (int)sizeof(T);   // an epilogue warp's way out
-template <typename T> constexpr int i8_ring = 227 * 1024 - 1024 - I8_EPI * i8_box<T> - I8_BARS - 16;
+constexpr int I8_EPI = 8, I8_THREADS = 64 + 32 * I8_EPI, I8_MAX_ST = 8, I8_BARS = 8 * (2 * I8_MAX_ST + 5);
+constexpr int I8_BOX = 32 * 128;                                         // an epilogue warp's way out: 32 rows of 128 bytes, whole lines (of 64 bytes: 106 us for 65536 x 768 x 2304)
+constexpr int I8_COLS = I8_EPI * 2 * 128 * 4;                            // every epilogue warp's scales of W and biases, of its 128 columns
+constexpr int I8_RING = 227 * 1024 - 1024 - I8_EPI * I8_BOX - I8_COLS - I8_BARS - 16;
 // D of 32-bit integers, A and B of signed bytes, both along k
 constexpr uint32_t I8_IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
 
@@ -42,24 +43,26 @@ __device__ __forceinline__ void mma_pair_i8(uint32_t d_tmem, uint32_t a_lo, uint
                  ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(I8_IDESC), "r"(accumulate), "r"(DESC_HI) : "memory");
 }
 
+__device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
+}
+
 struct I8Maps { CUtensorMap x, w, o; };
 
-// byte of (row, 16-byte piece) in a box whose rows are 64 or 128 bytes, swizzled as the tensor map of the output says
-template <typename T> __device__ __forceinline__ int box_at(int row, int piece) {
-    return sizeof(T) == 2 ? row * 64 + ((piece ^ ((row >> 1) & 3)) << 4) : row * 128 + ((piece ^ (row & 7)) << 4);
-}
+// byte of (row, 16-byte piece) in a box, swizzled as the tensor map of the output says
+__device__ __forceinline__ int box_at(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 
 template <typename T, bool STAT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
 int8_pair_kernel(const __grid_constant__ I8Maps maps, const Int8Params p, int KB, int ntn, int ntm, int nst, int boxed, int32_t* status) {
-    constexpr int BN = 256, COLS = 32, STAGE = I8_A + (STAT ? 0 : I8_B), V = 16 / (int)sizeof(T);
+    constexpr int BN = 256, COLS = 128, PIECE = 128 / (int)sizeof(T), STAGE = I8_A + (STAT ? 0 : I8_B), V = 16 / (int)sizeof(T);
     extern __shared__ uint8_t i8_smem_raw[];
     uint8_t* smem = i8_smem_raw + ((1024u - (smem_u32(i8_smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_rank();
     const int pair = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1, ntiles = ntm * ntn;
-    const uint32_t off_ring = STAT ? (uint32_t)KB * I8_B : 0u, off_out = off_ring + (uint32_t)nst * STAGE, off_bar = off_out + I8_EPI * i8_box<T>;
+    const uint32_t off_ring = STAT ? (uint32_t)KB * I8_B : 0u, off_out = off_ring + (uint32_t)nst * STAGE, off_cols = off_out + I8_EPI * I8_BOX, off_bar = off_cols + I8_COLS;
     const uint32_t bar_full = sbase + off_bar, bar_empty = bar_full + 8 * I8_MAX_ST, bar_acc_full = bar_empty + 8 * I8_MAX_ST, bar_acc_empty = bar_acc_full + 16,
                    bar_w = bar_acc_empty + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + off_bar + I8_BARS);
@@ -98,12 +101,15 @@ int8_pair_kernel(const __grid_constant__ I8Maps maps, const Int8Params p, int KB
         for (int tile = pair; tile < ntiles; tile += step) {
             const int row = (tile / ntn) * 256 + 128 * (int)rank, wrow = tile % ntn * BN + (rank ? BN / 2 : 0);
             for (int kb = 0; kb < KB; ++kb) {
-                waiter.wait_lite(bar_empty + 8 * st, phase ^ 1u);            // the MMAs of a ring ago have read the stage, in both CTAs
+                // the MMAs of a ring ago have read the stage, in both CTAs; asked first, since a wait costs hundreds of cycles even when its phase is over
+                if (!mbar_test_wait(bar_empty + 8 * st, phase ^ 1u)) waiter.wait_lite(bar_empty + 8 * st, phase ^ 1u);
                 if (*abort_flag) break;
                 if (lane == 0) {
                     if (rank == 0) mbar_expect_tx(bar_full + 8 * st, 2 * STAGE);
                     const uint32_t bar = map_rank(bar_full + 8 * st, 0), dst = sbase + off_ring + st * STAGE;
                     tma_load_2d_pair(dst, &maps.x, kb * I8_BK, row, bar);
+                    // the pairs of a row tile want the same box at the same time: it is on its way to L2 a tile ahead
+                    if (STAT && tile % ntn == kb % ntn && tile + step < ntiles) prefetch_2d(&maps.x, kb * I8_BK, row + step / ntn * 256);
                     if (!STAT) tma_load_2d_pair(dst + I8_A, &maps.w, kb * I8_BK, wrow, bar);
                 }
                 __syncwarp();
@@ -142,45 +148,61 @@ int8_pair_kernel(const __grid_constant__ I8Maps maps, const Int8Params p, int KB
                 if (issuer) tc_commit_pair(bar_acc_full + 8 * buf);
             }
         }
-    } else {                                             // ---- epilogue: a warp has a quarter of the rows and two pieces of 32 columns
+    } else {                                             // ---- epilogue: a warp has a quarter of the rows and half of the columns, a box of them at a time
         const int ew = warp - 2, part = ew >> 2;
         const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
-        uint8_t* box = smem + off_out + ew * i8_box<T>;
+        uint8_t* box = smem + off_out + ew * I8_BOX;
         const uint32_t drained = map_rank(bar_acc_empty, 0);
+        float* const cols = reinterpret_cast<float*>(smem + off_cols) + ew * 2 * COLS;    // scales, and behind them biases
+        int at_cols = -1;
         uint32_t it = 0;
         for (int tile = pair; tile < ntiles; tile += step, ++it) {
             const uint32_t buf = it & 1u, acc = tmem + lane_base + buf * 256u + COLS * part;
             const int row = (tile / ntn) * 256 + 128 * (int)rank + 32 * (warp & 3), col = (tile % ntn) * BN + COLS * part;
             const float xs = row + lane < p.M ? __ldg(p.xs + row + lane) : 0.f;
+            if (col != at_cols) {                        // in the stationary form once
+                at_cols = col;
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < COLS; i += 32) {
+                    const int n = col + i + lane;
+                    cols[i + lane] = n < p.N ? __ldg(p.ws + n) : 0.f;
+                    cols[COLS + i + lane] = n < p.N ? bias_at<T>(p.bias, n) : 0.f;
+                }
+            }
             waiter.wait_lite(bar_acc_full + 8 * buf, (it >> 1) & 1u);    // by the whole warp
             if (*abort_flag) break;
             tc_fence_after();
             __syncwarp();
-            float g[64];
-            tc_ld32(acc, g);
-            tc_ld32(acc + BN / 2, g + 32);
-            tc_wait_ld();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(drained + 8 * buf);
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int c = col + hf * (BN / 2);
+            for (int k = 0; k < COLS; k += PIECE) {
+                const int c = col + k;
+                float g[PIECE];
+#pragma unroll
+                for (int i = 0; i < PIECE; i += 32) tc_ld32(acc + k + i, g + i);
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the warp's earlier store has read the box
                 __syncwarp();
+                tc_wait_ld();
+                if (k + PIECE == COLS) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(drained + 8 * buf);
+                }
                 // the same addresses for all lanes
 #pragma unroll
-                for (int j = 0; j < 32 / V; ++j) {
+                for (int j = 0; j < 8; ++j) {
                     T e[V];
+                    float ws[V], b[V];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const int n = c + j * V + i;
-                        const float ws = n < p.N ? __ldg(p.ws + n) : 0.f, b = n < p.N ? bias_at<T>(p.bias, n) : 0.f;
-                        e[i] = DType<T>::from_f(fmaf((float)__float_as_int(g[32 * hf + j * V + i]), xs * ws, b));
+                    for (int i = 0; i < V; i += 4) {
+                        *(float4*)(ws + i) = *(const float4*)(cols + k + j * V + i);
+                        *(float4*)(b + i) = *(const float4*)(cols + COLS + k + j * V + i);
                     }
+#pragma unroll
+                    for (int i = 0; i < V; ++i) e[i] = DType<T>::from_f(fmaf((float)__float_as_int(g[j * V + i]), xs * ws[i], b[i]));
                     uint4 w;
                     memcpy(&w, e, 16);
-                    *reinterpret_cast<uint4*>(box + box_at<T>(lane, j)) = w;
+                    *reinterpret_cast<uint4*>(box + box_at(lane, j)) = w;
                 }
                 if (boxed) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -191,10 +213,13 @@ int8_pair_kernel(const __grid_constant__ I8Maps maps, const Int8Params p, int KB
                     }
                 } else {                                 // rows off 16 bytes: a lane has a column
                     __syncwarp();
-                    if (c + lane < p.N) {
-                        T* to = (T*)p.y + (int64_t)row * p.ldy + c + lane;
-                        for (int r = 0; r < 32 && row + r < p.M; ++r) to[r * p.ldy] = *reinterpret_cast<const T*>(box + box_at<T>(r, lane / V) + lane % V * sizeof(T));
+#pragma unroll
+                    for (int i = lane; i < PIECE; i += 32) {
+                        if (c + i >= p.N) break;
+                        T* to = (T*)p.y + (int64_t)row * p.ldy + c + i;
+                        for (int r = 0; r < 32 && row + r < p.M; ++r) to[r * p.ldy] = *reinterpret_cast<const T*>(box + box_at(r, i / V) + i % V * sizeof(T));
                     }
+                    __syncwarp();
                 }
             }
         }
@@ -222,10 +247,10 @@ bool map_of_bytes(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, 
 bool map_of_output(CUtensorMap* m, const Int8Params& p, int dtype) {
     const int size = dtype == VIG_DTYPE_F32 ? 4 : 2;
     MapKey key{};
-    key.base = p.y; key.rank = 2; key.dtype = dtype; key.swizzle = size == 2 ? 2 : 1;
+    key.base = p.y; key.rank = 2; key.dtype = dtype; key.swizzle = 1;
     key.dims[0] = (uint64_t)p.N; key.dims[1] = (uint64_t)p.M;
     key.strides[0] = (uint64_t)p.ldy * size;
-    key.box[0] = 32; key.box[1] = 32;
+    key.box[0] = 128 / size; key.box[1] = 32;
     return encode_cached(m, key);
 }
 
@@ -237,10 +262,10 @@ template <typename T> int pair_launch(const Int8Params& p, int dtype, int32_t* s
     const int64_t ntm = (p.M + 255) / 256;
     if (ntm * ntn > INT32_MAX) return VIG_ERR_SHAPE;
     // stationary by the rule of the 16-bit form: where W's columns leave a ring of four boxes of x, nearly all pairs have a column and each has a tile
-    const int xst = (i8_ring<T> - KB * I8_B) / I8_A;
+    const int xst = (I8_RING - KB * I8_B) / I8_A;
     const bool stat = xst >= 4 && all / ntn * ntn * 16 >= all * 15 && ntm * ntn >= all;
-    const int nst = stat ? (xst < I8_MAX_ST ? xst : I8_MAX_ST) : i8_ring<T> / (I8_A + I8_B);
-    const int smem = (stat ? KB * I8_B + nst * I8_A : nst * (I8_A + I8_B)) + I8_EPI * i8_box<T> + I8_BARS + 16 + 1024;
+    const int nst = stat ? (xst < I8_MAX_ST ? xst : I8_MAX_ST) : I8_RING / (I8_A + I8_B);
+    const int smem = (stat ? KB * I8_B + nst * I8_A : nst * (I8_A + I8_B)) + I8_EPI * I8_BOX + I8_COLS + I8_BARS + 16 + 1024;
     const int64_t pairs = stat ? all / ntn * ntn : ntm * ntn < all ? ntm * ntn : all;
     const auto kfn = stat ? int8_pair_kernel<T, true> : int8_pair_kernel<T, false>;
     if (const cudaError_t e = ensure_smem_attr((const void*)kfn, 227 * 1024)) return (int)e;

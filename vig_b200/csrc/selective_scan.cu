@@ -77,9 +77,11 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
         fetch_map<T>(mC, gC, p.s_c[1], t0, len, p.N, Npad, p.piece_maps, lane);
     };
     if (warp < ntiles) bring(warp);
+    const bool whole = p.N % (PARTS * S) == 0 && (uintptr_t)p.states % 16 == 0;
 
     for (int tile = warp; tile < ntiles; tile += W) {
         const int64_t t0 = (int64_t)tile * TILE;
+        float* const left = p.states ? p.states + (((int64_t)b * p.tiles + tile) * p.D + d) * p.N + part * S : nullptr;     // states that enter the tile
         copies_done();
         __syncwarp();
 #pragma unroll 1
@@ -144,10 +146,15 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
                     for (int s = 0; s < S / 2; ++s) *(F2*)(h_at + 2 * s) = E[0][s];
                 }
                 hand.pass(flag, (uint32_t)tile + 1);
-                if (p.states && run == 0) {
-                    float* to = p.states + (((int64_t)b * p.tiles + tile) * p.D + d + c) * p.N + n0 + part * S;
+                if (left && run == 0) {
+                    float* to = left + c * p.N + n0;
+                    if (whole) {
+                        if constexpr (S == 4) *(ulonglong2*)to = make_ulonglong2(h0[0][0], h0[0][1]);
+                        else *(F2*)to = h0[0][0];
+                    } else {
 #pragma unroll
-                    for (int s = 0; s < S; ++s) if (n0 + part * S + s < p.N) to[s] = s & 1 ? f2_hi(h0[0][s / 2]) : f2_lo(h0[0][s / 2]);
+                        for (int s = 0; s < S; ++s) if (n0 + part * S + s < p.N) to[s] = s & 1 ? f2_hi(h0[0][s / 2]) : f2_lo(h0[0][s / 2]);
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
