@@ -73,19 +73,28 @@ template <typename T, int NC> __device__ __forceinline__ void fetch(T* dst, cons
 
 // [64 tokens][Npad] of a map of this tile, by a warp; tokens from `len` on and states from N on are zeros
 template <typename T> __device__ __forceinline__ void fetch_map(T* dst, const T* src, int64_t stride, int64_t t0, int len, int N, int Npad, int piece, int lane) {
-    if (piece >= 4) {
-        const int bytes = Npad * (int)sizeof(T), have = N * (int)sizeof(T);       // whole pieces both
+    if (piece >= 16) {
+        const int n16 = Npad * (int)sizeof(T) / 16, have = N * (int)sizeof(T) / 16;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int t = lane + 32 * r;
             char* to = (char*)(dst + row_of(t) * Npad);
             const char* from = (const char*)(src + (t0 + t) * stride);
-            const int there = t0 + t < len ? have : 0;
-            int k = 0;
-            if (piece >= 16) for (; k < there; k += 16) copy16(to + k, from + k);
-            else if (piece >= 8) for (; k < there; k += 8) copy8(to + k, from + k);
-            else for (; k < there; k += 4) copy4(to + k, from + k);
-            for (; k < bytes; k += 4) *(uint32_t*)(to + k) = 0u;
+            for (int k = 0; k < n16; ++k) {
+                if (t0 + t < len && k < have) copy16(to + 16 * k, from + 16 * k);
+                else *(uint4*)(to + 16 * k) = make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+    } else if (piece >= 4) {
+        const int words = Npad * (int)sizeof(T) / 4, have = N * (int)sizeof(T) / 4;
+        for (int t = lane; t < TILE; t += 32) {
+            char* to = (char*)(dst + row_of(t) * Npad);
+            const char* from = (const char*)(src + (t0 + t) * stride);
+#pragma unroll 4
+            for (int k = 0; k < words; ++k) {
+                if (t0 + t < len && k < have) copy4(to + 4 * k, from + 4 * k);
+                else *(uint32_t*)(to + 4 * k) = 0u;
+            }
         }
     } else {
         for (int t = lane; t < TILE; t += 32)

@@ -25,7 +25,8 @@ template <typename T, int S, int CT> struct FwdSmem {
     static int bytes(int N, int W) { return W * warp_bytes(N) + (2 * CT * padded(N) + CT * padded(N) / NB + 2 * CT + 4) * 4; }
 };
 
-template <typename T, int S, int CT, int W>
+// LEAVE: the states that enter each tile are written too, for a backward
+template <typename T, int S, int CT, int W, bool LEAVE>
 __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kernel(const Params p) {
     using M = FwdSmem<T, S, CT>;
     constexpr int NB = M::NB, THREADS = 32 * W, HALF = M::STASH / 2;
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
 
     for (int tile = warp; tile < ntiles; tile += W) {
         const int64_t t0 = (int64_t)tile * TILE;
-        float* const left = p.states ? p.states + (((int64_t)b * p.tiles + tile) * p.D + d) * p.N + part * S : nullptr;     // states that enter the tile
+        float* const left = LEAVE ? p.states + (((int64_t)b * p.tiles + tile) * p.D + d) * p.N + part * S : nullptr;
         copies_done();
         __syncwarp();
 #pragma unroll 1
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
                     for (int s = 0; s < S / 2; ++s) *(F2*)(h_at + 2 * s) = E[0][s];
                 }
                 hand.pass(flag, (uint32_t)tile + 1);
-                if (left && run == 0) {
+                if (LEAVE && run == 0) {
                     float* to = left + c * p.N + n0;
                     if (whole) {
                         if constexpr (S == 4) *(ulonglong2*)to = make_ulonglong2(h0[0][0], h0[0][1]);
@@ -337,9 +338,9 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 *(float4*)v = *(const float4*)(from + c * TILE + run * RUN);
                 *(float4*)(v + 4) = *(const float4*)(from + c * TILE + run * RUN + 4);
             };
-            F2 s_y[RUN], s_b[RUN], s_a[RUN];                     // what is summed over the states
+            float s_y[RUN], s_b[RUN], s_a[RUN];                  // what is summed over the states
 #pragma unroll
-            for (int j = 0; j < RUN; ++j) s_y[j] = s_b[j] = s_a[j] = 0ull;
+            for (int j = 0; j < RUN; ++j) s_y[j] = s_b[j] = s_a[j] = 0.f;
 #pragma unroll 1
             for (int n0 = 0; n0 < Npad; n0 += NB) {
                 const int at = c * Npad + n0 + part * S;
@@ -359,23 +360,23 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 row(dr, dys);
                 landed<16>(mb);
                 landed<16>(mc);
+                kept();                                          // what the channel ahead has added, long since
                 recall<16>(col + 48, md);
 #pragma unroll
-                for (int j = 0; j < RUN; ++j) in[j][0] = f2_mul(f2_make(xr[j], xr[j]), f2_make(mb[2 * j], mb[2 * j + 1]));
+                for (int j = 0; j < RUN; ++j) in[j][0] = f2_make(xr[j] * mb[2 * j], xr[j] * mb[2 * j + 1]);
                 own_sum<S>(P, E, a, in);
                 Pb = P[0];
 #pragma unroll
-                for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), f2_make(dr[j], dr[j]), Q));
+                for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_make(fmaf(mc[2 * j], dr[j], f2_lo(Q)), fmaf(mc[2 * j + 1], dr[j], f2_hi(Q))));
                 pairs<float, S>(h0, st + at);
                 entering<S, 1>(&h[0], &E, &P, &h0, &a, &in, run, part);
                 landed<16>(md);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
                     h[j + 1][0] = f2_fma(a[j][0], h[j][0], in[j][0]);
-                    s_y[j] = f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), h[j + 1][0], s_y[j]);
-                    const F2 add = f2_fma(h[j + 1][0], f2_make(dr[j], dr[j]), f2_make(md[2 * j], md[2 * j + 1]));
-                    md[2 * j] = f2_lo(add);
-                    md[2 * j + 1] = f2_hi(add);
+                    s_y[j] = fmaf(mc[2 * j], f2_lo(h[j + 1][0]), fmaf(mc[2 * j + 1], f2_hi(h[j + 1][0]), s_y[j]));
+                    md[2 * j] = fmaf(f2_lo(h[j + 1][0]), dr[j], md[2 * j]);
+                    md[2 * j + 1] = fmaf(f2_hi(h[j + 1][0]), dr[j], md[2 * j + 1]);
                 }
                 keep<16>(col + 48, md);
                 recall<16>(col + 32, md);
@@ -407,15 +408,14 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 F2 dAs = 0ull;
 #pragma unroll
                 for (int j = RUN - 1; j >= 0; --j) {
-                    const F2 gr = f2_fma(f2_make(mc[2 * j], mc[2 * j + 1]), f2_make(dr[j], dr[j]), Q);
-                    s_b[j] = f2_fma(gr, f2_make(mb[2 * j], mb[2 * j + 1]), s_b[j]);
-                    const F2 add = f2_fma(gr, f2_make(xr[j], xr[j]), f2_make(md[2 * j], md[2 * j + 1]));
-                    md[2 * j] = f2_lo(add);
-                    md[2 * j + 1] = f2_hi(add);
+                    const F2 gr = f2_make(fmaf(mc[2 * j], dr[j], f2_lo(Q)), fmaf(mc[2 * j + 1], dr[j], f2_hi(Q)));
+                    s_b[j] = fmaf(f2_lo(gr), mb[2 * j], fmaf(f2_hi(gr), mb[2 * j + 1], s_b[j]));
+                    md[2 * j] = fmaf(f2_lo(gr), xr[j], md[2 * j]);
+                    md[2 * j + 1] = fmaf(f2_hi(gr), xr[j], md[2 * j + 1]);
                     Q = f2_mul(a[j][0], gr);
                     const F2 f = f2_mul(Q, h[j][0]);
-                    s_a[j] = f2_fma(f, A[0], s_a[j]);
-                    dAs = f2_fma(f, f2_make(dl[j], dl[j]), dAs);
+                    s_a[j] = fmaf(f2_lo(f), f2_lo(A[0]), fmaf(f2_hi(f), f2_hi(A[0]), s_a[j]));
+                    dAs = f2_make(fmaf(f2_lo(f), dl[j], f2_lo(dAs)), fmaf(f2_hi(f), dl[j], f2_hi(dAs)));
                 }
                 keep<16>(col + 32, md);
                 // dA over the runs: a lane of an even run keeps the first state's sum, of an odd one the second's
@@ -424,23 +424,13 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 v += __shfl_xor_sync(ALL, v, 2 * PARTS);
                 v += __shfl_xor_sync(ALL, v, 4 * PARTS);
                 if (run < 2) dA[at + run] += v;
-                kept();
             }
-            float v[RUN];
             const int to = c * TILE + run * RUN + part * 2;
-            if (z) {
-#pragma unroll
-                for (int j = 0; j < RUN; ++j) v[j] = f2_lo(s_y[j]) + f2_hi(s_y[j]);
-                *(float2*)(ys + to) = over_parts(v, part);
-            }
-#pragma unroll
-            for (int j = 0; j < RUN; ++j) v[j] = f2_lo(s_b[j]) + f2_hi(s_b[j]);
-            *(float2*)(gb + to) = over_parts(v, part);
-#pragma unroll
-            for (int j = 0; j < RUN; ++j) v[j] = f2_lo(s_a[j]) + f2_hi(s_a[j]);
-            *(float2*)(ga + to) = over_parts(v, part);
+            if (z) *(float2*)(ys + to) = over_parts(s_y, part);
+            *(float2*)(gb + to) = over_parts(s_b, part);
+            *(float2*)(ga + to) = over_parts(s_a, part);
         }
-        __syncwarp();
+        kept();
         // the tile's maps have their gradients from this CTA's channels
         for (int n0 = 0; n0 < Npad; n0 += NB) {
             float mb[RUN * S], mc[RUN * S];
@@ -621,8 +611,9 @@ template <typename T, int S, int CT, int W> int fwd_launch(Params& p, cudaStream
     const int64_t grid = (int64_t)p.B * p.G * p.ctiles;
     const int smem = FwdSmem<T, S, CT>::bytes(p.N, W);
     if (grid >= (1ll << 31)) return VIG_ERR_SHAPE;
-    if (const cudaError_t e = ensure_smem_attr((const void*)scan_fwd_kernel<T, S, CT, W>, smem)) return (int)e;
-    scan_fwd_kernel<T, S, CT, W><<<(unsigned)grid, 32 * W, smem, s>>>(p);
+    const auto kernel = p.states ? scan_fwd_kernel<T, S, CT, W, true> : scan_fwd_kernel<T, S, CT, W, false>;
+    if (const cudaError_t e = ensure_smem_attr((const void*)kernel, smem)) return (int)e;
+    kernel<<<(unsigned)grid, 32 * W, smem, s>>>(p);
     return (int)cudaGetLastError();
 }
 template <typename T> int bwd_launch(Params& p, cudaStream_t s) {
