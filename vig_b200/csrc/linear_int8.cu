@@ -1,8 +1,10 @@
 // Product of 8-bit integers: y[m, n] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + bias[n].  Sums are 32-bit integers and exact; scales and bias are
 // applied in fp32 and y is rounded once.  Three forms:
 //   pairs   (rows on 16 bytes): tcgen05.mma kind::i8 on CTA pairs, tiles of 256 x 256, k boxes of 128 bytes through TMA, as gemm_pair.cu does for 16 bits: the
-//           integer product is twice as fast and brings in half the bytes, so what bounds it is the output (65536 x 768 x 2304: 302 of 354 MB).
+//           integer product is twice as fast and brings in half the bytes, so what bounds it is the output (65536 x 768 x 2304: 302 of 354 MB).  That case takes
+//           96 us; 77 without the epilogue's work, 89 without its stores.
 //   skinny  (rows on 16 bytes, up to 64 of them): W is read once, by all SMs, straight into fragments of mma.sync; a warp takes 16 columns and a share of k.
+//           8 x 768 x 2304 2.5 us; as tiles of the form below 12.
 //   any     everything else: mma.sync on 64 x 64 tiles through shared memory.
 #include "tc_common.cuh"
 

@@ -6,7 +6,8 @@
 // Every (token, channel, state) costs an exponential and three multiply-adds, every (token, channel) three 16-bit values in and one out: with 16
 // states the exponentials bound it (MUFU, 16 a cycle and SM), not memory.  So each is taken once: the warps of a CTA take tiles of the same channels'
 // tokens in turn and hand the state from tile to tile, within a tile a warp's lanes divide tokens and states (scan_common.cuh); two passes over
-// independent chunks would take every exponential twice.
+// independent chunks would take every exponential twice.  1 x 16384 x 768 x 16 bf16 301 us, 8 x 4096 x 768 x 16 331 (45 and 90 by the exponentials), training the
+// latter 377 + 1040 + 45: issue slots at 45 to 50 %, ten warps an SM, 14 instructions a (token, channel, state) forward and 36 backward.
 #include "scan_common.cuh"
 
 namespace vig {

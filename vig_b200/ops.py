@@ -4,8 +4,8 @@
 ``fused_chunk_gla`` mirrors ``fla/ops/gla/chunk_fuse.py:554-572`` and ``chunk_gla``
 ``fla/ops/gla/chunk.py:561-580``; ``bi_gla`` is the explicit form of the merged operator.
 Tensors are ``[B, H, L, d]`` views with a contiguous last dimension; no copies are made.
-``bi_gla`` and the one-direction entry points are differentiable (``vig_bigla_bwd_full``), and so are ``gated_recurrence`` and
-``add_rmsnorm_train``; the block's other kernels are inference-only.
+``bi_gla`` and the one-direction entry points are differentiable (``vig_bigla_bwd_full``), and so are ``gated_recurrence``, ``selective_scan``,
+``causal_conv``, ``add_rmsnorm_train`` and ``add_layernorm_train``; the block's other kernels are inference-only.
 """
 import math
 
