@@ -254,6 +254,28 @@ def test_infinities_stay():
     assert (final[0, :, 2] == float("inf")).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_steps_of_nothing(dtype):
+    """A raw step of -inf, or of the type's lowest value, is one of nothing: the state passes as it was, the token has no gradient but the skip's, and nothing becomes a NaN."""
+    t = make(2, 100, 20, 16, 0, dtype, seed=7)
+    for i, v in enumerate((float("-inf"), torch.finfo(dtype).min)):
+        t["dt"][i, 10:80] = v
+    outs = compare(t)
+    assert not outs[3][:, 10:80].any()                           # the gradient of dt
+    c = {k: v.cuda() for k, v in t.items()}
+    state = c["initial_state"].clone()
+    y = vig_b200.selective_scan_step(c["u"][:, 20], c["dt"][:, 20], c["A"], c["B"][:, 20], c["C"][:, 20], state, c["D"], c["z"][:, 20], c["dt_bias"])
+    assert torch.equal(state, c["initial_state"]) and torch.isfinite(y).all()
+    t["dt"][0, 50, 3] = float("nan")
+    y, final = run(t)
+    assert y[0, 50:, 3].isnan().all() and final[0, 3].isnan().all()
+    y[0, :, 3] = final[0, 3] = 0
+    assert torch.isfinite(y).all() and torch.isfinite(final).all()
+    t["dt"][0, 50, 3], t["dt"][1, 60, 4], t["u"][1, 60, 4] = 0, float("inf"), 1
+    y, final = run(t)
+    assert not torch.isfinite(final[1, 4]).any() and torch.isfinite(final[0]).all()
+
+
 def test_graph_and_streams():
     """Captured with its backward and replayed on other values; on a stream of its own; the same bits every time."""
     t = make(2, 150, 48, 16, 0, torch.bfloat16, seed=4)

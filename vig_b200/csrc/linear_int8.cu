@@ -432,7 +432,7 @@ using namespace vig;
 extern "C" int vig_linear_int8_fwd(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw, const float* w_scales, const void* bias, void* y,
                                    int64_t ldy, int64_t M, int N, int K, int dtype, int32_t* status_dev, void* stream) {
     if (dtype < VIG_DTYPE_F32 || dtype > VIG_DTYPE_F16) return VIG_ERR_DTYPE;
-    if (M < 0 || N < 0 || K < 0 || K > 131072 || M >= (1ll << 31) || N > 4194240) return VIG_ERR_SHAPE;
+    if (M < 0 || N < 0 || K < 0 || K > 131072 || M > INT32_MAX - 1024 || N > 4194240) return VIG_ERR_SHAPE;
     if (!M || !N) return VIG_OK;
     if (!x_scales || !w_scales || !y || (K && (!x || !w))) return VIG_ERR_NULL;
     const Int8Params p{(const int8_t*)x, (const int8_t*)w, x_scales, w_scales, bias, y, ldx, ldw, ldy, M, N, K};

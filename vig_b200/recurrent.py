@@ -10,6 +10,8 @@ from .modules import RMSNorm
 
 
 class GatedRecurrence(nn.Module):
+    _type_8bit = torch.float8_e4m3fn        # also of modules that were pickled before they had a choice
+
     def __init__(self, d_model, d_inner=None, gate_logit_normalizer=16.0, eps=1e-6):
         super().__init__()
         self.d_model, self.d_inner = d_model, d_inner or d_model
@@ -17,7 +19,7 @@ class GatedRecurrence(nn.Module):
         self.norm = RMSNorm(d_model, eps=eps)
         self.in_proj = nn.Linear(d_model, 3 * self.d_inner, bias=False)
         self.out_proj = nn.Linear(self.d_inner, d_model, bias=False)
-        self._in_8bit, self._type_8bit = None, torch.float8_e4m3fn
+        self._in_8bit = None
 
     def forward(self, hidden, residual=None, state=None, output_final_state=False):
         """``hidden`` ``[B, L, d_model]`` and the residual stream (None: it begins with ``hidden``); ``state``: fp32 ``[B, d_inner]`` of the tokens
