@@ -520,6 +520,10 @@ VIG_API int vig_add_layernorm_bwd(const void* dy, int64_t ldy, const void* x, in
  * overflows), scaled in fp32, rounded once to dtype.  x: int8 [M, K] with row stride ldx; w: int8 [N, K] with row stride ldw; x_scales [M], w_scales [N]: fp32;
  * bias (optional): [N] of dtype; y: [M, N] with row stride ldy.  Any sizes and alignment.  status_dev: optional int32, bit 0 = a bounded wait ran out.
  */
+/* Whether the rows are better laid out first, by vig_int8_rows_lay_out into [rows, (K + 15) / 16 * 16] on 16 bytes with zeros behind the K bytes of a row (x and w both, the
+ * product then taken over the longer rows): a copy costs little beside a product of rows off 16 bytes. */
+VIG_API int vig_linear_int8_laid_out_first(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K);
+VIG_API int vig_int8_rows_lay_out(const void* src, int64_t ld, void* dst, int64_t rows, int K, void* stream);
 VIG_API int vig_linear_int8_fwd(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw, const float* w_scales, const void* bias, void* y,
                                 int64_t ldy, int64_t M, int N, int K, int dtype, int32_t* status_dev, void* stream);
 

@@ -39,6 +39,16 @@ def test_product(M, N, K, dtype):
     check(got, q, s, w, ws, b, dtype)
 
 
+def test_rows_off_16_bytes():
+    """Large products of rows that begin anywhere are taken over copies of them: odd K, and even ones behind an odd offset; K next to the largest is taken as it lies."""
+    for M, N, K, first in ((5000, 300, 333, 0), (700, 96, 768, 3), (40, 2304, 767, 1), (300, 64, 131071, 0)):
+        q, s, w, ws, b = make(M, N, K, torch.bfloat16, seed=K)
+        wide = torch.zeros(M, K + first, dtype=torch.int8, device="cuda")
+        wide[:, first:] = q.cuda()
+        got = vig_b200.linear_int8(wide[:, first:], s.cuda(), w.cuda(), ws.cuda(), b.cuda())
+        check(got, q, s, w, ws, b, torch.bfloat16)
+
+
 def test_many_tiles():
     """More tiles than CTA pairs, W's columns stationary and streamed."""
     for M, N, K in ((20000, 768, 768), (40000, 300, 256), (3000, 2304, 2048)):

@@ -84,6 +84,14 @@ def test_norm_and_product_entries():
     assert mul() == -1 and mul(dtype=3) == -3 and mul(M=-1) == -2 and mul(K=131073) == -2 and mul(N=-1) == -2 and mul(M=0) == 0 and mul(N=0) == 0
 
 
+def test_laying_out():
+    L_ = _lib.lib()
+    first = lambda x=256, ldx=64, M=4096, N=256, K=64: L_.vig_linear_int8_laid_out_first(x, ldx, 256, 64, M, N, K)  # noqa: E731
+    assert first() == 0 and first(x=257) == 1 and first(ldx=65) == 1 and first(K=63) == 1 and first(K=63, M=4) == 0 and first(M=0) == 0 and first(K=131071) == 0
+    lay = lambda src=None, dst=None, rows=1, K=5: L_.vig_int8_rows_lay_out(src, 5, dst, rows, K, None)  # noqa: E731
+    assert lay() == -1 and lay(rows=-1) == -2 and lay(K=131073) == -2 and lay(rows=0) == 0 and lay(K=0) == 0 and lay(src=256, dst=264) == -4
+
+
 def test_block_refuses_what_it_cannot_do():
     block = vig_b200.SelectiveStateSpace(16)
     with pytest.raises(RuntimeError, match="CUDA"):

@@ -83,6 +83,8 @@ _SIGNATURES = {
     "vig_add_layernorm_train_fwd": (c_int, [c_void_p, c_int64] * 2 + [c_void_p] * 2 + [c_int] + [c_void_p] * 2 + [c_int64, c_int, c_float, c_int, c_void_p]),
     "vig_add_layernorm_bwd_workspace_bytes": (c_size_t, [c_int64, c_int]),
     "vig_add_layernorm_bwd": (c_int, [c_void_p, c_int64] * 3 + [c_void_p, c_int] + [c_void_p, c_int64] + [c_void_p] * 3 + [c_int64, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "vig_linear_int8_laid_out_first": (c_int, [c_void_p, c_int64] * 2 + [c_int64] + [c_int] * 2),
+    "vig_int8_rows_lay_out": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p]),
     "vig_linear_int8_fwd": (c_int, [c_void_p, c_int64, c_void_p] * 2 + [c_void_p] * 2 + [c_int64] * 2 + [c_int] * 3 + [c_void_p] * 2),
     "vig_swiglu_fwd": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int64, c_int64, c_int, c_void_p]),
 }

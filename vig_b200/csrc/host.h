@@ -22,7 +22,7 @@ namespace py = pybind11;
     X(vig_add_rmsnorm_bwd_workspace_bytes) X(vig_adamw_step) X(vig_gated_recurrence_states_bytes) X(vig_gated_recurrence_train_fwd) X(vig_gated_recurrence_train_bwd) \
     X(vig_selective_scan_states_bytes) X(vig_selective_scan_fwd) X(vig_selective_scan_bwd_workspace_bytes) X(vig_selective_scan_bwd) X(vig_selective_scan_step) \
     X(vig_causal_conv_fwd) X(vig_causal_conv_bwd_workspace_bytes) X(vig_causal_conv_bwd) X(vig_causal_conv_step) X(vig_add_layernorm_train_fwd) \
-    X(vig_add_layernorm_bwd_workspace_bytes) X(vig_add_layernorm_bwd) X(vig_linear_int8_fwd)
+    X(vig_add_layernorm_bwd_workspace_bytes) X(vig_add_layernorm_bwd) X(vig_linear_int8_fwd) X(vig_linear_int8_laid_out_first) X(vig_int8_rows_lay_out)
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
     VIG_HOST_API(X)

@@ -414,10 +414,18 @@ std::optional<Tensor> linear_int8(const Tensor& q, const Tensor& scales, const T
     sizes.push_back(N);
     const Tensor y = fresh(sizes, q, type);
     const int64_t M = N ? y.numel() / N : 0;
-    const Tensor x = q.dim() == 2 && unit_last(q) ? q : rows(q.reshape({M ? M : (K ? q.numel() / K : 0), K}));
+    Tensor x = q.dim() == 2 && unit_last(q) ? q : rows(q.reshape({M ? M : (K ? q.numel() / K : 0), K})), w16 = w;
     const Tensor s = scales.contiguous(), ws = w_scales.contiguous();
-    ok(api.vig_linear_int8_fwd(ptr(x), x.size(0) > 1 ? x.stride(0) : K, (const float*)ptr(s), ptr(w), N > 1 ? w.stride(0) : K, (const float*)ptr(ws), ptr(bias), ptr(y), N, M, (int)N,
-                               (int)K, (int)out, status_ptr(q.get_device()), stream()), "vig_linear_int8_fwd");
+    int64_t ldx = x.size(0) > 1 ? x.stride(0) : K, ldw = N > 1 ? w.stride(0) : K, width = K;
+    if (api.vig_linear_int8_laid_out_first(ptr(x), ldx, ptr(w), ldw, M, (int)N, (int)K)) {
+        width = (K + 15) / 16 * 16;
+        const Tensor x2 = fresh({M, width}, q), w2 = fresh({N, width}, q);
+        ok(api.vig_int8_rows_lay_out(ptr(x), ldx, ptr(x2), M, (int)K, stream()), "vig_int8_rows_lay_out");
+        ok(api.vig_int8_rows_lay_out(ptr(w), ldw, ptr(w2), N, (int)K, stream()), "vig_int8_rows_lay_out");
+        x = x2; w16 = w2; ldx = ldw = width;
+    }
+    ok(api.vig_linear_int8_fwd(ptr(x), ldx, (const float*)ptr(s), ptr(w16), ldw, (const float*)ptr(ws), ptr(bias), ptr(y), N, M, (int)N, (int)width, (int)out,
+                               status_ptr(q.get_device()), stream()), "vig_linear_int8_fwd");
     return y;
 }
 

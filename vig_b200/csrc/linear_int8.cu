@@ -345,6 +345,17 @@ __device__ __forceinline__ uint32_t word_at(const int8_t* row, int k, int K, uin
     return v;
 }
 
+// Rows laid out on 16 bytes, zeros behind them: a thread puts 16 bytes together
+__global__ void __launch_bounds__(256) int8_lay_out_kernel(const int8_t* src, int64_t ld, uint4* dst, int64_t rows, int K, int pieces) {
+    const uintptr_t begin = (uintptr_t)src, end = begin + (uintptr_t)((rows - 1) * ld + K);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / pieces;
+        const int k = (int)(i - row * pieces) * 16;
+        const int8_t* from = src + row * ld;
+        dst[i] = make_uint4(word_at(from, k, K, begin, end), word_at(from, k + 4, K, begin, end), word_at(from, k + 8, K, begin, end), word_at(from, k + 12, K, begin, end));
+    }
+}
+
 template <typename T> __global__ void __launch_bounds__(128) int8_any_kernel(const Int8Params p) {
     __shared__ __align__(16) int8_t xs[BM * PITCH], ws[BN * PITCH];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
@@ -428,6 +439,24 @@ template <typename T> int int8_launch(const Int8Params& p, int dtype, int32_t* s
 }  // namespace vig
 
 using namespace vig;
+
+// Off 16 bytes the 64 x 64 form takes what is little, and what is more is laid out first: 65536 x 333 x 576 536 us as it lies.
+extern "C" int vig_linear_int8_laid_out_first(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0 || K > 131072 - 15) return 0;
+    const bool on_16 = K % 16 == 0 && ((uintptr_t)x | (uintptr_t)w) % 16 == 0 && (ldx | ldw) % 16 == 0 && ldx >= K && ldw >= K;
+    return !on_16 && (double)M * N * K >= 1 << 24;
+}
+
+extern "C" int vig_int8_rows_lay_out(const void* src, int64_t ld, void* dst, int64_t rows, int K, void* stream) {
+    if (rows < 0 || K < 0 || K > 131072) return VIG_ERR_SHAPE;
+    if (!rows || !K) return VIG_OK;
+    if (!src || !dst) return VIG_ERR_NULL;
+    if ((uintptr_t)dst % 16) return VIG_ERR_ALIGN;
+    const int pieces = (K + 15) / 16;
+    const int64_t blocks = (rows * pieces + 255) / 256, most = (int64_t)device_sms() * 16;
+    int8_lay_out_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, (cudaStream_t)stream>>>((const int8_t*)src, ld, (uint4*)dst, rows, K, pieces);
+    return (int)cudaGetLastError();
+}
 
 extern "C" int vig_linear_int8_fwd(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw, const float* w_scales, const void* bias, void* y,
                                    int64_t ldy, int64_t M, int N, int K, int dtype, int32_t* status_dev, void* stream) {
