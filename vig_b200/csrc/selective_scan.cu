@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
             }
             __syncwarp();
             if (n0 + NB >= Npad && tile + W < ntiles) bring(tile + W);       // all of this tile is elsewhere by now
-            if (!n0 && tile < W) hand.await(flags + have / W, (uint32_t)tile);    // warps begin some channels apart, or each hiccup of one is all the others'
+            if (W > 1 && !n0 && tile < W) hand.await(flags + have / W, (uint32_t)tile);    // warps begin some channels apart, or each hiccup of one is all the others'
 #pragma unroll 1
             for (int c = 0; c < have; ++c) {
                 float* const h_at = carry + c * Npad + n0 + part * S;
@@ -630,6 +630,8 @@ template <typename T> int bwd_launch(Params& p, cudaStream_t s) {
 // instruction: 1 x 16384 x 768 1004 / 531 / 303 us; 16 x 4096 x 768 711 / 705 / 817).
 template <typename T, int S> int fwd_width(Params& p, cudaStream_t s) {
     const int64_t wide = (int64_t)p.B * p.G * ((p.D / p.G + 15) / 16);
+    // a single tile is one warp's work: the others of a CTA would only hold its registers
+    if (p.tiles <= 1) return wide >= 4 * device_sms() ? fwd_launch<T, S, 16, 1>(p, s) : fwd_launch<T, S, 4, 1>(p, s);
     const auto fits = [&](int bytes) { return bytes <= 227 * 1024; };      // (maps of many states in fp32)
     if (wide >= 2 * device_sms() && fits(FwdSmem<T, S, 16>::bytes(p.N, 4))) return fwd_launch<T, S, 16, 4>(p, s);
     if (wide >= device_sms() || !fits(FwdSmem<T, S, 4>::bytes(p.N, 6))) return fwd_launch<T, S, 8, 4>(p, s);
