@@ -160,7 +160,7 @@ def test_lengths(dtype, lengths):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("B,L,D,N", [(1, 1500, 768, 16), (20, 200, 256, 16), (12, 130, 512, 8), (40, 70, 128, 16)])
+@pytest.mark.parametrize("B,L,D,N", [(1, 1500, 768, 16), (20, 200, 256, 16), (12, 130, 512, 8), (40, 70, 128, 16), (40, 128, 256, 16), (80, 60, 256, 16), (90, 100, 256, 5)])
 def test_every_width_of_a_block(B, L, D, N, dtype):
     """Few, some and many channels: sequences of a larger call against calls of their own, and against 64 bits."""
     t = make(B, L, D, N, 0, dtype, seed=3)

@@ -630,8 +630,9 @@ template <typename T> int bwd_launch(Params& p, cudaStream_t s) {
 // instruction: 1 x 16384 x 768 1004 / 531 / 303 us; 16 x 4096 x 768 711 / 705 / 817).
 template <typename T, int S> int fwd_width(Params& p, cudaStream_t s) {
     const int64_t wide = (int64_t)p.B * p.G * ((p.D / p.G + 15) / 16);
-    // a single tile is one warp's work: the others of a CTA would only hold its registers
+    // one or two tiles are one or two warps' work: the others of a CTA would only hold its registers (64 x 64 x 768 x 16 170 us with four warps, 75 with one)
     if (p.tiles <= 1) return wide >= 4 * device_sms() ? fwd_launch<T, S, 16, 1>(p, s) : fwd_launch<T, S, 4, 1>(p, s);
+    if (p.tiles == 2 && wide >= 4 * device_sms()) return fwd_launch<T, S, 16, 2>(p, s);
     const auto fits = [&](int bytes) { return bytes <= 227 * 1024; };      // (maps of many states in fp32)
     if (wide >= 2 * device_sms() && fits(FwdSmem<T, S, 16>::bytes(p.N, 4))) return fwd_launch<T, S, 16, 4>(p, s);
     if (wide >= device_sms() || !fits(FwdSmem<T, S, 4>::bytes(p.N, 6))) return fwd_launch<T, S, 8, 4>(p, s);
