@@ -6,8 +6,7 @@
 // The state that enters a tile comes from the warp of the tile before through shared memory (`carry`): everything that does not depend on it is done before it
 // is waited for, and what the next warp needs is sent on before the outputs are computed.  Warps meet nowhere else: while one waits for its rows,
 // others compute.  The maps (B and C, the same for all channels of a group)
-// are read once for a tile and kept in tensor memory, where each lane has a row of its own: registers have no room for them beside a run's decays, and out
-// of shared memory every access would take four turns.
+// are read once for a tile: the forward keeps them in registers over a warp's channels, the backward in tensor memory, where each lane has a row of its own.
 #pragma once
 #include "tc_common.cuh"
 
@@ -366,7 +365,7 @@ struct Params {
     int B, L, D, N, G, skip_f32, bias_f32, softplus;
     int32_t* status;
     int tiles, ctiles;                                           // tiles of tokens; CTAs of a group's channels
-    int piece, piece_maps, piece_state;                          // bytes of a copy that pointers and strides allow: rows, maps, states
+    int piece, piece_maps;                                       // bytes of a copy that pointers and strides allow: rows, maps
 };
 
 // a length is a number from 0 to L, whatever the caller's memory holds
