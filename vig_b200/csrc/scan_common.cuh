@@ -193,12 +193,25 @@ template <int S> __device__ __forceinline__ void own_sum(F2* P, F2* E, const F2 
         }
 }
 
+// 0, or NaN where a run's product of decays is past 2^32: of four it might leave the range.  Asked only where decays may be growth at all.
+__device__ __forceinline__ F2 grown(F2 P) {
+    const F2 two = f2_mul(P, P);
+    return f2_mul(f2_mul(two, two), 0ull);
+}
+
 // The states that enter each lane's run, of Q channels, from the runs' own sums and the states h0 that enter the tile; E of the last run becomes what leaves the
 // tile.  Runs are joined over the lanes by doubling.  An infinite state times a product that has left the type's range would be a NaN where the recurrence
-// token by token keeps the infinity: with a sum that is not finite the runs follow one another.
+// token by token keeps the infinity, and so would be a state of nothing times decays that grow (A above 0, or negative steps) past the range: with a sum that is
+// not finite, or (`grows`: where a decay may be above 1) a run's product past 2^32, of which four are multiplied, the runs follow one another.
 template <int S, int Q>
-__device__ __forceinline__ void entering(F2 (*in)[S / 2], F2 (*E)[S / 2], F2 (*P)[S / 2], const F2 (*h0)[S / 2], const F2 (*a)[RUN][S / 2], const F2 (*b)[RUN][S / 2], int run, int part) {
+__device__ __forceinline__ void entering(F2 (*in)[S / 2], F2 (*E)[S / 2], F2 (*P)[S / 2], const F2 (*h0)[S / 2], const F2 (*a)[RUN][S / 2], const F2 (*b)[RUN][S / 2], int run, int part, bool grows) {
     F2 probe = 0ull;                                             // 0, or NaN
+    if (grows) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int s = 0; s < S / 2; ++s) probe = f2_add(probe, grown(P[q][s]));
+    }
 #pragma unroll
     for (int q = 0; q < Q; ++q)
 #pragma unroll

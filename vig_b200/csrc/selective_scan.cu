@@ -8,6 +8,7 @@
 // tokens in turn and hand the state from tile to tile, within a tile a warp's lanes divide tokens and states (scan_common.cuh); two passes over
 // independent chunks would take every exponential twice.  1 x 16384 x 768 x 16 bf16 301 us, 8 x 4096 x 768 x 16 331 (45 and 90 by the exponentials), training the
 // latter 377 + 1040 + 45: issue slots at 45 to 50 %, ten warps an SM, 14 instructions a (token, channel, state) forward and 36 backward.
+#include <type_traits>
 #include "scan_common.cuh"
 
 namespace vig {
@@ -47,10 +48,12 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
     int* const given_up = (int*)(flags + CT * Npad / NB);
     const Handover hand{given_up, p.status};
 
+    bool up = !p.softplus;                                       // whether a decay may be above 1
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
         sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] * LOG2E : 0.f;
+        up |= sA[i] > 0.f;
         carry[i] = in && p.h0 ? p.h0[b * p.ld_h0 + (int64_t)(d + c) * p.N + n] : 0.f;
     }
     for (int i = tid; i < CT; i += THREADS) {
@@ -59,6 +62,7 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
     }
     for (int i = tid; i < CT * Npad / NB; i += THREADS) flags[i] = 0;
     if (tid == 0) *given_up = 0;
+    const bool grows = __syncthreads_or(up);
     const uint32_t tmem_base = tmem_take(&tmem_slot, (W > 4 ? 2 : 1) * M::COLUMNS);
     const uint32_t tmem = tmem_base + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * M::COLUMNS;
     const T *u = (const T*)p.u + b * p.s_u[0] + d, *dt = (const T*)p.dt + b * p.s_dt[0] + d, *z = p.z ? (const T*)p.z + b * p.s_z[0] + d : nullptr;
@@ -141,7 +145,7 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
                 own_sum<S>(P[0], E[0], a[0], in[0]);
                 hand.await(flag, (uint32_t)tile);
                 pairs<float, S>(h0[0], h_at);
-                entering<S, 1>(h, E, P, h0, a, in, run, part);
+                entering<S, 1>(h, E, P, h0, a, in, run, part, grows);
                 __syncwarp();
                 if (run == RUN - 1) {
 #pragma unroll
@@ -266,10 +270,12 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
     int* const given_up = (int*)(flags + CT * Npad / NB);
     const Handover hand{given_up, p.status};
 
+    bool up = !p.softplus;                                       // whether a decay may be above 1
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
         sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] : 0.f;
+        up |= sA[i] > 0.f;
         carry[i] = in && p.d_final ? p.d_final[((int64_t)b * p.D + d + c) * p.N + n] : 0.f;
     }
     for (int i = lane; i < 2 * CT * Npad; i += 32) st[i] = 0.f;
@@ -279,6 +285,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
     }
     for (int i = tid; i < CT * Npad / NB; i += THREADS) flags[i] = 0;
     if (tid == 0) *given_up = 0;
+    const bool grows = __syncthreads_or(up);
     const uint32_t tmem_base = tmem_take(&tmem_slot, columns), tmem = tmem_base + ((uint32_t)(32 * warp) << 16);      // [state block][B, C, dB, dC][8 tokens x 2 states]
     const T *u = (const T*)p.u + b * p.s_u[0] + d, *dt = (const T*)p.dt + b * p.s_dt[0] + d, *z = p.z ? (const T*)p.z + b * p.s_z[0] + d : nullptr;
     const T* dy = (const T*)p.dy + b * p.s_dy[0] + d;
@@ -330,10 +337,11 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
         }
         copies_done();
         __syncwarp();
-// (warps side by side here, not some channels apart as in the forward: they share the instructions that are fetched, 1371 -> 1198 us)
+        // (warps side by side here, not some channels apart as in the forward: they share the instructions that are fetched, 1371 -> 1198 us)
 
-#pragma unroll 1
-        for (int c = 0; c < have; ++c) {
+        // CAREFUL: a decay may be above 1, so that products of them may leave the range.  A form of its own: the questions in one form for all cost 7 % (1040 -> 1113 us).
+        const auto channel = [&](int c, auto careful) {
+            constexpr bool CAREFUL = decltype(careful)::value;
             // read again where they are used: registers are what this kernel is short of
             auto row = [&](float* v, const float* from) {
                 *(float4*)v = *(const float4*)(from + c * TILE + run * RUN);
@@ -370,7 +378,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
 #pragma unroll
                 for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_make(fmaf(mc[2 * j], dr[j], f2_lo(Q)), fmaf(mc[2 * j + 1], dr[j], f2_hi(Q))));
                 pairs<float, S>(h0, st + at);
-                entering<S, 1>(&h[0], &E, &P, &h0, &a, &in, run, part);
+                entering<S, 1>(&h[0], &E, &P, &h0, &a, &in, run, part, CAREFUL);
                 landed<16>(md);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
@@ -384,23 +392,42 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 // from the other end: q_t = a_t g_t is what token t - 1 gets
                 uint32_t* const flag = flags + n0 / NB * CT + c;
                 float* const q_at = carry + at;
-                F2 q0[1];
+                F2 q0[1], behind;                                // what enters the tile; what a run's last token gets
+                bool slow = false;
                 hand.await(flag, (uint32_t)back);
                 pairs<float, S>(q0, q_at);
-                Q = f2_fma(Pb, run == RUN - 1 ? q0[0] : 0ull, Q);
+                if (CAREFUL) {                                   // as in `entering`
+                    const F2 probe = f2_fma(q0[0], 0ull, f2_fma(Q, 0ull, grown(Pb)));
+                    slow = __any_sync(ALL, !(f2_lo(probe) + f2_hi(probe) == 0.f));
+                }
+                if (slow) {
+                    float dy8[RUN];
+                    row(dy8, dys);
+                    Q = q0[0];
+#pragma unroll 1
+                    for (int r = RUN - 1; r >= 0; --r) {
+                        if (run == r) behind = Q;
 #pragma unroll
-                for (int k = 1; k < RUN; k *= 2) {
-                    const F2 e = f2_shfl_down(Q, k * PARTS);
-                    Q = f2_fma(Pb, run + k < RUN ? e : 0ull, Q);
-                    if (2 * k < RUN) Pb = f2_mul(Pb, f2_shfl_down(Pb, k * PARTS));
+                        for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_make(fmaf(mc[2 * j], dy8[j], f2_lo(Q)), fmaf(mc[2 * j + 1], dy8[j], f2_hi(Q))));
+                        Q = f2_shfl(Q, r * PARTS + part);
+                    }
+                } else {
+                    Q = f2_fma(Pb, run == RUN - 1 ? q0[0] : 0ull, Q);
+#pragma unroll
+                    for (int k = 1; k < RUN; k *= 2) {
+                        const F2 e = f2_shfl_down(Q, k * PARTS);
+                        Q = f2_fma(Pb, run + k < RUN ? e : 0ull, Q);
+                        if (2 * k < RUN) Pb = f2_mul(Pb, f2_shfl_down(Pb, k * PARTS));
+                    }
                 }
                 __syncwarp();
                 if (run == 0) *(F2*)q_at = Q;
                 hand.pass(flag, (uint32_t)back + 1);
-                {
+                if (!slow) {
                     const F2 e = f2_shfl_down(Q, PARTS);
-                    Q = run == RUN - 1 ? q0[0] : e;
+                    behind = run == RUN - 1 ? q0[0] : e;
                 }
+                Q = behind;
                 float dl[RUN];
                 row(dl, delta);
                 row(xr, x);
@@ -430,6 +457,13 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
             if (z) *(float2*)(ys + to) = over_parts(s_y, part);
             *(float2*)(gb + to) = over_parts(s_b, part);
             *(float2*)(ga + to) = over_parts(s_a, part);
+        };
+        if (grows) {
+#pragma unroll 1
+            for (int c = 0; c < have; ++c) channel(c, std::true_type{});
+        } else {
+#pragma unroll 1
+            for (int c = 0; c < have; ++c) channel(c, std::false_type{});
         }
         kept();
         // the tile's maps have their gradients from this CTA's channels
