@@ -48,11 +48,12 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
     int* const given_up = (int*)(flags + CT * Npad / NB);
     const Handover hand{given_up, p.status};
 
+    const float none = p.softplus ? -1.f : 0.f;                  // a state that is not there: a step of +inf leaves nothing of it, and no NaN, which would go back to all tokens ahead
     bool up = !p.softplus;                                       // whether a decay may be above 1
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
-        sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] * LOG2E : 0.f;
+        sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] * LOG2E : none;
         up |= sA[i] > 0.f;
         carry[i] = in && p.h0 ? p.h0[b * p.ld_h0 + (int64_t)(d + c) * p.N + n] : 0.f;
     }
@@ -189,8 +190,13 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
             if (t0 + t < len) {
                 float uf[CT], out[CT];
                 read<T, CT>(uf, (const T*)stash, CT, 16);
+                if (p.skip) {
 #pragma unroll
-                for (int c = 0; c < CT; ++c) out[c] = fmaf(skip[c], uf[c], ys[c * TILE + t]);
+                    for (int c = 0; c < CT; ++c) out[c] = fmaf(skip[c], uf[c], ys[c * TILE + t]);
+                } else {                                         // (0 times an infinite input is a NaN)
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) out[c] = ys[c * TILE + t];
+                }
                 if (z) {
                     read<T, CT>(uf, (const T*)(stash + HALF), CT, 16);
 #pragma unroll
@@ -270,11 +276,12 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
     int* const given_up = (int*)(flags + CT * Npad / NB);
     const Handover hand{given_up, p.status};
 
+    const float none = p.softplus ? -1.f : 0.f;                  // a state that is not there: a step of +inf leaves nothing of it, and no NaN, which would go back to all tokens ahead
     bool up = !p.softplus;                                       // whether a decay may be above 1
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
-        sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] : 0.f;
+        sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] : none;
         up |= sA[i] > 0.f;
         carry[i] = in && p.d_final ? p.d_final[((int64_t)b * p.D + d + c) * p.N + n] : 0.f;
     }
@@ -354,7 +361,13 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
             for (int n0 = 0; n0 < Npad; n0 += NB) {
                 const int at = c * Npad + n0 + part * S;
                 const uint32_t col = tmem + n0 / NB * 64;
+                const int live = p.N - n0 - part * S;            // the lane's states that there are, or more; of the others nothing goes back
                 float mb[RUN * S], mc[RUN * S], md[RUN * S], xr[RUN], dr[RUN];
+                // g of token j, from what the token behind it gives back
+                const auto gradient = [&](int j, const float* dy, F2 q) {
+                    const F2 g = f2_make(fmaf(mc[2 * j], dy[j], f2_lo(q)), fmaf(mc[2 * j + 1], dy[j], f2_hi(q)));
+                    return CAREFUL ? f2_make(live > 0 ? f2_lo(g) : 0.f, live > 1 ? f2_hi(g) : 0.f) : g;
+                };
                 recall<16>(col, mb);
                 recall<16>(col + 16, mc);
                 F2 A[1], P[1], E[1], h0[1], h[RUN + 1][1], a[RUN][1], in[RUN][1], Q = 0ull, Pb;
@@ -373,10 +386,14 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 recall<16>(col + 48, md);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) in[j][0] = f2_make(xr[j] * mb[2 * j], xr[j] * mb[2 * j + 1]);
+                if (CAREFUL) {
+#pragma unroll
+                    for (int j = 0; j < RUN; ++j) a[j][0] = f2_make(live > 0 ? f2_lo(a[j][0]) : 0.f, live > 1 ? f2_hi(a[j][0]) : 0.f);
+                }
                 own_sum<S>(P, E, a, in);
                 Pb = P[0];
 #pragma unroll
-                for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_make(fmaf(mc[2 * j], dr[j], f2_lo(Q)), fmaf(mc[2 * j + 1], dr[j], f2_hi(Q))));
+                for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], gradient(j, dr, Q));
                 pairs<float, S>(h0, st + at);
                 entering<S, 1>(&h[0], &E, &P, &h0, &a, &in, run, part, CAREFUL);
                 landed<16>(md);
@@ -408,7 +425,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                     for (int r = RUN - 1; r >= 0; --r) {
                         if (run == r) behind = Q;
 #pragma unroll
-                        for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], f2_make(fmaf(mc[2 * j], dy8[j], f2_lo(Q)), fmaf(mc[2 * j + 1], dy8[j], f2_hi(Q))));
+                        for (int j = RUN - 1; j >= 0; --j) Q = f2_mul(a[j][0], gradient(j, dy8, Q));
                         Q = f2_shfl(Q, r * PARTS + part);
                     }
                 } else {
@@ -436,7 +453,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 F2 dAs = 0ull;
 #pragma unroll
                 for (int j = RUN - 1; j >= 0; --j) {
-                    const F2 gr = f2_make(fmaf(mc[2 * j], dr[j], f2_lo(Q)), fmaf(mc[2 * j + 1], dr[j], f2_hi(Q)));
+                    const F2 gr = gradient(j, dr, Q);
                     s_b[j] = fmaf(f2_lo(gr), mb[2 * j], fmaf(f2_hi(gr), mb[2 * j + 1], s_b[j]));
                     md[2 * j] = fmaf(f2_lo(gr), xr[j], md[2 * j]);
                     md[2 * j + 1] = fmaf(f2_hi(gr), xr[j], md[2 * j + 1]);
@@ -502,10 +519,15 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
                 }
                 put<T, CT>((T*)p.d_z + row, out, have, p.piece);
             }
+            if (p.skip) {
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                out[c] = fmaf(gb[c * TILE + t], delta[c * TILE + t], skip[c] * gf[c]);
-                keep_skip[c] = fmaf(gf[c], uf[c], keep_skip[c]);
+                for (int c = 0; c < CT; ++c) {
+                    out[c] = fmaf(gb[c * TILE + t], delta[c * TILE + t], skip[c] * gf[c]);
+                    keep_skip[c] = fmaf(gf[c], uf[c], keep_skip[c]);
+                }
+            } else {                                             // (0 times an infinite gradient is a NaN)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) out[c] = gb[c * TILE + t] * delta[c * TILE + t];
             }
             put<T, CT>((T*)p.d_u + row, out, have, p.piece);
             if (p.softplus) read<T, CT>(zf, dt + at * p.s_dt[1], have, p.piece);
@@ -629,7 +651,7 @@ template <typename T> __global__ void __launch_bounds__(128) scan_step_kernel(co
     y += __shfl_xor_sync(ALL, y, 2);
     y += __shfl_xor_sync(ALL, y, 1);
     if (in && part == 0) {
-        y = fmaf(skip, u, y);
+        if (p.skip) y = fmaf(skip, u, y);
         if (p.z) y *= zv * sigmoid(zv);
         ((T*)p.y)[b * p.s_y + d] = DType<T>::from_f(y);
     }
