@@ -48,6 +48,10 @@ __device__ __forceinline__ float slope(float x) {
 }
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-x * LOG2E)); }
 
+// A rate as it is taken: within +-2.3e38, so that its product with log2(e) is finite and with a step of nothing (a token behind the end of a sequence is one)
+// leaves a state as it was, where infinity * 0 would be a NaN.  Of a step above 1e-36 such a rate leaves nothing, as an infinite one does.
+__device__ __forceinline__ float rate_of(float A) { return A < -2.3e38f ? -2.3e38f : A > 2.3e38f ? 2.3e38f : A; }
+
 // where the row of token t of a tile's map lies: eight lanes that read token j of their runs read eight neighbouring rows
 __device__ __forceinline__ int row_of(int t) { return (t % RUN) * RUN + t / RUN; }
 

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
-        sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] * LOG2E : none;
+        sA[i] = in ? rate_of(p.A[(int64_t)(d + c) * p.N + n]) * LOG2E : none;
         up |= sA[i] > 0.f;
         carry[i] = in && p.h0 ? p.h0[b * p.ld_h0 + (int64_t)(d + c) * p.N + n] : 0.f;
     }
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
-        sA[i] = in ? p.A[(int64_t)(d + c) * p.N + n] : none;
+        sA[i] = in ? rate_of(p.A[(int64_t)(d + c) * p.N + n]) : none;
         up |= sA[i] > 0.f;
         carry[i] = in && p.d_final ? p.d_final[((int64_t)b * p.D + d + c) * p.N + n] : 0.f;
     }
@@ -636,7 +636,7 @@ template <typename T> __global__ void __launch_bounds__(128) scan_step_kernel(co
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            hv[k] = fmaf(ex2(dl * (av[k] * LOG2E)), hv[k], x * bv[k]);
+            hv[k] = fmaf(ex2(dl * (rate_of(av[k]) * LOG2E)), hv[k], x * bv[k]);
             y = fmaf(cv[k], hv[k], y);
         }
         if (in) {
