@@ -516,7 +516,7 @@ VIG_API int vig_add_layernorm_bwd(const void* dy, int64_t ldy, const void* x, in
                                   size_t workspace_bytes, void* stream);
 
 /*
- * Product of 8-bit integers: y[m, n] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + bias[n], summed in 32-bit integers (K <= 131072, so that no sum
+ * Product of 8-bit integers: y[m, n] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + bias[n], summed in 32-bit integers (K <= 131071, so that no sum
  * overflows), scaled in fp32, rounded once to dtype.  x: int8 [M, K] with row stride ldx; w: int8 [N, K] with row stride ldw; x_scales [M], w_scales [N]: fp32;
  * bias (optional): [N] of dtype; y: [M, N] with row stride ldy.  Any sizes and alignment.  status_dev: optional int32, bit 0 = a bounded wait ran out.
  */

@@ -401,7 +401,7 @@ std::optional<Tensor> linear_int8(const Tensor& q, const Tensor& scales, const T
     column.push_back(1);
     want(scales.sizes() == lead || scales.sizes() == at::IntArrayRef(column), "scales must have one value a row of q, [...] or [..., 1]; got " + shape_of(scales));
     want(w_scales.numel() == N && (w_scales.dim() == 1 || (w_scales.dim() == 2 && w_scales.size(1) == 1)), "weight_scales must be [N] or [N, 1]; got " + shape_of(w_scales));
-    want(K <= 131072 && N <= 4194240, "K must be 131072 at most (larger sums leave 32 bits), N 4194240");
+    want(K <= 131071 && N <= 4194240, "K must be 131071 at most (larger sums leave 32 bits), N 4194240");
     if (bias.defined()) {
         same_device(bias, q, "bias");
         want_type(bias.scalar_type() == type, "bias must have the output's dtype");

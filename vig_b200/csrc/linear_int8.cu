@@ -440,15 +440,18 @@ template <typename T> int int8_launch(const Int8Params& p, int dtype, int32_t* s
 
 using namespace vig;
 
+// Codes may be -128, whose product is 2^14: 2^17 of them are one more than a signed sum of 32 bits holds
+constexpr int I8_MOST_K = 131071;
+
 // Off 16 bytes the 64 x 64 form takes what is little, and what is more is laid out first: 65536 x 333 x 576 536 us as it lies.
 extern "C" int vig_linear_int8_laid_out_first(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0 || K > 131072 - 15) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || K > I8_MOST_K / 16 * 16) return 0;
     const bool on_16 = K % 16 == 0 && ((uintptr_t)x | (uintptr_t)w) % 16 == 0 && (ldx | ldw) % 16 == 0 && ldx >= K && ldw >= K;
     return !on_16 && (double)M * N * K >= 1 << 24;
 }
 
 extern "C" int vig_int8_rows_lay_out(const void* src, int64_t ld, void* dst, int64_t rows, int K, void* stream) {
-    if (rows < 0 || K < 0 || K > 131072) return VIG_ERR_SHAPE;
+    if (rows < 0 || K < 0 || K > I8_MOST_K) return VIG_ERR_SHAPE;
     if (!rows || !K) return VIG_OK;
     if (!src || !dst) return VIG_ERR_NULL;
     if ((uintptr_t)dst % 16) return VIG_ERR_ALIGN;
@@ -461,7 +464,7 @@ extern "C" int vig_int8_rows_lay_out(const void* src, int64_t ld, void* dst, int
 extern "C" int vig_linear_int8_fwd(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw, const float* w_scales, const void* bias, void* y,
                                    int64_t ldy, int64_t M, int N, int K, int dtype, int32_t* status_dev, void* stream) {
     if (dtype < VIG_DTYPE_F32 || dtype > VIG_DTYPE_F16) return VIG_ERR_DTYPE;
-    if (M < 0 || N < 0 || K < 0 || K > 131072 || M > INT32_MAX - 1024 || N > 4194240) return VIG_ERR_SHAPE;
+    if (M < 0 || N < 0 || K < 0 || K > I8_MOST_K || M > INT32_MAX - 1024 || N > 4194240) return VIG_ERR_SHAPE;
     if (!M || !N) return VIG_OK;
     if (!x_scales || !w_scales || !y || (K && (!x || !w))) return VIG_ERR_NULL;
     const Int8Params p{(const int8_t*)x, (const int8_t*)w, x_scales, w_scales, bias, y, ldx, ldw, ldy, M, N, K};

@@ -790,7 +790,7 @@ def add_layernorm_backward(d_y, r, weight, eps=1e-5, d_r=None, residual=None):
 def linear_int8(q, scales, weight, weight_scales, bias=None, dtype=torch.bfloat16):
     """``(q * scales) @ (weight * weight_scales[:, None]).T + bias`` of 8-bit integers, as ``add_rmsnorm_8bit`` gives them (with ``dtype=torch.int8``): ``q`` int8
     ``[..., K]``, ``scales`` fp32 ``[..., 1]`` (one value a row), ``weight`` int8 ``[N, K]``, ``weight_scales`` fp32 ``[N]``, ``bias`` ``[N]`` of ``dtype`` or None.  Returns
-    ``[..., N]`` of ``dtype`` (float32, bfloat16 or float16).  Sums are exact, scaled in fp32 and rounded once.  Any sizes (K up to 131072) and row strides; rows of
+    ``[..., N]`` of ``dtype`` (float32, bfloat16 or float16).  Sums are exact, scaled in fp32 and rounded once.  Any sizes (K up to 131071) and row strides; rows of
     whole 16 bytes on 16 bytes are what the fast forms take.  No gradient."""
     try:
         out = _lib.DTYPE_CODE[dtype]
