@@ -344,8 +344,10 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
         else ctx->save_for_backward({r.defined() ? r : x, w, Tensor()});
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["bias"] = get(bias).defined();
+        ctx->saved_data["residual"] = r.defined();
         variable_list out{y};
-        if (r.defined()) out.push_back(r);
+        // without a residual x itself, as a result of this node, so that what comes back through it is added before dx is rounded
+        if (r.defined() || x.requires_grad()) out.push_back(r.defined() ? r : x);
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list d) {
@@ -355,7 +357,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
         c10::cuda::CUDAGuard dev(x.device());
         const Tensor dy = d[0].defined() ? d[0] : at::zeros(x.sizes(), x.options());
         const auto [dx, dw, db] = layer_backward(dy, x, res, w, ctx->saved_data["bias"].toBool(), d.size() > 1 ? d[1] : Tensor(), ctx->saved_data["eps"].toDouble());
-        return {dx, dw, db, d.size() > 1 ? dx : Tensor(), Tensor()};
+        return {dx, dw, db, ctx->saved_data["residual"].toBool() ? dx : Tensor(), Tensor()};
     }
 };
 
@@ -367,7 +369,7 @@ std::pair<Tensor, Tensor> add_layernorm_train(const Tensor& x, const Tensor& w, 
     c10::cuda::CUDAGuard dev(x.device());
     if (wants_grad({&x, &w, &bias, &res})) {
         const auto out = LayerNode::apply(x, w, bias_, res_, eps);
-        return {out[0], res.defined() ? out[1] : x};
+        return {out[0], out.size() > 1 ? out[1] : x};
     }
     const auto [y, r] = layer_forward(x, w, bias, res, eps);
     return {y, r.defined() ? r : x};
