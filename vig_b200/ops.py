@@ -699,6 +699,82 @@ def add_rmsnorm_8bit(x, weight, residual=None, eps=1e-6, dtype=torch.float8_e4m3
 
 
 def add_rmsnorm_train(x, weight, residual=None, eps=1e-6):
+    """``(y, r)``: ``r = x + residual`` (``x`` itself without one), ``y = RMSNorm(r) * weight``; differentiable in ``x``, ``weight`` and
+    ``residual``, through both results.  Any N, any row strides; ``weight`` in ``x``'s dtype or fp32 (its gradient has the same).  The norm is
+    taken from the fp32 sum, where ``add_rmsnorm`` rounds the sum first."""
+    return _lib.host().add_rmsnorm_train(x, weight, residual, eps)
+
+
+def add_rmsnorm_backward(d_y, r, weight, eps=1e-6, d_r=None, residual=None):
+    """Gradients of ``add_rmsnorm_train`` at the sum ``r``, or at ``r + residual`` (taken in fp32: in 16 bits a rounded sum costs the weight's
+    gradient a third of its precision): ``(dx, dweight)``; ``dx`` is the residual's gradient too.  ``d_r``: what comes to the sum from elsewhere."""
+    return _lib.host().add_rmsnorm_backward(d_y, r, weight, eps, d_r, residual)
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, masters=None,
+               exp_avg_scales=None, exp_avg_sq_scales=None, grad_scale=None, found_inf=None):
+    """One AdamW step over lists of tensors, in place and in one launch for up to 400 of them (see ``vig_adamw_step`` for the formula).
+
+    ``params``, ``grads``: fp32, bf16 or fp16, mixed as they come; ``step`` counts from 1.  ``masters`` (entries may be None): fp32 copies that
+    are stepped in the parameters' place, these being their rounding.  States are fp32 tensors like the parameters, or, for tensors with
+    entries in both lists of scales (fp32, one value per 256 values begun, in memory order), ``float8_e4m3fn`` codes: ``exp_avg = code * scale``,
+    ``sqrt(exp_avg_sq) = code * scale``.  ``grad_scale`` / ``found_inf``: fp32 tensors of one value; gradients are multiplied by the first, and
+    nothing is written where the second is not 0.  Tensors must not overlap."""
+    beta1, beta2 = betas
+    _lib.host().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, masters, exp_avg_scales, exp_avg_sq_scales,
+                           grad_scale, found_inf)
+
+
+# --------------------------------------------------------------------------------------------------
+# Blocks with a selective state space: checks, outputs and autograd nodes are in ``csrc/host_state_space.cpp``.
+def _silu(activation):
+    if activation not in (None, "silu"):
+        raise ValueError(f"activation must be None or 'silu'; got {activation!r}")
+    return activation == "silu"
+
+
+def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=None, output_final_state=False, *, dt_softplus=True, lengths=None):
+    """Scan over ``N`` states a channel whose steps and maps change from token to token: ``delta = softplus(dt + dt_bias)``,
+    ``h_t[d, n] = exp(delta_t[d] A[d, n]) h_{t-1}[d, n] + delta_t[d] u_t[d] B_t[n]``, ``y_t[d] = (sum_n C_t[n] h_t[d, n] + D[d] u_t[d]) silu(z_t[d])``.
+
+    ``u``, ``dt``, ``z`` (optional): ``[B, L, D]`` of one dtype, any strides with a contiguous last dimension.  ``B``, ``C``: ``[B, L, N]``, or ``[B, L, G, N]``
+    for G groups of neighbouring channels, of the same dtype; 1 to 64 states.  ``A``: fp32 ``[D, N]`` (negative, for states that fade).  ``D``, ``dt_bias``
+    (optional): ``[D]`` of ``u``'s dtype or fp32.  ``initial_state``: fp32 ``[B, D, N]``.  ``dt_softplus=False``: ``delta = dt + dt_bias``.  ``lengths``: int
+    ``[B]``, how many tokens of each sequence count: behind them outputs and gradients are zeros, whatever stands there, and the final state is the one
+    behind the last that counts.  Returns ``(y, final_state)``, ``y`` in ``u``'s dtype, ``final_state`` fp32 or None.  Steps, states and sums are fp32.
+    Differentiable in every floating input, through both results."""
+    args = (u, dt, A, B, C, D, z, dt_bias, initial_state, output_final_state, dt_softplus, lengths)
+    res = _lib.host().selective_scan(*args)
+    if res is None:                         # the device's first call
+        status_word(u.device)
+        res = _lib.host().selective_scan(*args)
+    return res
+
+
+def selective_scan_step(u, dt, A, B, C, state, D=None, z=None, dt_bias=None, *, dt_softplus=True):
+    """One new token of ``selective_scan``: ``u``, ``dt``, ``z`` ``[B, D]``, ``B``, ``C`` ``[B, N]`` or ``[B, G, N]``; ``state`` (fp32 ``[B, D, N]``, a sequence's
+    part contiguous) is updated in place.  Returns ``y`` ``[B, D]``.  No gradient."""
+    return _lib.host().selective_scan_step(u, dt, A, B, C, state, D, z, dt_bias, dt_softplus)
+
+
+def causal_conv(x, weight, bias=None, initial_state=None, output_final_state=False, *, activation=None, lengths=None):
+    """Convolution of every channel with its own ``K`` taps over a token and the ``K - 1`` before it: ``y_t[d] = act(bias[d] + sum_k weight[d, k]
+    x_{t-K+1+k}[d])``, ``activation`` None or "silu".
+
+    ``x``: ``[B, L, D]``, any strides with a contiguous last dimension; ``weight``: ``[D, K]``, 1 to 8 taps, and ``bias``: ``[D]``, of ``x``'s dtype or fp32.
+    ``initial_state``: ``[B, K - 1, D]`` of ``x``'s dtype, the tokens before the first (None: zeros).  ``lengths`` as in ``selective_scan``.  Returns
+    ``(y, final_state)``, the last ``K - 1`` tokens, or None.  Sums are fp32.  Differentiable in ``x``, ``weight``, ``bias`` and ``initial_state``, through
+    both results."""
+    return _lib.host().causal_conv(x, weight, bias, initial_state, output_final_state, _silu(activation), lengths)
+
+
+def causal_conv_step(x, state, weight, bias=None, *, activation=None):
+    """One new token of ``causal_conv``: ``x`` ``[B, D]``; ``state`` (``[B, K - 1, D]`` of ``x``'s dtype, any strides with a contiguous last dimension) is moved on in
+    place.  Returns ``y`` ``[B, D]``.  No gradient."""
+    return _lib.host().causal_conv_step(x, state, weight, bias, _silu(activation))
+
+
+def add_layernorm_train(x, weight, bias=None, residual=None, eps=1e-5):
     """``(y, r)``: ``r = x + residual`` (without one ``x``, where a gradient is wanted as a result of this call), ``y = LayerNorm(r) * weight + bias``;
     differentiable in ``x``, ``weight``, ``bias`` and ``residual``, through both results.  Any N, any row strides; ``weight`` and ``bias`` in ``x``'s dtype or fp32
     (their gradients have the same).  Mean and variance are taken from the fp32 sum, where ``add_layernorm`` rounds the sum first."""
