@@ -39,7 +39,8 @@ class SelectiveStateSpace(nn.Module):
         return self.dt_proj(t), -torch.exp(self.A_log.float()), B, C
 
     def empty_state(self, batch, dtype=None, device=None):
-        """The state ahead of the first token, for ``step``: ``(last tokens of the convolution, states of the scan)``."""
+        """The state ahead of the first token, for ``step`` and ``forward``: ``(last tokens of the convolution, states of the scan)``.  The tokens are of ``dtype`` (None: the
+        weights'); in fp32 they take 16-bit ones too, as they are under ``torch.autocast``."""
         w = self.in_proj.weight
         return (torch.zeros(batch, self.d_conv - 1, self.d_inner, dtype=dtype or w.dtype, device=device or w.device),
                 torch.zeros(batch, self.d_inner, self.d_state, dtype=torch.float32, device=device or w.device))
@@ -50,7 +51,9 @@ class SelectiveStateSpace(nn.Module):
         y, residual = self._normed(hidden, residual)
         x, z = self.in_proj(y).chunk(2, -1)
         window, h = state if state is not None else (None, None)
-        x, window = ops.causal_conv(x, self.conv_weight, self.conv_bias, window, output_final_state, activation="silu", lengths=lengths)
+        # (autocast: tokens in 16 bits, and of `empty_state` a window in the weights' fp32, which goes on as such)
+        x, window = ops.causal_conv(self._widened(x, window), self.conv_weight, self.conv_bias, window, output_final_state, activation="silu", lengths=lengths)
+        x = x.to(z.dtype)
         dt, A, B, C = self._steps_and_maps(x)
         y, h = ops.selective_scan(x, dt, A, B, C, self.D, z, self.dt_bias, h, output_final_state, lengths=lengths)
         return self.out_proj(y), residual, (window, h) if output_final_state else None
@@ -60,7 +63,7 @@ class SelectiveStateSpace(nn.Module):
         """One token: ``hidden``, ``residual`` ``[B, d_model]`` (``residual`` may be None); ``state`` is updated in place.  Returns ``(output, residual)``."""
         y, residual = self._normed(hidden, residual)
         x, z = self.in_proj(y).chunk(2, -1)
-        x = ops.causal_conv_step(x, state[0], self.conv_weight, self.conv_bias, activation="silu")
+        x = ops.causal_conv_step(self._widened(x, state[0]), state[0], self.conv_weight, self.conv_bias, activation="silu").to(z.dtype)
         dt, A, B, C = self._steps_and_maps(x)
         y = ops.selective_scan_step(x, dt, A, B, C, state[1], self.D, z, self.dt_bias)
         return self.out_proj(y), residual
