@@ -213,7 +213,7 @@ template <typename T, int K, int V, int U> __global__ void __launch_bounds__(32 
     for (int64_t i = (int64_t)blockIdx.y * ROWS + row; i < all && in; i += (int64_t)gridDim.y * ROWS) {
         const int r = (int)(i % p.runs), b = (int)(i / p.runs), len = length_of(p, b);
         const int first = r * p.run, t1 = min(p.L, first + p.run), t0 = r == 0 && p.d_state ? -(K - 1) : first, end = t1 + K - 1;
-        const int calm = min(t1, len) - (p.d_out ? K - 1 : 0);   // up to where a block asks nothing
+        const int stop = min(t1, len), calm = stop - (p.d_out ? K - 1 : 0);   // tokens of the run that count; up to where a block asks nothing
         const T *const x = (const T*)p.x + b * p.s_x[0] + d, *const dy = (const T*)p.dy + b * p.s_dy[0] + d;
         const T* const st = p.state ? (const T*)p.state + b * p.s_st[0] + d : nullptr;
         T* const dx = (T*)p.dx + (int64_t)b * p.L * p.D + d;
@@ -258,7 +258,7 @@ template <typename T, int K, int V, int U> __global__ void __launch_bounds__(32 
                     float g = p.silu ? act : own;
                     if (!Q && (tj < 0 || tj >= len)) g = 0.f;
                     P[K - 1 + j][e] = g;
-                    if (Q || (tj >= first && tj < t1)) {         // whose share of dw is this run's
+                    if (Q || (tj >= first && tj < stop)) {       // whose share of dw is this run's
                         db[e] += g;
 #pragma unroll
                         for (int k = 0; k < K; ++k) dw[k][e] = fmaf(g, X[j + k][e], dw[k][e]);
