@@ -316,14 +316,15 @@ __device__ __forceinline__ void kept() {
     tc_wait_st();
 }
 
-__device__ __forceinline__ uint32_t tmem_take(uint32_t* slot, int columns) {
+// ... and, at the barrier that this takes, whether `any` holds for one of the CTA's threads
+__device__ __forceinline__ uint32_t tmem_take(uint32_t* slot, int columns, bool& any) {
     __syncwarp();
     if (threadIdx.x < 32) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(columns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
-    __syncthreads();
+    any = __syncthreads_or(any);
     tc_fence_after();
     return *slot;
 }

@@ -49,12 +49,12 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
     const Handover hand{given_up, p.status};
 
     const float none = p.softplus ? -1.f : 0.f;                  // a state that is not there: a step of +inf leaves nothing of it, and no NaN, which would go back to all tokens ahead
-    bool up = !p.softplus;                                       // whether a decay may be above 1
+    bool grows = !p.softplus;                                    // whether a decay may be above 1
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
         sA[i] = in ? rate_of(p.A[(int64_t)(d + c) * p.N + n]) * LOG2E : none;
-        up |= sA[i] > 0.f;
+        grows |= sA[i] > 0.f;
         carry[i] = in && p.h0 ? p.h0[b * p.ld_h0 + (int64_t)(d + c) * p.N + n] : 0.f;
     }
     for (int i = tid; i < CT; i += THREADS) {
@@ -63,8 +63,7 @@ __global__ void __launch_bounds__(32 * W, (S == 4 ? 12 : 16) / W) scan_fwd_kerne
     }
     for (int i = tid; i < CT * Npad / NB; i += THREADS) flags[i] = 0;
     if (tid == 0) *given_up = 0;
-    const bool grows = __syncthreads_or(up);
-    const uint32_t tmem_base = tmem_take(&tmem_slot, (W > 4 ? 2 : 1) * M::COLUMNS);
+    const uint32_t tmem_base = tmem_take(&tmem_slot, (W > 4 ? 2 : 1) * M::COLUMNS, grows);
     const uint32_t tmem = tmem_base + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * M::COLUMNS;
     const T *u = (const T*)p.u + b * p.s_u[0] + d, *dt = (const T*)p.dt + b * p.s_dt[0] + d, *z = p.z ? (const T*)p.z + b * p.s_z[0] + d : nullptr;
     const T *gB = (const T*)p.b + b * p.s_b[0] + g * p.s_b[2], *gC = (const T*)p.c + b * p.s_c[0] + g * p.s_c[2];
@@ -277,12 +276,12 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
     const Handover hand{given_up, p.status};
 
     const float none = p.softplus ? -1.f : 0.f;                  // a state that is not there: a step of +inf leaves nothing of it, and no NaN, which would go back to all tokens ahead
-    bool up = !p.softplus;                                       // whether a decay may be above 1
+    bool grows = !p.softplus;                                    // whether a decay may be above 1
     for (int i = tid; i < CT * Npad; i += THREADS) {
         const int c = i / Npad, n = i - c * Npad;
         const bool in = c < have && n < p.N;
         sA[i] = in ? rate_of(p.A[(int64_t)(d + c) * p.N + n]) : none;
-        up |= sA[i] > 0.f;
+        grows |= sA[i] > 0.f;
         carry[i] = in && p.d_final ? p.d_final[((int64_t)b * p.D + d + c) * p.N + n] : 0.f;
     }
     for (int i = lane; i < 2 * CT * Npad; i += 32) st[i] = 0.f;
@@ -292,8 +291,7 @@ __global__ void __launch_bounds__(BTHREADS, 3) scan_bwd_kernel(const Params p) {
     }
     for (int i = tid; i < CT * Npad / NB; i += THREADS) flags[i] = 0;
     if (tid == 0) *given_up = 0;
-    const bool grows = __syncthreads_or(up);
-    const uint32_t tmem_base = tmem_take(&tmem_slot, columns), tmem = tmem_base + ((uint32_t)(32 * warp) << 16);      // [state block][B, C, dB, dC][8 tokens x 2 states]
+    const uint32_t tmem_base = tmem_take(&tmem_slot, columns, grows), tmem = tmem_base + ((uint32_t)(32 * warp) << 16);      // [state block][B, C, dB, dC][8 tokens x 2 states]
     const T *u = (const T*)p.u + b * p.s_u[0] + d, *dt = (const T*)p.dt + b * p.s_dt[0] + d, *z = p.z ? (const T*)p.z + b * p.s_z[0] + d : nullptr;
     const T* dy = (const T*)p.dy + b * p.s_dy[0] + d;
     const T *gB = (const T*)p.b + b * p.s_b[0] + g * p.s_b[2], *gC = (const T*)p.c + b * p.s_c[0] + g * p.s_c[2];
