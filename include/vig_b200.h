@@ -445,14 +445,15 @@ VIG_API int vig_adamw_step(int count, void* const* params, const void* const* gr
  * Selective scan: delta = softplus(dt + dt_bias) (softplus 0: dt + dt_bias), h_t[d,n] = exp(delta_t[d] A[d,n]) h_{t-1}[d,n] + delta_t[d] u_t[d] b_t[n],
  * y_t[d] = (sum_n c_t[n] h_t[d,n] + skip[d] u_t[d]) silu(z_t[d]).  All pointers are device pointers; optional ones are NULL.
  *   u, dt, z (optional), y, d_y: [B, L, D] of dtype, unit stride over D, element strides (b, l).  b, c: [B, L, G, N] of dtype, unit stride over N,
- *   strides (b, l, g); channel d reads group d / (D / G), D % G == 0, 1 <= N <= 64.  A: fp32 [D, N] contiguous.  skip, dt_bias (optional): [D] of
+ *   strides (b, l, g); channel d reads group d / (D / G), D % G == 0, 1 <= N <= 64.  A: fp32 [D, N] contiguous, taken within +-2.3e38.  skip, dt_bias (optional): [D] of
  *   skip_dtype, bias_dtype (dtype or fp32).  lengths (optional): int32 [B], tokens of a sequence that count (taken into 0..L): behind them y
  *   and gradients are zeros and states stay.  h0 (optional), h_final (optional): fp32 [B, D, N], sequences ld_h0 / ld_final apart, channels N apart;
  *   h_final may be h0.  Any alignment.  B * D < 2^31, D < 2^28, L < 2^30.
  * vig_selective_scan_fwd: y and h_final; with `states` (vig_selective_scan_states_bytes) also the states that enter every 64th token, for a backward.
  * vig_selective_scan_bwd: from the inputs, these states, d_y and d_final (optional, fp32 [B, D, N] contiguous): d_u, d_dt, d_z [B, L, D] and d_b,
  *   d_c [B, L, G, N] of dtype, d_A fp32 [D, N], d_skip, d_bias (optional) [D] of their types, d_h0 (optional) fp32 [B, D, N], all contiguous.  Sums over
- *   channels, tokens and sequences are fp32 in a fixed order.
+ *   channels, tokens and sequences are fp32 in a fixed order.  Its workspace holds their shares, most of them those of d_b and d_c: 4 (2 ceil(D / G / 16) B L G N +
+ *   B D (N + 2)) bytes, which is N / 2 bytes for each of B L D values (8 x 4096 x 768 with 16 states: 202 MB, u 50 MB), and the states 4 B ceil(L / 64) D N bytes.
  * vig_selective_scan_step: L = 1; h_final is the state, updated in place (h0 and lengths are not looked at).
  * status: optional int32 on the device, bit 0 = a bounded wait ran out.
  */

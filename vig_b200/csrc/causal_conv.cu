@@ -3,7 +3,8 @@
 //
 // Bound by memory: x in, y out; backward x and dy in, dx out.  A thread walks a run of tokens of a few neighbouring channels and keeps the
 // window in registers, so that each value is read once and, at the border of two runs, K - 1 times more out of the cache.  16 x 4096 x 768 bf16, 4 taps: forward
-// 51 us (4.0 TB/s), backward 136 (2.2 TB/s; 30 instructions a value bound it, at 16 warps an SM).
+// 50 us (4.0 TB/s; 25 instructions a value, issue slots at 71 %), backward 136 (2.2 TB/s; 51 instructions a value, issue slots at 57 % with 16 warps an SM; at the 128
+// registers that these allow, 4 taps of 4 channels in 16 bits spill 120 bytes).
 #include <type_traits>
 #include "tc_common.cuh"
 
@@ -51,7 +52,8 @@ template <typename T, int V> struct Piece {
 
 template <typename T> __device__ __forceinline__ float weight(const void* w, int64_t i, int f32) { return f32 ? ((const float*)w)[i] : DType<T>::to_f(((const T*)w)[i]); }
 
-// the taps and biases of V neighbouring channels: whole pieces of 16 bytes where the channels are, since they lie one behind the other
+// the taps and biases of V neighbouring channels: those in fp32 in whole pieces of 16 bytes, since they lie one behind the other; those in 16 bits, whose V biases
+// are 8 bytes, one at a time
 template <typename T, typename W, int K, int V> __device__ __forceinline__ void taps_of(const W* w, const W* bias, int d, int whole, float (*f)[V], float* b) {
     W e[V * K], c[V];
     constexpr bool PIECES = V * (int)sizeof(W) % 16 == 0;

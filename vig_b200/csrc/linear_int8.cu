@@ -1,10 +1,11 @@
 // Product of 8-bit integers: y[m, n] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + bias[n].  Sums are 32-bit integers and exact; scales and bias are
 // applied in fp32 and y is rounded once.  Three forms:
 //   pairs   (rows on 16 bytes): tcgen05.mma kind::i8 on CTA pairs, tiles of 256 x 256, k boxes of 128 bytes through TMA, as gemm_pair.cu does for 16 bits: the
-//           integer product is twice as fast and brings in half the bytes, so what bounds it is the output (65536 x 768 x 2304: 302 of 354 MB).  That case takes
-//           96 us; 77 without the epilogue's work, 89 without its stores.
+//           integer product is twice as fast and brings in half the bytes.  65536 x 768 x 2304 takes 97 us; 77 without the epilogue's work, 89 without its
+//           stores; 70 would be the products by themselves, 54 the bytes (302 of 354 MB are the output).
 //   skinny  (rows on 16 bytes, up to 64 of them): W is read once, by all SMs, straight into fragments of mma.sync; a warp takes 16 columns and a share of k.
-//           8 x 768 x 2304 2.5 us; as tiles of the form below 12.
+//           768 x 2304 with W in L2, this form and pairs: 8 rows 2.4 and 6.6 us, 32 rows 5.1 and 6.7, 64 rows 6.8 and 6.9.  With W out of memory: 8 rows 4.2 and
+//           7.3, 24 rows 7.7 and 7.4, 64 rows 11.9 and 7.5, so that there a border at 16 would be the better one.
 //   any     everything else: mma.sync on 64 x 64 tiles through shared memory.
 #include "tc_common.cuh"
 

@@ -6,8 +6,9 @@
 // Every (token, channel, state) costs an exponential and three multiply-adds, every (token, channel) three 16-bit values in and one out: with 16
 // states the exponentials bound it (MUFU, 16 a cycle and SM), not memory.  So each is taken once: the warps of a CTA take tiles of the same channels'
 // tokens in turn and hand the state from tile to tile, within a tile a warp's lanes divide tokens and states (scan_common.cuh); two passes over
-// independent chunks would take every exponential twice.  1 x 16384 x 768 x 16 bf16 301 us, 8 x 4096 x 768 x 16 331 (45 and 90 by the exponentials), training the
-// latter 377 + 1040 + 45: issue slots at 45 to 50 %, ten warps an SM, 14 instructions a (token, channel, state) forward and 36 backward.
+// independent chunks would take every exponential twice.  1 x 16384 x 768 x 16 bf16 306 us, 8 x 4096 x 768 x 16 336 (45 and 90 by the exponentials), training the
+// latter 383 + 1055 + 45: issue slots at 41 to 45 %, ten warps an SM, 15 instructions a (token, channel, state) forward and 41 backward, the polls among them.
+// Sixteen channels and four warps is the backward's only shape: one long sequence, 1 x 16384 x 768, leaves it 48 CTAs and takes 346 + 2852 + 23.
 #include <type_traits>
 #include "scan_common.cuh"
 

@@ -738,10 +738,11 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, initial_state=N
     ``h_t[d, n] = exp(delta_t[d] A[d, n]) h_{t-1}[d, n] + delta_t[d] u_t[d] B_t[n]``, ``y_t[d] = (sum_n C_t[n] h_t[d, n] + D[d] u_t[d]) silu(z_t[d])``.
 
     ``u``, ``dt``, ``z`` (optional): ``[B, L, D]`` of one dtype, any strides with a contiguous last dimension.  ``B``, ``C``: ``[B, L, N]``, or ``[B, L, G, N]``
-    for G groups of neighbouring channels, of the same dtype; 1 to 64 states.  ``A``: fp32 ``[D, N]`` (negative, for states that fade).  ``D``, ``dt_bias``
+    for G groups of neighbouring channels, of the same dtype; 1 to 64 states.  ``A``: fp32 ``[D, N]`` (negative, for states that fade; taken within +-2.3e38).  ``D``, ``dt_bias``
     (optional): ``[D]`` of ``u``'s dtype or fp32.  ``initial_state``: fp32 ``[B, D, N]``.  ``dt_softplus=False``: ``delta = dt + dt_bias``.  ``lengths``: int
     ``[B]``, how many tokens of each sequence count: behind them outputs and gradients are zeros, whatever stands there, and the final state is the one
-    behind the last that counts.  Returns ``(y, final_state)``, ``y`` in ``u``'s dtype, ``final_state`` fp32 or None.  Steps, states and sums are fp32.
+    behind the last that counts.  Returns ``(y, final_state)``, ``y`` in ``u``'s dtype, ``final_state`` fp32 or None.  Steps, states and sums are fp32; an infinite state
+    stays one, and what comes of an infinite input or gradient is an infinity or a NaN.
     Differentiable in every floating input, through both results."""
     args = (u, dt, A, B, C, D, z, dt_bias, initial_state, output_final_state, dt_softplus, lengths)
     res = _lib.host().selective_scan(*args)

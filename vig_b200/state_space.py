@@ -20,7 +20,7 @@ class SelectiveStateSpace(nn.Module):
         self.conv_bias = nn.Parameter(torch.zeros(self.d_inner))
         self.x_proj = nn.Linear(self.d_inner, self.dt_rank + 2 * d_state, bias=False)
         self.dt_proj = nn.Linear(self.dt_rank, self.d_inner, bias=False)
-        # steps between dt_min and dt_max, rates 1 to d_state: memories of all lengths to begin with
+        # steps between dt_min and dt_max, evenly in their logarithm, rates 1 to d_state: memories of all lengths to begin with (Gu and Dao 2023, with the selective scan)
         step = torch.exp(torch.rand(self.d_inner) * math.log(dt_max / dt_min) + math.log(dt_min))
         self.dt_bias = nn.Parameter(step + torch.log(-torch.expm1(-step)))
         self.A_log = nn.Parameter(torch.log(torch.arange(1, d_state + 1, dtype=torch.float32)).repeat(self.d_inner, 1))
