@@ -177,13 +177,18 @@ __device__ __forceinline__ F2 f2_shfl_up(F2 v, int lanes) { return f2_make(__shf
 __device__ __forceinline__ F2 f2_shfl_down(F2 v, int lanes) { return f2_make(__shfl_down_sync(ALL, f2_lo(v), lanes), __shfl_down_sync(ALL, f2_hi(v), lanes)); }
 __device__ __forceinline__ F2 f2_shfl(F2 v, int lane) { return f2_make(__shfl_sync(ALL, f2_lo(v), lane), __shfl_sync(ALL, f2_hi(v), lane)); }
 
+// The unit's 2^x is below the value by 0.1 to 0.5 of 2^-24 on average over arguments from 0 to -0.6, and tokens of like steps multiply that up.  Its argument, rounded once with
+// the product, is raised by what makes 0.2 of it good, which leaves between -0.27 and 0.12 and 2^0 = 1: dA of training 8 x 1024 x 256 x 16 fp32 1.6e-6 -> 7.6e-7
+// from 64 bits (5.7e-7 with expf), at the same time.
+constexpr float EX2_LOW = 0.2f / 16777216.f * LOG2E;
+
 // decays of a run, exp(delta A) with A in log2 units
 template <int S> __device__ __forceinline__ void decays(F2 (*a)[S / 2], const float* delta, const F2* A2) {
 #pragma unroll
     for (int j = 0; j < RUN; ++j)
 #pragma unroll
         for (int s = 0; s < S / 2; ++s) {
-            const F2 x = f2_mul(f2_make(delta[j], delta[j]), A2[s]);
+            const F2 x = f2_fma(f2_make(delta[j], delta[j]), A2[s], f2_make(EX2_LOW, EX2_LOW));
             a[j][s] = f2_make(ex2(f2_lo(x)), ex2(f2_hi(x)));
         }
 }

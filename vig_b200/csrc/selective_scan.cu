@@ -635,7 +635,7 @@ template <typename T> __global__ void __launch_bounds__(128) scan_step_kernel(co
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            hv[k] = fmaf(ex2(dl * (rate_of(av[k]) * LOG2E)), hv[k], x * bv[k]);
+            hv[k] = fmaf(ex2(fmaf(dl, rate_of(av[k]) * LOG2E, EX2_LOW)), hv[k], x * bv[k]);
             y = fmaf(cv[k], hv[k], y);
         }
         if (in) {
